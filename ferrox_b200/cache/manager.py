@@ -73,6 +73,16 @@ class LayerCache:
     def v(self) -> Optional[torch.Tensor]:
         return self.pages.get("v")
 
+    @property
+    def fp8(self) -> bool:
+        """Whether keys and values are e4m3 elements with exponents beside them (``cache.specs.in_8_bits``)."""
+        return "k_exp" in self.pages
+
+    @property
+    def fp8_operands(self):
+        """An 8-bit cache as the kernels' entry points take it: pages, exponents, block table, page size."""
+        return self.pages["k"], self.pages["v"], self.pages["k_exp"], self.pages["v_exp"], self.block_table, self.page_size
+
 
 _CHECKS = {
     1: "a page is mapped outside a live request's held range", 2: "a hole in a request's held range",

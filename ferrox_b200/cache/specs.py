@@ -14,7 +14,7 @@ fixed recurrent state for its linear-attention model.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import Optional, Tuple
 
 import torch
@@ -54,6 +54,16 @@ def KvCacheSpec(n_kv_heads: int, head_dim: int, window: Optional[int] = None, ke
     shape = (int(n_kv_heads), int(head_dim))
     return PagedSpec((PagedTensorSpec("k", shape, lead_dims=1), PagedTensorSpec("v", shape, lead_dims=1)), window,
                      int(keep_first) if window is not None else 0, chunk)
+
+
+def in_8_bits(paged: PagedSpec) -> PagedSpec:
+    """Keys and values of :func:`KvCacheSpec` as e4m3 elements with one power of two a position and kv head: ``k`` and ``v`` of
+    that type, their exponents ``k_exp`` and ``v_exp`` [n_pages, n_kv_heads, page_size] bytes (kernels.ops.rope_kv_write_fp8)."""
+    if {t.name for t in paged.tensors} != {"k", "v"} or any(len(t.token_shape) != 2 or t.lead_dims != 1 for t in paged.tensors):
+        raise ValueError("an 8-bit cache holds keys and values [n_kv_heads, head_dim] of a position")
+    tensors = [replace(t, dtype=torch.float8_e4m3fn) for t in paged.tensors]
+    tensors += [PagedTensorSpec(t.name + "_exp", t.token_shape[:1], lead_dims=1, dtype=torch.uint8) for t in paged.tensors]
+    return replace(paged, tensors=tuple(tensors))
 
 
 @dataclass(frozen=True)

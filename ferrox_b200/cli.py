@@ -10,9 +10,9 @@ Options keep the reference's names, defaults and meanings where it has them
 ``-e/--escape``, ``--ignore-eos``, ``--verbose-prompt``.  A leading ``run`` is
 accepted and optional, as the reference inserts it itself (main.rs:254-296).
 ``-m`` names a model folder (config.json + safetensors) instead of a GGUF file.
-Options without a counterpart here (threads, devices, GPU layers, KV dtype) are
+Options without a counterpart here (threads, devices, GPU layers) are
 not offered: there is one backend.  Added: ``--tokens`` (prompt as token ids),
-``--dtype``, ``--page-size``, ``--num-pages``, ``--max-batch-tokens``, ``--random``.
+``--dtype``, ``--kv-cache`` (8-bit keys and values), ``--page-size``, ``--num-pages``, ``--max-batch-tokens``, ``--random``.
 
 Text prompts use the byte-level tokenizer (tokenizer.rs:40-56); the generated text
 goes to stdout and, as in the reference (run.rs:680-695), one line to stderr:
@@ -48,6 +48,8 @@ def build_parser() -> argparse.ArgumentParser:
                     help="sum the device time of every class of kernel and print the table to stderr at the end "
                          "(launches then run one by one, without CUDA graphs: for looking, not for speed)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--kv-cache", default="model", choices=["model", "fp8"],
+                    help="how keys and values are held: in the compute type, or in 8 bits (e4m3 and a power of two a position and head)")
     ap.add_argument("--page-size", type=int, default=64)
     ap.add_argument("--num-pages", type=int, default=0, help="cache pages per layer group (0 = one context's worth)")
     ap.add_argument("--max-batch-tokens", type=int, default=2048, help="token budget of one step")
@@ -83,7 +85,7 @@ def main(argv=None) -> int:
     if args.trace_kernels:
         Engine.trace_start()   # before the engine is made: it then leaves CUDA graphs off
     t0 = time.time()
-    cache = dict(page_size=args.page_size, max_slots=4)
+    cache = dict(page_size=args.page_size, max_slots=4, kv_cache=None if args.kv_cache == "model" else args.kv_cache)
     if args.ctx_size:
         cache["max_positions"] = args.ctx_size
     if args.random:

@@ -77,6 +77,22 @@ int fx_rope_kv_write(void* qkv, int dtype, long ld, const int* positions, const 
                      const float* inv_freq, const float* cos_sin, int rotary_dim, int pairing, void* k_pages, void* v_pages, const int* block_table,
                      int table_width, int page_size, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
                      int write_cache, int* status, void* stream);
+// The 8-bit cache (fp8.cuh): bytes of e4m3 [page][kv head][position][head_dim], exponents [page][kv head][position]; n_slots rows
+// of table_width entries in the block table, n_pages pages.  Positions and pages outside them are treated as missing.
+int fx_rope_kv_write_fp8(void* qkv, int dtype, long ld, const int* positions, const int* token_seq, const int* seq_slot,
+                         const float* inv_freq, const float* cos_sin, int rotary_dim, int pairing, void* k_pages, void* v_pages,
+                         void* k_exp, void* v_exp, const int* block_table, int n_slots, int table_width, int page_size, int n_pages,
+                         int n_tokens, int n_heads, int n_kv_heads, int head_dim, int write_cache, int* status, void* stream);
+// spans null: k_out, v_out [n_rows][kv heads][head_dim] at the listed positions; else pages of n_spans stretches
+int fx_read_kv_fp8(const void* k_pages, const void* v_pages, const void* k_exp, const void* v_exp, const int* block_table, int n_slots,
+                   int table_width, int page_size, int n_pages, const int* positions, const int* token_seq, const int* seq_slot,
+                   const int* spans, int n_spans, int n_rows, void* k_out, void* v_out, int dtype, int n_kv_heads, int head_dim,
+                   void* stream);
+// tokens (optional): the n_tokens rows of q and out that are taken
+int fx_attention_fp8(const void* q, long ldq, int dtype, const void* k_pages, const void* v_pages, const void* k_exp,
+                     const void* v_exp, const int* block_table, int n_slots, int table_width, int page_size, int n_pages,
+                     const int* positions, const int* token_seq, const int* seq_slot, const int* tokens, int n_tokens, void* out,
+                     long ldo, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap, void* stream);
 int fx_moe_combine(float* h, const void* y, int dtype, const int* inv_perm, const float* topk_w, int top_k,
                    const void* shared, const float* shared_gate_logit, long gate_ld, int n_tokens, int hidden,
                    void* stream);

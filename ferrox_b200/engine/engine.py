@@ -43,9 +43,11 @@ def _dtype(d) -> torch.dtype:
 
 class Engine:
     def __init__(self, config, spec, model, *, page_size=64, n_pages=None, max_tokens=None, max_slots=64,
-                 max_positions=None, cuda_graphs=True):
+                 max_positions=None, cuda_graphs=True, kv_cache=None):
         """Use :meth:`from_folder` or :meth:`from_random`.  The cache pool holds
-        ``n_pages`` pages per group, or enough for ``max_tokens`` positions."""
+        ``n_pages`` pages per group, or enough for ``max_tokens`` positions.  ``kv_cache="fp8"``: keys and values are held
+        in 8 bits (e4m3 elements with one power of two a position and kv head), half of a bfloat16 cache's bytes; for models
+        whose attention layers all take it so (refused by name otherwise)."""
         self.config = config
         self.spec = spec
         self.model = model
@@ -57,7 +59,7 @@ class Engine:
                 max_tokens = min(max_positions * 4, 65536)
             n_pages = (max_tokens + page_size - 1) // page_size
         self.cache = CacheManager(
-            model.cache_specs(), page_size=page_size, n_pages=n_pages, max_slots=max_slots,
+            model.cache_specs(kv_cache), page_size=page_size, n_pages=n_pages, max_slots=max_slots,
             max_positions=max_positions, device=self.rt.device, dtype=self.rt.dtype,
         )
         # decode steps replay CUDA graphs when every part of the model can be captured (and no kernel trace is on:

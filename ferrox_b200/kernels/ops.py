@@ -123,6 +123,9 @@ _SIGNATURES = {
     "fx_gemm_skinny": [_P, _L, _P, _P, _L, _L, _P, _I, _P, _I, _L, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _I, _I, _I, _P],
     "fx_decode_attention": [_P, _L, _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P, _L, _P, _P, _I, _I, _I, _I, _I, _F, _I,
                             _I, _P, _P, _I, _I, _I, _P, _F, _P, _P],
+    "fx_rope_kv_write_fp8": [_P, _I, _L, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "fx_read_kv_fp8": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _P],
+    "fx_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F, _P],
     "fx_argmax": [_P, _L, _I, _I, _P, _P],
     "fx_repetition_penalty": [_P, _L, _I, _I, _P, _P, _P, _P],
     "fx_sample": [_P, _L, _I, _I, _P, _P, _P, _P, _P, _P],
@@ -1991,6 +1994,330 @@ def gemm_tc2(x, w, out, *, bias=None, accumulate=False, gated=False, unary=None,
          _ptr(out), code(out), _rows(out), int(accumulate), M, N, K, int(_gated_or_unary(gated, unary)), N if gated else 0, lim, alpha,
          int(tile), _ptr(status), stream if stream is not None else stream_ptr())
     return out
+
+
+# ---- the 8-bit cache: e4m3 elements and one exponent a position and head (csrc/fp8.cuh) --------------------------------------
+FP8_MAX_DIM = 256                 # elements of a head
+FP8_LARGEST, FP8_MIN_EXP, FP8_NAN = 448.0, -119, 255
+
+
+def _on_current_device(name, *tensors):
+    """A launch goes to the current device: operands elsewhere are refused."""
+    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.device.index == device):
+            raise KernelError(f"{name}: an operand on {t.device}, the current device is " + (f"cuda:{device}" if device >= 0 else "none"))
+
+
+def _int32(name, what, *tensors):
+    for t in tensors:
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise KernelError(f"{name}: {what} are contiguous int32, found {t.dtype} with strides {t.stride()}")
+
+
+def _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size):
+    """Checks an 8-bit cache; its (pages, kv heads, head size)."""
+    if k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn or k_exp.dtype != torch.uint8 or v_exp.dtype != torch.uint8:
+        raise KernelError(f"{name}: pages are float8_e4m3fn and their exponents uint8, found {k_pages.dtype}, {v_pages.dtype}, {k_exp.dtype}, {v_exp.dtype}")
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or k_exp.shape != shape[:3] or v_exp.shape != shape[:3] or shape[2] != page_size:
+        raise KernelError(f"{name}: pages [pages, kv heads, {page_size}, head size] and exponents [pages, kv heads, {page_size}], found "
+                          f"{tuple(shape)}, {tuple(v_pages.shape)}, {tuple(k_exp.shape)}, {tuple(v_exp.shape)}")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and k_exp.is_contiguous() and v_exp.is_contiguous()):
+        raise KernelError(f"{name}: pages and exponents are contiguous")
+    if block_table.dim() != 2 or block_table.shape[1] == 0:
+        raise KernelError(f"{name}: the block table is [slots, pages of a request], found {tuple(block_table.shape)}")
+    _int32(name, "block tables", block_table)
+    if not 0 < shape[3] <= FP8_MAX_DIM or shape[0] == 0:
+        raise KernelError(f"{name}: heads of 1 to {FP8_MAX_DIM} elements and at least one page, found {tuple(shape)}")
+    return shape[0], shape[1], shape[3]
+
+
+def rope_kv_write_fp8(qkv, positions, token_seq, seq_slot, inv_freq, rotary_dim, k_pages, v_pages, k_exp, v_exp, block_table,
+                      page_size, n_heads, n_kv_heads, head_dim, write_cache=True, status=None, stream=None, cos_sin=None,
+                      pairing=PAIR_HALVES):
+    """:func:`rope_kv_write` into an 8-bit cache: q and k rotated in place (``inv_freq`` None: neither), k and v quantised as they
+    are written.  ``k_pages``, ``v_pages`` float8_e4m3fn [pages, kv heads, page, head_dim] and ``k_exp``, ``v_exp`` uint8 [pages, kv
+    heads, page]: element i of a position stands for e4m3_i * 2^(E - 127), with e = E - 127 the smallest whole number for which the
+    row's largest |x| is at most 448 * 2^e (at least -119), and e4m3_i = x_i / 2^e rounded to nearest, ties to even (numbers beyond
+    240 * 2^120 as that: the next one is infinite in 32 bits).  A row with an
+    element that is infinite or no number gets E = 255 and reads as NaN.  A position without a page, or outside its table, is
+    written nowhere and raises ``status`` 2.  Positions of a call are distinct."""
+    name = "rope_kv_write_fp8"
+    n_pages, G, D = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
+    T = qkv.shape[0]
+    if (G, D) != (n_kv_heads, head_dim) or qkv.dim() != 2 or qkv.shape[1] < (n_heads + 2 * n_kv_heads) * head_dim:
+        raise KernelError(f"{name}: rows of {n_heads} + 2 * {n_kv_heads} heads of {head_dim} for pages of {G} heads of {D}, found {tuple(qkv.shape)}")
+    if positions.numel() != T or token_seq.numel() != T:
+        raise KernelError(f"{name}: a position and an entry for each of {T} rows, found {positions.numel()} and {token_seq.numel()}")
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or 2 * inv_freq.numel() < rotary_dim):
+        raise KernelError(f"{name}: {rotary_dim // 2} contiguous 32-bit frequencies, found {inv_freq.dtype} {tuple(inv_freq.shape)}")
+    if cos_sin is not None and (cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.numel() < T * rotary_dim):
+        raise KernelError(f"{name}: contiguous 32-bit (cos, sin) pairs [{T}, {rotary_dim // 2}, 2], found {cos_sin.dtype} {tuple(cos_sin.shape)}")
+    _int32(name, "positions, entries and slots", positions, token_seq, seq_slot)
+    _on_current_device(name, qkv, positions, token_seq, seq_slot, inv_freq, cos_sin, k_pages, v_pages, k_exp, v_exp, block_table, status)
+    call("fx_rope_kv_write_fp8", _ptr(qkv), code(qkv), _rows(qkv), _ptr(positions), _ptr(token_seq), _ptr(seq_slot), _ptr(inv_freq),
+         _ptr(cos_sin), rotary_dim, int(pairing), _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table),
+         block_table.shape[0], block_table.shape[1], page_size, n_pages, T, n_heads, n_kv_heads, head_dim, int(write_cache), _ptr(status),
+         stream if stream is not None else stream_ptr())
+
+
+def _read_kv_fp8(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, spans, n_rows, k_out,
+                 v_out, shape, stream):
+    n_pages, G, D = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
+    shape = shape(G, D)
+    if k_out.dtype != v_out.dtype or k_out.shape != shape or v_out.shape != shape or not (k_out.is_contiguous() and v_out.is_contiguous()):
+        raise KernelError(f"{name}: two contiguous results {tuple(shape)} of one type, found {tuple(k_out.shape)} {k_out.dtype} and "
+                          f"{tuple(v_out.shape)} {v_out.dtype}")
+    _int32(name, "positions, entries, slots and spans", positions, token_seq, seq_slot, spans)
+    _on_current_device(name, k_pages, v_pages, k_exp, v_exp, block_table, positions, token_seq, seq_slot, spans, k_out, v_out)
+    call("fx_read_kv_fp8", _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table), block_table.shape[0],
+         block_table.shape[1], page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot), _ptr(spans),
+         spans.shape[0] if spans is not None else 0, n_rows, _ptr(k_out), _ptr(v_out), code(k_out), G, D,
+         stream if stream is not None else stream_ptr())
+
+
+def read_kv_fp8(k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, k_out, v_out, stream=None):
+    """What an 8-bit cache holds at the given positions: ``k_out``, ``v_out`` [tokens, kv heads, head_dim] (bfloat16, in which every
+    value is exact, or float32).  A position without a page reads as 0."""
+    T = positions.numel()
+    if token_seq.numel() != T:
+        raise KernelError(f"read_kv_fp8: an entry for each of {T} positions, found {token_seq.numel()}")
+    _read_kv_fp8("read_kv_fp8", k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, None, T, k_out,
+                 v_out, lambda G, D: (T, G, D), stream)
+
+
+def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, spans, n_rows, seq_slot, k_out, v_out, stream=None):
+    """Stretches of requests out of an 8-bit cache into pages that the other attention kernels take: ``k_out``, ``v_out`` [n_rows /
+    page, kv heads, page, head_dim].  ``spans``: int32 [n, 4] rows of (entry, first position, end, first row), first positions and
+    rows multiples of the page, the rows in order and without gaps up to ``n_rows``.  What lies behind a stretch's end in its last
+    page is 0, and so is a page that its request does not have."""
+    if n_rows % page_size or n_rows < 0 or spans.dim() != 2 or spans.shape[1] != 4 or (n_rows and not spans.shape[0]):
+        raise KernelError(f"read_kv_fp8_spans: spans [n, 4] over a multiple of {page_size} rows, found {tuple(spans.shape)} over {n_rows}")
+    _read_kv_fp8("read_kv_fp8_spans", k_pages, v_pages, k_exp, v_exp, block_table, page_size, None, None, seq_slot, spans, n_rows, k_out,
+                 v_out, lambda G, D: (n_rows // page_size, G, page_size, D), stream)
+
+
+def _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, tokens, out,
+                         n_heads, n_kv_heads, head_dim, window, scale, softcap):
+    n_pages, G, D = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
+    T = positions.numel()
+    if (G, D) != (n_kv_heads, head_dim) or n_heads < 1 or n_heads % n_kv_heads:
+        raise KernelError(f"{name}: {n_heads} heads on {n_kv_heads} of {head_dim} for pages of {G} heads of {D}")
+    if out.dtype != q.dtype or q.dim() != 2 or q.shape[0] != T or q.shape[1] < n_heads * head_dim or out.dim() != 2 or out.shape[0] != T \
+            or out.shape[1] < n_heads * head_dim or token_seq.numel() != T:
+        raise KernelError(f"{name}: {T} rows of {n_heads} heads of {head_dim}, found queries {tuple(q.shape)} {q.dtype}, results "
+                          f"{tuple(out.shape)} {out.dtype}, {token_seq.numel()} entries")
+    if (window is not None and window < 1) or (softcap is not None and not softcap > 0) or not abs(scale) < float("inf"):
+        raise KernelError(f"{name}: window={window}, softcap={softcap}, scale={scale}: positive (or None), positive (or None), finite")
+    _int32(name, "positions, entries, slots and tokens", positions, token_seq, seq_slot, tokens)
+    _on_current_device(name, q, k_pages, v_pages, k_exp, v_exp, block_table, positions, token_seq, seq_slot, tokens, out)
+    return n_pages
+
+
+def decode_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, out, n_heads,
+                         n_kv_heads, head_dim, window, scale, softcap=None, status=None, tokens=None, stream=None):
+    """Attention of few tokens a request over an 8-bit cache (:func:`rope_kv_write_fp8`): ``q`` rows that start with the query heads,
+    in 16 or 32 bits as ``out``; token t sees the positions max(0, p - window + 1) .. p of its request, its own among them.
+    ``tokens`` (int32, optional): the rows of ``q`` and ``out`` that are taken; the others stay as they are.  Positions without a
+    page do not count; a token that sees none gets zeros."""
+    name = "decode_attention_fp8"
+    n_pages = _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, tokens,
+                                   out, n_heads, n_kv_heads, head_dim, window, scale, softcap)
+    n = positions.numel() if tokens is None else tokens.numel()
+    call("fx_attention_fp8", _ptr(q), _rows(q), code(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table),
+         block_table.shape[0], block_table.shape[1], page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot), _ptr(tokens), n,
+         _ptr(out), _rows(out), n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0),
+         stream if stream is not None else stream_ptr())
+    return out
+
+
+FP8_FEW_TOKENS = 8                # entries that bring at most this many tokens are left to decode_attention_fp8
+FP8_READ_BACK_MAX = 1 << 30       # bytes of keys and values that are read back at a time
+
+
+def _stream_on(device):
+    return torch.cuda.current_stream(device) if device.type == "cuda" else None
+
+
+def _elsewhere(stream) -> bool:
+    """Whether a named stream is another than the one that scratch is taken on."""
+    return stream is not None and stream != _scoped_stream and stream != torch.cuda.current_stream().cuda_stream
+
+
+class PrefillFp8Plan:
+    """The work of :func:`prefill_attention_fp8` for a step's ``entries``, (tokens, first position) of each in the order of the
+    flattened batch: made once a step and used by every layer.  Lists that a layer's window, heads or type ask for are made and
+    uploaded by the first layer that needs them."""
+
+    def __init__(self, entries, page_size, device):
+        self.entries, self.page_size, self.device = [(int(n), int(start)) for n, start in entries], int(page_size), torch.device(device)
+        if self.page_size < 1 or any(n < 0 or start < 0 for n, start in self.entries):
+            raise KernelError(f"prefill_fp8_plan: entries {self.entries} of pages of {page_size}")
+        self.n_tokens = sum(n for n, _ in self.entries)
+        self._kept, self._streams = {}, {}
+
+    def kept(self, key, make):
+        """What ``make`` returns, made once: a tuple's numpy arrays as tensors on the device."""
+        x = self._kept.get(key)
+        if x is None:
+            x = make()
+            if isinstance(x, tuple):
+                x = tuple(upload(v, self.device) if hasattr(v, "__array__") else v for v in x)
+                self._streams[key] = [_stream_on(self.device)]
+            self._kept[key] = x
+        elif isinstance(x, tuple):
+            # used on a stream other than the one that copied it: ordered behind the copy, and not freed under its kernels
+            now, seen = _stream_on(self.device), self._streams[key]
+            if now is not None and all(now != s for s in seen):
+                now.wait_stream(seen[0])
+                for t in x:
+                    if isinstance(t, torch.Tensor) and t.numel():
+                        t.record_stream(now)
+                seen.append(now)
+        return x
+
+    def few(self):
+        """Flat indices of the tokens of entries that bring few, or None."""
+        import numpy as np
+
+        def make():
+            at, flat = [], 0
+            for n, _ in self.entries:
+                if n <= FP8_FEW_TOKENS:
+                    at += range(flat, flat + n)
+                flat += n
+            return (np.asarray(at, dtype=np.int32),)
+        t = self.kept("few", make)[0]
+        return t if t.numel() else None
+
+    def parts(self, window, row_bytes):
+        """Neighbouring entries whose visible keys and values are read back together: (first token, tokens, entries, spans, rows,
+        block table over the rows' pages, its slots), at most FP8_READ_BACK_MAX bytes each where that holds an entry at all."""
+        groups = self.kept(("groups", window, row_bytes), lambda: self._groups(window, row_bytes))
+        return [self.kept(("part", window, row_bytes, g[0][0]), lambda: self._part(window, g)) for g in groups]
+
+    def _rows_of(self, n, start, window):
+        p0 = first_key(start, window) // self.page_size * self.page_size
+        return p0, -(-(start + n - p0) // self.page_size) * self.page_size
+
+    def _groups(self, window, row_bytes):
+        groups, flat, rows, end = [], 0, 0, -1
+        for b, (n, start) in enumerate(self.entries):
+            if n > FP8_FEW_TOKENS:
+                need = self._rows_of(n, start, window)[1]
+                if end != flat or (rows + need) * row_bytes > FP8_READ_BACK_MAX:
+                    groups.append([])
+                    rows = 0
+                groups[-1].append((b, flat, n, start))
+                rows, end = rows + need, flat + n
+            flat += n
+        return groups
+
+    def _part(self, window, group):
+        import numpy as np
+
+        P, spans, row = self.page_size, [], 0
+        for b, _, n, start in group:
+            p0, rows = self._rows_of(n, start, window)
+            spans.append((b, p0, start + n, row))
+            row += rows
+        table = np.full((len(group), max(-(-s[2] // P) for s in spans)), -1, dtype=np.int32)
+        for i, (_, p0, end, r) in enumerate(spans):
+            table[i, p0 // P:-(-end // P)] = r // P + np.arange(-(-end // P) - p0 // P)
+        return (group[0][1], sum(n for _, _, n, _ in group), [(n, start) for _, _, n, start in group], np.asarray(spans, dtype=np.int32), row,
+                table, np.arange(len(group), dtype=np.int32))
+
+
+def prefill_fp8_plan(entries, page_size, device) -> PrefillFp8Plan:
+    return PrefillFp8Plan(entries, page_size, device)
+
+
+def _query_tiles(entries, rows: int):
+    import numpy as np
+
+    out, flat = [], 0
+    for b, (n, start) in enumerate(entries):
+        out += [(flat + i, min(rows, n - i), b, start + i) for i in range(0, n, rows)]
+        flat += n
+    return np.asarray(out, dtype=np.int32).reshape(-1, 4)
+
+
+def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, plan, positions, token_seq, seq_slot, out, n_heads,
+                          n_kv_heads, head_dim, window, scale, softcap=None, status=None, stream=None):
+    """Attention of a step's prompt portions over an 8-bit cache that holds their own positions already; operands as
+    :func:`decode_attention_fp8`, ``plan``: :func:`prefill_fp8_plan` of the step's entries.
+
+    The keys and values that a portion sees are read back once into pages of q's type (exact: an element has four significant bits
+    and a power of two) and the attention kernels for such pages take them from there: a tile of queries then meets operands that
+    the tensor cores take as they are, where conversion in the attention kernel would be paid again for every tile and query head.
+    Entries of up to FP8_FEW_TOKENS tokens, and shapes that no tiled kernel takes, go to :func:`decode_attention_fp8`."""
+    name = "prefill_attention_fp8"
+    _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, None, out, n_heads,
+                         n_kv_heads, head_dim, window, scale, softcap)
+    if plan.n_tokens != q.shape[0] or plan.page_size != page_size or len(plan.entries) > seq_slot.numel():
+        raise KernelError(f"{name}: a plan of {len(plan.entries)} entries, {plan.n_tokens} tokens and pages of {plan.page_size} for "
+                          f"{seq_slot.numel()} entries, {q.shape[0]} tokens and pages of {page_size}")
+    if _elsewhere(stream):               # (scratch and lists belong to the stream that the kernels run on)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream)):
+            return prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, plan, positions, token_seq, seq_slot,
+                                         out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status)
+    st = stream if stream is not None else stream_ptr()
+    cache = (k_pages, v_pages, k_exp, v_exp, block_table, page_size)
+    step = (positions, token_seq, seq_slot)
+    f32 = q.dtype == torch.float32
+    # (asked with q in the pages' place: pages that are read back have its type and lie on the allocator's grid)
+    if not (prefill_f32_ok(q, out, q, head_dim) if f32 else prefill_ok(q, out, q, head_dim)):
+        return decode_attention_fp8(q, *cache, *step, out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status,
+                                    stream=stream)
+    few = plan.few()
+    if few is not None:
+        decode_attention_fp8(q, *cache, *step, out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status, tokens=few,
+                             stream=stream)
+    for tok0, n, entries, spans, rows, table, slots in plan.parts(window, 2 * n_kv_heads * head_dim * q.element_size()):
+        k, v = torch.empty((2, rows // page_size, n_kv_heads, page_size, head_dim), dtype=q.dtype, device=q.device)
+        read_kv_fp8_spans(*cache, spans, rows, seq_slot, k, v, stream=stream)
+        _prefill_read_back(q[tok0:tok0 + n], k, v, table, page_size, plan, (tok0, window), entries, slots, out[tok0:tok0 + n], n_heads,
+                           n_kv_heads, head_dim, window, scale, softcap, status, st)
+    return out
+
+
+def _prefill_read_back(q, k, v, table, page_size, plan, key, entries, slots, out, n_heads, n_kv_heads, head_dim, window, scale, softcap,
+                       status, stream):
+    """Prompt attention of neighbouring entries over pages of q's type, by the kernel that the attention mixer takes for such pages."""
+    tail = dict(stream=stream, softcap=softcap)
+    heads = (n_heads, n_kv_heads, head_dim, window, scale)
+    if q.dtype == torch.float32:
+        tiles = None
+        if prefill_f32_tc_ok(q, out, k, page_size, head_dim):
+            items, spans, rest, n_items, rows = plan.kept(("f32", head_dim) + key, lambda: _f32_lists(entries, window, head_dim))
+            if prefill_f32_tc_fits(n_items, q.shape[0], rows, n_heads, n_kv_heads, head_dim):
+                prefill_attention_f32_tc(q, k, v, table, page_size, items, spans, rows, slots, out, *heads, status=status, **tail)
+                tiles = rest
+        if tiles is None:
+            tiles = plan.kept(("tiles", F32_PREFILL_TILE) + key, lambda: (_query_tiles(entries, F32_PREFILL_TILE),))[0]
+        if tiles.shape[0]:
+            prefill_attention_f32(q, k, v, table, page_size, tiles, slots, out, *heads, **tail)
+        return
+    capped = softcap is not None
+    if (prefill_tc_general_ok(q, q.stride(0), head_dim, k, v, page_size, out, out.stride(0), head_dim, head_dim, head_dim, scale, softcap)
+            and prefill_tc_better(entries, window, n_heads, head_dim, head_dim, capped=True) if capped
+            else prefill_tc_ok(q, out, k, page_size, head_dim, scale=scale)):
+        items, merges, parts = plan.kept(("tc", n_heads) + key, lambda: prefill_tc_plan(entries, window, n_heads))
+        part_o = part_ml = None
+        if parts:
+            part_o = torch.empty(parts, n_heads, WIDE_PREFILL_TILE, prefill_value_width(head_dim), dtype=torch.float32, device=q.device)
+            part_ml = torch.empty(parts, n_heads, WIDE_PREFILL_TILE, 2, dtype=torch.float32, device=q.device)
+        prefill_attention_tc(q, k, v, table, page_size, items, slots, out, *heads, status=status, merges=merges, part_o=part_o,
+                             part_ml=part_ml, general=capped, **tail)
+    else:
+        tiles = plan.kept(("tiles", PREFILL_TILE) + key, lambda: (_query_tiles(entries, PREFILL_TILE),))[0]
+        prefill_attention(q, k, v, table, page_size, tiles, slots, out, *heads, **tail)
+
+
+def _f32_lists(entries, window, head_dim):
+    items, spans, rows, rest = prefill_f32_tc_plan(entries, window, head_dim)
+    return items, spans, rest, len(items), rows
 
 
 def gather_rows(x, rows, out, stream=None):

@@ -207,6 +207,10 @@ class GqaAttention(Mixer):
                                              self.keep_first, self.chunk))
         return CacheSpec(paged=KvCacheSpec(s.n_kv_heads, s.head_dim, s.window, self.keep_first, self.chunk))
 
+    @property
+    def takes_fp8_cache(self):
+        return not self.general
+
     def tensor_decls(self):
         s, n = self.spec, self._names
         sizes = dict(q=self.q_size, k=self.kv_size, v=self.v_size)
@@ -306,13 +310,15 @@ class GqaAttention(Mixer):
         # stores the keys and values itself (one launch less on every layer's path); else the position part does.
         in_kernel = None
         capped = self.softcap is not None
-        if (batch.max_new == 1 and T <= ROTARY_IN_DECODE_KERNEL_MAX_TOKENS and not capped
+        if (batch.max_new == 1 and T <= ROTARY_IN_DECODE_KERNEL_MAX_TOKENS and not capped and not cache.fp8
                 and ops.decode_store_ok(qkv, cache.k, s.head_dim, cache.page_size)):
             in_kernel = self.position.in_decode_kernel(batch, s.head_dim)
         if in_kernel is None:
             self.position.rotate_and_store(qkv, batch, cache, s.n_heads, s.n_kv_heads, s.head_dim)
         attn = self.rt.empty(T, self.q_size)
-        if batch.max_new <= DECODE_ATTENTION_MAX_NEW and ops.decode_ok(qkv, s.head_dim):
+        if cache.fp8:
+            self._attend_fp8(qkv, attn, batch, cache)
+        elif batch.max_new <= DECODE_ATTENTION_MAX_NEW and ops.decode_ok(qkv, s.head_dim):
             # few query tokens: split each request's keys over many blocks
             group = s.n_heads // s.n_kv_heads
             # (capped scores: not the kernel that streams pages by TMA)
@@ -389,6 +395,21 @@ class GqaAttention(Mixer):
         # (the attention's last blocks only add up key ranges: the memory system is idle under them)
         ops.linear(attn, self.w_o, h, bias=self.b_o, accumulate=accumulate, status=batch.status, stream=batch.stream,
                    after_short_kernel=True)
+
+    def _attend_fp8(self, qkv, attn, batch, cache):
+        """Attention over pages of 8 bits, which hold the step's own positions already."""
+        s = self.spec
+        step = (batch.positions, batch.token_seq, batch.seq_slot, attn, s.n_heads, s.n_kv_heads, s.head_dim, s.window, self.scale)
+        tail = dict(softcap=self.softcap, status=batch.status, stream=batch.stream)
+        if batch.max_new <= ops.FP8_FEW_TOKENS:
+            ops.decode_attention_fp8(qkv, *cache.fp8_operands, *step, **tail)
+            return
+        key = ("attention 8-bit plan", cache.page_size)
+        plan = batch.shared.get(key)
+        if plan is None:
+            plan = batch.shared[key] = ops.prefill_fp8_plan([(len(e.tokens), e.start) for e in batch.entries], cache.page_size,
+                                                            batch.token_ids.device)
+        ops.prefill_attention_fp8(qkv, *cache.fp8_operands, plan, *step, **tail)
 
     def _forward_general(self, x, out, batch, cache, accumulate):
         """The form with normed queries, keys or values, a query temperature, a distance bias, kept first positions,

@@ -120,6 +120,9 @@ class Norm(Part):
 
 
 class Mixer(Part):
+    # True when ``forward`` also takes a cache whose keys and values are held in 8 bits (``cache.specs.in_8_bits``)
+    takes_fp8_cache = False
+
     def cache_spec(self):
         return None
 

@@ -36,6 +36,10 @@ class MixerSum(Mixer):
     def graph_safe(self):
         return all(m.graph_safe for m in self.mixers)
 
+    @property
+    def takes_fp8_cache(self):
+        return any(m.takes_fp8_cache for m in self.mixers)      # (only one keeps pages)
+
     def tensor_decls(self):
         return [d for m in self.mixers for d in m.tensor_decls()]
 

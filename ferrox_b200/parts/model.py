@@ -8,10 +8,12 @@ are wanted (reference: final norm and head crates/ferrox-models/src/decoder.rs:
 """
 from __future__ import annotations
 
+from dataclasses import replace
 from typing import List
 
 import torch
 
+from ..cache.specs import in_8_bits
 from ..kernels import ops
 from ..weights.loader import TensorDecl
 from .base import Part, Runtime, build_part
@@ -40,11 +42,20 @@ class DecoderModel(Part):
                 raise ValueError(f"cache {e.cache} is shared by layers whose cache needs differ")
             seen[e.cache] = cs
 
-    def cache_specs(self) -> list:
-        """One entry per cache index: what the layers bound to it need."""
+    def cache_specs(self, kv_cache=None) -> list:
+        """One entry per cache index: what the layers bound to it need.  ``kv_cache="fp8"``: keys and values in 8 bits; every
+        mixer that keeps pages has to take them so."""
+        if kv_cache not in (None, "fp8"):
+            raise ValueError(f"kv_cache={kv_cache!r}: None (the compute type) or 'fp8'")
         out = [None] * self.spec.n_caches
         for e in self.spec.schedule:
-            out[e.cache] = self.layers[e.layer].mixer.cache_spec()
+            mixer = self.layers[e.layer].mixer
+            cs = mixer.cache_spec()
+            if kv_cache and cs is not None and cs.paged is not None:
+                if not mixer.takes_fp8_cache:
+                    raise ValueError(f"kv_cache='fp8': layer {e.layer} has a mixer ({mixer.spec.kind}) whose pages are not held in 8 bits")
+                cs = replace(cs, paged=in_8_bits(cs.paged))
+            out[e.cache] = cs
         return out
 
     def tensor_decls(self) -> List[TensorDecl]:

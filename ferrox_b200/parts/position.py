@@ -34,6 +34,14 @@ class PositionEncoding(Part):
         return None
 
 
+def _rotate_and_store(qkv, batch, cache, n_heads, n_kv_heads, head_dim, inv_freq, rotary_dim, **rotation):
+    """The rotary kernel for the pages that the layer has: of the compute type, or of 8 bits."""
+    write, pages = (ops.rope_kv_write_fp8, cache.fp8_operands) if cache.fp8 else (
+        ops.rope_kv_write, (cache.k, cache.v, cache.block_table, cache.page_size))
+    write(qkv, batch.positions, batch.token_seq, batch.seq_slot, inv_freq, rotary_dim, *pages, n_heads, n_kv_heads, head_dim,
+          write_cache=cache.writes, status=batch.status, stream=batch.stream, **rotation)
+
+
 class RotaryEncoding(PositionEncoding):
     """Rotation of element pairs by pos * inv_freq[i]: a frequency table, a pairing rule and a rotary width.
     Subclasses set them in ``load`` (or override :meth:`frequencies`)."""
@@ -75,11 +83,8 @@ class RotaryEncoding(PositionEncoding):
     def rotate_and_store(self, qkv, batch, cache, n_heads, n_kv_heads, head_dim):
         if self.rotary_dim > head_dim:
             raise ValueError(f"rotary_dim={self.rotary_dim} exceeds head_dim={head_dim}")
-        ops.rope_kv_write(
-            qkv, batch.positions, batch.token_seq, batch.seq_slot, self.inv_freq, self.rotary_dim, cache.k, cache.v,
-            cache.block_table, cache.page_size, n_heads, n_kv_heads, head_dim, write_cache=cache.writes,
-            status=batch.status, stream=batch.stream, cos_sin=self.table(batch), pairing=self.pairing,
-        )
+        _rotate_and_store(qkv, batch, cache, n_heads, n_kv_heads, head_dim, self.inv_freq, self.rotary_dim,
+                          cos_sin=self.table(batch), pairing=self.pairing)
 
 
 class RopeNeox(RotaryEncoding):
@@ -142,11 +147,7 @@ class NoPosition(PositionEncoding):
         return (None,)
 
     def rotate_and_store(self, qkv, batch, cache, n_heads, n_kv_heads, head_dim):
-        ops.rope_kv_write(
-            qkv, batch.positions, batch.token_seq, batch.seq_slot, None, 0, cache.k, cache.v, cache.block_table,
-            cache.page_size, n_heads, n_kv_heads, head_dim, write_cache=cache.writes, status=batch.status,
-            stream=batch.stream,
-        )
+        _rotate_and_store(qkv, batch, cache, n_heads, n_kv_heads, head_dim, None, 0)
 
 
 register_part("rope_neox", RopeNeox, replace=True)

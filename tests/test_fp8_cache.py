@@ -1,0 +1,187 @@
+"""The 8-bit cache on the CPU: the form's definition, what the entry points refuse, how a prompt step is planned."""
+import math
+
+import pytest
+import torch
+
+import plain_fp8_cache as plain
+from ferrox_b200.cache.specs import CacheSpec, KvCacheSpec, PagedSpec, PagedTensorSpec, in_8_bits
+from ferrox_b200.config.registry import resolve
+from ferrox_b200.kernels import ops
+from ferrox_b200.parts.build import build_model
+from tiny_configs import TINY_A
+
+
+# ---- the definition -------------------------------------------------------------------------------------------------
+def test_the_plain_form_rounds_to_nearest_even():
+    v, e = plain.quantise(torch.tensor([[448.0, 17.0, 19.0, 18.0, 0.0, -17.0, 2.0 ** -9, 2.0 ** -10, 3 * 2.0 ** -10]]))
+    assert e.tolist() == [127]
+    assert v.tolist() == [[448.0, 16.0, 20.0, 18.0, 0.0, -16.0, 2.0 ** -9, 0.0, 2 * 2.0 ** -9]]
+
+
+@pytest.mark.parametrize("amax,e", [(448.0, 0), (448.5, 1), (449.0, 1), (224.0, -1), (3.3e38, 120), (1e-40, -119), (0.0, -119)])
+def test_the_exponent_is_the_smallest_that_fits(amax, e):
+    v, got = plain.quantise(torch.tensor([[amax, 0.0]], dtype=torch.float64))
+    assert int(got[0]) == e + 127 and float(v.abs().max()) <= 448.0
+
+
+def test_an_error_is_at_most_half_a_step():
+    x = torch.randn(50, 64, dtype=torch.float64) * torch.exp(torch.randn(50, 1, dtype=torch.float64) * 5)
+    y = plain.values(*plain.quantise(x))
+    small = torch.exp2(plain.quantise(x)[1].double() - 127)[:, None] * 2.0 ** -10      # half a step of the smallest numbers
+    assert ((x - y).abs() <= torch.maximum(x.abs() * 2.0 ** -4, small)).all()
+
+
+def test_values_are_exact_in_16_bits():
+    exps = torch.arange(8, 248)
+    x = plain.values(plain.TABLE[:127][None].expand(240, -1), exps)
+    x = x[x <= plain.MOST]
+    assert torch.equal(x.to(torch.bfloat16).double(), x)
+
+
+# ---- specs and models -----------------------------------------------------------------------------------------------
+def test_pages_in_8_bits():
+    p = in_8_bits(KvCacheSpec(3, 48, window=7))
+    assert [(t.name, t.dtype, t.page_shape(16)) for t in p.tensors] == [
+        ("k", torch.float8_e4m3fn, (3, 16, 48)), ("v", torch.float8_e4m3fn, (3, 16, 48)), ("k_exp", torch.uint8, (3, 16)),
+        ("v_exp", torch.uint8, (3, 16))] and p.window == 7
+    with pytest.raises(ValueError, match="8-bit cache"):
+        in_8_bits(PagedSpec((PagedTensorSpec("kv", (64,)),)))
+
+
+def test_a_model_gives_its_caches_in_8_bits():
+    model = build_model(resolve(TINY_A)[1])
+    assert all(isinstance(c, CacheSpec) and len(c.paged.tensors) == 4 for c in model.cache_specs("fp8"))
+    assert all(len(c.paged.tensors) == 2 for c in model.cache_specs())
+    with pytest.raises(ValueError, match="kv_cache='int4'"):
+        model.cache_specs("int4")
+
+
+def test_a_layer_that_cannot_is_refused_by_name():
+    from zanezen_configs import ZANEZEN_A
+    model = build_model(resolve(ZANEZEN_A)[1])
+    with pytest.raises(ValueError, match="not held in 8 bits"):
+        model.cache_specs("fp8")
+
+
+# ---- refusals: before anything is launched --------------------------------------------------------------------------
+def _cache(pages=3, G=2, P=16, D=32, **other):
+    c = dict(k_pages=torch.zeros(pages, G, P, D, dtype=torch.float8_e4m3fn), v_pages=torch.zeros(pages, G, P, D, dtype=torch.float8_e4m3fn),
+             k_exp=torch.zeros(pages, G, P, dtype=torch.uint8), v_exp=torch.zeros(pages, G, P, dtype=torch.uint8),
+             block_table=torch.zeros(2, 4, dtype=torch.int32), page_size=P)
+    c.update(other)
+    return c
+
+
+def _step(T=3):
+    return dict(positions=torch.arange(T, dtype=torch.int32), token_seq=torch.zeros(T, dtype=torch.int32), seq_slot=torch.zeros(1, dtype=torch.int32))
+
+
+BAD_CACHES = [
+    dict(k_pages=torch.zeros(3, 2, 16, 32)), dict(v_pages=torch.zeros(3, 2, 16, 32, dtype=torch.float8_e5m2)),
+    dict(k_exp=torch.zeros(3, 2, 16)), dict(v_exp=torch.zeros(3, 2, 15, dtype=torch.uint8)), dict(page_size=8),
+    dict(v_pages=torch.zeros(3, 2, 16, 64, dtype=torch.float8_e4m3fn)), dict(block_table=torch.zeros(2, 4, dtype=torch.int64)),
+    dict(block_table=torch.zeros(8, dtype=torch.int32)), dict(block_table=torch.zeros(4, 2, dtype=torch.int32).T),
+    dict(k_pages=torch.zeros(3, 16, 2, 32, dtype=torch.float8_e4m3fn).transpose(1, 2)), dict(block_table=torch.zeros(2, 0, dtype=torch.int32)),
+]
+BAD_STEPS = [dict(positions=torch.zeros(3, dtype=torch.int64)), dict(token_seq=torch.zeros(2, dtype=torch.int32)),
+             dict(seq_slot=torch.zeros(1, dtype=torch.int64)), dict(positions=torch.zeros(6, dtype=torch.int32)[::2])]
+
+
+def _calls(cache, step, T=3, H=4, G=2, D=32, dtype=torch.bfloat16, **over):
+    qkv, out = torch.zeros(T, (H + 2 * G) * D, dtype=dtype), torch.zeros(T, H * D, dtype=dtype)
+    rows = torch.zeros(T, G, D, dtype=dtype)
+    plan = ops.prefill_fp8_plan([(T, 0)], cache["page_size"], "cpu")
+    shape = dict(n_heads=H, n_kv_heads=G, head_dim=D)
+    attend = dict(window=None, scale=1.0)
+    return [
+        lambda **o: ops.rope_kv_write_fp8(**{**dict(qkv=qkv, inv_freq=None, rotary_dim=0), **cache, **step, **shape, **over, **o}),
+        lambda **o: ops.read_kv_fp8(**{**cache, **step, **dict(k_out=rows, v_out=rows), **over, **o}),
+        lambda **o: ops.decode_attention_fp8(**{**dict(q=qkv, out=out), **cache, **step, **shape, **attend, **over, **o}),
+        lambda **o: ops.prefill_attention_fp8(**{**dict(q=qkv, out=out, plan=plan), **cache, **step, **shape, **attend, **over, **o}),
+    ]
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("bad", range(len(BAD_CACHES)))
+def test_bad_caches(which, bad):
+    with pytest.raises(ops.KernelError):
+        _calls(_cache(**BAD_CACHES[bad]), _step())[which]()
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("bad", range(len(BAD_STEPS)))
+def test_bad_steps(which, bad):
+    with pytest.raises(ops.KernelError):
+        _calls(_cache(), {**_step(), **BAD_STEPS[bad]})[which]()
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_tensors_of_the_host(which):
+    with pytest.raises(ops.KernelError, match="an operand on cpu"):
+        _calls(_cache(), _step())[which]()
+
+
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("bad", [dict(n_heads=3), dict(n_heads=0), dict(head_dim=64), dict(n_kv_heads=4), dict(window=0), dict(window=-3),
+                                 dict(softcap=0.0), dict(softcap=-1.0), dict(scale=math.inf), dict(scale=math.nan),
+                                 dict(out=torch.zeros(3, 128)), dict(out=torch.zeros(3, 100, dtype=torch.bfloat16)),
+                                 dict(out=torch.zeros(2, 128, dtype=torch.bfloat16)), dict(q=torch.zeros(3, 96, dtype=torch.bfloat16))])
+def test_bad_attention(which, bad):
+    with pytest.raises(ops.KernelError, match="fp8"):
+        _calls(_cache(), _step())[which](**bad)
+
+
+@pytest.mark.parametrize("bad", [dict(n_heads=8), dict(head_dim=16), dict(inv_freq=torch.zeros(3), rotary_dim=32),
+                                 dict(inv_freq=torch.zeros(16, dtype=torch.float64), rotary_dim=32),
+                                 dict(inv_freq=torch.zeros(16), rotary_dim=32, cos_sin=torch.zeros(2, 16, 2))])
+def test_bad_writes(bad):
+    with pytest.raises(ops.KernelError, match="rope_kv_write_fp8"):
+        _calls(_cache(), _step())[0](**bad)
+
+
+def test_bad_reads():
+    c, slot = _cache(), torch.zeros(1, dtype=torch.int32)
+    k = torch.zeros(2, 2, 16, 32)
+    for spans, rows, a, b in [(torch.zeros(1, 4, dtype=torch.int32), 30, k, k), (torch.zeros(4, dtype=torch.int32), 32, k, k),
+                              (torch.zeros(0, 4, dtype=torch.int32), 32, k, k), (torch.zeros(1, 4, dtype=torch.int64), 32, k, k),
+                              (torch.zeros(1, 4, dtype=torch.int32), 32, k, k.bfloat16()), (torch.zeros(1, 4, dtype=torch.int32), 48, k, k)]:
+        with pytest.raises(ops.KernelError, match="read_kv_fp8"):
+            ops.read_kv_fp8_spans(**c, spans=spans, n_rows=rows, seq_slot=slot, k_out=a, v_out=b)
+
+
+def test_a_plan_of_another_step():
+    c, s = _cache(), _step()
+    for plan in (ops.prefill_fp8_plan([(2, 0)], 16, "cpu"), ops.prefill_fp8_plan([(3, 0)], 32, "cpu"), ops.prefill_fp8_plan([(2, 0), (1, 5)], 16, "cpu")):
+        with pytest.raises(ops.KernelError):
+            _calls(c, s)[3](plan=plan)
+    for entries, page in (([(-1, 0)], 16), ([(1, -1)], 16), ([(1, 0)], 0)):
+        with pytest.raises(ops.KernelError, match="prefill_fp8_plan"):
+            ops.prefill_fp8_plan(entries, page, "cpu")
+
+
+# ---- how a prompt step is planned -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("window", [None, 5, 40])
+@pytest.mark.parametrize("most", [1, 3000, 1 << 30])
+def test_parts_hold_what_the_tokens_see(window, most, monkeypatch):
+    monkeypatch.setattr(ops, "FP8_READ_BACK_MAX", most)
+    P, entries = 16, [(40, 0), (3, 100), (17, 33), (9, 0), (0, 12), (200, 7), (8, 0)]
+    plan = ops.prefill_fp8_plan(entries, P, "cpu")
+    few = plan.few().tolist()
+    seen, first = set(few), [0]
+    for n, _ in entries:
+        first.append(first[-1] + n)
+    for tok0, n, own, spans, rows, table, slots in plan.parts(window, 10):
+        assert sum(m for m, _ in own) == n and slots.tolist() == list(range(len(own))) and (len(own) == 1 or rows * 10 <= most)
+        at, row = tok0, 0
+        for (m, start), (b, p0, end, r), pages in zip(own, spans.tolist(), table.tolist()):
+            assert (m, start) == entries[b] and at == first[b] and end == start + m and r == row and p0 % P == 0
+            assert p0 <= ops.first_key(start, window) < p0 + P
+            for p in range(len(pages)):
+                inside = p0 <= p * P < end
+                assert pages[p] == (row // P + p - p0 // P if inside else -1)
+            seen |= set(range(at, at + m))
+            at += m
+            row += -(-(end - p0) // P) * P
+        assert row == rows
+    assert seen == set(range(first[-1])) and len(few) == 3 + 8
