@@ -1,0 +1,577 @@
+// Attention of few tokens a request over 8-bit cache pages (the form: fp8.cuh) on the 5th-generation tensor cores, which take
+// the pages' bytes as they are: nothing converts a cached element.
+//
+//   grid = (token, kv head x block of HB query heads, run of keys); a tile is 128 positions.
+//
+//   S^T = K Q^T     tcgen05.mma kind::f8f6f4, 128 keys x (heads x parts) x head_dim.  K as TMA lays it down ([key][128 bytes],
+//                   128-byte swizzle).  A query is e4m3 in PARTS parts: with q' = q 2^-x (its largest element between 128 and
+//                   256), part 1 is q' rounded to e4m3, part n + 1 what is left times 16 rounded again, each part a column of
+//                   its own; two parts hold a bfloat16 element exactly (4 + 4 bits), six a 32-bit one.
+//   softmax         a thread owns a key: it adds up its heads' parts in 32 bits, multiplies by the key's 2^K, caps and masks,
+//                   and makes p = 2^(s - ref) for the denominator and w = p 2^V / 2^refw for the second product.
+//   O^T += V^T W^T  tcgen05.mma, 128 elements x (heads x parts) x 128 keys.  V as TMA lays it down is its transpose with the
+//                   elements side by side (M-major A); W in three parts of e4m3 (six in 32 bits), written [key][64 bytes] with
+//                   the 64-byte swizzle (N-major B).
+//
+// Why parts: e4m3 keeps 4 bits, and products of e4m3 are added up in 32 bits (measured: beside a sum of 2^16 in the same
+// instruction a product of 2^-9 is kept, in the next one of 2^-7), so that the sum over the parts is the product of the wider
+// number.  Weights are first rounded to 16-bit floating numbers (2^-12 of the weight) for 16-bit rows; the third part ends at
+// 2^-13 of a weight and at 2^-18 of 1 where the largest weight lies between 2^5 and 2^8, six parts at 2^-24 and 2^-30.
+// What it costs is columns, of which the instruction has more than 16 heads need.
+//
+// The references ref and refw are whole powers of two, for each head, the same in all threads: ref for the sum of weights, refw
+// for the weights times 2^V (a cached value's scale belongs to its key, and with it the weight may be of any size).  They are
+// raised when a score passes ref by 6 or a weighted scale refw by 8; then O in tensor memory is multiplied by the power of two
+// between the old and the new one.  After the first tile that is rare.  One barrier a tile asks all 128 threads.
+//
+// Warp 0 asks for tiles (TMA, a ring of 3 stages; a stage of heads up to 128 elements is 32 KB, two blocks an SM), warp 1 issues
+// the products in the order S(j + 1), O(j), warps 2 - 5 are the softmax threads.  Every wait is bounded (status 3).
+//
+// Positions outside the run or without a page: their boxes are asked for behind the last page, where TMA fills in zeros without
+// reading; their weights are 0.  Bytes of pages are finite (the writer makes no other), so that 0 times them is 0.  A position
+// whose row is not finite has E = 255: its scale is NaN, and so is the result of the queries that see it.
+//
+// Runs of a token's keys leave (mean of the values, ref, sum of weights) and a second kernel adds them up in their order.
+#include "fp8.cuh"
+#include "tc_common.cuh"
+#include "api.h"
+
+namespace {
+using namespace fxtc;
+
+constexpr int TK = 128, NSOFT = 128, NTHREADS = 192, STAGES = 3, SLAB = TK * 128, P_BYTES = TK * 64;
+constexpr float NO_REF = -1e30f;                                 // no score yet
+constexpr float RAISE = 6.f, RAISE_W = 8.f, ROOM = 2.f, ROOM_W = 5.f;
+
+struct Args {
+    const void* q; long ldq;
+    const uint8_t *k_exp, *v_exp;
+    const int* block_table; int n_slots, table_width, page_size, n_pages, box;
+    const int *positions, *token_seq, *seq_slot, *tokens;
+    void* out; long ldo;
+    float *part_o, *part_ml;
+    int n_heads, n_kv_heads, head_dim, window, n_splits;
+    float q_scale, cap;                                          // cap 0: scores in powers of two; else scale / cap, and cap in powers of two
+    int* status;
+};
+
+// The keys [k_begin, k_end) of run `split`: whole tiles of the token's visible ones, as even as they go.
+__device__ __forceinline__ void run_of(int pos, int lo, int split, int n_splits, int& k_begin, int& k_end)
+{
+    const int first = lo / TK, n = pos / TK - first + 1, per = (n + n_splits - 1) / n_splits;
+    k_begin = max(lo, (first + split * per) * TK);
+    k_end = min(pos + 1, (first + min((split + 1) * per, n)) * TK);
+    if (split * per >= n || pos < 0) k_end = k_begin;
+}
+
+template <typename T, int HB, int SLABS> struct Lay {
+    static constexpr int PARTS_Q = sizeof(T) == 2 ? 2 : 6, PARTS_W = sizeof(T) == 2 ? 3 : 6;
+    static constexpr int NS = (HB * PARTS_Q + 15) / 16 * 16, NO = (HB * PARTS_W + 15) / 16 * 16;      // columns (M = 128: in steps of 16)
+    static constexpr int COLS_O = 2 * NS, COLS = COLS_O + SLABS * NO;
+    static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+    static constexpr int STAGE = 2 * SLABS * SLAB;                                                    // K slabs, V slabs
+    static constexpr int Q_OFF = STAGES * STAGE, W_OFF = Q_OFF + SLABS * NS * 128, TOTAL = W_OFF + P_BYTES + 1024;
+    static_assert(NO <= 64 && COLS <= 256, "a key's weights are a row of 64 bytes; two blocks share the SM's tensor memory");
+};
+
+__device__ __forceinline__ void mma8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// Instruction descriptor: e4m3 operands, 32-bit sums; a_mn, b_mn: the operand's M (N) extent is the contiguous one.
+__host__ __device__ constexpr uint32_t idesc8(int m, int n, int a_mn, int b_mn) {
+    return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// 64-byte swizzle: rows of 64 bytes, 8-row groups 512 bytes apart
+__device__ __forceinline__ uint64_t desc64(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(P_BYTES >> 4) << 16) | ((uint64_t)(512 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)4 << 61);
+}
+
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                   "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ float warp_max_f32(float v) {         // (numbers that are none have no say unless there is no other)
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {            // 2^x to 2 steps; 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ bool any_of_soft(bool x) {            // a barrier of the softmax threads that asks all of them
+    uint32_t r;
+    asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 1, %2, p; selp.u32 %0, 1, 0, q;}"
+                 : "=r"(r) : "r"((uint32_t)x), "n"(NSOFT) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(NSOFT) : "memory"); }
+__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(uint32_t v) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(v));
+    return r;
+}
+// A wait that does not give up when another role has (bounded all the same).
+__device__ __forceinline__ void settle(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(bar, parity); ++i) { }
+}
+// 16 (x - y), two 16-bit floating numbers, exact here
+__device__ __forceinline__ uint32_t rest_f16x2(uint32_t x, uint32_t y) {
+    uint32_t r;
+    asm("{.reg .b32 d; sub.f16x2 d, %1, %2; mul.f16x2 %0, d, %3;}" : "=r"(r) : "r"(x), "r"(y), "r"(0x4c004c00u));
+    return r;
+}
+
+template <typename T, int HB, int SLABS>
+__global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                                 const __grid_constant__ CUtensorMap map_v,
+                                                                                 const __grid_constant__ Args a)
+{
+    using L = Lay<T, HB, SLABS>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int abort_flag_s;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ __align__(8) uint64_t bars_s[2 * STAGES + 6];
+    __shared__ __align__(16) float c_s[HB];
+    __shared__ float red_s[2][4][HB];
+    volatile int* abort_flag = &abort_flag_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto full = [&](int s) { return smem_u32(&bars_s[s]); };
+    auto empty = [&](int s) { return smem_u32(&bars_s[STAGES + s]); };
+    auto s_full = [&](int b) { return smem_u32(&bars_s[2 * STAGES + b]); };
+    const uint32_t w_full = smem_u32(&bars_s[2 * STAGES + 2]), o_done = smem_u32(&bars_s[2 * STAGES + 3]), q_full = smem_u32(&bars_s[2 * STAGES + 4]),
+                   drained = smem_u32(&bars_s[2 * STAGES + 5]);
+
+    if (threadIdx.x == 0) {
+        abort_flag_s = 0;
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        mbar_init(s_full(0), 1); mbar_init(s_full(1), 1); mbar_init(w_full, 4); mbar_init(o_done, 1); mbar_init(q_full, 4); mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    fx_pdl_wait_only();
+    const int group = a.n_heads / a.n_kv_heads, blocks_g = (group + HB - 1) / HB;
+    const int kvh = blockIdx.y / blocks_g, h0 = kvh * group + blockIdx.y % blocks_g * HB, nh = min(HB, kvh * group + group - h0);
+    const int tkn = a.tokens ? a.tokens[blockIdx.x] : blockIdx.x, split = blockIdx.z, D = a.head_dim;
+    const int pos = a.positions[tkn], slot = a.seq_slot[a.token_seq[tkn]];
+    int k_begin, k_end;
+    run_of(pos, fx_first_key(pos, a.window, 0), split, a.n_splits, k_begin, k_end);
+    if (slot < 0 || slot >= a.n_slots) k_end = k_begin;
+    if (k_begin >= k_end) {                       // (the whole block) no key: zeros, or a run that the merge counts for nothing
+        for (int i = threadIdx.x; i < nh * D; i += NTHREADS) {
+            if (a.n_splits == 1) reinterpret_cast<T*>(a.out)[(long)tkn * a.ldo + (long)h0 * D + i] = from_f32<T>(0.f);
+            else if (i < nh) {
+                const long at = ((long)blockIdx.x * a.n_heads + h0 + i) * a.n_splits + split;
+                a.part_ml[2 * at] = NO_REF; a.part_ml[2 * at + 1] = 0.f;
+            }
+        }
+        return;
+    }
+    const int* table = a.block_table + (long)slot * a.table_width;
+    const int first_tile = k_begin / TK, n_tiles = (k_end - 1) / TK - first_tile + 1;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* sm = smem_raw + (base - smem_u32(smem_raw));
+
+    // Tensor memory is taken behind the wait for the kernel before and ahead of the leave for the kernel behind to be set up:
+    // neither can hold it while waiting for this one.
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&tmem_base_s)), "r"((uint32_t)L::TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    fx_pdl_trigger();
+    const uint32_t tmem = tmem_base_s;
+
+    if (warp == 0) {
+        // ---------------- producer: lane b asks for the tile's box b of a.box keys ----------------
+        const int n_boxes = TK / a.box;
+        auto page_of = [&](int j) {                                      // of this lane's box in tile j; behind the pool: zeros
+            const int key = (first_tile + j) * TK + lane * a.box;
+            if (lane >= n_boxes || j >= n_tiles || key >= k_end || key + a.box <= k_begin) return -1;
+            return fx_page_of(table, a.table_width, a.n_pages, key, a.page_size);
+        };
+        int page_next = page_of(0), asked = 0;
+        for (int j = 0; j < n_tiles; ++j, ++asked) {
+            const int s = j % STAGES, page = page_next < 0 ? a.n_pages : page_next;
+            const int off = page_next < 0 ? 0 : ((first_tile + j) * TK + lane * a.box) % a.page_size;
+            page_next = page_of(j + 1);
+            bool ok = true;
+            if (j >= STAGES) ok = mbar_wait(empty(s), (uint32_t)(j / STAGES - 1) & 1u, abort_flag);
+            if (__any_sync(0xffffffffu, !ok)) break;
+            if (lane == 0) mbar_expect_tx(full(s), (uint32_t)L::STAGE);
+            __syncwarp();
+            if (lane < n_boxes) {
+                const uint32_t dst = base + s * L::STAGE + lane * a.box * 128;
+#pragma unroll
+                for (int sl = 0; sl < SLABS; ++sl) {
+                    tma_load_4d(dst + sl * SLAB, &map_k, sl * 128, off, kvh, page, full(s));
+                    tma_load_4d(dst + (SLABS + sl) * SLAB, &map_v, sl * 128, off, kvh, page, full(s));
+                }
+            }
+            __syncwarp();
+        }
+        if (asked < n_tiles)                                             // given up: the copies under way still have to land
+            for (int j = max(0, asked - STAGES); j < asked; ++j) settle(full(j % STAGES), (uint32_t)(j / STAGES) & 1u);
+    } else if (warp == 1) {
+        // ---------------- tensor cores ----------------
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = idesc8(TK, L::NS, 0, 0), idesc_o = idesc8(128, L::NO, 1, 1);
+            const int steps = (D + 31) / 32;                             // of 32 elements
+            bool ok = mbar_wait(q_full, 0, abort_flag);
+            auto issue_s = [&](int j) {
+                const int s = j % STAGES;
+                if (!mbar_wait(full(s), (uint32_t)(j / STAGES) & 1u, abort_flag)) return false;
+                tc_fence_after();
+                const uint32_t k = base + s * L::STAGE, q = base + L::Q_OFF;
+#pragma unroll
+                for (int ks = 0; ks < 4 * SLABS; ++ks)
+                    if (ks < steps)
+                        mma8(tmem + (j & 1) * L::NS, smem_desc(k + ks / 4 * SLAB + ks % 4 * 32), smem_desc(q + ks / 4 * L::NS * 128 + ks % 4 * 32),
+                             idesc_s, ks != 0);
+                tc_commit(s_full(j & 1));
+                return true;
+            };
+            if (ok) ok = issue_s(0);
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                // (the place of S(j + 1) was read for W(j - 1), which O(j - 1) has waited for)
+                if (j + 1 < n_tiles) ok = issue_s(j + 1);
+                if (!ok || !mbar_wait(w_full, (uint32_t)j & 1u, abort_flag)) break;
+                tc_fence_after();
+                const uint32_t v = base + j % STAGES * L::STAGE + SLABS * SLAB, w = base + L::W_OFF;
+#pragma unroll
+                for (int sl = 0; sl < SLABS; ++sl)
+#pragma unroll
+                    for (int ks = 0; ks < TK / 32; ++ks)                 // 32 keys: four 8-key groups, 1024 bytes apart in V, 512 in W
+                        mma8(tmem + L::COLS_O + sl * L::NO, smem_desc_lbo_sbo(v + sl * SLAB + ks * 4096, SLAB, 1024), desc64(w + ks * 2048), idesc_o,
+                             (j | ks) != 0);
+                tc_commit(empty(j % STAGES));
+                tc_commit(o_done);
+            }
+            if (*abort_flag) { tc_commit(drained); settle(drained, 0); }  // given up: no product may outlive tensor memory
+        }
+        __syncwarp();
+    } else {
+        // ---------------- softmax: a key a thread ----------------
+        const int st = threadIdx.x - 64, sw = warp - 2, quad = warp & 3, r = quad * 32 + lane;      // (tensor memory: a warp may touch lanes 32 (warp % 4) ..)
+        // this thread's page, two tiles ahead, and its key's exponents, one tile ahead
+        auto page_at = [&](int j) {
+            const int key = (first_tile + j) * TK + r;
+            return j < n_tiles && key >= k_begin && key < k_end ? fx_page_of(table, a.table_width, a.n_pages, key, a.page_size) : -1;
+        };
+        auto exps_at = [&](int j, int page) {                            // K and V exponents, -1: the key does not count
+            if (page < 0) return -1;
+            const long at = ((long)page * a.n_kv_heads + kvh) * a.page_size + ((first_tile + j) * TK + r) % a.page_size;
+            return (int)a.k_exp[at] | (int)a.v_exp[at] << 8;
+        };
+        int page_1 = page_at(1), exps_next = exps_at(0, page_at(0));
+
+        // the queries in parts: a warp a head; rows of the columns that no head has are zeros
+        for (int i = st; i < SLABS * L::NS * 8; i += NSOFT) reinterpret_cast<uint4*>(sm + L::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
+        soft_sync();
+        for (int h = sw; h < HB; h += 4) {
+            float x[SLABS * 4];
+            const T* row = reinterpret_cast<const T*>(a.q) + (long)tkn * a.ldq + (long)(h0 + min(h, nh - 1)) * D;
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < SLABS * 4; ++i) {
+                const int e = lane + 32 * i;
+                x[i] = e < D && h < nh ? to_f32(row[e]) : 0.f;
+                most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+            }
+            most = __reduce_max_sync(0xffffffffu, most);
+            // q 2^-x in [128, 256): the exponent field of its largest element, less 7 (at least 2^-126; an element that is no
+            // finite number makes the head's factor none)
+            const int field = max((int)(most >> 23), 8);
+            const float inv = __uint_as_float((uint32_t)(min(254 - field + 7, 254)) << 23);
+            if (lane == 0) c_s[h] = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.q_scale / inv;
+#pragma unroll
+            for (int i = 0; i < SLABS * 4; ++i) {
+                const int e = lane + 32 * i;
+                if (e >= D || h >= nh || most >= 0x7f800000u) continue;
+                float v = x[i] * inv;
+#pragma unroll
+                for (int p = 0; p < L::PARTS_Q; ++p) {
+                    const uint32_t b = fx_fp8_pack2(v, 0.f);
+                    const int n = p * HB + h, c = e & 127;
+                    sm[L::Q_OFF + (e >> 7) * L::NS * 128 + n * 128 + (((c >> 4) ^ (n & 7)) << 4) + (c & 15)] = (uint8_t)b;
+                    v = (v - fx_fp8_float2(b).x) * 16.f;
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        soft_sync();
+        if (lane == 0) mbar_arrive(q_full);
+
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+        float l[HB], ref[HB], refw[HB], ratio[HB];                       // ratio = 2^(ref - refw)
+#pragma unroll
+        for (int h = 0; h < HB; ++h) { l[h] = 0.f; ref[h] = refw[h] = NO_REF; ratio[h] = 1.f; }
+        bool fine = true;
+
+        for (int j = 0; j < n_tiles; ++j) {
+            const int exps = exps_next;
+            exps_next = exps_at(j + 1, page_1);
+            page_1 = page_at(j + 2);
+            const bool live = exps >= 0;
+            const float k_scale = fx_fp8_scale(exps & 255), v_scale = live ? fx_fp8_scale(exps >> 8 & 255) : 0.f;
+            bool ok = mbar_wait(s_full(j & 1), (uint32_t)(j >> 1) & 1u, abort_flag);
+            tc_fence_after();
+            uint32_t raw[L::NS];
+#pragma unroll
+            for (int c = 0; c < L::NS; c += 16) tc_ld16(lanes + (j & 1) * L::NS + c, raw + c);
+            tc_ld_wait();
+            float s[HB], p[HB], w[HB];
+            bool raise = false;
+#pragma unroll
+            for (int h = 0; h < HB; ++h) {
+                float x = __uint_as_float(raw[(L::PARTS_Q - 1) * HB + h]);
+#pragma unroll
+                for (int n = L::PARTS_Q - 2; n >= 0; --n) x = fmaf(x, 0.0625f, __uint_as_float(raw[n * HB + h]));
+                x *= k_scale * c_s[h];
+                if (a.cap > 0.f) x = a.cap * tanhf(x);
+                s[h] = live ? x : -INFINITY;
+            }
+            auto weigh = [&]() {
+#pragma unroll
+                for (int h = 0; h < HB; ++h) {
+                    p[h] = exp2_fast(s[h] - ref[h]);
+                    w[h] = p[h] * v_scale * ratio[h];
+                }
+            };
+            weigh();
+#pragma unroll
+            for (int h = 0; h < HB; ++h) raise |= s[h] - ref[h] > RAISE || w[h] > 256.f;
+            if (any_of_soft(raise || !ok)) {
+                if (any_of_soft(!ok)) { fine = false; break; }
+                const float v_log = (float)((exps >> 8 & 255) - 127);
+#pragma unroll
+                for (int h = 0; h < HB; ++h) {
+                    const float m = warp_max_f32(s[h]), mw = warp_max_f32(s[h] + v_log);
+                    if (lane == 0) { red_s[0][sw][h] = m; red_s[1][sw][h] = mw; }
+                }
+                if (j > 0) ok = mbar_wait(o_done, (uint32_t)(j - 1) & 1u, abort_flag);      // O as it stands, and nobody adds to it
+                if (any_of_soft(!ok)) { fine = false; break; }
+                tc_fence_after();
+                float down[HB];
+#pragma unroll
+                for (int h = 0; h < HB; ++h) {
+                    const float m = fmaxf(fmaxf(red_s[0][0][h], red_s[0][1][h]), fmaxf(red_s[0][2][h], red_s[0][3][h]));
+                    const float mw = fmaxf(fmaxf(red_s[1][0][h], red_s[1][1][h]), fmaxf(red_s[1][2][h], red_s[1][3][h]));
+                    const float ref_old = ref[h], refw_old = refw[h];
+                    if (m - ref[h] > RAISE) ref[h] = ceilf(m) - ROOM;
+                    if (mw - refw[h] > RAISE_W) refw[h] = ceilf(mw) - ROOM_W;
+                    l[h] *= exp2_fast(ref_old - ref[h]);
+                    down[h] = exp2_fast(refw_old - refw[h]);
+                    ratio[h] = exp2_fast(ref[h] - refw[h]);
+                }
+                if (j > 0) {
+#pragma unroll 1
+                    for (int c = 0; c < SLABS * L::NO; c += 16) {
+                        uint32_t o[16];
+                        tc_ld16(lanes + L::COLS_O + c, o);
+                        tc_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down[i % HB]);   // (HB divides 16)
+                        tc_st16(lanes + L::COLS_O + c, o);
+                    }
+                    tc_st_wait();
+                }
+                soft_sync();                                             // red_s is read
+                weigh();
+            } else if (j > 0) {
+                // W(j - 1) has been multiplied: its place is free
+                ok = mbar_wait(o_done, (uint32_t)(j - 1) & 1u, abort_flag);
+            }
+            uint32_t word[L::NO / 4];
+#pragma unroll
+            for (int i = 0; i < L::NO / 4; ++i) word[i] = 0u;
+#pragma unroll
+            for (int h = 0; h < HB; h += 2) {
+                l[h] += p[h]; l[h + 1] += p[h + 1];
+                uint32_t part[L::PARTS_W];
+                if constexpr (sizeof(T) == 2) {
+                    uint32_t x = f16x2_of(w[h], w[h + 1]);
+#pragma unroll
+                    for (int n = 0; n < L::PARTS_W; ++n) {
+                        part[n] = pack_f16x2(x);
+                        if (n + 1 < L::PARTS_W) x = rest_f16x2(x, fx_fp8_unpack2(part[n]));
+                    }
+                } else {
+                    float x = w[h], y = w[h + 1];
+#pragma unroll
+                    for (int n = 0; n < L::PARTS_W; ++n) {
+                        part[n] = fx_fp8_pack2(x, y);
+                        const float2 f = fx_fp8_float2(part[n]);
+                        x = (x - f.x) * 16.f; y = (y - f.y) * 16.f;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < L::PARTS_W; ++n) word[(n * HB + h) / 4] |= part[n] << (n * HB + h) % 4 * 8;
+            }
+            uint8_t* row = sm + L::W_OFF + r * 64;
+#pragma unroll
+            for (int c = 0; c < L::NO / 16; ++c)
+                *reinterpret_cast<uint4*>(row + ((c ^ (r >> 1 & 3)) << 4)) = make_uint4(word[4 * c], word[4 * c + 1], word[4 * c + 2], word[4 * c + 3]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(w_full);
+            if (!ok) fine = false;                                       // (seen by all at the next barrier, or behind the loop)
+        }
+
+        // ---- the run's result: this thread has element r of every slab ----
+        bool ok = fine && mbar_wait(o_done, (uint32_t)(n_tiles - 1) & 1u, abort_flag);
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < HB; ++h) {
+            const float sum = warp_sum(l[h]);
+            if (lane == 0) red_s[0][sw][h] = sum;
+        }
+        if (!any_of_soft(!ok)) {
+#pragma unroll
+            for (int sl = 0; sl < SLABS; ++sl) {
+                uint32_t o[L::NO];
+#pragma unroll
+                for (int c = 0; c < L::NO; c += 16) tc_ld16(lanes + L::COLS_O + sl * L::NO + c, o + c);
+                tc_ld_wait();
+                const int e = sl * 128 + r;
+#pragma unroll
+                for (int h = 0; h < HB; ++h) {
+                    if (h >= nh || e >= D) continue;
+                    float x = __uint_as_float(o[(L::PARTS_W - 1) * HB + h]);
+#pragma unroll
+                    for (int n = L::PARTS_W - 2; n >= 0; --n) x = fmaf(x, 0.0625f, __uint_as_float(o[n * HB + h]));
+                    const float sum = (red_s[0][0][h] + red_s[0][1][h]) + (red_s[0][2][h] + red_s[0][3][h]);
+                    x = sum == 0.f ? 0.f : x / sum * exp2_fast(refw[h] - ref[h]);
+                    if (a.n_splits == 1) {
+                        reinterpret_cast<T*>(a.out)[(long)tkn * a.ldo + (long)(h0 + h) * D + e] = from_f32<T>(x);
+                    } else {
+                        const long at = ((long)blockIdx.x * a.n_heads + h0 + h) * a.n_splits + split;
+                        a.part_o[at * D + e] = x;
+                        if (e == 0) { a.part_ml[2 * at] = ref[h]; a.part_ml[2 * at + 1] = sum; }
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::TMEM));
+    if (threadIdx.x == 0 && abort_flag_s && a.status) atomicExch(a.status, STATUS_TC_TIMEOUT);
+}
+
+// The runs of a (token, head): sum_s l_s 2^(m_s - m) mean_s / sum_s l_s 2^(m_s - m), in the order of the runs.
+constexpr int MERGE_THREADS = 128, MAX_RUNS = 128;
+
+template <typename T> __global__ void __launch_bounds__(MERGE_THREADS) decode_fp8_merge_kernel(const __grid_constant__ Args a)
+{
+    __shared__ float w_s[MAX_RUNS], top_s[MERGE_THREADS / 32];
+    fx_pdl_wait();
+    const int n = a.n_splits, D = a.head_dim, h = blockIdx.y, lane = threadIdx.x & 31;
+    const int tkn = a.tokens ? a.tokens[blockIdx.x] : blockIdx.x;
+    const long at = ((long)blockIdx.x * a.n_heads + h) * n;
+    const bool mine = (int)threadIdx.x < n;
+    const float m = mine ? a.part_ml[2 * (at + threadIdx.x)] : NO_REF, l = mine ? a.part_ml[2 * (at + threadIdx.x) + 1] : 0.f;
+    const float top = warp_max(m);
+    if (lane == 0) top_s[threadIdx.x >> 5] = top;
+    __syncthreads();
+    float ref = top_s[0];
+    for (int i = 1; i < MERGE_THREADS / 32; ++i) ref = fmaxf(ref, top_s[i]);
+    if (mine) w_s[threadIdx.x] = l == 0.f ? 0.f : l * exp2f(m - ref);
+    __syncthreads();
+    float sum = 0.f;
+    for (int i = 0; i < n; ++i) sum += w_s[i];
+    for (int e = threadIdx.x; e < D; e += MERGE_THREADS) {
+        float acc = 0.f;
+        for (int i0 = 0; i0 < n; i0 += 8) {
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = i0 + i < n && w_s[i0 + i] != 0.f ? a.part_o[(at + i0 + i) * D + e] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (i0 + i < n) acc = fmaf(w_s[i0 + i], o[i], acc);
+        }
+        reinterpret_cast<T*>(a.out)[(long)tkn * a.ldo + (long)h * D + e] = from_f32<T>(sum == 0.f ? 0.f : acc / sum);
+    }
+}
+
+template <typename T, int HB, int SLABS> int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, dim3 grid, cudaStream_t s)
+{
+    auto kern = decode_fp8_kernel<T, HB, SLABS>;
+    // of the current device: asked for each time
+    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<T, HB, SLABS>::TOTAL)) return (int)e;
+    fx_launch_pdl(kern, grid, NTHREADS, Lay<T, HB, SLABS>::TOTAL, s, mk, mv, a);
+    return fx_launch_status();
+}
+
+bool encode(CUtensorMap* map, const void* ptr, const Args& a)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t D = a.head_dim, P = a.page_size, G = a.n_kv_heads;
+    const cuuint64_t dims[4] = {D, P, G, (cuuint64_t)a.n_pages}, strides[3] = {D, P * D, G * P * D};
+    const cuuint32_t box[4] = {128, (cuuint32_t)a.box, 1, 1}, ones[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T> int run(const CUtensorMap& mk, const CUtensorMap& mv, Args& a, int n_tokens, cudaStream_t s)
+{
+    // heads a block takes: as few columns as the group needs, 16 at most (32 bits: 8, whose parts are 48 columns)
+    const int group = a.n_heads / a.n_kv_heads, hb = group <= 4 ? 4 : group <= 8 || sizeof(T) == 4 ? 8 : 16;
+    const dim3 grid(n_tokens, a.n_kv_heads * ((group + hb - 1) / hb), a.n_splits);
+    if (grid.y > 65535u) return FX_ERR_SIZE;
+    int rc;
+    if constexpr (sizeof(T) == 2) {
+        if (hb == 16) rc = a.head_dim <= 128 ? launch<T, 16, 1>(mk, mv, a, grid, s) : launch<T, 16, 2>(mk, mv, a, grid, s);
+    }
+    if (hb == 8) rc = a.head_dim <= 128 ? launch<T, 8, 1>(mk, mv, a, grid, s) : launch<T, 8, 2>(mk, mv, a, grid, s);
+    if (hb == 4) rc = a.head_dim <= 128 ? launch<T, 4, 1>(mk, mv, a, grid, s) : launch<T, 4, 2>(mk, mv, a, grid, s);
+    if (rc || a.n_splits == 1) return rc;
+    fx_launch_pdl(decode_fp8_merge_kernel<T>, dim3(n_tokens, a.n_heads), MERGE_THREADS, 0, s, a);
+    return fx_launch_status();
+}
+
+}  // namespace
+
+extern "C" int fx_decode_attention_fp8(const void* q, long ldq, int dtype, const void* k_pages, const void* v_pages, const void* k_exp,
+                                       const void* v_exp, const int* block_table, int n_slots, int table_width, int page_size, int n_pages,
+                                       const int* positions, const int* token_seq, const int* seq_slot, const int* tokens, int n_tokens,
+                                       void* out, long ldo, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap,
+                                       int n_splits, float* part_o, float* part_ml, int* status, void* stream)
+{
+    if (n_tokens <= 0) return FX_OK;
+    if (head_dim <= 0 || head_dim > 256 || head_dim % 16 || page_size <= 0 || page_size % 16 || n_pages <= 0 || n_slots <= 0 || table_width <= 0 ||
+        n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads > 65535 || window < 0 || softcap < 0.f || n_splits < 1 ||
+        n_splits > MAX_RUNS || (n_splits > 1 && (!part_o || !part_ml))) return FX_ERR_SIZE;
+    if ((uintptr_t)k_pages % 16 || (uintptr_t)v_pages % 16) return FX_ERR_ALIGN;
+    int box = TK;                                                        // keys a TMA box: the largest that stays in a page
+    while (page_size % box) box /= 2;
+    constexpr float LOG2E = 1.4426950408889634f;
+    Args a = {q, ldq, (const uint8_t*)k_exp, (const uint8_t*)v_exp, block_table, n_slots, table_width, page_size, n_pages, box, positions, token_seq,
+              seq_slot, tokens, out, ldo, part_o, part_ml, n_heads, n_kv_heads, head_dim, window, n_splits,
+              softcap > 0.f ? scale / softcap : scale * LOG2E, softcap * LOG2E, status};
+    CUtensorMap mk, mv;
+    if (!encode(&mk, k_pages, a) || !encode(&mv, v_pages, a)) return FX_ERR_SIZE;
+    if (dtype == FX_F32) return run<float>(mk, mv, a, n_tokens, (cudaStream_t)stream);
+    if (dtype == FX_BF16) return run<bf16>(mk, mv, a, n_tokens, (cudaStream_t)stream);
+    return FX_ERR_DTYPE;
+}

@@ -125,6 +125,8 @@ _SIGNATURES = {
                             _I, _P, _P, _I, _I, _I, _P, _F, _P, _P],
     "fx_rope_kv_write_fp8": [_P, _I, _L, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "fx_read_kv_fp8": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _P],
+    "fx_decode_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F,
+                                _I, _P, _P, _P, _P],
     "fx_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F, _P],
     "fx_argmax": [_P, _L, _I, _I, _P, _P],
     "fx_repetition_penalty": [_P, _L, _I, _I, _P, _P, _P, _P],
@@ -2115,6 +2117,33 @@ def _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, p
     return n_pages
 
 
+def decode_fp8_ok(k_pages, v_pages, head_dim: int, page_size: int) -> bool:
+    """Whether the tensor-core kernel takes these pages (head sizes and pages in steps of 16); others go to a warp a (token, head)."""
+    return head_dim % 16 == 0 and page_size % 16 == 0 and k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0
+
+
+FP8_TILE = 128                    # positions a tile of the decode kernel holds
+FP8_MAX_RUNS = 64
+# In the time a tile takes a block: what a run costs beside its tiles, and the second kernel that adds the runs up.
+FP8_RUN_OVERHEAD, FP8_MERGE_COST = 3.0, 2.0
+
+
+@functools.lru_cache(maxsize=4096)
+def decode_fp8_runs(n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, f32: bool, reach: int) -> int:
+    """Into how many runs :func:`decode_attention_fp8` cuts a token's keys: those whose rounds of blocks (two an SM, one for heads of
+    more than 128 elements) come to the least.  A function of the step's size and of ``reach``, the most positions a token may see, and
+    not of the lengths, so that a captured step keeps its grid."""
+    group = n_heads // n_kv_heads
+    per = 4 if group <= 4 else 8 if group <= 8 or f32 else 16
+    blocks, slots, tiles = max(1, n_tokens * n_kv_heads * -(-group // per)), sm_count() * (2 if head_dim <= 128 else 1), -(-reach // FP8_TILE)
+    best, best_cost = 1, None
+    for n in range(1, min(FP8_MAX_RUNS, tiles) + 1):
+        cost = -(-blocks * n // slots) * (-(-tiles // n) + FP8_RUN_OVERHEAD) + (FP8_MERGE_COST if n > 1 else 0)
+        if best_cost is None or cost < best_cost:
+            best, best_cost = n, cost
+    return best
+
+
 def decode_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, out, n_heads,
                          n_kv_heads, head_dim, window, scale, softcap=None, status=None, tokens=None, stream=None):
     """Attention of few tokens a request over an 8-bit cache (:func:`rope_kv_write_fp8`): ``q`` rows that start with the query heads,
@@ -2125,10 +2154,30 @@ def decode_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_si
     n_pages = _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, tokens,
                                    out, n_heads, n_kv_heads, head_dim, window, scale, softcap)
     n = positions.numel() if tokens is None else tokens.numel()
-    call("fx_attention_fp8", _ptr(q), _rows(q), code(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table),
-         block_table.shape[0], block_table.shape[1], page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot), _ptr(tokens), n,
-         _ptr(out), _rows(out), n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0),
-         stream if stream is not None else stream_ptr())
+    operands = (_ptr(q), _rows(q), code(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table),
+                block_table.shape[0], block_table.shape[1], page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot),
+                _ptr(tokens), n, _ptr(out), _rows(out), n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0))
+    st = stream if stream is not None else stream_ptr()
+    if not decode_fp8_ok(k_pages, v_pages, head_dim, page_size):
+        call("fx_attention_fp8", *operands, st)
+        return out
+    reach = block_table.shape[1] * page_size
+    if window is not None:
+        reach = min(reach, (window + FP8_TILE - 2) // FP8_TILE * FP8_TILE + FP8_TILE)      # (the tiles that it straddles)
+    runs = decode_fp8_runs(n, n_heads, n_kv_heads, head_dim, q.dtype == torch.float32, reach)
+    if runs == 1:
+        call("fx_decode_attention_fp8", *operands, 1, None, None, _ptr(status), st)
+        return out
+    global _launches
+    _launches += 1
+    size = n * n_heads * runs * (head_dim + 2)
+    if _elsewhere(stream):                     # (scratch belongs to the stream that the kernels run on)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream)):
+            work = torch.empty(size, dtype=torch.float32, device=q.device)
+    else:
+        work = torch.empty(size, dtype=torch.float32, device=q.device)
+    base = work.data_ptr()
+    call("fx_decode_attention_fp8", *operands, runs, base, base + 4 * n * n_heads * runs * head_dim, _ptr(status), st)
     return out
 
 
