@@ -39,7 +39,7 @@
 namespace {
 using namespace fxtc;
 
-constexpr int TK = 128, NSOFT = 128, NTHREADS = 192, STAGES = 3, SLAB = TK * 128, P_BYTES = TK * 64;
+constexpr int TK = 128, NSOFT = 128, NTHREADS = 64 + 2 * NSOFT, STAGES = 3, S_PLACES = 3, SLAB = TK * 128, P_BYTES = TK * 64;
 constexpr float NO_REF = -1e30f;                                 // no score yet
 constexpr float RAISE = 6.f, RAISE_W = 8.f, ROOM = 2.f, ROOM_W = 5.f;
 
@@ -67,11 +67,11 @@ __device__ __forceinline__ void run_of(int pos, int lo, int split, int n_splits,
 template <typename T, int HB, int SLABS> struct Lay {
     static constexpr int PARTS_Q = sizeof(T) == 2 ? 2 : 6, PARTS_W = sizeof(T) == 2 ? 3 : 6;
     static constexpr int NS = (HB * PARTS_Q + 15) / 16 * 16, NO = (HB * PARTS_W + 15) / 16 * 16;      // columns (M = 128: in steps of 16)
-    static constexpr int COLS_O = 2 * NS, COLS = COLS_O + SLABS * NO;
-    static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+    static constexpr int COLS_O = S_PLACES * NS, COLS = COLS_O + 2 * SLABS * NO;                      // (O of either group)
+    static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int STAGE = 2 * SLABS * SLAB;                                                    // K slabs, V slabs
     static constexpr int Q_OFF = STAGES * STAGE, W_OFF = Q_OFF + SLABS * NS * 128, TOTAL = W_OFF + P_BYTES + 1024;
-    static_assert(NO <= 64 && COLS <= 256, "a key's weights are a row of 64 bytes; two blocks share the SM's tensor memory");
+    static_assert(NO <= 64 && COLS <= (SLABS == 1 ? 256 : 512), "a key's weights are a row of 64 bytes; two blocks share the SM's tensor memory");
 };
 
 __device__ __forceinline__ void mma8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -110,13 +110,24 @@ __device__ __forceinline__ float exp2_fast(float x) {            // 2^x to 2 ste
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ bool any_of_soft(bool x) {            // a barrier of the softmax threads that asks all of them
+// Barriers of a group's 128 threads: one that asks all of them, a plain one, and one that only the group's first warp waits at.
+__device__ __forceinline__ bool any_of_group(int g, bool x) {
     uint32_t r;
-    asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 1, %2, p; selp.u32 %0, 1, 0, q;}"
-                 : "=r"(r) : "r"((uint32_t)x), "n"(NSOFT) : "memory");
+    asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, %2, %3, p; selp.u32 %0, 1, 0, q;}"
+                 : "=r"(r) : "r"((uint32_t)x), "r"(1 + g), "n"(NSOFT) : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(NSOFT) : "memory"); }
+__device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(NSOFT) : "memory"); }
+__device__ __forceinline__ void group_written(int g, bool waits) {
+    if (waits) asm volatile("bar.sync %0, %1;" ::"r"(3 + g), "n"(NSOFT) : "memory");
+    else asm volatile("bar.arrive %0, %1;" ::"r"(3 + g), "n"(NSOFT) : "memory");
+}
+__device__ __forceinline__ bool any_of_soft(bool x) {            // of both groups
+    uint32_t r;
+    asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 5, %2, p; selp.u32 %0, 1, 0, q;}"
+                 : "=r"(r) : "r"((uint32_t)x), "n"(2 * NSOFT) : "memory");
+    return r != 0;
+}
 __device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -147,21 +158,28 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag_s;
     __shared__ uint32_t tmem_base_s;
-    __shared__ __align__(8) uint64_t bars_s[2 * STAGES + 6];
-    __shared__ __align__(16) float c_s[HB];
-    __shared__ float red_s[2][4][HB];
+    __shared__ __align__(8) uint64_t bars_s[2 * STAGES + 2 * S_PLACES + 6];
+    __shared__ __align__(16) float c_s[HB];                              // what a head's raw score is multiplied with
+    // of a group: references of its heads, 2^(ref - refw); while they are raised: maxima of its warps, what sums and O shrink by
+    __shared__ __align__(16) float ref_s[2][HB], refw_s[2][HB], ratio_s[2][HB], shrink_s[2][HB], shrink_o_s[2][16], most_s[2][2][4][HB];
+    __shared__ float sum_s[2][4][HB];
     volatile int* abort_flag = &abort_flag_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto full = [&](int s) { return smem_u32(&bars_s[s]); };
     auto empty = [&](int s) { return smem_u32(&bars_s[STAGES + s]); };
     auto s_full = [&](int b) { return smem_u32(&bars_s[2 * STAGES + b]); };
-    const uint32_t w_full = smem_u32(&bars_s[2 * STAGES + 2]), o_done = smem_u32(&bars_s[2 * STAGES + 3]), q_full = smem_u32(&bars_s[2 * STAGES + 4]),
-                   drained = smem_u32(&bars_s[2 * STAGES + 5]);
+    auto s_empty = [&](int b) { return smem_u32(&bars_s[2 * STAGES + S_PLACES + b]); };
+    const uint32_t q_full = smem_u32(&bars_s[2 * STAGES + 2 * S_PLACES]);
+    auto o_done = [&](int j) { return q_full + 8 + 8u * (j & 1); };      // of the group that tile j belongs to, phase j / 2
+    auto drained = [&](int i) { return q_full + 24 + 8u * i; };
 
     if (threadIdx.x == 0) {
         abort_flag_s = 0;
         for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        mbar_init(s_full(0), 1); mbar_init(s_full(1), 1); mbar_init(w_full, 4); mbar_init(o_done, 1); mbar_init(q_full, 4); mbar_init(drained, 1);
+        for (int b = 0; b < S_PLACES; ++b) { mbar_init(s_full(b), 1); mbar_init(s_empty(b), 4); }
+        mbar_init(q_full, 8);
+        for (int i = 0; i < 2; ++i) mbar_init(o_done(i), 1);
+        for (int i = 0; i < 3; ++i) mbar_init(drained(i), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -232,62 +250,67 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
         if (asked < n_tiles)                                             // given up: the copies under way still have to land
             for (int j = max(0, asked - STAGES); j < asked; ++j) settle(full(j % STAGES), (uint32_t)(j / STAGES) & 1u);
     } else if (warp == 1) {
-        // ---------------- tensor cores ----------------
+        // ---------------- scores: S(j) as soon as its keys and a place for it are there ----------------
         if (lane == 0) {
-            constexpr uint32_t idesc_s = idesc8(TK, L::NS, 0, 0), idesc_o = idesc8(128, L::NO, 1, 1);
+            constexpr uint32_t idesc_s = idesc8(TK, L::NS, 0, 0);
             const int steps = (D + 31) / 32;                             // of 32 elements
             bool ok = mbar_wait(q_full, 0, abort_flag);
-            auto issue_s = [&](int j) {
-                const int s = j % STAGES;
-                if (!mbar_wait(full(s), (uint32_t)(j / STAGES) & 1u, abort_flag)) return false;
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                const int s = j % STAGES, b = j % S_PLACES;
+                ok = mbar_wait(full(s), (uint32_t)(j / STAGES) & 1u, abort_flag);
+                if (ok && j >= S_PLACES) ok = mbar_wait(s_empty(b), (uint32_t)(j / S_PLACES - 1) & 1u, abort_flag);
+                if (!ok) break;
                 tc_fence_after();
                 const uint32_t k = base + s * L::STAGE, q = base + L::Q_OFF;
 #pragma unroll
                 for (int ks = 0; ks < 4 * SLABS; ++ks)
                     if (ks < steps)
-                        mma8(tmem + (j & 1) * L::NS, smem_desc(k + ks / 4 * SLAB + ks % 4 * 32), smem_desc(q + ks / 4 * L::NS * 128 + ks % 4 * 32),
+                        mma8(tmem + b * L::NS, smem_desc(k + ks / 4 * SLAB + ks % 4 * 32), smem_desc(q + ks / 4 * L::NS * 128 + ks % 4 * 32),
                              idesc_s, ks != 0);
-                tc_commit(s_full(j & 1));
-                return true;
-            };
-            if (ok) ok = issue_s(0);
-            for (int j = 0; j < n_tiles && ok; ++j) {
-                // (the place of S(j + 1) was read for W(j - 1), which O(j - 1) has waited for)
-                if (j + 1 < n_tiles) ok = issue_s(j + 1);
-                if (!ok || !mbar_wait(w_full, (uint32_t)j & 1u, abort_flag)) break;
-                tc_fence_after();
-                const uint32_t v = base + j % STAGES * L::STAGE + SLABS * SLAB, w = base + L::W_OFF;
-#pragma unroll
-                for (int sl = 0; sl < SLABS; ++sl)
-#pragma unroll
-                    for (int ks = 0; ks < TK / 32; ++ks)                 // 32 keys: four 8-key groups, 1024 bytes apart in V, 512 in W
-                        mma8(tmem + L::COLS_O + sl * L::NO, smem_desc_lbo_sbo(v + sl * SLAB + ks * 4096, SLAB, 1024), desc64(w + ks * 2048), idesc_o,
-                             (j | ks) != 0);
-                tc_commit(empty(j % STAGES));
-                tc_commit(o_done);
+                tc_commit(s_full(b));
             }
-            if (*abort_flag) { tc_commit(drained); settle(drained, 0); }  // given up: no product may outlive tensor memory
+            if (*abort_flag) { tc_commit(drained(2)); settle(drained(2), 0); }   // given up: no product may outlive tensor memory
         }
         __syncwarp();
     } else {
-        // ---------------- softmax: a key a thread ----------------
-        const int st = threadIdx.x - 64, sw = warp - 2, quad = warp & 3, r = quad * 32 + lane;      // (tensor memory: a warp may touch lanes 32 (warp % 4) ..)
-        // this thread's page, two tiles ahead, and its key's exponents, one tile ahead
-        auto page_at = [&](int j) {
-            const int key = (first_tile + j) * TK + r;
-            return j < n_tiles && key >= k_begin && key < k_end ? fx_page_of(table, a.table_width, a.n_pages, key, a.page_size) : -1;
+        // ---------------- softmax: a key a thread; group g takes the tiles g, g + 2, ... ----------------
+        const int g = (warp - 2) >> 2, sw = (warp - 2) & 3, st = threadIdx.x - 64;
+        const int quad = warp & 3, r = quad * 32 + lane;                 // (tensor memory: a warp may touch lanes 32 (warp % 4) ..)
+        // Where this thread's keys lie: entry `at` of the table and position `off` of a page, moved on by two tiles at a time.
+        // A key's page is looked up two of the group's tiles ahead, its exponents one ahead (-1: the key does not count).
+        const int hop = 2 * TK / a.page_size, hop_off = 2 * TK % a.page_size;
+        int key_p = (first_tile + g) * TK + r, at_p = key_p / a.page_size, off_p = key_p - at_p * a.page_size;
+        int off_e = off_p;
+        auto next_page = [&]() {
+            int page = -1;
+            if (key_p >= k_begin && key_p < k_end && at_p < a.table_width) {
+                page = table[at_p];
+                if (page >= a.n_pages) page = -1;
+            }
+            key_p += 2 * TK; at_p += hop; off_p += hop_off;
+            if (off_p >= a.page_size) { off_p -= a.page_size; ++at_p; }
+            return page;
         };
-        auto exps_at = [&](int j, int page) {                            // K and V exponents, -1: the key does not count
-            if (page < 0) return -1;
-            const long at = ((long)page * a.n_kv_heads + kvh) * a.page_size + ((first_tile + j) * TK + r) % a.page_size;
-            return (int)a.k_exp[at] | (int)a.v_exp[at] << 8;
+        auto next_exps = [&](int page) {
+            int e = -1;
+            if (page >= 0) {
+                const long at = ((long)page * a.n_kv_heads + kvh) * a.page_size + off_e;
+                e = (int)a.k_exp[at] | (int)a.v_exp[at] << 8;
+            }
+            off_e += hop_off;
+            if (off_e >= a.page_size) off_e -= a.page_size;
+            return e;
         };
-        int page_1 = page_at(1), exps_next = exps_at(0, page_at(0));
+        int page_next = next_page();
+        int exps_next = next_exps(page_next);
+        page_next = next_page();
 
         // the queries in parts: a warp a head; rows of the columns that no head has are zeros
-        for (int i = st; i < SLABS * L::NS * 8; i += NSOFT) reinterpret_cast<uint4*>(sm + L::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
-        soft_sync();
-        for (int h = sw; h < HB; h += 4) {
+        for (int i = st; i < SLABS * L::NS * 8; i += 2 * NSOFT) reinterpret_cast<uint4*>(sm + L::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
+        if (st < 2 * HB) { (&ref_s[0][0])[st] = NO_REF; (&refw_s[0][0])[st] = NO_REF; (&ratio_s[0][0])[st] = 1.f; }
+        any_of_soft(false);
+        if (warp - 2 < HB) {
+            const int h = warp - 2;
             float x[SLABS * 4];
             const T* row = reinterpret_cast<const T*>(a.q) + (long)tkn * a.ldq + (long)(h0 + min(h, nh - 1)) * D;
             uint32_t most = 0;
@@ -298,10 +321,10 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
                 most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
             }
             most = __reduce_max_sync(0xffffffffu, most);
-            // q 2^-x in [128, 256): the exponent field of its largest element, less 7 (at least 2^-126; an element that is no
+            // q 2^-x in [128, 256): the exponent field of its largest element, less 7 (at least 2^-119; an element that is no
             // finite number makes the head's factor none)
             const int field = max((int)(most >> 23), 8);
-            const float inv = __uint_as_float((uint32_t)(min(254 - field + 7, 254)) << 23);
+            const float inv = __uint_as_float((uint32_t)(254 - field + 7) << 23);
             if (lane == 0) c_s[h] = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.q_scale / inv;
 #pragma unroll
             for (int i = 0; i < SLABS * 4; ++i) {
@@ -318,114 +341,125 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        soft_sync();
+        any_of_soft(false);
         if (lane == 0) mbar_arrive(q_full);
 
-        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-        float l[HB], ref[HB], refw[HB], ratio[HB];                       // ratio = 2^(ref - refw)
+        constexpr uint32_t idesc_o = idesc8(128, L::NO, 1, 1);
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), col_o = L::COLS_O + g * SLABS * L::NO;
+        float l[HB];
 #pragma unroll
-        for (int h = 0; h < HB; ++h) { l[h] = 0.f; ref[h] = refw[h] = NO_REF; ratio[h] = 1.f; }
+        for (int h = 0; h < HB; ++h) l[h] = 0.f;
         bool fine = true;
 
-        for (int j = 0; j < n_tiles; ++j) {
-            const int exps = exps_next;
-            exps_next = exps_at(j + 1, page_1);
-            page_1 = page_at(j + 2);
+        for (int j = g; j < n_tiles; j += 2) {
+            const int exps = exps_next, b = j % S_PLACES;
+            exps_next = next_exps(page_next);
+            page_next = next_page();
             const bool live = exps >= 0;
             const float k_scale = fx_fp8_scale(exps & 255), v_scale = live ? fx_fp8_scale(exps >> 8 & 255) : 0.f;
-            bool ok = mbar_wait(s_full(j & 1), (uint32_t)(j >> 1) & 1u, abort_flag);
+            bool ok = mbar_wait(s_full(b), (uint32_t)(j / S_PLACES) & 1u, abort_flag);
             tc_fence_after();
-            uint32_t raw[L::NS];
-#pragma unroll
-            for (int c = 0; c < L::NS; c += 16) tc_ld16(lanes + (j & 1) * L::NS + c, raw + c);
-            tc_ld_wait();
             float s[HB], p[HB], w[HB];
-            bool raise = false;
+            {
+                uint32_t raw[L::NS];
 #pragma unroll
-            for (int h = 0; h < HB; ++h) {
-                float x = __uint_as_float(raw[(L::PARTS_Q - 1) * HB + h]);
+                for (int c = 0; c < L::NS; c += 16) tc_ld16(lanes + b * L::NS + c, raw + c);
+                tc_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_empty(b));
 #pragma unroll
-                for (int n = L::PARTS_Q - 2; n >= 0; --n) x = fmaf(x, 0.0625f, __uint_as_float(raw[n * HB + h]));
-                x *= k_scale * c_s[h];
-                if (a.cap > 0.f) x = a.cap * tanhf(x);
-                s[h] = live ? x : -INFINITY;
+                for (int h = 0; h < HB; ++h) {
+                    float x = __uint_as_float(raw[(L::PARTS_Q - 1) * HB + h]);
+#pragma unroll
+                    for (int n = L::PARTS_Q - 2; n >= 0; --n) x = fmaf(x, 0.0625f, __uint_as_float(raw[n * HB + h]));
+                    s[h] = x * (k_scale * c_s[h]);
+                }
             }
+            if (a.cap > 0.f) {
+#pragma unroll
+                for (int h = 0; h < HB; ++h) s[h] = a.cap * tanhf(s[h]);
+            }
+            if (!__all_sync(0xffffffffu, live)) {
+#pragma unroll
+                for (int h = 0; h < HB; ++h) s[h] = live ? s[h] : -INFINITY;
+            }
+            float over = -INFINITY, over_w = 0.f;                        // how far a score passes its reference; the largest weight
             auto weigh = [&]() {
 #pragma unroll
                 for (int h = 0; h < HB; ++h) {
-                    p[h] = exp2_fast(s[h] - ref[h]);
-                    w[h] = p[h] * v_scale * ratio[h];
+                    const float x = s[h] - ref_s[g][h];
+                    p[h] = exp2_fast(x);
+                    w[h] = p[h] * v_scale * ratio_s[g][h];
+                    over = fmaxf(over, x);
+                    over_w = fmaxf(over_w, w[h]);
                 }
             };
             weigh();
-#pragma unroll
-            for (int h = 0; h < HB; ++h) raise |= s[h] - ref[h] > RAISE || w[h] > 256.f;
-            if (any_of_soft(raise || !ok)) {
-                if (any_of_soft(!ok)) { fine = false; break; }
+            if (any_of_group(g, over > RAISE || over_w > 256.f || !ok)) {
+                if (any_of_group(g, !ok)) { fine = false; break; }
                 const float v_log = (float)((exps >> 8 & 255) - 127);
 #pragma unroll
                 for (int h = 0; h < HB; ++h) {
                     const float m = warp_max_f32(s[h]), mw = warp_max_f32(s[h] + v_log);
-                    if (lane == 0) { red_s[0][sw][h] = m; red_s[1][sw][h] = mw; }
+                    if (lane == 0) { most_s[g][0][sw][h] = m; most_s[g][1][sw][h] = mw; }
                 }
-                if (j > 0) ok = mbar_wait(o_done, (uint32_t)(j - 1) & 1u, abort_flag);      // O as it stands, and nobody adds to it
-                if (any_of_soft(!ok)) { fine = false; break; }
+                if (j > 0) ok = mbar_wait(o_done(j - 1), (uint32_t)((j - 1) >> 1) & 1u, abort_flag);      // the group's O as it stands, and nobody adds to it
+                if (any_of_group(g, !ok)) { fine = false; break; }
                 tc_fence_after();
-                float down[HB];
-#pragma unroll
-                for (int h = 0; h < HB; ++h) {
-                    const float m = fmaxf(fmaxf(red_s[0][0][h], red_s[0][1][h]), fmaxf(red_s[0][2][h], red_s[0][3][h]));
-                    const float mw = fmaxf(fmaxf(red_s[1][0][h], red_s[1][1][h]), fmaxf(red_s[1][2][h], red_s[1][3][h]));
-                    const float ref_old = ref[h], refw_old = refw[h];
-                    if (m - ref[h] > RAISE) ref[h] = ceilf(m) - ROOM;
-                    if (mw - refw[h] > RAISE_W) refw[h] = ceilf(mw) - ROOM_W;
-                    l[h] *= exp2_fast(ref_old - ref[h]);
-                    down[h] = exp2_fast(refw_old - refw[h]);
-                    ratio[h] = exp2_fast(ref[h] - refw[h]);
+                if ((st & 127) < HB) {
+                    const int h = st & 127;
+                    const float m = fmaxf(fmaxf(most_s[g][0][0][h], most_s[g][0][1][h]), fmaxf(most_s[g][0][2][h], most_s[g][0][3][h]));
+                    const float mw = fmaxf(fmaxf(most_s[g][1][0][h], most_s[g][1][1][h]), fmaxf(most_s[g][1][2][h], most_s[g][1][3][h]));
+                    const float ref = ref_s[g][h], refw = refw_s[g][h];
+                    const float now = m - ref > RAISE ? ceilf(m) - ROOM : ref, now_w = mw - refw > RAISE_W ? ceilf(mw) - ROOM_W : refw;
+                    shrink_s[g][h] = exp2_fast(ref - now);
+                    for (int i = h; i < 16; i += HB) shrink_o_s[g][i] = exp2_fast(refw - now_w);      // (columns repeat their heads)
+                    ratio_s[g][h] = exp2_fast(now - now_w);
+                    ref_s[g][h] = now; refw_s[g][h] = now_w;
                 }
-                if (j > 0) {
+                group_sync(g);
+#pragma unroll
+                for (int h = 0; h < HB; ++h) l[h] *= shrink_s[g][h];
+                if (j > 1) {
 #pragma unroll 1
                     for (int c = 0; c < SLABS * L::NO; c += 16) {
                         uint32_t o[16];
-                        tc_ld16(lanes + L::COLS_O + c, o);
+                        tc_ld16(lanes + col_o + c, o);
                         tc_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down[i % HB]);   // (HB divides 16)
-                        tc_st16(lanes + L::COLS_O + c, o);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink_o_s[g][i]);
+                        tc_st16(lanes + col_o + c, o);
                     }
                     tc_st_wait();
                 }
-                soft_sync();                                             // red_s is read
                 weigh();
             } else if (j > 0) {
-                // W(j - 1) has been multiplied: its place is free
-                ok = mbar_wait(o_done, (uint32_t)(j - 1) & 1u, abort_flag);
+                ok = mbar_wait(o_done(j - 1), (uint32_t)((j - 1) >> 1) & 1u, abort_flag);                 // W(j - 1) has been multiplied: its place is free
             }
             uint32_t word[L::NO / 4];
 #pragma unroll
             for (int i = 0; i < L::NO / 4; ++i) word[i] = 0u;
 #pragma unroll
-            for (int h = 0; h < HB; h += 2) {
-                l[h] += p[h]; l[h + 1] += p[h + 1];
-                uint32_t part[L::PARTS_W];
-                if constexpr (sizeof(T) == 2) {
-                    uint32_t x = f16x2_of(w[h], w[h + 1]);
+            for (int h = 0; h < HB; h += 4) {
+                uint32_t x[2];
+                float y[4] = {w[h], w[h + 1], w[h + 2], w[h + 3]};
+                if (sizeof(T) == 2) { x[0] = f16x2_of(y[0], y[1]); x[1] = f16x2_of(y[2], y[3]); }
 #pragma unroll
-                    for (int n = 0; n < L::PARTS_W; ++n) {
-                        part[n] = pack_f16x2(x);
-                        if (n + 1 < L::PARTS_W) x = rest_f16x2(x, fx_fp8_unpack2(part[n]));
-                    }
-                } else {
-                    float x = w[h], y = w[h + 1];
+                for (int i = 0; i < 4; ++i) l[h + i] += p[h + i];
 #pragma unroll
-                    for (int n = 0; n < L::PARTS_W; ++n) {
-                        part[n] = fx_fp8_pack2(x, y);
-                        const float2 f = fx_fp8_float2(part[n]);
-                        x = (x - f.x) * 16.f; y = (y - f.y) * 16.f;
+                for (int n = 0; n < L::PARTS_W; ++n) {
+                    uint32_t lo, hi;
+                    if constexpr (sizeof(T) == 2) {
+                        lo = pack_f16x2(x[0]); hi = pack_f16x2(x[1]);
+                        if (n + 1 < L::PARTS_W) { x[0] = rest_f16x2(x[0], fx_fp8_unpack2(lo)); x[1] = rest_f16x2(x[1], fx_fp8_unpack2(hi)); }
+                    } else {
+                        lo = fx_fp8_pack2(y[0], y[1]); hi = fx_fp8_pack2(y[2], y[3]);
+                        const float2 f = fx_fp8_float2(lo), f2 = fx_fp8_float2(hi);
+                        y[0] = (y[0] - f.x) * 16.f; y[1] = (y[1] - f.y) * 16.f; y[2] = (y[2] - f2.x) * 16.f; y[3] = (y[3] - f2.y) * 16.f;
                     }
+                    word[(n * HB + h) / 4] = __byte_perm(lo, hi, 0x5410);
                 }
-#pragma unroll
-                for (int n = 0; n < L::PARTS_W; ++n) word[(n * HB + h) / 4] |= part[n] << (n * HB + h) % 4 * 8;
             }
             uint8_t* row = sm + L::W_OFF + r * 64;
 #pragma unroll
@@ -433,41 +467,74 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
                 *reinterpret_cast<uint4*>(row + ((c ^ (r >> 1 & 3)) << 4)) = make_uint4(word[4 * c], word[4 * c + 1], word[4 * c + 2], word[4 * c + 3]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_before();
+            // O += V^T W^T, by the group's first thread when all its keys' weights are written
+            group_written(g, sw == 0);
+            if (sw == 0 && lane == 0) {
+                tc_fence_after();
+                const uint32_t v = base + j % STAGES * L::STAGE + SLABS * SLAB, wt = base + L::W_OFF;
+#pragma unroll
+                for (int sl = 0; sl < SLABS; ++sl)
+#pragma unroll
+                    for (int ks = 0; ks < TK / 32; ++ks)                 // 32 keys: four 8-key groups, 1024 bytes apart in V, 512 in W
+                        mma8(tmem + col_o + sl * L::NO, smem_desc_lbo_sbo(v + sl * SLAB + ks * 4096, SLAB, 1024), desc64(wt + ks * 2048), idesc_o,
+                             j > 1 || ks > 0);
+                tc_commit(empty(j % STAGES));
+                tc_commit(o_done(j));
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive(w_full);
             if (!ok) fine = false;                                       // (seen by all at the next barrier, or behind the loop)
         }
 
-        // ---- the run's result: this thread has element r of every slab ----
-        bool ok = fine && mbar_wait(o_done, (uint32_t)(n_tiles - 1) & 1u, abort_flag);
+        if (!fine && sw == 0 && lane == 0) { tc_commit(drained(g)); settle(drained(g), 0); }
+
+        // ---- the run's result: this thread has element r of every slab, its group half of the heads, over both groups' tiles ----
+        bool ok = fine && mbar_wait(o_done(n_tiles - 1), (uint32_t)((n_tiles - 1) >> 1) & 1u, abort_flag);
         tc_fence_after();
 #pragma unroll
         for (int h = 0; h < HB; ++h) {
             const float sum = warp_sum(l[h]);
-            if (lane == 0) red_s[0][sw][h] = sum;
+            if (lane == 0) sum_s[g][sw][h] = sum;
         }
         if (!any_of_soft(!ok)) {
+            const bool two = n_tiles > 1;
 #pragma unroll
             for (int sl = 0; sl < SLABS; ++sl) {
-                uint32_t o[L::NO];
-#pragma unroll
-                for (int c = 0; c < L::NO; c += 16) tc_ld16(lanes + L::COLS_O + sl * L::NO + c, o + c);
-                tc_ld_wait();
                 const int e = sl * 128 + r;
+                uint32_t o[2][L::NO];
+#pragma unroll
+                for (int c = 0; c < L::NO; c += 16) tc_ld16(lanes + L::COLS_O + sl * L::NO + c, o[0] + c);
+                if (two) {
+#pragma unroll
+                    for (int c = 0; c < L::NO; c += 16) tc_ld16(lanes + L::COLS_O + (SLABS + sl) * L::NO + c, o[1] + c);
+                }
+                tc_ld_wait();
 #pragma unroll
                 for (int h = 0; h < HB; ++h) {
-                    if (h >= nh || e >= D) continue;
-                    float x = __uint_as_float(o[(L::PARTS_W - 1) * HB + h]);
+                    if (h / (HB / 2) != g || h >= nh || e >= D) continue;
+                    float x[2], sum[2];
 #pragma unroll
-                    for (int n = L::PARTS_W - 2; n >= 0; --n) x = fmaf(x, 0.0625f, __uint_as_float(o[n * HB + h]));
-                    const float sum = (red_s[0][0][h] + red_s[0][1][h]) + (red_s[0][2][h] + red_s[0][3][h]);
-                    x = sum == 0.f ? 0.f : x / sum * exp2_fast(refw[h] - ref[h]);
+                    for (int i = 0; i < 2; ++i) {
+                        x[i] = __uint_as_float(o[i][(L::PARTS_W - 1) * HB + h]);
+#pragma unroll
+                        for (int n = L::PARTS_W - 2; n >= 0; --n) x[i] = fmaf(x[i], 0.0625f, __uint_as_float(o[i][n * HB + h]));
+                        sum[i] = (sum_s[i][0][h] + sum_s[i][1][h]) + (sum_s[i][2][h] + sum_s[i][3][h]);
+                    }
+                    // either group's mean of the values, and its share of the weights
+                    const float ref = two ? fmaxf(ref_s[0][h], ref_s[1][h]) : ref_s[0][h];
+                    float all = sum[0] * exp2_fast(ref_s[0][h] - ref);
+                    float v = sum[0] == 0.f ? 0.f : x[0] / sum[0] * exp2_fast(refw_s[0][h] - ref_s[0][h]);
+                    if (two && sum[1] != 0.f) {
+                        const float share = sum[1] * exp2_fast(ref_s[1][h] - ref), v1 = x[1] / sum[1] * exp2_fast(refw_s[1][h] - ref_s[1][h]);
+                        const float whole = all + share;
+                        v = all == 0.f ? v1 : fmaf(v, all / whole, v1 * (share / whole));
+                        all = whole;
+                    }
                     if (a.n_splits == 1) {
-                        reinterpret_cast<T*>(a.out)[(long)tkn * a.ldo + (long)(h0 + h) * D + e] = from_f32<T>(x);
+                        reinterpret_cast<T*>(a.out)[(long)tkn * a.ldo + (long)(h0 + h) * D + e] = from_f32<T>(v);
                     } else {
                         const long at = ((long)blockIdx.x * a.n_heads + h0 + h) * a.n_splits + split;
-                        a.part_o[at * D + e] = x;
-                        if (e == 0) { a.part_ml[2 * at] = ref[h]; a.part_ml[2 * at + 1] = sum; }
+                        a.part_o[at * D + e] = v;
+                        if (e == 0) { a.part_ml[2 * at] = ref; a.part_ml[2 * at + 1] = all; }
                     }
                 }
             }
@@ -535,16 +602,13 @@ bool encode(CUtensorMap* map, const void* ptr, const Args& a)
 
 template <typename T> int run(const CUtensorMap& mk, const CUtensorMap& mv, Args& a, int n_tokens, cudaStream_t s)
 {
-    // heads a block takes: as few columns as the group needs, 16 at most (32 bits: 8, whose parts are 48 columns)
-    const int group = a.n_heads / a.n_kv_heads, hb = group <= 4 ? 4 : group <= 8 || sizeof(T) == 4 ? 8 : 16;
+    // heads a block takes: 4, or 8, whose registers leave two blocks an SM; more heads of a kv head: blocks side by side
+    const int group = a.n_heads / a.n_kv_heads, hb = group <= 4 ? 4 : 8;
     const dim3 grid(n_tokens, a.n_kv_heads * ((group + hb - 1) / hb), a.n_splits);
     if (grid.y > 65535u) return FX_ERR_SIZE;
     int rc;
-    if constexpr (sizeof(T) == 2) {
-        if (hb == 16) rc = a.head_dim <= 128 ? launch<T, 16, 1>(mk, mv, a, grid, s) : launch<T, 16, 2>(mk, mv, a, grid, s);
-    }
     if (hb == 8) rc = a.head_dim <= 128 ? launch<T, 8, 1>(mk, mv, a, grid, s) : launch<T, 8, 2>(mk, mv, a, grid, s);
-    if (hb == 4) rc = a.head_dim <= 128 ? launch<T, 4, 1>(mk, mv, a, grid, s) : launch<T, 4, 2>(mk, mv, a, grid, s);
+    else rc = a.head_dim <= 128 ? launch<T, 4, 1>(mk, mv, a, grid, s) : launch<T, 4, 2>(mk, mv, a, grid, s);
     if (rc || a.n_splits == 1) return rc;
     fx_launch_pdl(decode_fp8_merge_kernel<T>, dim3(n_tokens, a.n_heads), MERGE_THREADS, 0, s, a);
     return fx_launch_status();

@@ -2123,7 +2123,7 @@ def decode_fp8_ok(k_pages, v_pages, head_dim: int, page_size: int) -> bool:
 
 
 FP8_TILE = 128                    # positions a tile of the decode kernel holds
-FP8_MAX_RUNS = 64
+FP8_MAX_RUNS = 128
 # In the time a tile takes a block: what a run costs beside its tiles, and the second kernel that adds the runs up.
 FP8_RUN_OVERHEAD, FP8_MERGE_COST = 3.0, 2.0
 
@@ -2134,7 +2134,7 @@ def decode_fp8_runs(n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
     more than 128 elements) come to the least.  A function of the step's size and of ``reach``, the most positions a token may see, and
     not of the lengths, so that a captured step keeps its grid."""
     group = n_heads // n_kv_heads
-    per = 4 if group <= 4 else 8 if group <= 8 or f32 else 16
+    per = 4 if group <= 4 else 8
     blocks, slots, tiles = max(1, n_tokens * n_kv_heads * -(-group // per)), sm_count() * (2 if head_dim <= 128 else 1), -(-reach // FP8_TILE)
     best, best_cost = 1, None
     for n in range(1, min(FP8_MAX_RUNS, tiles) + 1):
@@ -2217,8 +2217,9 @@ class PrefillFp8Plan:
             self._kept[key] = x
         elif isinstance(x, tuple):
             # used on a stream other than the one that copied it: ordered behind the copy, and not freed under its kernels
+            # (a capture begins behind everything that was under way, and its graph needs the plan for as long as it lives)
             now, seen = _stream_on(self.device), self._streams[key]
-            if now is not None and all(now != s for s in seen):
+            if now is not None and all(now != s for s in seen) and not torch.cuda.is_current_stream_capturing():
                 now.wait_stream(seen[0])
                 for t in x:
                     if isinstance(t, torch.Tensor) and t.numel():
