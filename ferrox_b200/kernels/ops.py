@@ -265,6 +265,8 @@ def _call_traced(name: str, args) -> None:
 
 _scoped_stream = None
 _sm_count = 0
+# a device's current stream without an object made for it (3 us of a call)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def sm_count() -> int:
@@ -282,7 +284,7 @@ def stream_ptr() -> int:
     """The stream kernels go to when none is named: the one a step has announced, else torch's current stream."""
     if _scoped_stream is not None:
         return _scoped_stream
-    return torch.cuda.current_stream().cuda_stream
+    return _current_stream(torch.cuda.current_device())
 
 
 _beside_step = False     # inside a scope within a step's own: work that runs on another stream beside the step
@@ -2003,36 +2005,42 @@ FP8_MAX_DIM = 256                 # elements of a head
 FP8_LARGEST, FP8_MIN_EXP, FP8_NAN = 448.0, -119, 255
 
 
-def _on_current_device(name, *tensors):
+_E4M3, _U8, _I32 = torch.float8_e4m3fn, torch.uint8, torch.int32
+
+
+def _on_current_device(name, first, *others):
     """A launch goes to the current device: operands elsewhere are refused."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for t in tensors:
-        if t is not None and not (t.is_cuda and t.device.index == device):
-            raise KernelError(f"{name}: an operand on {t.device}, the current device is " + (f"cuda:{device}" if device >= 0 else "none"))
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"{name}: an operand on {t.device}, another on {first.device}")
+    if device < 0 or device != torch.cuda.current_device():
+        raise KernelError(f"{name}: an operand on {first.device}, which is not the current CUDA device")
 
 
 def _int32(name, what, *tensors):
     for t in tensors:
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+        if t is not None and (t.dtype is not _I32 or not t.is_contiguous()):
             raise KernelError(f"{name}: {what} are contiguous int32, found {t.dtype} with strides {t.stride()}")
 
 
 def _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size):
-    """Checks an 8-bit cache; its (pages, kv heads, head size)."""
-    if k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn or k_exp.dtype != torch.uint8 or v_exp.dtype != torch.uint8:
+    """Checks an 8-bit cache; its (pages, kv heads, head size, slots, pages of a request)."""
+    shape, exp_shape, table_shape = k_pages.shape, k_exp.shape, block_table.shape
+    if not (k_pages.dtype is _E4M3 and v_pages.dtype is _E4M3 and k_exp.dtype is _U8 and v_exp.dtype is _U8):
         raise KernelError(f"{name}: pages are float8_e4m3fn and their exponents uint8, found {k_pages.dtype}, {v_pages.dtype}, {k_exp.dtype}, {v_exp.dtype}")
-    shape = k_pages.shape
-    if len(shape) != 4 or v_pages.shape != shape or k_exp.shape != shape[:3] or v_exp.shape != shape[:3] or shape[2] != page_size:
+    if len(shape) != 4 or v_pages.shape != shape or exp_shape != shape[:3] or v_exp.shape != exp_shape or shape[2] != page_size:
         raise KernelError(f"{name}: pages [pages, kv heads, {page_size}, head size] and exponents [pages, kv heads, {page_size}], found "
                           f"{tuple(shape)}, {tuple(v_pages.shape)}, {tuple(k_exp.shape)}, {tuple(v_exp.shape)}")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous() and k_exp.is_contiguous() and v_exp.is_contiguous()):
         raise KernelError(f"{name}: pages and exponents are contiguous")
-    if block_table.dim() != 2 or block_table.shape[1] == 0:
-        raise KernelError(f"{name}: the block table is [slots, pages of a request], found {tuple(block_table.shape)}")
-    _int32(name, "block tables", block_table)
-    if not 0 < shape[3] <= FP8_MAX_DIM or shape[0] == 0:
+    if len(table_shape) != 2 or table_shape[1] == 0 or block_table.dtype is not _I32 or not block_table.is_contiguous():
+        raise KernelError(f"{name}: the block table is contiguous int32 [slots, pages of a request], found {block_table.dtype} {tuple(table_shape)} "
+                          f"with strides {block_table.stride()}")
+    n_pages, G, _, D = shape
+    if not 0 < D <= FP8_MAX_DIM or n_pages == 0:
         raise KernelError(f"{name}: heads of 1 to {FP8_MAX_DIM} elements and at least one page, found {tuple(shape)}")
-    return shape[0], shape[1], shape[3]
+    return n_pages, G, D, table_shape[0], table_shape[1]
 
 
 def rope_kv_write_fp8(qkv, positions, token_seq, seq_slot, inv_freq, rotary_dim, k_pages, v_pages, k_exp, v_exp, block_table,
@@ -2046,9 +2054,10 @@ def rope_kv_write_fp8(qkv, positions, token_seq, seq_slot, inv_freq, rotary_dim,
     element that is infinite or no number gets E = 255 and reads as NaN.  A position without a page, or outside its table, is
     written nowhere and raises ``status`` 2.  Positions of a call are distinct."""
     name = "rope_kv_write_fp8"
-    n_pages, G, D = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
-    T = qkv.shape[0]
-    if (G, D) != (n_kv_heads, head_dim) or qkv.dim() != 2 or qkv.shape[1] < (n_heads + 2 * n_kv_heads) * head_dim:
+    n_pages, G, D, n_slots, width = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
+    shape = qkv.shape
+    T = shape[0]
+    if G != n_kv_heads or D != head_dim or len(shape) != 2 or shape[1] < (n_heads + 2 * n_kv_heads) * head_dim:
         raise KernelError(f"{name}: rows of {n_heads} + 2 * {n_kv_heads} heads of {head_dim} for pages of {G} heads of {D}, found {tuple(qkv.shape)}")
     if positions.numel() != T or token_seq.numel() != T:
         raise KernelError(f"{name}: a position and an entry for each of {T} rows, found {positions.numel()} and {token_seq.numel()}")
@@ -2060,21 +2069,21 @@ def rope_kv_write_fp8(qkv, positions, token_seq, seq_slot, inv_freq, rotary_dim,
     _on_current_device(name, qkv, positions, token_seq, seq_slot, inv_freq, cos_sin, k_pages, v_pages, k_exp, v_exp, block_table, status)
     call("fx_rope_kv_write_fp8", _ptr(qkv), code(qkv), _rows(qkv), _ptr(positions), _ptr(token_seq), _ptr(seq_slot), _ptr(inv_freq),
          _ptr(cos_sin), rotary_dim, int(pairing), _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table),
-         block_table.shape[0], block_table.shape[1], page_size, n_pages, T, n_heads, n_kv_heads, head_dim, int(write_cache), _ptr(status),
+         n_slots, width, page_size, n_pages, T, n_heads, n_kv_heads, head_dim, int(write_cache), _ptr(status),
          stream if stream is not None else stream_ptr())
 
 
 def _read_kv_fp8(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, spans, n_rows, k_out,
-                 v_out, shape, stream):
-    n_pages, G, D = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
-    shape = shape(G, D)
+                 v_out, stream):
+    n_pages, G, D, n_slots, width = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
+    shape = (n_rows, G, D) if spans is None else (n_rows // page_size, G, page_size, D)
     if k_out.dtype != v_out.dtype or k_out.shape != shape or v_out.shape != shape or not (k_out.is_contiguous() and v_out.is_contiguous()):
         raise KernelError(f"{name}: two contiguous results {tuple(shape)} of one type, found {tuple(k_out.shape)} {k_out.dtype} and "
                           f"{tuple(v_out.shape)} {v_out.dtype}")
     _int32(name, "positions, entries, slots and spans", positions, token_seq, seq_slot, spans)
     _on_current_device(name, k_pages, v_pages, k_exp, v_exp, block_table, positions, token_seq, seq_slot, spans, k_out, v_out)
-    call("fx_read_kv_fp8", _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table), block_table.shape[0],
-         block_table.shape[1], page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot), _ptr(spans),
+    call("fx_read_kv_fp8", _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table), n_slots,
+         width, page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot), _ptr(spans),
          spans.shape[0] if spans is not None else 0, n_rows, _ptr(k_out), _ptr(v_out), code(k_out), G, D,
          stream if stream is not None else stream_ptr())
 
@@ -2086,7 +2095,7 @@ def read_kv_fp8(k_pages, v_pages, k_exp, v_exp, block_table, page_size, position
     if token_seq.numel() != T:
         raise KernelError(f"read_kv_fp8: an entry for each of {T} positions, found {token_seq.numel()}")
     _read_kv_fp8("read_kv_fp8", k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, None, T, k_out,
-                 v_out, lambda G, D: (T, G, D), stream)
+                 v_out, stream)
 
 
 def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, spans, n_rows, seq_slot, k_out, v_out, stream=None):
@@ -2097,24 +2106,24 @@ def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, sp
     if n_rows % page_size or n_rows < 0 or spans.dim() != 2 or spans.shape[1] != 4 or (n_rows and not spans.shape[0]):
         raise KernelError(f"read_kv_fp8_spans: spans [n, 4] over a multiple of {page_size} rows, found {tuple(spans.shape)} over {n_rows}")
     _read_kv_fp8("read_kv_fp8_spans", k_pages, v_pages, k_exp, v_exp, block_table, page_size, None, None, seq_slot, spans, n_rows, k_out,
-                 v_out, lambda G, D: (n_rows // page_size, G, page_size, D), stream)
+                 v_out, stream)
 
 
 def _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, tokens, out,
                          n_heads, n_kv_heads, head_dim, window, scale, softcap):
-    n_pages, G, D = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
-    T = positions.numel()
-    if (G, D) != (n_kv_heads, head_dim) or n_heads < 1 or n_heads % n_kv_heads:
+    n_pages, G, D, n_slots, width = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
+    T, qs, os = positions.numel(), q.shape, out.shape
+    if G != n_kv_heads or D != head_dim or n_heads < 1 or n_heads % n_kv_heads:
         raise KernelError(f"{name}: {n_heads} heads on {n_kv_heads} of {head_dim} for pages of {G} heads of {D}")
-    if out.dtype != q.dtype or q.dim() != 2 or q.shape[0] != T or q.shape[1] < n_heads * head_dim or out.dim() != 2 or out.shape[0] != T \
-            or out.shape[1] < n_heads * head_dim or token_seq.numel() != T:
-        raise KernelError(f"{name}: {T} rows of {n_heads} heads of {head_dim}, found queries {tuple(q.shape)} {q.dtype}, results "
-                          f"{tuple(out.shape)} {out.dtype}, {token_seq.numel()} entries")
+    need = n_heads * head_dim
+    if out.dtype is not q.dtype or len(qs) != 2 or len(os) != 2 or qs[0] != T or os[0] != T or qs[1] < need or os[1] < need or token_seq.numel() != T:
+        raise KernelError(f"{name}: {T} rows of {n_heads} heads of {head_dim}, found queries {tuple(qs)} {q.dtype}, results "
+                          f"{tuple(os)} {out.dtype}, {token_seq.numel()} entries")
     if (window is not None and window < 1) or (softcap is not None and not softcap > 0) or not abs(scale) < float("inf"):
         raise KernelError(f"{name}: window={window}, softcap={softcap}, scale={scale}: positive (or None), positive (or None), finite")
     _int32(name, "positions, entries, slots and tokens", positions, token_seq, seq_slot, tokens)
     _on_current_device(name, q, k_pages, v_pages, k_exp, v_exp, block_table, positions, token_seq, seq_slot, tokens, out)
-    return n_pages
+    return n_pages, n_slots, width, T
 
 
 def decode_fp8_ok(k_pages, v_pages, head_dim: int, page_size: int) -> bool:
@@ -2151,20 +2160,21 @@ def decode_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_si
     ``tokens`` (int32, optional): the rows of ``q`` and ``out`` that are taken; the others stay as they are.  Positions without a
     page do not count; a token that sees none gets zeros."""
     name = "decode_attention_fp8"
-    n_pages = _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, tokens,
+    n_pages, n_slots, width, n = _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, tokens,
                                    out, n_heads, n_kv_heads, head_dim, window, scale, softcap)
-    n = positions.numel() if tokens is None else tokens.numel()
+    if tokens is not None:
+        n = tokens.numel()
     operands = (_ptr(q), _rows(q), code(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table),
-                block_table.shape[0], block_table.shape[1], page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot),
+                n_slots, width, page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot),
                 _ptr(tokens), n, _ptr(out), _rows(out), n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0))
     st = stream if stream is not None else stream_ptr()
     if not decode_fp8_ok(k_pages, v_pages, head_dim, page_size):
         call("fx_attention_fp8", *operands, st)
         return out
-    reach = block_table.shape[1] * page_size
+    reach = width * page_size
     if window is not None:
         reach = min(reach, (window + FP8_TILE - 2) // FP8_TILE * FP8_TILE + FP8_TILE)      # (the tiles that it straddles)
-    runs = decode_fp8_runs(n, n_heads, n_kv_heads, head_dim, q.dtype == torch.float32, reach)
+    runs = decode_fp8_runs(n, n_heads, n_kv_heads, head_dim, q.dtype is torch.float32, reach)
     if runs == 1:
         call("fx_decode_attention_fp8", *operands, 1, None, None, _ptr(status), st)
         return out
@@ -2185,13 +2195,9 @@ FP8_FEW_TOKENS = 8                # entries that bring at most this many tokens 
 FP8_READ_BACK_MAX = 1 << 30       # bytes of keys and values that are read back at a time
 
 
-def _stream_on(device):
-    return torch.cuda.current_stream(device) if device.type == "cuda" else None
-
-
 def _elsewhere(stream) -> bool:
     """Whether a named stream is another than the one that scratch is taken on."""
-    return stream is not None and stream != _scoped_stream and stream != torch.cuda.current_stream().cuda_stream
+    return stream is not None and stream != _scoped_stream and stream != _current_stream(torch.cuda.current_device())
 
 
 class PrefillFp8Plan:
@@ -2205,6 +2211,7 @@ class PrefillFp8Plan:
             raise KernelError(f"prefill_fp8_plan: entries {self.entries} of pages of {page_size}")
         self.n_tokens = sum(n for n, _ in self.entries)
         self._kept, self._streams = {}, {}
+        self._index = self.device.index if self.device.index is not None or self.device.type != "cuda" else torch.cuda.current_device()
 
     def kept(self, key, make):
         """What ``make`` returns, made once: a tuple's numpy arrays as tensors on the device."""
@@ -2213,19 +2220,23 @@ class PrefillFp8Plan:
             x = make()
             if isinstance(x, tuple):
                 x = tuple(upload(v, self.device) if hasattr(v, "__array__") else v for v in x)
-                self._streams[key] = [_stream_on(self.device)]
+                self._streams[key] = [self._stream()]
             self._kept[key] = x
         elif isinstance(x, tuple):
             # used on a stream other than the one that copied it: ordered behind the copy, and not freed under its kernels
             # (a capture begins behind everything that was under way, and its graph needs the plan for as long as it lives)
-            now, seen = _stream_on(self.device), self._streams[key]
-            if now is not None and all(now != s for s in seen) and not torch.cuda.is_current_stream_capturing():
-                now.wait_stream(seen[0])
+            now, seen = self._stream(), self._streams[key]
+            if now not in seen and not torch.cuda.is_current_stream_capturing():
+                stream = torch.cuda.current_stream(self.device)
+                stream.wait_stream(torch.cuda.ExternalStream(seen[0], device=self.device))
                 for t in x:
                     if isinstance(t, torch.Tensor) and t.numel():
-                        t.record_stream(now)
+                        t.record_stream(stream)
                 seen.append(now)
         return x
+
+    def _stream(self):
+        return _current_stream(self._index) if self.device.type == "cuda" else None
 
     def few(self):
         """Flat indices of the tokens of entries that bring few, or None."""
