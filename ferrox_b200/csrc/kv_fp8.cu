@@ -30,110 +30,151 @@ struct WriteArgs {
 
 constexpr int WRITE_WARPS = 4, MAX_DIM = 256;
 
-// Elements a lane holds: NE neighbours from lane * NE on (WHOLE: rows of 32 NE elements on the vectors' grid, a rotation of
-// the whole head in halves or none), else lane, lane + 32, ...
-template <typename T, int NE, bool WHOLE>
-__global__ void __launch_bounds__(WRITE_WARPS * 32) write_kernel(WriteArgs a)
+// Where token t's position lies; -1: nowhere.
+__device__ __forceinline__ int page_of_token(const int* positions, const int* token_seq, const int* seq_slot, const int* block_table, int n_slots,
+                                             int table_width, int n_pages, int page_size, int t, int pos)
 {
-    __shared__ float row_s[WHOLE ? 1 : WRITE_WARPS][WHOLE ? 1 : MAX_DIM];
+    const int slot = seq_slot[token_seq[t]];
+    return slot >= 0 && slot < n_slots ? fx_page_of(block_table + (long)slot * table_width, table_width, n_pages, pos, page_size) : -1;
+}
+
+// An element of pair i behind its rotation: its own value p, its partner's q.
+__device__ __forceinline__ float turned(const WriteArgs& a, int t, int pos, float p, float q, int i, bool second)
+{
+    float s, c;
+    if (a.cos_sin) {
+        const float2 cs = *reinterpret_cast<const float2*>(a.cos_sin + ((long)t * (a.rotary_dim >> 1) + i) * 2);
+        c = cs.x; s = cs.y;
+    } else sincosf((float)pos * a.inv_freq[i], &s, &c);
+    return second ? q * s + p * c : p * c - q * s;
+}
+
+// Rows of LANES lanes with 16 bytes each (or 32 lanes with 32 bytes), a rotation of the whole head in halves or none.  A block
+// takes a token's rows, or a share of them (blockIdx.y); a lane loads R rows' parts before it works on the first.  What bounds
+// it is how many bytes are under way: the place of a token's position is four loads that hang on one another, beside which its
+// rows arrive.  B200, 2,709 tokens of 32 heads of 128 and their reading back: one row a warp 34.4 us, four rows a lane see DESIGN.
+template <typename T, int DIM, int R>
+__global__ void __launch_bounds__(WRITE_WARPS * 32) write_rows_kernel(WriteArgs a)
+{
+    constexpr int NE = DIM * (int)sizeof(T) / 16 > 32 ? DIM / 32 : 16 / (int)sizeof(T), LANES = DIM / NE, PER = 32 / LANES * WRITE_WARPS;
+    fx_pdl_wait();
+    const int t = blockIdx.x, sub = threadIdx.x % LANES, heads = a.n_heads + 2 * a.n_kv_heads;
+    const int h_first = a.first_head + blockIdx.y * PER * R + threadIdx.x / LANES;
+    const int pos = a.positions[t];
+    T* rows = reinterpret_cast<T*>(a.qkv) + (long)t * a.ld + sub * NE;
+    float x[R][NE];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int h = h_first + u * PER;
+#pragma unroll
+        for (int i = 0; i < NE; i += Pack<T>::N) {
+            if (h < heads) Pack<T>::load(rows + (long)h * DIM + i, x[u] + i);
+            else
+#pragma unroll
+                for (int e = 0; e < Pack<T>::N; ++e) x[u][i + e] = 0.f;
+        }
+    }
+    int page = -1;
+    if (a.write_cache) {
+        page = page_of_token(a.positions, a.token_seq, a.seq_slot, a.block_table, a.n_slots, a.table_width, a.n_pages, a.page_size, t, pos);
+        if (page < 0 && threadIdx.x == 0 && a.status) atomicExch(a.status, 2);
+    }
+    const long at0 = (long)page * a.n_kv_heads * a.page_size + pos % a.page_size;
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int h = h_first + u * PER;                                   // (the lanes of a row agree on it, a warp's may not)
+        float* y = x[u];
+        if (a.inv_freq) {
+            const bool rotated = h < a.n_heads + a.n_kv_heads;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const float other = __shfl_xor_sync(0xffffffffu, y[i], LANES / 2);
+                if (rotated) y[i] = to_f32(from_f32<T>(turned(a, t, pos, y[i], other, (sub % (LANES / 2)) * NE + i, sub >= LANES / 2)));
+            }
+            if (rotated)
+#pragma unroll
+                for (int i = 0; i < NE; i += Pack<T>::N) Pack<T>::store(rows + (long)h * DIM + i, y + i);
+        }
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) most = max(most, __float_as_uint(y[i]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (page < 0 || h < a.n_heads || h >= heads) continue;
+        const int exponent = fx_fp8_exponent(most);
+        const bool none = exponent == FX_FP8_NAN, is_v = h >= a.n_heads + a.n_kv_heads;
+        if (exponent == FX_FP8_MAX_BYTE)
+#pragma unroll
+            for (int i = 0; i < NE; ++i) y[i] = fminf(fmaxf(y[i], -FX_FP8_MOST), FX_FP8_MOST);
+        const float inv = none ? 0.f : fx_fp8_inverse(exponent);
+        const long at = at0 + (long)(h - a.n_heads - (is_v ? a.n_kv_heads : 0)) * a.page_size;
+        uint32_t w[NE / 4];
+#pragma unroll
+        for (int i = 0; i < NE; i += 4)
+            w[i / 4] = none ? 0u : fx_fp8_pack2(y[i] * inv, y[i + 1] * inv) | fx_fp8_pack2(y[i + 2] * inv, y[i + 3] * inv) << 16;
+        uint8_t* dst = (is_v ? a.v_pages : a.k_pages) + at * DIM + sub * NE;
+        if constexpr (NE == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+        if (sub == 0) (is_v ? a.v_exp : a.k_exp)[at] = (uint8_t)exponent;
+    }
+}
+
+// Any other row of up to MAX_DIM elements, a warp a row: a lane has the elements lane, lane + 32, ...
+template <typename T>
+__global__ void __launch_bounds__(WRITE_WARPS * 32) write_any_kernel(WriteArgs a)
+{
+    constexpr int NE = MAX_DIM / 32;
+    __shared__ float row_s[WRITE_WARPS][MAX_DIM];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = a.head_dim;
     const int heads = a.n_heads + 2 * a.n_kv_heads - a.first_head;         // rows of a token that are looked at
     fx_pdl_wait();
     const long item = (long)blockIdx.x * WRITE_WARPS + warp;
     if (item >= (long)a.n_tokens * heads) return;
     const int t = (int)(item / heads), h = a.first_head + (int)(item - (long)t * heads);
-    const bool rotated = a.inv_freq && h < a.n_heads + a.n_kv_heads, cached = a.write_cache && h >= a.n_heads;
+    const bool rotated = a.inv_freq && h < a.n_heads + a.n_kv_heads;
     const int pos = a.positions[t];
     T* row = reinterpret_cast<T*>(a.qkv) + (long)t * a.ld + (long)h * D;
     float x[NE];
-    if (WHOLE) {
-        if constexpr (NE * sizeof(T) >= 16) {
 #pragma unroll
-            for (int i = 0; i < NE; i += Pack<T>::N) Pack<T>::load(row + lane * NE + i, x + i);
-        } else if constexpr (NE * sizeof(T) == 8 && sizeof(T) == 2) {
-            const uint2 w = *reinterpret_cast<const uint2*>(row + lane * NE);
-            x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xffff0000u);
-            x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xffff0000u);
-        } else {
-#pragma unroll
-            for (int i = 0; i < NE; ++i) x[i] = to_f32(row[lane * NE + i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < NE; ++i) x[i] = lane + 32 * i < D ? to_f32(row[lane + 32 * i]) : 0.f;
-    }
-    int page = -1, slot = 0;
-    if (cached) {
-        slot = a.seq_slot[a.token_seq[t]];
-        if (slot >= 0 && slot < a.n_slots)
-            page = fx_page_of(a.block_table + (long)slot * a.table_width, a.table_width, a.n_pages, pos, a.page_size);
+    for (int i = 0; i < NE; ++i) x[i] = lane + 32 * i < D ? to_f32(row[lane + 32 * i]) : 0.f;
+    int page = -1;
+    if (a.write_cache && h >= a.n_heads) {
+        page = page_of_token(a.positions, a.token_seq, a.seq_slot, a.block_table, a.n_slots, a.table_width, a.n_pages, a.page_size, t, pos);
         if (page < 0 && lane == 0 && a.status) atomicExch(a.status, 2);
     }
     if (rotated) {
         const int half = a.rotary_dim >> 1;
-        auto turn = [&](float p, float q, int i, bool second) {            // element of pair i: its own value p, its partner's q
-            float s, c;
-            if (a.cos_sin) {
-                const float2 cs = *reinterpret_cast<const float2*>(a.cos_sin + ((long)t * half + i) * 2);
-                c = cs.x; s = cs.y;
-            } else sincosf((float)pos * a.inv_freq[i], &s, &c);
-            return second ? q * s + p * c : p * c - q * s;
-        };
-        if (WHOLE) {
 #pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                const float other = __shfl_xor_sync(0xffffffffu, x[i], 16);
-                x[i] = turn(x[i], other, (lane & 15) * NE + i, lane >= 16);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NE; ++i)
-                if (lane + 32 * i < D) row_s[warp][lane + 32 * i] = x[i];
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                const int e = lane + 32 * i;
-                if (e >= a.rotary_dim) continue;
-                const bool second = a.pairing ? e & 1 : e >= half;
-                x[i] = turn(x[i], row_s[warp][a.pairing ? e ^ 1 : second ? e - half : e + half], a.pairing ? e >> 1 : second ? e - half : e, second);
-            }
-        }
+        for (int i = 0; i < NE; ++i)
+            if (lane + 32 * i < D) row_s[warp][lane + 32 * i] = x[i];
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
-            const T y = from_f32<T>(x[i]);
+            const int e = lane + 32 * i;
+            if (e >= a.rotary_dim) continue;
+            const bool second = a.pairing ? e & 1 : e >= half;
+            const T y = from_f32<T>(turned(a, t, pos, x[i], row_s[warp][a.pairing ? e ^ 1 : second ? e - half : e + half],
+                                           a.pairing ? e >> 1 : second ? e - half : e, second));
             x[i] = to_f32(y);
-            const int e = WHOLE ? lane * NE + i : lane + 32 * i;
-            if (WHOLE || e < a.rotary_dim) row[e] = y;
+            row[e] = y;
         }
     }
     if (page < 0) return;                                                  // (a whole warp)
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < NE; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-    most = __reduce_max_sync(0xffffffffu, most);
-    const int exponent = fx_fp8_exponent(most);
+    const int exponent = fx_fp8_exponent(__reduce_max_sync(0xffffffffu, most));
     if (exponent == FX_FP8_MAX_BYTE)
 #pragma unroll
         for (int i = 0; i < NE; ++i) x[i] = fminf(fmaxf(x[i], -FX_FP8_MOST), FX_FP8_MOST);
-    const float inv = exponent == FX_FP8_NAN ? 0.f : fx_fp8_inverse(exponent);
-    const bool is_v = h >= a.n_heads + a.n_kv_heads;
+    const bool none = exponent == FX_FP8_NAN, is_v = h >= a.n_heads + a.n_kv_heads;
+    const float inv = none ? 0.f : fx_fp8_inverse(exponent);
     const long at = ((long)page * a.n_kv_heads + (h - a.n_heads - (is_v ? a.n_kv_heads : 0))) * a.page_size + pos % a.page_size;
     uint8_t* dst = (is_v ? a.v_pages : a.k_pages) + at * D;
     if (lane == 0) (is_v ? a.v_exp : a.k_exp)[at] = (uint8_t)exponent;
-    auto byte2 = [&](float p, float q) { return exponent == FX_FP8_NAN ? 0u : fx_fp8_pack2(p * inv, q * inv); };
-    if (WHOLE) {
-        if constexpr (NE == 2) {
-            *reinterpret_cast<uint16_t*>(dst + lane * 2) = (uint16_t)byte2(x[0], x[1]);
-        } else {
 #pragma unroll
-            for (int i = 0; i < NE; i += 4)
-                *reinterpret_cast<uint32_t*>(dst + lane * NE + i) = byte2(x[i], x[i + 1]) | byte2(x[i + 2], x[i + 3]) << 16;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < NE; ++i)
-            if (lane + 32 * i < D) dst[lane + 32 * i] = (uint8_t)byte2(x[i], 0.f);
-    }
+    for (int i = 0; i < NE; ++i)
+        if (lane + 32 * i < D) dst[lane + 32 * i] = none ? 0 : (uint8_t)fx_fp8_pack2(x[i] * inv, 0.f);
 }
 
 struct ReadArgs {
@@ -159,26 +200,41 @@ template <typename T> __device__ __forceinline__ void put16(T* dst, uint4 w, flo
     for (int i = 0; i < 16; i += Pack<T>::N) Pack<T>::store(dst + i, f + i);
 }
 
-// The rows of a step: k_out, v_out [tokens][kv heads][head_dim].  VEC elements a thread.
+// The rows of a step: k_out, v_out [tokens][kv heads][head_dim].  A block takes a token's rows, or a share of them
+// (blockIdx.y); a thread READ_AHEAD times VEC elements, all asked for before the first is written.
+constexpr int READ_THREADS = 128, READ_AHEAD = 4;
+
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) read_rows_kernel(ReadArgs a)
+__global__ void __launch_bounds__(READ_THREADS) read_rows_kernel(ReadArgs a)
 {
     fx_pdl_wait();
-    const int D = a.head_dim, per_row = D / VEC;
-    const long n = (long)a.n_rows * a.n_kv_heads * per_row * 2;
-    for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) {
-        const int c = (int)(i % per_row);
-        const long rest = i / per_row;
-        const bool is_v = rest & 1;
-        const int h = (int)((rest >> 1) % a.n_kv_heads), t = (int)((rest >> 1) / a.n_kv_heads);
-        const int slot = a.seq_slot[a.token_seq[t]], pos = a.positions[t];
-        const int page = slot >= 0 && slot < a.n_slots ? fx_page_of(a.block_table + (long)slot * a.table_width, a.table_width, a.n_pages, pos, a.page_size) : -1;
-        T* dst = reinterpret_cast<T*>(is_v ? a.v_out : a.k_out) + ((long)t * a.n_kv_heads + h) * D + c * VEC;
-        const long at = ((long)max(page, 0) * a.n_kv_heads + h) * a.page_size + (page < 0 ? 0 : pos % a.page_size);
-        const uint8_t* src = (is_v ? a.v_pages : a.k_pages) + at * D + c * VEC;
-        const float scale = page < 0 ? 0.f : fx_fp8_scale((is_v ? a.v_exp : a.k_exp)[at]);
-        if constexpr (VEC == 16) put16(dst, page < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(src), scale);
-        else *dst = from_f32<T>(page < 0 ? 0.f : fx_fp8_float2(*src).x * scale);
+    const int D = a.head_dim, per_row = D / VEC, n = 2 * a.n_kv_heads * per_row, t = blockIdx.x, pos = a.positions[t];
+    const int slot = a.seq_slot[a.token_seq[t]];
+    const int page = slot >= 0 && slot < a.n_slots ? fx_page_of(a.block_table + (long)slot * a.table_width, a.table_width, a.n_pages, pos, a.page_size) : -1;
+    const long at0 = page < 0 ? 0 : (long)page * a.n_kv_heads * a.page_size + pos % a.page_size;
+    uint4 w[READ_AHEAD];
+    int e[READ_AHEAD];
+#pragma unroll
+    for (int u = 0; u < READ_AHEAD; ++u) {
+        const int i = (blockIdx.y * READ_AHEAD + u) * READ_THREADS + threadIdx.x, row = i / per_row, h = row % a.n_kv_heads;
+        w[u] = make_uint4(0, 0, 0, 0);
+        e[u] = 0;
+        if (i >= n || page < 0) continue;
+        const bool is_v = row >= a.n_kv_heads;
+        const long at = at0 + (long)h * a.page_size;
+        const uint8_t* src = (is_v ? a.v_pages : a.k_pages) + at * D + (i - row * per_row) * VEC;
+        if constexpr (VEC == 16) w[u] = *reinterpret_cast<const uint4*>(src);
+        else w[u].x = *src;
+        e[u] = (is_v ? a.v_exp : a.k_exp)[at];
+    }
+#pragma unroll
+    for (int u = 0; u < READ_AHEAD; ++u) {
+        const int i = (blockIdx.y * READ_AHEAD + u) * READ_THREADS + threadIdx.x, row = i / per_row, h = row % a.n_kv_heads;
+        if (i >= n) continue;
+        T* dst = reinterpret_cast<T*>(row >= a.n_kv_heads ? a.v_out : a.k_out) + ((long)t * a.n_kv_heads + h) * D + (i - row * per_row) * VEC;
+        const float scale = fx_fp8_scale(e[u]);
+        if constexpr (VEC == 16) put16(dst, w[u], scale);
+        else *dst = from_f32<T>(fx_fp8_float2(w[u].x).x * scale);
     }
 }
 
@@ -215,15 +271,23 @@ __global__ void __launch_bounds__(256) read_spans_kernel(ReadArgs a)
     }
 }
 
-template <typename T> void launch_write(const WriteArgs& a, unsigned blocks, bool whole, cudaStream_t s)
+template <typename T, int DIM> void launch_rows(const WriteArgs& a, cudaStream_t s)
 {
-    const int n = WRITE_WARPS * 32;
-    if (whole && a.head_dim == 64) return fx_launch_pdl(write_kernel<T, 2, true>, blocks, n, 0, s, a);
-    if (whole && a.head_dim == 128) return fx_launch_pdl(write_kernel<T, 4, true>, blocks, n, 0, s, a);
-    if (whole && a.head_dim == 256) return fx_launch_pdl(write_kernel<T, 8, true>, blocks, n, 0, s, a);
-    if (a.head_dim <= 64) return fx_launch_pdl(write_kernel<T, 2, false>, blocks, n, 0, s, a);
-    if (a.head_dim <= 128) return fx_launch_pdl(write_kernel<T, 4, false>, blocks, n, 0, s, a);
-    return fx_launch_pdl(write_kernel<T, 8, false>, blocks, n, 0, s, a);
+    constexpr int NE = DIM * (int)sizeof(T) / 16 > 32 ? DIM / 32 : 16 / (int)sizeof(T), PER = 32 / (DIM / NE) * WRITE_WARPS;
+    const int heads = a.n_heads + 2 * a.n_kv_heads - a.first_head;
+    // (few tokens: every row a block of its own fills the machine sooner)
+    if ((long)a.n_tokens * fx_cdiv(heads, PER) >= 8L * fx_sm_count())
+        fx_launch_pdl(write_rows_kernel<T, DIM, 4>, dim3(a.n_tokens, (unsigned)fx_cdiv(heads, 4 * PER)), WRITE_WARPS * 32, 0, s, a);
+    else
+        fx_launch_pdl(write_rows_kernel<T, DIM, 1>, dim3(a.n_tokens, (unsigned)fx_cdiv(heads, PER)), WRITE_WARPS * 32, 0, s, a);
+}
+template <typename T> void launch_write(const WriteArgs& a, bool whole, cudaStream_t s)
+{
+    if (whole && a.head_dim == 64) return launch_rows<T, 64>(a, s);
+    if (whole && a.head_dim == 128) return launch_rows<T, 128>(a, s);
+    if (whole && a.head_dim == 256) return launch_rows<T, 256>(a, s);
+    const long rows = (long)a.n_tokens * (a.n_heads + 2 * a.n_kv_heads - a.first_head);
+    fx_launch_pdl(write_any_kernel<T>, (unsigned)fx_cdiv(rows, WRITE_WARPS), WRITE_WARPS * 32, 0, s, a);
 }
 
 }  // namespace
@@ -242,13 +306,12 @@ extern "C" int fx_rope_kv_write_fp8(void* qkv, int dtype, long ld, const int* po
     const WriteArgs a = {qkv, ld, positions, token_seq, seq_slot, inv_freq, cos_sin, rotary_dim, pairing, (uint8_t*)k_pages, (uint8_t*)v_pages,
                          (uint8_t*)k_exp, (uint8_t*)v_exp, block_table, n_slots, table_width, page_size, n_pages, n_tokens, n_heads, n_kv_heads,
                          head_dim, inv_freq ? 0 : n_heads, write_cache, status};
-    const long blocks = fx_cdiv((long)n_tokens * (n_heads + 2 * n_kv_heads - a.first_head), WRITE_WARPS);
-    if (blocks > 0x7fffffffL) return FX_ERR_SIZE;
+    if ((long)n_tokens * (n_heads + 2 * n_kv_heads) > 0x7fffffffL || n_heads + 2 * n_kv_heads > 65535) return FX_ERR_SIZE;
     const int es = dtype == FX_F32 ? 4 : 2;
     const bool whole = (!inv_freq || (rotary_dim == head_dim && pairing == 0)) && (head_dim == 64 || head_dim == 128 || head_dim == 256) &&
-                       ld * es % 16 == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)k_pages % 4 == 0 && (uintptr_t)v_pages % 4 == 0;
-    if (dtype == FX_F32) launch_write<float>(a, (unsigned)blocks, whole, (cudaStream_t)stream);
-    else if (dtype == FX_BF16) launch_write<bf16>(a, (unsigned)blocks, whole, (cudaStream_t)stream);
+                       ld * es % 16 == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)k_pages % 8 == 0 && (uintptr_t)v_pages % 8 == 0;
+    if (dtype == FX_F32) launch_write<float>(a, whole, (cudaStream_t)stream);
+    else if (dtype == FX_BF16) launch_write<bf16>(a, whole, (cudaStream_t)stream);
     else return FX_ERR_DTYPE;
     return fx_launch_status();
 }
@@ -273,10 +336,9 @@ extern "C" int fx_read_kv_fp8(const void* k_pages, const void* v_pages, const vo
         else vec ? fx_launch_pdl(read_spans_kernel<bf16, 16>, grid, 256, 0, s, a) : fx_launch_pdl(read_spans_kernel<bf16, 1>, grid, 256, 0, s, a);
         return fx_launch_status();
     }
-    const long n = (long)n_rows * n_kv_heads * 2 * (head_dim / (vec ? 16 : 1));
-    const long most = fx_sm_count() * 8L;
-    const unsigned blocks = (unsigned)(fx_cdiv(n, 256) < most ? fx_cdiv(n, 256) : most);
-    if (dtype == FX_F32) vec ? fx_launch_pdl(read_rows_kernel<float, 16>, blocks, 256, 0, s, a) : fx_launch_pdl(read_rows_kernel<float, 1>, blocks, 256, 0, s, a);
-    else vec ? fx_launch_pdl(read_rows_kernel<bf16, 16>, blocks, 256, 0, s, a) : fx_launch_pdl(read_rows_kernel<bf16, 1>, blocks, 256, 0, s, a);
+    const dim3 blocks(n_rows, (unsigned)fx_cdiv(2L * n_kv_heads * (head_dim / (vec ? 16 : 1)), READ_THREADS * READ_AHEAD));
+    if (blocks.y > 65535u) return FX_ERR_SIZE;
+    if (dtype == FX_F32) vec ? fx_launch_pdl(read_rows_kernel<float, 16>, blocks, READ_THREADS, 0, s, a) : fx_launch_pdl(read_rows_kernel<float, 1>, blocks, READ_THREADS, 0, s, a);
+    else vec ? fx_launch_pdl(read_rows_kernel<bf16, 16>, blocks, READ_THREADS, 0, s, a) : fx_launch_pdl(read_rows_kernel<bf16, 1>, blocks, READ_THREADS, 0, s, a);
     return fx_launch_status();
 }
