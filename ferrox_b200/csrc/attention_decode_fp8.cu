@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag_s;
     __shared__ uint32_t tmem_base_s;
-    __shared__ __align__(8) uint64_t bars_s[2 * STAGES + 2 * S_PLACES + 6];
+    __shared__ __align__(8) uint64_t bars_s[2 * STAGES + 2 * S_PLACES + 5];
     __shared__ __align__(16) float c_s[HB];                              // what a head's raw score is multiplied with
     // of a group: references of its heads, 2^(ref - refw); while they are raised: maxima of its warps, what sums and O shrink by
     __shared__ __align__(16) float ref_s[2][HB], refw_s[2][HB], ratio_s[2][HB], shrink_s[2][HB], shrink_o_s[2][16], most_s[2][2][4][HB];
@@ -169,15 +169,13 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
     auto empty = [&](int s) { return smem_u32(&bars_s[STAGES + s]); };
     auto s_full = [&](int b) { return smem_u32(&bars_s[2 * STAGES + b]); };
     auto s_empty = [&](int b) { return smem_u32(&bars_s[2 * STAGES + S_PLACES + b]); };
-    const uint32_t q_full = smem_u32(&bars_s[2 * STAGES + 2 * S_PLACES]);
-    auto o_done = [&](int j) { return q_full + 8 + 8u * (j & 1); };      // of the group that tile j belongs to, phase j / 2
-    auto drained = [&](int i) { return q_full + 24 + 8u * i; };
+    auto o_done = [&](int j) { return smem_u32(&bars_s[2 * STAGES + 2 * S_PLACES + (j & 1)]); };   // of the group that tile j belongs to, phase j / 2
+    auto drained = [&](int i) { return smem_u32(&bars_s[2 * STAGES + 2 * S_PLACES + 2 + i]); };
 
     if (threadIdx.x == 0) {
         abort_flag_s = 0;
         for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         for (int b = 0; b < S_PLACES; ++b) { mbar_init(s_full(b), 1); mbar_init(s_empty(b), 4); }
-        mbar_init(q_full, 8);
         for (int i = 0; i < 2; ++i) mbar_init(o_done(i), 1);
         for (int i = 0; i < 3; ++i) mbar_init(drained(i), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -206,105 +204,72 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* sm = smem_raw + (base - smem_u32(smem_raw));
 
-    // Tensor memory is taken behind the wait for the kernel before and ahead of the leave for the kernel behind to be set up:
-    // neither can hold it while waiting for this one.
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(&tmem_base_s)), "r"((uint32_t)L::TMEM) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    fx_pdl_trigger();
-    const uint32_t tmem = tmem_base_s;
-
-    if (warp == 0) {
-        // ---------------- producer: lane b asks for the tile's box b of a.box keys ----------------
-        const int n_boxes = TK / a.box;
-        auto page_of = [&](int j) {                                      // of this lane's box in tile j; behind the pool: zeros
-            const int key = (first_tile + j) * TK + lane * a.box;
-            if (lane >= n_boxes || j >= n_tiles || key >= k_end || key + a.box <= k_begin) return -1;
-            return fx_page_of(table, a.table_width, a.n_pages, key, a.page_size);
-        };
-        int page_next = page_of(0), asked = 0;
-        for (int j = 0; j < n_tiles; ++j, ++asked) {
-            const int s = j % STAGES, page = page_next < 0 ? a.n_pages : page_next;
-            const int off = page_next < 0 ? 0 : ((first_tile + j) * TK + lane * a.box) % a.page_size;
-            page_next = page_of(j + 1);
-            bool ok = true;
-            if (j >= STAGES) ok = mbar_wait(empty(s), (uint32_t)(j / STAGES - 1) & 1u, abort_flag);
-            if (__any_sync(0xffffffffu, !ok)) break;
-            if (lane == 0) mbar_expect_tx(full(s), (uint32_t)L::STAGE);
-            __syncwarp();
-            if (lane < n_boxes) {
-                const uint32_t dst = base + s * L::STAGE + lane * a.box * 128;
+    // The producer's warp: lane b asks for a tile's box b of a.box keys.  The first tiles are asked for before the block meets.
+    const int n_boxes = TK / a.box;
+    int page_next = -1, asked = min(STAGES, n_tiles);
+    auto page_of = [&](int j) {                                          // of this lane's box in tile j; behind the pool: zeros
+        const int key = (first_tile + j) * TK + lane * a.box;
+        if (lane >= n_boxes || j >= n_tiles || key >= k_end || key + a.box <= k_begin) return -1;
+        return fx_page_of(table, a.table_width, a.n_pages, key, a.page_size);
+    };
+    auto ask = [&](int j, int found) {
+        const int s = j % STAGES, page = found < 0 ? a.n_pages : found;
+        const int off = found < 0 ? 0 : ((first_tile + j) * TK + lane * a.box) % a.page_size;
+        if (lane == 0) mbar_expect_tx(full(s), (uint32_t)L::STAGE);
+        __syncwarp();
+        if (lane < n_boxes) {
+            const uint32_t dst = base + s * L::STAGE + lane * a.box * 128;
 #pragma unroll
-                for (int sl = 0; sl < SLABS; ++sl) {
-                    tma_load_4d(dst + sl * SLAB, &map_k, sl * 128, off, kvh, page, full(s));
-                    tma_load_4d(dst + (SLABS + sl) * SLAB, &map_v, sl * 128, off, kvh, page, full(s));
-                }
+            for (int sl = 0; sl < SLABS; ++sl) {
+                tma_load_4d(dst + sl * SLAB, &map_k, sl * 128, off, kvh, page, full(s));
+                tma_load_4d(dst + (SLABS + sl) * SLAB, &map_v, sl * 128, off, kvh, page, full(s));
             }
-            __syncwarp();
-        }
-        if (asked < n_tiles)                                             // given up: the copies under way still have to land
-            for (int j = max(0, asked - STAGES); j < asked; ++j) settle(full(j % STAGES), (uint32_t)(j / STAGES) & 1u);
-    } else if (warp == 1) {
-        // ---------------- scores: S(j) as soon as its keys and a place for it are there ----------------
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = idesc8(TK, L::NS, 0, 0);
-            const int steps = (D + 31) / 32;                             // of 32 elements
-            bool ok = mbar_wait(q_full, 0, abort_flag);
-            for (int j = 0; j < n_tiles && ok; ++j) {
-                const int s = j % STAGES, b = j % S_PLACES;
-                ok = mbar_wait(full(s), (uint32_t)(j / STAGES) & 1u, abort_flag);
-                if (ok && j >= S_PLACES) ok = mbar_wait(s_empty(b), (uint32_t)(j / S_PLACES - 1) & 1u, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t k = base + s * L::STAGE, q = base + L::Q_OFF;
-#pragma unroll
-                for (int ks = 0; ks < 4 * SLABS; ++ks)
-                    if (ks < steps)
-                        mma8(tmem + b * L::NS, smem_desc(k + ks / 4 * SLAB + ks % 4 * 32), smem_desc(q + ks / 4 * L::NS * 128 + ks % 4 * 32),
-                             idesc_s, ks != 0);
-                tc_commit(s_full(b));
-            }
-            if (*abort_flag) { tc_commit(drained(2)); settle(drained(2), 0); }   // given up: no product may outlive tensor memory
         }
         __syncwarp();
-    } else {
-        // ---------------- softmax: a key a thread; group g takes the tiles g, g + 2, ... ----------------
-        const int g = (warp - 2) >> 2, sw = (warp - 2) & 3, st = threadIdx.x - 64;
-        const int quad = warp & 3, r = quad * 32 + lane;                 // (tensor memory: a warp may touch lanes 32 (warp % 4) ..)
-        // Where this thread's keys lie: entry `at` of the table and position `off` of a page, moved on by two tiles at a time.
-        // A key's page is looked up two of the group's tiles ahead, its exponents one ahead (-1: the key does not count).
-        const int hop = 2 * TK / a.page_size, hop_off = 2 * TK % a.page_size;
-        int key_p = (first_tile + g) * TK + r, at_p = key_p / a.page_size, off_p = key_p - at_p * a.page_size;
-        int off_e = off_p;
-        auto next_page = [&]() {
-            int page = -1;
-            if (key_p >= k_begin && key_p < k_end && at_p < a.table_width) {
-                page = table[at_p];
-                if (page >= a.n_pages) page = -1;
-            }
-            key_p += 2 * TK; at_p += hop; off_p += hop_off;
-            if (off_p >= a.page_size) { off_p -= a.page_size; ++at_p; }
-            return page;
-        };
-        auto next_exps = [&](int page) {
-            int e = -1;
-            if (page >= 0) {
-                const long at = ((long)page * a.n_kv_heads + kvh) * a.page_size + off_e;
-                e = (int)a.k_exp[at] | (int)a.v_exp[at] << 8;
-            }
-            off_e += hop_off;
-            if (off_e >= a.page_size) off_e -= a.page_size;
-            return e;
-        };
-        int page_next = next_page();
-        int exps_next = next_exps(page_next);
-        page_next = next_page();
+    };
+    if (warp == 0) {
+        int first[STAGES];
+#pragma unroll
+        for (int j = 0; j < STAGES; ++j) first[j] = page_of(j);
+#pragma unroll
+        for (int j = 0; j < STAGES; ++j)
+            if (j < n_tiles) ask(j, first[j]);
+        page_next = page_of(STAGES);
+    }
 
+    // The softmax threads: a key a thread; group g takes the tiles g, g + 2, ...
+    const int g = (warp - 2) >> 2, sw = (warp - 2) & 3, st = threadIdx.x - 64;
+    const int quad = warp & 3, r = quad * 32 + lane;                     // (tensor memory: a warp may touch lanes 32 (warp % 4) ..)
+    // Where this thread's keys lie: entry `at` of the table and position `off` of a page, moved on by two tiles at a time.
+    // A key's page is looked up two of the group's tiles ahead, its exponents one ahead (-1: the key does not count).
+    const int hop = 2 * TK / a.page_size, hop_off = 2 * TK % a.page_size;
+    int key_p = (first_tile + g) * TK + r, at_p = key_p / a.page_size, off_p = key_p - at_p * a.page_size;
+    int off_e = off_p;
+    auto next_page = [&]() {
+        int page = -1;
+        if (key_p >= k_begin && key_p < k_end && at_p < a.table_width) {
+            page = table[at_p];
+            if (page >= a.n_pages) page = -1;
+        }
+        key_p += 2 * TK; at_p += hop; off_p += hop_off;
+        if (off_p >= a.page_size) { off_p -= a.page_size; ++at_p; }
+        return page;
+    };
+    auto next_exps = [&](int page) {
+        int e = -1;
+        if (page >= 0) {
+            const long at = ((long)page * a.n_kv_heads + kvh) * a.page_size + off_e;
+            e = (int)a.k_exp[at] | (int)a.v_exp[at] << 8;
+        }
+        off_e += hop_off;
+        if (off_e >= a.page_size) off_e -= a.page_size;
+        return e;
+    };
+    int exps_next = -1;
+    if (warp >= 2) {
+        page_next = next_page();
+        exps_next = next_exps(page_next);
+        page_next = next_page();
         // the queries in parts: a warp a head; rows of the columns that no head has are zeros
         for (int i = st; i < SLABS * L::NS * 8; i += 2 * NSOFT) reinterpret_cast<uint4*>(sm + L::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
         if (st < 2 * HB) { (&ref_s[0][0])[st] = NO_REF; (&refw_s[0][0])[st] = NO_REF; (&ratio_s[0][0])[st] = 1.f; }
@@ -341,9 +306,54 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        any_of_soft(false);
-        if (lane == 0) mbar_arrive(q_full);
+    }
 
+    // Tensor memory is taken behind the wait for the kernel before and ahead of the leave for the kernel behind to be set up:
+    // neither can hold it while waiting for this one.
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&tmem_base_s)), "r"((uint32_t)L::TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    fx_pdl_trigger();
+    const uint32_t tmem = tmem_base_s;
+
+    if (warp == 0) {
+        // ---------------- producer: the other tiles, each when its stage is free ----------------
+        for (int j = STAGES; j < n_tiles; ++j, ++asked) {
+            const bool ok = mbar_wait(empty(j % STAGES), (uint32_t)(j / STAGES - 1) & 1u, abort_flag);
+            if (__any_sync(0xffffffffu, !ok)) break;
+            ask(j, page_next);
+            page_next = page_of(j + 1);
+        }
+    } else if (warp == 1) {
+        // ---------------- scores: S(j) as soon as its keys and a place for it are there ----------------
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = idesc8(TK, L::NS, 0, 0);
+            const int steps = (D + 31) / 32;                             // of 32 elements
+            bool ok = true;
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                const int s = j % STAGES, b = j % S_PLACES;
+                ok = mbar_wait(full(s), (uint32_t)(j / STAGES) & 1u, abort_flag);
+                if (ok && j >= S_PLACES) ok = mbar_wait(s_empty(b), (uint32_t)(j / S_PLACES - 1) & 1u, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t k = base + s * L::STAGE, q = base + L::Q_OFF;
+#pragma unroll
+                for (int ks = 0; ks < 4 * SLABS; ++ks)
+                    if (ks < steps)
+                        mma8(tmem + b * L::NS, smem_desc(k + ks / 4 * SLAB + ks % 4 * 32), smem_desc(q + ks / 4 * L::NS * 128 + ks % 4 * 32),
+                             idesc_s, ks != 0);
+                tc_commit(s_full(b));
+            }
+            if (*abort_flag) { tc_commit(drained(2)); settle(drained(2), 0); }   // given up: no product may outlive tensor memory
+        }
+        __syncwarp();
+    } else {
+        // ---------------- softmax ----------------
         constexpr uint32_t idesc_o = idesc8(128, L::NO, 1, 1);
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), col_o = L::COLS_O + g * SLABS * L::NO;
         float l[HB];
@@ -490,11 +500,20 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
         // ---- the run's result: this thread has element r of every slab, its group half of the heads, over both groups' tiles ----
         bool ok = fine && mbar_wait(o_done(n_tiles - 1), (uint32_t)((n_tiles - 1) >> 1) & 1u, abort_flag);
         tc_fence_after();
+        // HB sums over 32 lanes: half of what a lane has goes to its partner, until each has one head's; the rest as ever
 #pragma unroll
-        for (int h = 0; h < HB; ++h) {
-            const float sum = warp_sum(l[h]);
-            if (lane == 0) sum_s[g][sw][h] = sum;
+        for (int n = HB / 2, o = 16; n > 0; n >>= 1, o >>= 1) {
+            const bool up = lane & o;
+#pragma unroll
+            for (int h = 0; h < n; ++h) {
+                const float give = up ? l[h] : l[h + n], keep = up ? l[h + n] : l[h];
+                l[h] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
         }
+#pragma unroll
+        for (int o = 16 / HB; o > 0; o >>= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+        // (lane's bits from the highest on choose the upper or lower half: they are the head's)
+        if (lane % (32 / HB) == 0) sum_s[g][sw][lane / (32 / HB)] = l[0];
         if (!any_of_soft(!ok)) {
             const bool two = n_tiles > 1;
 #pragma unroll
@@ -543,39 +562,56 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
     tc_fence_before();
     __syncthreads();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::TMEM));
-    if (threadIdx.x == 0 && abort_flag_s && a.status) atomicExch(a.status, STATUS_TC_TIMEOUT);
+    if (threadIdx.x == 0 && abort_flag_s) {
+        for (int j = max(0, asked - STAGES); j < asked; ++j) settle(full(j % STAGES), (uint32_t)(j / STAGES) & 1u);   // (copies still under way land first)
+        if (a.status) atomicExch(a.status, STATUS_TC_TIMEOUT);
+    }
 }
 
-// The runs of a (token, head): sum_s l_s 2^(m_s - m) mean_s / sum_s l_s 2^(m_s - m), in the order of the runs.
-constexpr int MERGE_THREADS = 128, MAX_RUNS = 128;
+// The runs of a (token, head): sum_s l_s 2^(m_s - m) mean_s / sum_s l_s 2^(m_s - m).  A warp takes every eighth run, a lane four
+// elements at a time, and the warps' sums are added up in their order.  Bound by latency: with a thread an element that walks all
+// runs the 74 of one long request took longer to add up than an eighth of the attention itself.
+constexpr int MERGE_WARPS = 8, MAX_RUNS = 128, MERGE_DIM = 256;
 
-template <typename T> __global__ void __launch_bounds__(MERGE_THREADS) decode_fp8_merge_kernel(const __grid_constant__ Args a)
+template <typename T> __global__ void __launch_bounds__(MERGE_WARPS * 32) decode_fp8_merge_kernel(const __grid_constant__ Args a)
 {
-    __shared__ float w_s[MAX_RUNS], top_s[MERGE_THREADS / 32];
+    __shared__ float w_s[MAX_RUNS], top_s[MERGE_WARPS], sum_s[MERGE_WARPS];
+    __shared__ __align__(16) float acc_s[MERGE_WARPS][MERGE_DIM];
     fx_pdl_wait();
-    const int n = a.n_splits, D = a.head_dim, h = blockIdx.y, lane = threadIdx.x & 31;
+    const int n = a.n_splits, D = a.head_dim, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tkn = a.tokens ? a.tokens[blockIdx.x] : blockIdx.x;
     const long at = ((long)blockIdx.x * a.n_heads + h) * n;
     const bool mine = (int)threadIdx.x < n;
     const float m = mine ? a.part_ml[2 * (at + threadIdx.x)] : NO_REF, l = mine ? a.part_ml[2 * (at + threadIdx.x) + 1] : 0.f;
     const float top = warp_max(m);
-    if (lane == 0) top_s[threadIdx.x >> 5] = top;
+    if (lane == 0) top_s[warp] = top;
     __syncthreads();
     float ref = top_s[0];
-    for (int i = 1; i < MERGE_THREADS / 32; ++i) ref = fmaxf(ref, top_s[i]);
-    if (mine) w_s[threadIdx.x] = l == 0.f ? 0.f : l * exp2f(m - ref);
+#pragma unroll
+    for (int i = 1; i < MERGE_WARPS; ++i) ref = fmaxf(ref, top_s[i]);
+    const float w = l == 0.f ? 0.f : l * exp2f(m - ref), part = warp_sum(w);
+    if (mine) w_s[threadIdx.x] = w;
+    if (lane == 0) sum_s[warp] = part;
     __syncthreads();
     float sum = 0.f;
-    for (int i = 0; i < n; ++i) sum += w_s[i];
-    for (int e = threadIdx.x; e < D; e += MERGE_THREADS) {
-        float acc = 0.f;
-        for (int i0 = 0; i0 < n; i0 += 8) {
-            float o[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = i0 + i < n && w_s[i0 + i] != 0.f ? a.part_o[(at + i0 + i) * D + e] : 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) if (i0 + i < n) acc = fmaf(w_s[i0 + i], o[i], acc);
+    for (int i = 0; i < MERGE_WARPS; ++i) sum += sum_s[i];
+    for (int e = 4 * lane; e < D; e += 128) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = warp; i < n; i += MERGE_WARPS) {
+            const float wi = w_s[i];
+            if (wi == 0.f) continue;                                     // (a run without keys has written no values)
+            const float4 o = *reinterpret_cast<const float4*>(a.part_o + (at + i) * D + e);
+            acc.x = fmaf(wi, o.x, acc.x); acc.y = fmaf(wi, o.y, acc.y); acc.z = fmaf(wi, o.z, acc.z); acc.w = fmaf(wi, o.w, acc.w);
         }
+        *reinterpret_cast<float4*>(&acc_s[warp][e]) = acc;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < D; e += MERGE_WARPS * 32) {
+        float acc = 0.f;
+#pragma unroll
+        for (int i = 0; i < MERGE_WARPS; ++i) acc += acc_s[i][e];
         reinterpret_cast<T*>(a.out)[(long)tkn * a.ldo + (long)h * D + e] = from_f32<T>(sum == 0.f ? 0.f : acc / sum);
     }
 }
@@ -610,7 +646,7 @@ template <typename T> int run(const CUtensorMap& mk, const CUtensorMap& mv, Args
     if (hb == 8) rc = a.head_dim <= 128 ? launch<T, 8, 1>(mk, mv, a, grid, s) : launch<T, 8, 2>(mk, mv, a, grid, s);
     else rc = a.head_dim <= 128 ? launch<T, 4, 1>(mk, mv, a, grid, s) : launch<T, 4, 2>(mk, mv, a, grid, s);
     if (rc || a.n_splits == 1) return rc;
-    fx_launch_pdl(decode_fp8_merge_kernel<T>, dim3(n_tokens, a.n_heads), MERGE_THREADS, 0, s, a);
+    fx_launch_pdl(decode_fp8_merge_kernel<T>, dim3(n_tokens, a.n_heads), MERGE_WARPS * 32, 0, s, a);
     return fx_launch_status();
 }
 
