@@ -174,10 +174,123 @@ static PyObject* set_slow(PyObject* module, PyObject* args)
     Py_RETURN_NONE;
 }
 
+// ---- operands looked at in one go ------------------------------------------------------------------------------------
+// An entry point of a dozen tensors costs more in questions about them (50 to 150 ns each) than in its launch.  look(spec,
+// tensors...) asks for each tensor once, by DLPack's exchange interface, and compares it with what the call needs; what is not
+// so, or what the interface does not give, is left to the caller, who names the error.
+//
+// spec: a word a tensor: its type (e: e4m3, u: unsigned byte, i: 32-bit integer, f: 32-bit float, x: 32-bit float or bfloat16,
+// the same for all of them), then a letter a dimension; the same letter is the same size wherever it stands.  Tensors are
+// contiguous, or with ~ at the word's end rows of contiguous elements.  ? at the beginning: the tensor may be None.
+// Returns None, or (device, current stream there, x's code, addresses, sizes of the letters in their order of appearance, -1
+// for one of an absent tensor, row strides of the words with ~).
+typedef struct { int32_t device_type, device_id; } DlDevice;
+typedef struct { uint8_t code, bits; uint16_t lanes; } DlType;
+typedef struct { void* data; DlDevice device; int32_t ndim; DlType dtype; int64_t *shape, *strides; uint64_t byte_offset; } DlTensor;
+typedef struct {
+    struct { uint32_t major, minor; } version;
+    void *prev, *allocate, *managed_from, *managed_to;
+    int (*tensor_from)(void* object, DlTensor* out);
+    int (*stream_of)(int32_t device_type, int32_t device_id, void** out);
+} DlExchange;
+enum { DL_CUDA = 2, DL_INT = 0, DL_UINT = 1, DL_FLOAT = 2, DL_BFLOAT = 4, DL_E4M3 = 10, MAX_LOOKED = 16, MAX_LETTERS = 16 };
+static const DlExchange* exchange;
+
+static int type_fits(char want, DlType t, int* x_code)
+{
+    if (t.lanes != 1) return 0;
+    switch (want) {
+        case 'e': return t.code == DL_E4M3 && t.bits == 8;
+        case 'u': return t.code == DL_UINT && t.bits == 8;
+        case 'i': return t.code == DL_INT && t.bits == 32;
+        case 'f': return t.code == DL_FLOAT && t.bits == 32;
+        default: {
+            const int code = t.code == DL_FLOAT && t.bits == 32 ? 0 : t.code == DL_BFLOAT && t.bits == 16 ? 1 : -1;
+            if (code < 0 || (*x_code >= 0 && *x_code != code)) return 0;
+            *x_code = code;
+            return 1;
+        }
+    }
+}
+
+static PyObject* look(PyObject* module, PyObject* const* args, Py_ssize_t n)
+{
+    if (!exchange || n < 2 || n > MAX_LOOKED + 1) Py_RETURN_NONE;
+    const char* c = PyUnicode_AsUTF8(args[0]);
+    if (!c) return NULL;
+    W address[MAX_LOOKED], size[MAX_LETTERS], row[MAX_LOOKED];
+    char letter[MAX_LETTERS];
+    int letters = 0, rows = 0, device = -1, x_code = -1;
+    for (Py_ssize_t i = 1; i < n; ++i) {
+        while (*c == ' ') ++c;
+        const int absent = *c == '?' && args[i] == Py_None;
+        if (*c == '?') ++c;
+        DlTensor t = {0};
+        const char type = *c++;
+        if (!absent) {
+            if (!type || exchange->tensor_from(args[i], &t)) { PyErr_Clear(); Py_RETURN_NONE; }
+            if (t.device.device_type != DL_CUDA || (device >= 0 && t.device.device_id != device) || !type_fits(type, t.dtype, &x_code)) Py_RETURN_NONE;
+            device = t.device.device_id;
+        }
+        address[i - 1] = absent ? 0 : (W)(uintptr_t)t.data + (W)t.byte_offset;
+        int dims = 0;
+        for (; *c && *c != ' ' && *c != '~'; ++c, ++dims) {
+            int k = 0;
+            while (k < letters && letter[k] != *c) ++k;
+            if (k == letters) {
+                if (letters == MAX_LETTERS) Py_RETURN_NONE;
+                letter[letters] = *c;
+                size[letters++] = -1;
+            }
+            if (absent) continue;
+            if (dims >= t.ndim || (size[k] >= 0 && size[k] != t.shape[dims])) Py_RETURN_NONE;
+            size[k] = t.shape[dims];
+        }
+        const int by_rows = *c == '~';
+        if (by_rows) ++c;
+        if (absent) { if (by_rows) row[rows++] = 0; continue; }
+        if (dims != t.ndim || (by_rows && dims != 2)) Py_RETURN_NONE;
+        W step = 1;
+        int empty = 0;
+        for (int d = 0; d < dims; ++d) empty |= t.shape[d] == 0;
+        for (int d = dims - 1; d >= by_rows; --d) {
+            if (!empty && t.strides && t.shape[d] > 1 && t.strides[d] != step) Py_RETURN_NONE;
+            step *= t.shape[d];
+        }
+        if (by_rows) {                                       // (a single row's stride says nothing)
+            row[rows] = t.shape[0] > 1 && t.strides ? t.strides[0] : t.shape[1];
+            if (row[rows++] < 0) Py_RETURN_NONE;
+        }
+    }
+    void* stream = NULL;
+    if (device < 0 || exchange->stream_of(DL_CUDA, device, &stream)) { PyErr_Clear(); Py_RETURN_NONE; }
+    const Py_ssize_t total = 3 + (n - 1) + letters + rows;
+    PyObject* out = PyTuple_New(total);
+    if (!out) return NULL;
+    for (Py_ssize_t i = 0; i < total; ++i) {
+        const Py_ssize_t a = i - 3, l = a - (n - 1), r = l - letters;
+        PyObject* v = PyLong_FromLongLong(i == 0 ? device : i == 1 ? (W)(uintptr_t)stream : i == 2 ? x_code : a < n - 1 ? address[a] : l < letters ? size[l] : row[r]);
+        if (!v) { Py_DECREF(out); return NULL; }
+        PyTuple_SET_ITEM(out, i, v);
+    }
+    return out;
+}
+
+// exchange(capsule): DLPack's exchange interface of the tensors' library; whether it is of a kind that is read here
+static PyObject* set_exchange(PyObject* module, PyObject* capsule)
+{
+    const DlExchange* e = PyCapsule_GetPointer(capsule, "dlpack_exchange_api");
+    if (!e) return NULL;
+    exchange = e->version.major == 1 && e->tensor_from && e->stream_of ? e : NULL;
+    return PyBool_FromLong(exchange != NULL);
+}
+
 static PyMethodDef methods[] = {
     {"ptr", ptr, METH_O, "A CUDA tensor's address, None for None."},
     {"rows", rows, METH_O, "The row stride of a two-dimensional tensor with contiguous rows."},
     {"set_slow", set_slow, METH_VARARGS, "set_slow(ptr, rows): what takes the arguments that these do not."},
+    {"look", (PyCFunction)(void (*)(void))look, METH_FASTCALL, "look(spec, tensors...): what a call needs to know of them, or None."},
+    {"set_exchange", set_exchange, METH_O, "set_exchange(capsule): where look finds the tensors' descriptions."},
     {"bind", bind, METH_VARARGS, "bind(address, codes): the C entry point there as a callable, or None."},
     {NULL, NULL, 0, NULL},
 };

@@ -345,6 +345,62 @@ def _use_extension():
         _ptr, _rows = m.ptr, m.rows
 
 
+@functools.lru_cache(maxsize=None)
+def _look():
+    """``look`` of the extension module (csrc/py/fastcall.c), or what says None to everything."""
+    m, api = fastcall.module(), getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+    return m.look if m is not None and api is not None and m.set_exchange(api) else lambda *a: None
+
+
+_LOOK_TYPES = {"e": (torch.float8_e4m3fn,), "u": (torch.uint8,), "i": (torch.int32,), "f": (torch.float32,), "x": (torch.float32, torch.bfloat16)}
+
+
+def _operands(name, spec, labels, *tensors):
+    """What a call needs to know of its tensors: (device, current stream, element code, addresses, sizes, row strides) by ``spec``
+    (``look`` of csrc/py/fastcall.c says how it reads); tensors that are not so are refused by their labels."""
+    found = _look()(spec, *tensors)
+    if found is None:
+        found = _operands_slowly(name, spec, labels, tensors)
+    if found[0] != torch._C._cuda_getDevice():
+        raise KernelError(f"{name}: operands on cuda:{found[0]}, which is not the current device")
+    return found
+
+
+def _operands_slowly(name, spec, labels, tensors):
+    sizes, where, addresses, rows, device, x_type = {}, {}, [], [], None, None
+    for word, label, t in zip(spec.split(), labels, tensors):
+        optional, word = word[0] == "?", word.lstrip("?")
+        by_rows, kind, dims = word[-1] == "~", word[0], word[1:].rstrip("~")
+        for d in dims:
+            sizes.setdefault(d, -1)
+        if t is None and optional:
+            addresses.append(0)
+            rows += [0] * by_rows
+            continue
+        shape = "[" + ", ".join(f"{d}" if sizes[d] < 0 else f"{sizes[d]} ({d} of {where[d]})" for d in dims) + "]"
+        wanted = f"{name}: {label} is a {' or '.join(str(x)[6:] for x in _LOOK_TYPES[kind])} tensor {shape}, " \
+                 f"{'with contiguous rows' if by_rows else 'contiguous'}"
+        if not isinstance(t, torch.Tensor):
+            raise KernelError(f"{wanted}: found {type(t).__name__}")
+        bad = (t.dtype not in _LOOK_TYPES[kind] or t.dim() != len(dims) or any(sizes[d] not in (-1, n) for d, n in zip(dims, t.shape))
+               or (kind == "x" and x_type not in (None, t.dtype)))
+        for d, n in zip(dims, t.shape):
+            bad = bad or sizes[d] not in (-1, n)         # (a letter twice in one word)
+            sizes[d], where[d] = n, where.get(d, label)
+        if bad or not (t.stride(1) == 1 or t.shape[1] <= 1 if by_rows else t.is_contiguous()):
+            raise KernelError(f"{wanted}{f' of type {x_type}' if kind == 'x' and x_type else ''}: found {t.dtype} {tuple(t.shape)} with "
+                              f"strides {t.stride()}")
+        if not t.is_cuda or device not in (None, t.device):
+            raise KernelError(f"{name}: an operand on {t.device} ({label}): kernels take tensors of one CUDA device")
+        device, x_type = t.device, t.dtype if kind == "x" else x_type
+        addresses.append(t.data_ptr())
+        if by_rows:
+            rows.append(t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    if device is None:
+        raise KernelError(f"{name}: no operands")
+    return (device.index, _current_stream(device.index), -1 if x_type is None else _CODES[x_type], *addresses, *sizes.values(), *rows)
+
+
 def upload(values, device) -> torch.Tensor:
     """A numpy array's copy on ``device``, ordered on the current stream without waiting for it: by way of pinned memory,
     which torch's allocator hands out again only when the copy is done.  (A pageable copy waits for everything the
@@ -2005,42 +2061,19 @@ FP8_MAX_DIM = 256                 # elements of a head
 FP8_LARGEST, FP8_MIN_EXP, FP8_NAN = 448.0, -119, 255
 
 
-_E4M3, _U8, _I32 = torch.float8_e4m3fn, torch.uint8, torch.int32
+_CACHE_FP8 = ("k_pages", "v_pages", "k_exp", "v_exp", "block_table")
+_STEP = ("positions", "token_seq", "seq_slot")
 
 
-def _on_current_device(name, first, *others):
-    """A launch goes to the current device: operands elsewhere are refused."""
-    device = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != device:
-            raise KernelError(f"{name}: an operand on {t.device}, another on {first.device}")
-    if device < 0 or device != torch.cuda.current_device():
-        raise KernelError(f"{name}: an operand on {first.device}, which is not the current CUDA device")
+def _check_fp8(name, found, page_size, n_kv_heads, head_dim):
+    """The sizes of an 8-bit cache, which come first in ``found``: pages, kv heads, page, head size."""
+    N, G, P, D = found
+    if P != page_size or N == 0 or not 0 < D <= FP8_MAX_DIM or (n_kv_heads is not None and (G != n_kv_heads or D != head_dim)):
+        raise KernelError(f"{name}: pages of {page_size} positions, {n_kv_heads or 'any'} heads of {head_dim or 'up to'} {'' if head_dim else FP8_MAX_DIM}"
+                          f" elements (at most {FP8_MAX_DIM}), at least one: found [{N}, {G}, {P}, {D}]")
 
 
-def _int32(name, what, *tensors):
-    for t in tensors:
-        if t is not None and (t.dtype is not _I32 or not t.is_contiguous()):
-            raise KernelError(f"{name}: {what} are contiguous int32, found {t.dtype} with strides {t.stride()}")
-
-
-def _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size):
-    """Checks an 8-bit cache; its (pages, kv heads, head size, slots, pages of a request)."""
-    shape, exp_shape, table_shape = k_pages.shape, k_exp.shape, block_table.shape
-    if not (k_pages.dtype is _E4M3 and v_pages.dtype is _E4M3 and k_exp.dtype is _U8 and v_exp.dtype is _U8):
-        raise KernelError(f"{name}: pages are float8_e4m3fn and their exponents uint8, found {k_pages.dtype}, {v_pages.dtype}, {k_exp.dtype}, {v_exp.dtype}")
-    if len(shape) != 4 or v_pages.shape != shape or exp_shape != shape[:3] or v_exp.shape != exp_shape or shape[2] != page_size:
-        raise KernelError(f"{name}: pages [pages, kv heads, {page_size}, head size] and exponents [pages, kv heads, {page_size}], found "
-                          f"{tuple(shape)}, {tuple(v_pages.shape)}, {tuple(k_exp.shape)}, {tuple(v_exp.shape)}")
-    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and k_exp.is_contiguous() and v_exp.is_contiguous()):
-        raise KernelError(f"{name}: pages and exponents are contiguous")
-    if len(table_shape) != 2 or table_shape[1] == 0 or block_table.dtype is not _I32 or not block_table.is_contiguous():
-        raise KernelError(f"{name}: the block table is contiguous int32 [slots, pages of a request], found {block_table.dtype} {tuple(table_shape)} "
-                          f"with strides {block_table.stride()}")
-    n_pages, G, _, D = shape
-    if not 0 < D <= FP8_MAX_DIM or n_pages == 0:
-        raise KernelError(f"{name}: heads of 1 to {FP8_MAX_DIM} elements and at least one page, found {tuple(shape)}")
-    return n_pages, G, D, table_shape[0], table_shape[1]
+_WRITE_FP8 = "eNGPD eNGPD uNGP uNGP iSW iT iT iB xTQ~ ?fF ?fThc ?iZ"
 
 
 def rope_kv_write_fp8(qkv, positions, token_seq, seq_slot, inv_freq, rotary_dim, k_pages, v_pages, k_exp, v_exp, block_table,
@@ -2050,52 +2083,34 @@ def rope_kv_write_fp8(qkv, positions, token_seq, seq_slot, inv_freq, rotary_dim,
     are written.  ``k_pages``, ``v_pages`` float8_e4m3fn [pages, kv heads, page, head_dim] and ``k_exp``, ``v_exp`` uint8 [pages, kv
     heads, page]: element i of a position stands for e4m3_i * 2^(E - 127), with e = E - 127 the smallest whole number for which the
     row's largest |x| is at most 448 * 2^e (at least -119), and e4m3_i = x_i / 2^e rounded to nearest, ties to even (numbers beyond
-    240 * 2^120 as that: the next one is infinite in 32 bits).  A row with an
-    element that is infinite or no number gets E = 255 and reads as NaN.  A position without a page, or outside its table, is
-    written nowhere and raises ``status`` 2.  Positions of a call are distinct."""
+    240 * 2^120 as that: the next one is infinite in 32 bits).  A row with an element that is infinite or no number gets E = 255 and
+    reads as NaN.  A position without a page, or outside its table, is written nowhere and raises ``status`` 2.  Positions of a
+    request are distinct."""
     name = "rope_kv_write_fp8"
-    n_pages, G, D, n_slots, width = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
-    shape = qkv.shape
-    T = shape[0]
-    if G != n_kv_heads or D != head_dim or len(shape) != 2 or shape[1] < (n_heads + 2 * n_kv_heads) * head_dim:
-        raise KernelError(f"{name}: rows of {n_heads} + 2 * {n_kv_heads} heads of {head_dim} for pages of {G} heads of {D}, found {tuple(qkv.shape)}")
-    if positions.numel() != T or token_seq.numel() != T:
-        raise KernelError(f"{name}: a position and an entry for each of {T} rows, found {positions.numel()} and {token_seq.numel()}")
-    if inv_freq is not None and (inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or 2 * inv_freq.numel() < rotary_dim):
-        raise KernelError(f"{name}: {rotary_dim // 2} contiguous 32-bit frequencies, found {inv_freq.dtype} {tuple(inv_freq.shape)}")
-    if cos_sin is not None and (cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.numel() < T * rotary_dim):
-        raise KernelError(f"{name}: contiguous 32-bit (cos, sin) pairs [{T}, {rotary_dim // 2}, 2], found {cos_sin.dtype} {tuple(cos_sin.shape)}")
-    _int32(name, "positions, entries and slots", positions, token_seq, seq_slot)
-    _on_current_device(name, qkv, positions, token_seq, seq_slot, inv_freq, cos_sin, k_pages, v_pages, k_exp, v_exp, block_table, status)
-    call("fx_rope_kv_write_fp8", _ptr(qkv), code(qkv), _rows(qkv), _ptr(positions), _ptr(token_seq), _ptr(seq_slot), _ptr(inv_freq),
-         _ptr(cos_sin), rotary_dim, int(pairing), _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table),
-         n_slots, width, page_size, n_pages, T, n_heads, n_kv_heads, head_dim, int(write_cache), _ptr(status),
-         stream if stream is not None else stream_ptr())
+    (_, now, x, kp, vp, kep, vep, tp, pp, sp, lp, qp, fp, cp, zp, N, G, P, D, S, W, T, _, Q, F, h, c, _, ld) = _operands(
+        name, _WRITE_FP8, _CACHE_FP8 + _STEP + ("qkv", "inv_freq", "cos_sin", "status"), k_pages, v_pages, k_exp, v_exp, block_table,
+        positions, token_seq, seq_slot, qkv, inv_freq, cos_sin, status)
+    _check_fp8(name, (N, G, P, D), page_size, n_kv_heads, head_dim)
+    half = rotary_dim // 2
+    if n_heads < 0 or Q < (n_heads + 2 * G) * D or W == 0 or (inv_freq is not None and F < half) or (cos_sin is not None and (h != half or c != 2)):
+        raise KernelError(f"{name}: rows of {n_heads} + 2 * {G} heads of {D}, {half} frequencies, (cos, sin) pairs [{T}, {half}, 2]: found rows of "
+                          f"{Q}, {F} frequencies, pairs [{T}, {h}, {c}], {W} pages a request")
+    call("fx_rope_kv_write_fp8", qp, x, ld, pp, sp, lp, fp, cp, rotary_dim, int(pairing), kp, vp, kep, vep, tp, S, W, page_size, N, T, n_heads,
+         G, D, int(write_cache), zp, stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
 
 
-def _read_kv_fp8(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, spans, n_rows, k_out,
-                 v_out, stream):
-    n_pages, G, D, n_slots, width = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
-    shape = (n_rows, G, D) if spans is None else (n_rows // page_size, G, page_size, D)
-    if k_out.dtype != v_out.dtype or k_out.shape != shape or v_out.shape != shape or not (k_out.is_contiguous() and v_out.is_contiguous()):
-        raise KernelError(f"{name}: two contiguous results {tuple(shape)} of one type, found {tuple(k_out.shape)} {k_out.dtype} and "
-                          f"{tuple(v_out.shape)} {v_out.dtype}")
-    _int32(name, "positions, entries, slots and spans", positions, token_seq, seq_slot, spans)
-    _on_current_device(name, k_pages, v_pages, k_exp, v_exp, block_table, positions, token_seq, seq_slot, spans, k_out, v_out)
-    call("fx_read_kv_fp8", _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table), n_slots,
-         width, page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot), _ptr(spans),
-         spans.shape[0] if spans is not None else 0, n_rows, _ptr(k_out), _ptr(v_out), code(k_out), G, D,
-         stream if stream is not None else stream_ptr())
+_READ_FP8, _READ_FP8_SPANS = "eNGPD eNGPD uNGP uNGP iSW iT iT iB xTGD xTGD", "eNGPD eNGPD uNGP uNGP iSW in4 iB xMGPD xMGPD"
 
 
 def read_kv_fp8(k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, k_out, v_out, stream=None):
     """What an 8-bit cache holds at the given positions: ``k_out``, ``v_out`` [tokens, kv heads, head_dim] (bfloat16, in which every
     value is exact, or float32).  A position without a page reads as 0."""
-    T = positions.numel()
-    if token_seq.numel() != T:
-        raise KernelError(f"read_kv_fp8: an entry for each of {T} positions, found {token_seq.numel()}")
-    _read_kv_fp8("read_kv_fp8", k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, None, T, k_out,
-                 v_out, stream)
+    (_, now, x, kp, vp, kep, vep, tp, pp, sp, lp, ko, vo, N, G, P, D, S, W, T, _) = _operands(
+        "read_kv_fp8", _READ_FP8, _CACHE_FP8 + _STEP + ("k_out", "v_out"), k_pages, v_pages, k_exp, v_exp, block_table, positions, token_seq,
+        seq_slot, k_out, v_out)
+    _check_fp8("read_kv_fp8", (N, G, P, D), page_size, None, None)
+    call("fx_read_kv_fp8", kp, vp, kep, vep, tp, S, W, page_size, N, pp, sp, lp, 0, 0, T, ko, vo, x, G, D,
+         stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
 
 
 def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, spans, n_rows, seq_slot, k_out, v_out, stream=None):
@@ -2103,32 +2118,36 @@ def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, sp
     page, kv heads, page, head_dim].  ``spans``: int32 [n, 4] rows of (entry, first position, end, first row), first positions and
     rows multiples of the page, the rows in order and without gaps up to ``n_rows``.  What lies behind a stretch's end in its last
     page is 0, and so is a page that its request does not have."""
-    if n_rows % page_size or n_rows < 0 or spans.dim() != 2 or spans.shape[1] != 4 or (n_rows and not spans.shape[0]):
-        raise KernelError(f"read_kv_fp8_spans: spans [n, 4] over a multiple of {page_size} rows, found {tuple(spans.shape)} over {n_rows}")
-    _read_kv_fp8("read_kv_fp8_spans", k_pages, v_pages, k_exp, v_exp, block_table, page_size, None, None, seq_slot, spans, n_rows, k_out,
-                 v_out, stream)
+    name = "read_kv_fp8_spans"
+    (_, now, x, kp, vp, kep, vep, tp, np_, lp, ko, vo, N, G, P, D, S, W, n, four, _, M) = _operands(
+        name, _READ_FP8_SPANS, _CACHE_FP8 + ("spans", "seq_slot", "k_out", "v_out"), k_pages, v_pages, k_exp, v_exp, block_table, spans, seq_slot,
+        k_out, v_out)
+    _check_fp8(name, (N, G, P, D), page_size, None, None)
+    if n_rows != M * P or four != 4 or (M and not n):
+        raise KernelError(f"{name}: spans [n, 4] over {n_rows} rows, {M} pages of {P}: found [{n}, {four}]")
+    call("fx_read_kv_fp8", kp, vp, kep, vep, tp, S, W, page_size, N, 0, 0, lp, np_, n, n_rows, ko, vo, x, G, D,
+         stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
 
 
-def _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, tokens, out,
-                         n_heads, n_kv_heads, head_dim, window, scale, softcap):
-    n_pages, G, D, n_slots, width = _fp8_cache(name, k_pages, v_pages, k_exp, v_exp, block_table, page_size)
-    T, qs, os = positions.numel(), q.shape, out.shape
-    if G != n_kv_heads or D != head_dim or n_heads < 1 or n_heads % n_kv_heads:
-        raise KernelError(f"{name}: {n_heads} heads on {n_kv_heads} of {head_dim} for pages of {G} heads of {D}")
+_ATTEND_FP8 = "eNGPD eNGPD uNGP uNGP iSW iT iT iB xTQ~ xTO~ ?iZ ?in"
+
+
+def _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, status, tokens, out,
+                           n_heads, n_kv_heads, head_dim, window, scale, softcap):
+    found = _operands(name, _ATTEND_FP8, _CACHE_FP8 + _STEP + ("q", "out", "status", "tokens"), k_pages, v_pages, k_exp, v_exp, block_table, positions,
+                      token_seq, seq_slot, q, out, status, tokens)
+    _check_fp8(name, found[15:19], page_size, n_kv_heads, head_dim)
     need = n_heads * head_dim
-    if out.dtype is not q.dtype or len(qs) != 2 or len(os) != 2 or qs[0] != T or os[0] != T or qs[1] < need or os[1] < need or token_seq.numel() != T:
-        raise KernelError(f"{name}: {T} rows of {n_heads} heads of {head_dim}, found queries {tuple(qs)} {q.dtype}, results "
-                          f"{tuple(os)} {out.dtype}, {token_seq.numel()} entries")
+    if n_heads < 1 or n_heads % n_kv_heads or found[20] == 0 or found[23] < need or found[24] < need:
+        raise KernelError(f"{name}: {n_heads} heads on {n_kv_heads} of {head_dim}, {found[20]} pages a request: found rows of {found[23]} and {found[24]}")
     if (window is not None and window < 1) or (softcap is not None and not softcap > 0) or not abs(scale) < float("inf"):
         raise KernelError(f"{name}: window={window}, softcap={softcap}, scale={scale}: positive (or None), positive (or None), finite")
-    _int32(name, "positions, entries, slots and tokens", positions, token_seq, seq_slot, tokens)
-    _on_current_device(name, q, k_pages, v_pages, k_exp, v_exp, block_table, positions, token_seq, seq_slot, tokens, out)
-    return n_pages, n_slots, width, T
+    return found
 
 
-def decode_fp8_ok(k_pages, v_pages, head_dim: int, page_size: int) -> bool:
-    """Whether the tensor-core kernel takes these pages (head sizes and pages in steps of 16); others go to a warp a (token, head)."""
-    return head_dim % 16 == 0 and page_size % 16 == 0 and k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0
+def decode_fp8_ok(k_address: int, v_address: int, head_dim: int, page_size: int) -> bool:
+    """Whether the tensor-core kernel takes such pages (head sizes and pages in steps of 16); others go to a warp a (token, head)."""
+    return head_dim % 16 == 0 and page_size % 16 == 0 and k_address % 16 == 0 and v_address % 16 == 0
 
 
 FP8_TILE = 128                    # positions a tile of the decode kernel holds
@@ -2159,45 +2178,41 @@ def decode_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_si
     in 16 or 32 bits as ``out``; token t sees the positions max(0, p - window + 1) .. p of its request, its own among them.
     ``tokens`` (int32, optional): the rows of ``q`` and ``out`` that are taken; the others stay as they are.  Positions without a
     page do not count; a token that sees none gets zeros."""
-    name = "decode_attention_fp8"
-    n_pages, n_slots, width, n = _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, tokens,
-                                   out, n_heads, n_kv_heads, head_dim, window, scale, softcap)
-    if tokens is not None:
-        n = tokens.numel()
-    operands = (_ptr(q), _rows(q), code(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_exp), _ptr(v_exp), _ptr(block_table),
-                n_slots, width, page_size, n_pages, _ptr(positions), _ptr(token_seq), _ptr(seq_slot),
-                _ptr(tokens), n, _ptr(out), _rows(out), n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0))
-    st = stream if stream is not None else stream_ptr()
-    if not decode_fp8_ok(k_pages, v_pages, head_dim, page_size):
-        call("fx_attention_fp8", *operands, st)
-        return out
-    reach = width * page_size
+    found = _look_at_attention_fp8("decode_attention_fp8", q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq,
+                                   seq_slot, status, tokens, out, n_heads, n_kv_heads, head_dim, window, scale, softcap)
+    _decode_fp8(found, page_size, n_heads, window, scale, softcap, stream)
+    return out
+
+
+def _decode_fp8(found, page_size, n_heads, window, scale, softcap, stream):
+    (device, now, x, kp, vp, kep, vep, tp, pp, sp, lp, qp, op, zp, ip, N, G, _, D, S, W, T, _, _, _, _, n, ldq, ldo) = found
+    if ip == 0 and n < 0:
+        n = T
+    operands = (qp, ldq, x, kp, vp, kep, vep, tp, S, W, page_size, N, pp, sp, lp, ip, n, op, ldo, n_heads, G, D, int(window or 0), float(scale),
+                float(softcap or 0.0))
+    st = stream if stream is not None else _scoped_stream if _scoped_stream is not None else now
+    if not decode_fp8_ok(kp, vp, D, page_size):
+        return call("fx_attention_fp8", *operands, st)
+    reach = W * page_size
     if window is not None:
         reach = min(reach, (window + FP8_TILE - 2) // FP8_TILE * FP8_TILE + FP8_TILE)      # (the tiles that it straddles)
-    runs = decode_fp8_runs(n, n_heads, n_kv_heads, head_dim, q.dtype is torch.float32, reach)
+    runs = decode_fp8_runs(n, n_heads, G, D, x == F32, reach)
     if runs == 1:
-        call("fx_decode_attention_fp8", *operands, 1, None, None, _ptr(status), st)
-        return out
+        return call("fx_decode_attention_fp8", *operands, 1, 0, 0, zp, st)
     global _launches
     _launches += 1
-    size = n * n_heads * runs * (head_dim + 2)
-    if _elsewhere(stream):                     # (scratch belongs to the stream that the kernels run on)
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream)):
-            work = torch.empty(size, dtype=torch.float32, device=q.device)
+    size = n * n_heads * runs * (D + 2)
+    if st != now:                              # (scratch belongs to the stream that the kernels run on)
+        with torch.cuda.stream(torch.cuda.ExternalStream(st)):
+            work = torch.empty(size, dtype=torch.float32, device=device)
     else:
-        work = torch.empty(size, dtype=torch.float32, device=q.device)
+        work = torch.empty(size, dtype=torch.float32, device=device)
     base = work.data_ptr()
-    call("fx_decode_attention_fp8", *operands, runs, base, base + 4 * n * n_heads * runs * head_dim, _ptr(status), st)
-    return out
+    call("fx_decode_attention_fp8", *operands, runs, base, base + 4 * n * n_heads * runs * D, zp, st)
 
 
 FP8_FEW_TOKENS = 8                # entries that bring at most this many tokens are left to decode_attention_fp8
 FP8_READ_BACK_MAX = 1 << 30       # bytes of keys and values that are read back at a time
-
-
-def _elsewhere(stream) -> bool:
-    """Whether a named stream is another than the one that scratch is taken on."""
-    return stream is not None and stream != _scoped_stream and stream != _current_stream(torch.cuda.current_device())
 
 
 class PrefillFp8Plan:
@@ -2314,30 +2329,30 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     the tensor cores take as they are, where conversion in the attention kernel would be paid again for every tile and query head.
     Entries of up to FP8_FEW_TOKENS tokens, and shapes that no tiled kernel takes, go to :func:`decode_attention_fp8`."""
     name = "prefill_attention_fp8"
-    _check_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, None, out, n_heads,
-                         n_kv_heads, head_dim, window, scale, softcap)
+    found = _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, status, None,
+                                   out, n_heads, n_kv_heads, head_dim, window, scale, softcap)
     if plan.n_tokens != q.shape[0] or plan.page_size != page_size or len(plan.entries) > seq_slot.numel():
         raise KernelError(f"{name}: a plan of {len(plan.entries)} entries, {plan.n_tokens} tokens and pages of {plan.page_size} for "
                           f"{seq_slot.numel()} entries, {q.shape[0]} tokens and pages of {page_size}")
-    if _elsewhere(stream):               # (scratch and lists belong to the stream that the kernels run on)
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream)):
+    st = stream if stream is not None else _scoped_stream if _scoped_stream is not None else found[1]
+    if st != found[1]:                   # (scratch and lists belong to the stream that the kernels run on)
+        with torch.cuda.stream(torch.cuda.ExternalStream(st)), stream_scope(st):
             return prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, plan, positions, token_seq, seq_slot,
                                          out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status)
-    st = stream if stream is not None else stream_ptr()
     cache = (k_pages, v_pages, k_exp, v_exp, block_table, page_size)
     step = (positions, token_seq, seq_slot)
     f32 = q.dtype == torch.float32
     # (asked with q in the pages' place: pages that are read back have its type and lie on the allocator's grid)
     if not (prefill_f32_ok(q, out, q, head_dim) if f32 else prefill_ok(q, out, q, head_dim)):
-        return decode_attention_fp8(q, *cache, *step, out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status,
-                                    stream=stream)
+        _decode_fp8(found, page_size, n_heads, window, scale, softcap, st)
+        return out
     few = plan.few()
     if few is not None:
         decode_attention_fp8(q, *cache, *step, out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status, tokens=few,
-                             stream=stream)
+                             stream=st)
     for tok0, n, entries, spans, rows, table, slots in plan.parts(window, 2 * n_kv_heads * head_dim * q.element_size()):
         k, v = torch.empty((2, rows // page_size, n_kv_heads, page_size, head_dim), dtype=q.dtype, device=q.device)
-        read_kv_fp8_spans(*cache, spans, rows, seq_slot, k, v, stream=stream)
+        read_kv_fp8_spans(*cache, spans, rows, seq_slot, k, v, stream=st)
         _prefill_read_back(q[tok0:tok0 + n], k, v, table, page_size, plan, (tok0, window), entries, slots, out[tok0:tok0 + n], n_heads,
                            n_kv_heads, head_dim, window, scale, softcap, status, st)
     return out

@@ -563,3 +563,34 @@ def test_a_request_from_prompt_to_tokens(dtype):
             ops.decode_attention_fp8(q, *c.operands, *st, out, H, G, D, None, 0.125)
         check(out, c, entries, q, H, None, 0.125, None, PROMPT_WEIGHT[dtype])
         done = [d + n for d, n in zip(done, news)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_operands_are_found_the_same_without_the_extension(dtype, monkeypatch):
+    """What the extension module says of a call's tensors is what the plain look at them says, and what it does not take is
+    refused by the plain one."""
+    H, G, D, P = 4, 2, 64, 16
+    c = Cache([70, 9, 33], G, D, P, 40)
+    q = rows(3, H, G, D, DTYPES[dtype], 41, extra=8)
+    st = step([(1, 69), (1, 8), (1, 32)], c.slots)
+    out = torch.zeros(3, H * D + 4, dtype=q.dtype, device=DEV)
+    k, v, ke, ve, table, _ = c.operands
+    status, some = torch.zeros(1, dtype=torch.int32, device=DEV), torch.tensor([2, 0], dtype=torch.int32, device=DEV)
+    assert ops._look()("iT", st[0]) is not None                            # (it is there at all)
+    for tensors in ([k, v, ke, ve, table, *st, q, out, status, some], [k, v, ke, ve, table, *st, q[:1].expand(3, -1), out[:, :H * D], None, None],
+                    [k, v, ke, ve, table, *st, q[::2].repeat(2, 1)[:3], out, status, some[:0]]):
+        labels = ops._CACHE_FP8 + ops._STEP + ("q", "out", "status", "tokens")
+        assert ops._operands("x", ops._ATTEND_FP8, labels, *tensors) == ops._operands_slowly("x", ops._ATTEND_FP8, labels, tensors)
+    for at, bad in ((0, k.view(torch.uint8)), (1, v[:1]), (2, ke.float()), (4, table.long()), (5, st[0][:2]), (8, q.double()), (8, q.T), (9, out.to(torch.float16)),
+                    (0, k.transpose(1, 2)), (6, st[1].cpu()), (9, out[:, ::2]), (8, None)):
+        t = [k, v, ke, ve, table, *st, q, out, status, some]
+        t[at] = bad
+        assert ops._look()(ops._ATTEND_FP8, *t) is None
+        with pytest.raises(ops.KernelError):
+            ops._operands("x", ops._ATTEND_FP8, ops._CACHE_FP8 + ops._STEP + ("q", "out", "status", "tokens"), *t)
+    want = torch.empty(3, H * D, dtype=q.dtype, device=DEV)
+    ops.decode_attention_fp8(q, *c.operands, *st, want, H, G, D, 40, 0.1)
+    monkeypatch.setattr(ops, "_look", lambda: lambda *a: None)
+    got = torch.empty_like(want)
+    ops.decode_attention_fp8(q, *c.operands, *st, got, H, G, D, 40, 0.1)
+    assert torch.equal(got, want)
