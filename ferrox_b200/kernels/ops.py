@@ -1291,13 +1291,13 @@ def prefill_f32_ok(q, out, k_pages, head_dim) -> bool:
 F32_TC_TILE, F32_TC_KEYS = 128, 64     # queries a tile and keys a block of attention_f32_tc.cu
 
 
-def prefill_f32_tc_plan(entries, window, head_dim):
+def prefill_f32_tc_plan(entries, window, head_dim, least=None):
     """The work of :func:`prefill_attention_f32_tc` for a step.  ``entries``: (tokens, first position) of each entry, in the order
     of the flattened batch.  Returns (items int32 [n, 8], spans int32 [m, 4], plane rows, rest int32 [k, 4]): tiles of up to 128
     queries, the most key blocks first; the positions of every entry that its queries see, in rows of the planes that begin at
     multiples of 64; and the entries that the tensor cores do not take, as the tiles of :func:`prefill_attention_f32`.
 
-    They take an entry that sees 64 keys or more (128 with heads of 64 elements or fewer).  The line was drawn while operands' parts
+    ``least`` given: they take an entry that sees that many keys or more.  Else they take one that sees 64 keys or more (128 with heads of 64 elements or fewer).  The line was drawn while operands' parts
     were cut off instead of rounded, where the result is then no further from 64 bits than FFMA's; rounded, it is nearer from 9 keys on.
     B200, one request from position 0, FFMA and tensor cores, error and time: 16 heads of 128, 33 keys: 1.51e-7 and 1.17e-7, 18 and 11
     us; 64: 1.74e-7 and 1.33e-7, 18 and 12 us; 517: 2.65e-7 and 1.70e-7, 145 and 42 us; 2000: 3.81e-7 and 1.87e-7, 1299 and 135 us.  8
@@ -1306,7 +1306,7 @@ def prefill_f32_tc_plan(entries, window, head_dim):
     import numpy as np
 
     items, spans, rest, flat, row = [], [], [], 0, 0
-    least = 64 if head_dim > 64 else 128
+    least = least or (64 if head_dim > 64 else 128)
     for b, (n, start) in enumerate(entries):
         if min(start + n, window or start + n) < least:
             rest += [(flat + i, min(F32_PREFILL_TILE, n - i), b, start + i) for i in range(0, n, F32_PREFILL_TILE)]
@@ -2392,7 +2392,9 @@ def _prefill_read_back(q, k, v, table, page_size, plan, key, entries, slots, out
 
 
 def _f32_lists(entries, window, head_dim):
-    items, spans, rows, rest = prefill_f32_tc_plan(entries, window, head_dim)
+    # (from 9 keys on the tensor cores are nearer to 64 bits than FFMA and no slower: one kernel for all entries but the shortest.
+    # B200, three prompts of 300, 193 and 97 tokens, 4 heads of 64 on 2: 50 us with the shortest left to FFMA)
+    items, spans, rows, rest = prefill_f32_tc_plan(entries, window, head_dim, least=9)
     return items, spans, rest, len(items), rows
 
 
