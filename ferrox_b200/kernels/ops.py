@@ -2225,8 +2225,20 @@ class PrefillFp8Plan:
         if self.page_size < 1 or any(n < 0 or start < 0 for n, start in self.entries):
             raise KernelError(f"prefill_fp8_plan: entries {self.entries} of pages of {page_size}")
         self.n_tokens = sum(n for n, _ in self.entries)
-        self._kept, self._streams = {}, {}
-        self._index = self.device.index if self.device.index is not None or self.device.type != "cuda" else torch.cuda.current_device()
+        self.has_few = any(0 < n <= FP8_FEW_TOKENS for n, _ in self.entries)
+        self._kept, self._tensors, self._stream = {}, [], None
+
+    def on_stream(self, stream: int):
+        """The next uses are on the (current) stream ``stream``: behind the uses before on another one, which copied the lists, and
+        the lists are not freed under its kernels.  (A capture begins behind everything that was under way, and its graph needs
+        the plan for as long as it lives.)"""
+        if self._stream != stream:
+            if self._stream is not None and not torch.cuda.is_current_stream_capturing():
+                now = torch.cuda.current_stream(self.device)
+                now.wait_stream(torch.cuda.ExternalStream(self._stream, device=self.device))
+                for t in self._tensors:
+                    t.record_stream(now)
+            self._stream = stream
 
     def kept(self, key, make):
         """What ``make`` returns, made once: a tuple's numpy arrays as tensors on the device."""
@@ -2235,26 +2247,12 @@ class PrefillFp8Plan:
             x = make()
             if isinstance(x, tuple):
                 x = tuple(upload(v, self.device) if hasattr(v, "__array__") else v for v in x)
-                self._streams[key] = [self._stream()]
+                self._tensors += [v for v in x if isinstance(v, torch.Tensor) and v.numel() and v.is_cuda]
             self._kept[key] = x
-        elif isinstance(x, tuple):
-            # used on a stream other than the one that copied it: ordered behind the copy, and not freed under its kernels
-            # (a capture begins behind everything that was under way, and its graph needs the plan for as long as it lives)
-            now, seen = self._stream(), self._streams[key]
-            if now not in seen and not torch.cuda.is_current_stream_capturing():
-                stream = torch.cuda.current_stream(self.device)
-                stream.wait_stream(torch.cuda.ExternalStream(seen[0], device=self.device))
-                for t in x:
-                    if isinstance(t, torch.Tensor) and t.numel():
-                        t.record_stream(stream)
-                seen.append(now)
         return x
 
-    def _stream(self):
-        return _current_stream(self._index) if self.device.type == "cuda" else None
-
     def few(self):
-        """Flat indices of the tokens of entries that bring few, or None."""
+        """Flat indices of the tokens of entries that bring few."""
         import numpy as np
 
         def make():
@@ -2264,14 +2262,13 @@ class PrefillFp8Plan:
                     at += range(flat, flat + n)
                 flat += n
             return (np.asarray(at, dtype=np.int32),)
-        t = self.kept("few", make)[0]
-        return t if t.numel() else None
+        return self.kept("few", make)[0]
 
     def parts(self, window, row_bytes):
         """Neighbouring entries whose visible keys and values are read back together: (first token, tokens, entries, spans, rows,
         block table over the rows' pages, its slots), at most FP8_READ_BACK_MAX bytes each where that holds an entry at all."""
-        groups = self.kept(("groups", window, row_bytes), lambda: self._groups(window, row_bytes))
-        return [self.kept(("part", window, row_bytes, g[0][0]), lambda: self._part(window, g)) for g in groups]
+        return self.kept((window, row_bytes), lambda: [self.kept(("part", window, row_bytes, g[0][0]), lambda: self._part(window, g))
+                                                       for g in self._groups(window, row_bytes)])
 
     def _rows_of(self, n, start, window):
         p0 = first_key(start, window) // self.page_size * self.page_size
@@ -2331,9 +2328,10 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     name = "prefill_attention_fp8"
     found = _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, status, None,
                                    out, n_heads, n_kv_heads, head_dim, window, scale, softcap)
-    if plan.n_tokens != q.shape[0] or plan.page_size != page_size or len(plan.entries) > seq_slot.numel():
+    T, B = found[21:23]
+    if plan.n_tokens != T or plan.page_size != page_size or len(plan.entries) > B:
         raise KernelError(f"{name}: a plan of {len(plan.entries)} entries, {plan.n_tokens} tokens and pages of {plan.page_size} for "
-                          f"{seq_slot.numel()} entries, {q.shape[0]} tokens and pages of {page_size}")
+                          f"{B} entries, {T} tokens and pages of {page_size}")
     st = stream if stream is not None else _scoped_stream if _scoped_stream is not None else found[1]
     if st != found[1]:                   # (scratch and lists belong to the stream that the kernels run on)
         with torch.cuda.stream(torch.cuda.ExternalStream(st)), stream_scope(st):
@@ -2346,15 +2344,16 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     if not (prefill_f32_ok(q, out, q, head_dim) if f32 else prefill_ok(q, out, q, head_dim)):
         _decode_fp8(found, page_size, n_heads, window, scale, softcap, st)
         return out
-    few = plan.few()
-    if few is not None:
-        decode_attention_fp8(q, *cache, *step, out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status, tokens=few,
-                             stream=st)
+    plan.on_stream(st)
+    if plan.has_few:
+        decode_attention_fp8(q, *cache, *step, out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status,
+                             tokens=plan.few(), stream=st)
     for tok0, n, entries, spans, rows, table, slots in plan.parts(window, 2 * n_kv_heads * head_dim * q.element_size()):
-        k, v = torch.empty((2, rows // page_size, n_kv_heads, page_size, head_dim), dtype=q.dtype, device=q.device)
+        k, v = (torch.empty(rows // page_size, n_kv_heads, page_size, head_dim, dtype=q.dtype, device=q.device) for _ in range(2))
         read_kv_fp8_spans(*cache, spans, rows, seq_slot, k, v, stream=st)
-        _prefill_read_back(q[tok0:tok0 + n], k, v, table, page_size, plan, (tok0, window), entries, slots, out[tok0:tok0 + n], n_heads,
-                           n_kv_heads, head_dim, window, scale, softcap, status, st)
+        q_part, out_part = (q, out) if n == plan.n_tokens else (q[tok0:tok0 + n], out[tok0:tok0 + n])
+        _prefill_read_back(q_part, k, v, table, page_size, plan, (tok0, window), entries, slots, out_part, n_heads, n_kv_heads, head_dim,
+                           window, scale, softcap, status, st)
     return out
 
 
