@@ -92,7 +92,7 @@ int fx_read_kv_fp8(const void* k_pages, const void* v_pages, const void* k_exp, 
 // n_splits > 1: part_o [tokens][heads][n_splits][head_dim], part_ml [tokens][heads][n_splits][2]; fx_attention_fp8: any up to 256
 int fx_decode_attention_fp8(const void* q, long ldq, int dtype, const void* k_pages, const void* v_pages, const void* k_exp,
                             const void* v_exp, const int* block_table, int n_slots, int table_width, int page_size, int n_pages,
-                            const int* positions, const int* token_seq, const int* seq_slot, const int* tokens, int n_tokens,
+                            const int* positions, const int* token_seq, const int* seq_slot, int n_entries, const int* tokens, int n_tokens,
                             void* out, long ldo, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap,
                             int n_splits, float* part_o, float* part_ml, int* status, void* stream);
 int fx_attention_fp8(const void* q, long ldq, int dtype, const void* k_pages, const void* v_pages, const void* k_exp,

@@ -39,7 +39,7 @@
 namespace {
 using namespace fxtc;
 
-constexpr int TK = 128, NSOFT = 128, NTHREADS = 64 + 2 * NSOFT, STAGES = 3, S_PLACES = 3, SLAB = TK * 128, P_BYTES = TK * 64;
+constexpr int TK = 128, NSOFT = 128, NTHREADS = 64 + 2 * NSOFT, STAGES = 3, S_PLACES = 3, SLAB = TK * 128, W_ROW = 32, W_BYTES = TK * W_ROW;
 constexpr float NO_REF = -1e30f;                                 // no score yet
 constexpr float RAISE = 6.f, RAISE_W = 8.f, ROOM = 2.f, ROOM_W = 5.f;
 
@@ -50,7 +50,7 @@ struct Args {
     const int *positions, *token_seq, *seq_slot, *tokens;
     void* out; long ldo;
     float *part_o, *part_ml;
-    int n_heads, n_kv_heads, head_dim, window, n_splits;
+    int n_entries, n_heads, n_kv_heads, head_dim, window, n_splits;
     float q_scale, cap;                                          // cap 0: scores in powers of two; else scale / cap, and cap in powers of two
     int* status;
 };
@@ -70,8 +70,8 @@ template <typename T, int HB, int SLABS> struct Lay {
     static constexpr int COLS_O = S_PLACES * NS, COLS = COLS_O + 2 * SLABS * NO;                      // (O of either group)
     static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int STAGE = 2 * SLABS * SLAB;                                                    // K slabs, V slabs
-    static constexpr int Q_OFF = STAGES * STAGE, W_OFF = Q_OFF + SLABS * NS * 128, TOTAL = W_OFF + P_BYTES + 1024;
-    static_assert(NO <= 64 && COLS <= (SLABS == 1 ? 256 : 512), "a key's weights are a row of 64 bytes; two blocks share the SM's tensor memory");
+    static constexpr int Q_OFF = STAGES * STAGE, W_OFF = Q_OFF + SLABS * NS * 128, TOTAL = W_OFF + 2 * W_BYTES + 1024;
+    static_assert(NO <= W_ROW && COLS <= (SLABS == 1 ? 256 : 512), "a key's weights are a row of 32 bytes; two blocks share the SM's tensor memory");
 };
 
 __device__ __forceinline__ void mma8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -85,9 +85,9 @@ __device__ __forceinline__ void mma8(uint32_t d, uint64_t a, uint64_t b, uint32_
 __host__ __device__ constexpr uint32_t idesc8(int m, int n, int a_mn, int b_mn) {
     return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// 64-byte swizzle: rows of 64 bytes, 8-row groups 512 bytes apart
-__device__ __forceinline__ uint64_t desc64(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(P_BYTES >> 4) << 16) | ((uint64_t)(512 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)4 << 61);
+// 32-byte swizzle: rows of 32 bytes, 8-row groups 256 bytes apart
+__device__ __forceinline__ uint64_t desc32(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(W_BYTES >> 4) << 16) | ((uint64_t)(256 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)6 << 61);
 }
 
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* r) {
@@ -110,14 +110,13 @@ __device__ __forceinline__ float exp2_fast(float x) {            // 2^x to 2 ste
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Barriers of a group's 128 threads: one that asks all of them, a plain one, and one that only the group's first warp waits at.
+// Barriers of a group's 128 threads: one that asks all of them, and one that only the group's first warp waits at.
 __device__ __forceinline__ bool any_of_group(int g, bool x) {
     uint32_t r;
     asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, %2, %3, p; selp.u32 %0, 1, 0, q;}"
                  : "=r"(r) : "r"((uint32_t)x), "r"(1 + g), "n"(NSOFT) : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(NSOFT) : "memory"); }
 __device__ __forceinline__ void group_written(int g, bool waits) {
     if (waits) asm volatile("bar.sync %0, %1;" ::"r"(3 + g), "n"(NSOFT) : "memory");
     else asm volatile("bar.arrive %0, %1;" ::"r"(3 + g), "n"(NSOFT) : "memory");
@@ -165,11 +164,13 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
     __shared__ float sum_s[2][4][HB];
     volatile int* abort_flag = &abort_flag_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* sm = smem_raw + (base - smem_u32(smem_raw));
     auto full = [&](int s) { return smem_u32(&bars_s[s]); };
     auto empty = [&](int s) { return smem_u32(&bars_s[STAGES + s]); };
     auto s_full = [&](int b) { return smem_u32(&bars_s[2 * STAGES + b]); };
     auto s_empty = [&](int b) { return smem_u32(&bars_s[2 * STAGES + S_PLACES + b]); };
-    auto o_done = [&](int j) { return smem_u32(&bars_s[2 * STAGES + 2 * S_PLACES + (j & 1)]); };   // of the group that tile j belongs to, phase j / 2
+    auto o_done = [&](int i) { return smem_u32(&bars_s[2 * STAGES + 2 * S_PLACES + i]); };         // of a group, a phase for each of its tiles
     auto drained = [&](int i) { return smem_u32(&bars_s[2 * STAGES + 2 * S_PLACES + 2 + i]); };
 
     if (threadIdx.x == 0) {
@@ -185,7 +186,9 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
     const int group = a.n_heads / a.n_kv_heads, blocks_g = (group + HB - 1) / HB;
     const int kvh = blockIdx.y / blocks_g, h0 = kvh * group + blockIdx.y % blocks_g * HB, nh = min(HB, kvh * group + group - h0);
     const int tkn = a.tokens ? a.tokens[blockIdx.x] : blockIdx.x, split = blockIdx.z, D = a.head_dim;
-    const int pos = a.positions[tkn], slot = a.seq_slot[a.token_seq[tkn]];
+    // (a decode step's token t is mostly its entry t: the slot that would be its is asked for beside the answer)
+    const int likely = a.seq_slot[min(tkn, a.n_entries - 1)], seq = a.token_seq[tkn], pos = a.positions[tkn];
+    const int slot = seq == tkn ? likely : a.seq_slot[seq];
     int k_begin, k_end;
     run_of(pos, fx_first_key(pos, a.window, 0), split, a.n_splits, k_begin, k_end);
     if (slot < 0 || slot >= a.n_slots) k_end = k_begin;
@@ -201,8 +204,6 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
     }
     const int* table = a.block_table + (long)slot * a.table_width;
     const int first_tile = k_begin / TK, n_tiles = (k_end - 1) / TK - first_tile + 1;
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* sm = smem_raw + (base - smem_u32(smem_raw));
 
     // The producer's warp: lane b asks for a tile's box b of a.box keys.  The first tiles are asked for before the block meets.
     const int n_boxes = TK / a.box;
@@ -212,28 +213,31 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
         if (lane >= n_boxes || j >= n_tiles || key >= k_end || key + a.box <= k_begin) return -1;
         return fx_page_of(table, a.table_width, a.n_pages, key, a.page_size);
     };
-    auto ask = [&](int j, int found) {
+    auto ask_box = [&](int j, int b, int found, int off) {
         const int s = j % STAGES, page = found < 0 ? a.n_pages : found;
-        const int off = found < 0 ? 0 : ((first_tile + j) * TK + lane * a.box) % a.page_size;
-        if (lane == 0) mbar_expect_tx(full(s), (uint32_t)L::STAGE);
-        __syncwarp();
-        if (lane < n_boxes) {
-            const uint32_t dst = base + s * L::STAGE + lane * a.box * 128;
+        const uint32_t dst = base + s * L::STAGE + b * a.box * 128;
 #pragma unroll
-            for (int sl = 0; sl < SLABS; ++sl) {
-                tma_load_4d(dst + sl * SLAB, &map_k, sl * 128, off, kvh, page, full(s));
-                tma_load_4d(dst + (SLABS + sl) * SLAB, &map_v, sl * 128, off, kvh, page, full(s));
-            }
+        for (int sl = 0; sl < SLABS; ++sl) {
+            tma_load_4d(dst + sl * SLAB, &map_k, sl * 128, off, kvh, page, full(s));
+            tma_load_4d(dst + (SLABS + sl) * SLAB, &map_v, sl * 128, off, kvh, page, full(s));
         }
+    };
+    auto ask = [&](int j, int found) {
+        if (lane == 0) mbar_expect_tx(full(j % STAGES), (uint32_t)L::STAGE);
+        __syncwarp();
+        if (lane < n_boxes) ask_box(j, lane, found, found < 0 ? 0 : ((first_tile + j) * TK + lane * a.box) % a.page_size);
         __syncwarp();
     };
     if (warp == 0) {
-        int first[STAGES];
-#pragma unroll
-        for (int j = 0; j < STAGES; ++j) first[j] = page_of(j);
-#pragma unroll
-        for (int j = 0; j < STAGES; ++j)
-            if (j < n_tiles) ask(j, first[j]);
+        // the first tiles' boxes, a lane each
+        const int j = lane / n_boxes, b = lane - j * n_boxes, key = (first_tile + j) * TK + b * a.box;
+        const bool mine = j < asked;
+        int page = -1;
+        if (mine && key < k_end && key + a.box > k_begin) page = fx_page_of(table, a.table_width, a.n_pages, key, a.page_size);
+        if (lane < asked) mbar_expect_tx(full(lane), (uint32_t)L::STAGE);
+        __syncwarp();
+        if (mine) ask_box(j, b, page, page < 0 ? 0 : key % a.page_size);
+        __syncwarp();
         page_next = page_of(STAGES);
     }
 
@@ -267,24 +271,20 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
     };
     int exps_next = -1;
     if (warp >= 2) {
-        page_next = next_page();
-        exps_next = next_exps(page_next);
-        page_next = next_page();
         // the queries in parts: a warp a head; rows of the columns that no head has are zeros
+        const int h = warp - 2;
+        const T* row = reinterpret_cast<const T*>(a.q) + (long)tkn * a.ldq + (long)(h0 + min(h, nh - 1)) * D;
+        float x[SLABS * 4];
+#pragma unroll
+        for (int i = 0; i < SLABS * 4; ++i) x[i] = lane + 32 * i < D && h < nh ? to_f32(row[lane + 32 * i]) : 0.f;
+        page_next = next_page();
         for (int i = st; i < SLABS * L::NS * 8; i += 2 * NSOFT) reinterpret_cast<uint4*>(sm + L::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
         if (st < 2 * HB) { (&ref_s[0][0])[st] = NO_REF; (&refw_s[0][0])[st] = NO_REF; (&ratio_s[0][0])[st] = 1.f; }
         any_of_soft(false);
-        if (warp - 2 < HB) {
-            const int h = warp - 2;
-            float x[SLABS * 4];
-            const T* row = reinterpret_cast<const T*>(a.q) + (long)tkn * a.ldq + (long)(h0 + min(h, nh - 1)) * D;
+        if (h < HB) {
             uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < SLABS * 4; ++i) {
-                const int e = lane + 32 * i;
-                x[i] = e < D && h < nh ? to_f32(row[e]) : 0.f;
-                most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-            }
+            for (int i = 0; i < SLABS * 4; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
             most = __reduce_max_sync(0xffffffffu, most);
             // q 2^-x in [128, 256): the exponent field of its largest element, less 7 (at least 2^-119; an element that is no
             // finite number makes the head's factor none)
@@ -306,6 +306,8 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        exps_next = next_exps(page_next);
+        page_next = next_page();
     }
 
     // Tensor memory is taken behind the wait for the kernel before and ahead of the leave for the kernel behind to be set up:
@@ -405,33 +407,33 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
                     over_w = fmaxf(over_w, w[h]);
                 }
             };
-            weigh();
-            if (any_of_group(g, over > RAISE || over_w > 256.f || !ok)) {
-                if (any_of_group(g, !ok)) { fine = false; break; }
+            const bool first = j == g;                                   // (no reference yet)
+            if (!first) weigh();
+            if (first || any_of_group(g, over > RAISE || over_w > 256.f || !ok)) {
                 const float v_log = (float)((exps >> 8 & 255) - 127);
+                const int h = lane % HB;
+                const float ref = ref_s[g][h], refw = refw_s[g][h];
 #pragma unroll
-                for (int h = 0; h < HB; ++h) {
-                    const float m = warp_max_f32(s[h]), mw = warp_max_f32(s[h] + v_log);
-                    if (lane == 0) { most_s[g][0][sw][h] = m; most_s[g][1][sw][h] = mw; }
+                for (int i = 0; i < HB; ++i) {
+                    const float m = warp_max_f32(s[i]), mw = warp_max_f32(s[i] + v_log);
+                    if (lane == 0) { most_s[g][0][sw][i] = m; most_s[g][1][sw][i] = mw; }
                 }
-                if (j > 0) ok = mbar_wait(o_done(j - 1), (uint32_t)((j - 1) >> 1) & 1u, abort_flag);      // the group's O as it stands, and nobody adds to it
+                if (!first && !mbar_wait(o_done(g), (uint32_t)((j >> 1) - 1) & 1u, abort_flag)) ok = false;      // O as it stands, and nobody adds to it
                 if (any_of_group(g, !ok)) { fine = false; break; }
                 tc_fence_after();
-                if ((st & 127) < HB) {
-                    const int h = st & 127;
+                {   // every warp the same, a lane a head (the values before were read ahead of the barrier)
                     const float m = fmaxf(fmaxf(most_s[g][0][0][h], most_s[g][0][1][h]), fmaxf(most_s[g][0][2][h], most_s[g][0][3][h]));
                     const float mw = fmaxf(fmaxf(most_s[g][1][0][h], most_s[g][1][1][h]), fmaxf(most_s[g][1][2][h], most_s[g][1][3][h]));
-                    const float ref = ref_s[g][h], refw = refw_s[g][h];
                     const float now = m - ref > RAISE ? ceilf(m) - ROOM : ref, now_w = mw - refw > RAISE_W ? ceilf(mw) - ROOM_W : refw;
                     shrink_s[g][h] = exp2_fast(ref - now);
-                    for (int i = h; i < 16; i += HB) shrink_o_s[g][i] = exp2_fast(refw - now_w);      // (columns repeat their heads)
+                    shrink_o_s[g][lane % 16] = exp2_fast(refw - now_w);   // (columns repeat their heads)
                     ratio_s[g][h] = exp2_fast(now - now_w);
                     ref_s[g][h] = now; refw_s[g][h] = now_w;
                 }
-                group_sync(g);
+                __syncwarp();
+                if (!first) {
 #pragma unroll
-                for (int h = 0; h < HB; ++h) l[h] *= shrink_s[g][h];
-                if (j > 1) {
+                    for (int i = 0; i < HB; ++i) l[i] *= shrink_s[g][i];
 #pragma unroll 1
                     for (int c = 0; c < SLABS * L::NO; c += 16) {
                         uint32_t o[16];
@@ -444,8 +446,8 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
                     tc_st_wait();
                 }
                 weigh();
-            } else if (j > 0) {
-                ok = mbar_wait(o_done(j - 1), (uint32_t)((j - 1) >> 1) & 1u, abort_flag);                 // W(j - 1) has been multiplied: its place is free
+            } else {
+                ok = mbar_wait(o_done(g), (uint32_t)((j >> 1) - 1) & 1u, abort_flag);        // the group's W before this one: its place is free
             }
             uint32_t word[L::NO / 4];
 #pragma unroll
@@ -471,25 +473,25 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
                     word[(n * HB + h) / 4] = __byte_perm(lo, hi, 0x5410);
                 }
             }
-            uint8_t* row = sm + L::W_OFF + r * 64;
+            uint8_t* row = sm + L::W_OFF + g * W_BYTES + r * W_ROW;
 #pragma unroll
             for (int c = 0; c < L::NO / 16; ++c)
-                *reinterpret_cast<uint4*>(row + ((c ^ (r >> 1 & 3)) << 4)) = make_uint4(word[4 * c], word[4 * c + 1], word[4 * c + 2], word[4 * c + 3]);
+                *reinterpret_cast<uint4*>(row + ((c ^ (r >> 2 & 1)) << 4)) = make_uint4(word[4 * c], word[4 * c + 1], word[4 * c + 2], word[4 * c + 3]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_before();
             // O += V^T W^T, by the group's first thread when all its keys' weights are written
             group_written(g, sw == 0);
             if (sw == 0 && lane == 0) {
                 tc_fence_after();
-                const uint32_t v = base + j % STAGES * L::STAGE + SLABS * SLAB, wt = base + L::W_OFF;
+                const uint32_t v = base + j % STAGES * L::STAGE + SLABS * SLAB, wt = base + L::W_OFF + g * W_BYTES;
 #pragma unroll
                 for (int sl = 0; sl < SLABS; ++sl)
 #pragma unroll
-                    for (int ks = 0; ks < TK / 32; ++ks)                 // 32 keys: four 8-key groups, 1024 bytes apart in V, 512 in W
-                        mma8(tmem + col_o + sl * L::NO, smem_desc_lbo_sbo(v + sl * SLAB + ks * 4096, SLAB, 1024), desc64(wt + ks * 2048), idesc_o,
+                    for (int ks = 0; ks < TK / 32; ++ks)                 // 32 keys: four 8-key groups, 1024 bytes apart in V, 256 in W
+                        mma8(tmem + col_o + sl * L::NO, smem_desc_lbo_sbo(v + sl * SLAB + ks * 4096, SLAB, 1024), desc32(wt + ks * 32 * W_ROW), idesc_o,
                              j > 1 || ks > 0);
                 tc_commit(empty(j % STAGES));
-                tc_commit(o_done(j));
+                tc_commit(o_done(g));
             }
             __syncwarp();
             if (!ok) fine = false;                                       // (seen by all at the next barrier, or behind the loop)
@@ -498,8 +500,8 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
         if (!fine && sw == 0 && lane == 0) { tc_commit(drained(g)); settle(drained(g), 0); }
 
         // ---- the run's result: this thread has element r of every slab, its group half of the heads, over both groups' tiles ----
-        bool ok = fine && mbar_wait(o_done(n_tiles - 1), (uint32_t)((n_tiles - 1) >> 1) & 1u, abort_flag);
-        tc_fence_after();
+        const int own = (n_tiles - g + 1) / 2;                           // the group's tiles
+        const bool ok = fine && (own == 0 || mbar_wait(o_done(g), (uint32_t)(own - 1) & 1u, abort_flag));
         // HB sums over 32 lanes: half of what a lane has goes to its partner, until each has one head's; the rest as ever
 #pragma unroll
         for (int n = HB / 2, o = 16; n > 0; n >>= 1, o >>= 1) {
@@ -515,7 +517,25 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
         // (lane's bits from the highest on choose the upper or lower half: they are the head's)
         if (lane % (32 / HB) == 0) sum_s[g][sw][lane / (32 / HB)] = l[0];
         if (!any_of_soft(!ok)) {
+            tc_fence_after();
+            // what a head's O of either group is multiplied with: 2^(refw - ref) over all weights' sum; a lane a head
             const bool two = n_tiles > 1;
+            float factor[2], all;
+            {
+                const int h = lane % HB;
+                const float ref = two ? fmaxf(ref_s[0][h], ref_s[1][h]) : ref_s[0][h];
+                const float s0 = (sum_s[0][0][h] + sum_s[0][1][h]) + (sum_s[0][2][h] + sum_s[0][3][h]);
+                const float s1 = (sum_s[1][0][h] + sum_s[1][1][h]) + (sum_s[1][2][h] + sum_s[1][3][h]);
+                all = s0 * exp2_fast(ref_s[0][h] - ref);
+                if (two) all = fmaf(s1, exp2_fast(ref_s[1][h] - ref), all);
+                const float over = all == 0.f ? 0.f : 1.f / all;
+                factor[0] = exp2_fast(refw_s[0][h] - ref) * over;
+                factor[1] = two ? exp2_fast(refw_s[1][h] - ref) * over : 0.f;
+                if (a.n_splits > 1 && warp == 2 && lane < nh) {
+                    const long at = ((long)blockIdx.x * a.n_heads + h0 + h) * a.n_splits + split;
+                    a.part_ml[2 * at] = ref; a.part_ml[2 * at + 1] = all;
+                }
+            }
 #pragma unroll
             for (int sl = 0; sl < SLABS; ++sl) {
                 const int e = sl * 128 + r;
@@ -529,32 +549,20 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
                 tc_ld_wait();
 #pragma unroll
                 for (int h = 0; h < HB; ++h) {
-                    if (h / (HB / 2) != g || h >= nh || e >= D) continue;
-                    float x[2], sum[2];
+                    if (h / (HB / 2) != g) continue;                     // (a group takes half of the heads)
+                    float v = 0.f;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        x[i] = __uint_as_float(o[i][(L::PARTS_W - 1) * HB + h]);
+                        const float f = __shfl_sync(0xffffffffu, factor[i], h);
+                        if (i == 1 && !two) continue;
+                        float x = __uint_as_float(o[i][(L::PARTS_W - 1) * HB + h]);
 #pragma unroll
-                        for (int n = L::PARTS_W - 2; n >= 0; --n) x[i] = fmaf(x[i], 0.0625f, __uint_as_float(o[i][n * HB + h]));
-                        sum[i] = (sum_s[i][0][h] + sum_s[i][1][h]) + (sum_s[i][2][h] + sum_s[i][3][h]);
+                        for (int n = L::PARTS_W - 2; n >= 0; --n) x = fmaf(x, 0.0625f, __uint_as_float(o[i][n * HB + h]));
+                        v = fmaf(x, f, v);
                     }
-                    // either group's mean of the values, and its share of the weights
-                    const float ref = two ? fmaxf(ref_s[0][h], ref_s[1][h]) : ref_s[0][h];
-                    float all = sum[0] * exp2_fast(ref_s[0][h] - ref);
-                    float v = sum[0] == 0.f ? 0.f : x[0] / sum[0] * exp2_fast(refw_s[0][h] - ref_s[0][h]);
-                    if (two && sum[1] != 0.f) {
-                        const float share = sum[1] * exp2_fast(ref_s[1][h] - ref), v1 = x[1] / sum[1] * exp2_fast(refw_s[1][h] - ref_s[1][h]);
-                        const float whole = all + share;
-                        v = all == 0.f ? v1 : fmaf(v, all / whole, v1 * (share / whole));
-                        all = whole;
-                    }
-                    if (a.n_splits == 1) {
-                        reinterpret_cast<T*>(a.out)[(long)tkn * a.ldo + (long)(h0 + h) * D + e] = from_f32<T>(v);
-                    } else {
-                        const long at = ((long)blockIdx.x * a.n_heads + h0 + h) * a.n_splits + split;
-                        a.part_o[at * D + e] = v;
-                        if (e == 0) { a.part_ml[2 * at] = ref; a.part_ml[2 * at + 1] = all; }
-                    }
+                    if (h >= nh || e >= D) continue;
+                    if (a.n_splits == 1) reinterpret_cast<T*>(a.out)[(long)tkn * a.ldo + (long)(h0 + h) * D + e] = from_f32<T>(v);
+                    else a.part_o[(((long)blockIdx.x * a.n_heads + h0 + h) * a.n_splits + split) * D + e] = v;
                 }
             }
         }
@@ -638,13 +646,16 @@ bool encode(CUtensorMap* map, const void* ptr, const Args& a)
 
 template <typename T> int run(const CUtensorMap& mk, const CUtensorMap& mv, Args& a, int n_tokens, cudaStream_t s)
 {
-    // heads a block takes: 4, or 8, whose registers leave two blocks an SM; more heads of a kv head: blocks side by side
-    const int group = a.n_heads / a.n_kv_heads, hb = group <= 4 ? 4 : 8;
+    // heads a block takes: 4, or 8, whose columns and registers leave two blocks an SM (32 bits, with six parts: 4); more heads of
+    // a kv head: blocks side by side
+    const int group = a.n_heads / a.n_kv_heads, hb = group <= 4 || sizeof(T) == 4 ? 4 : 8;
     const dim3 grid(n_tokens, a.n_kv_heads * ((group + hb - 1) / hb), a.n_splits);
     if (grid.y > 65535u) return FX_ERR_SIZE;
     int rc;
-    if (hb == 8) rc = a.head_dim <= 128 ? launch<T, 8, 1>(mk, mv, a, grid, s) : launch<T, 8, 2>(mk, mv, a, grid, s);
-    else rc = a.head_dim <= 128 ? launch<T, 4, 1>(mk, mv, a, grid, s) : launch<T, 4, 2>(mk, mv, a, grid, s);
+    if constexpr (sizeof(T) == 2) {
+        if (hb == 8) rc = a.head_dim <= 128 ? launch<T, 8, 1>(mk, mv, a, grid, s) : launch<T, 8, 2>(mk, mv, a, grid, s);
+    }
+    if (hb == 4) rc = a.head_dim <= 128 ? launch<T, 4, 1>(mk, mv, a, grid, s) : launch<T, 4, 2>(mk, mv, a, grid, s);
     if (rc || a.n_splits == 1) return rc;
     fx_launch_pdl(decode_fp8_merge_kernel<T>, dim3(n_tokens, a.n_heads), MERGE_WARPS * 32, 0, s, a);
     return fx_launch_status();
@@ -654,20 +665,20 @@ template <typename T> int run(const CUtensorMap& mk, const CUtensorMap& mv, Args
 
 extern "C" int fx_decode_attention_fp8(const void* q, long ldq, int dtype, const void* k_pages, const void* v_pages, const void* k_exp,
                                        const void* v_exp, const int* block_table, int n_slots, int table_width, int page_size, int n_pages,
-                                       const int* positions, const int* token_seq, const int* seq_slot, const int* tokens, int n_tokens,
-                                       void* out, long ldo, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap,
+                                       const int* positions, const int* token_seq, const int* seq_slot, int n_entries, const int* tokens,
+                                       int n_tokens, void* out, long ldo, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap,
                                        int n_splits, float* part_o, float* part_ml, int* status, void* stream)
 {
     if (n_tokens <= 0) return FX_OK;
     if (head_dim <= 0 || head_dim > 256 || head_dim % 16 || page_size <= 0 || page_size % 16 || n_pages <= 0 || n_slots <= 0 || table_width <= 0 ||
-        n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads > 65535 || window < 0 || softcap < 0.f || n_splits < 1 ||
+        n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads > 65535 || n_entries <= 0 || window < 0 || softcap < 0.f || n_splits < 1 ||
         n_splits > MAX_RUNS || (n_splits > 1 && (!part_o || !part_ml))) return FX_ERR_SIZE;
     if ((uintptr_t)k_pages % 16 || (uintptr_t)v_pages % 16) return FX_ERR_ALIGN;
     int box = TK;                                                        // keys a TMA box: the largest that stays in a page
     while (page_size % box) box /= 2;
     constexpr float LOG2E = 1.4426950408889634f;
     Args a = {q, ldq, (const uint8_t*)k_exp, (const uint8_t*)v_exp, block_table, n_slots, table_width, page_size, n_pages, box, positions, token_seq,
-              seq_slot, tokens, out, ldo, part_o, part_ml, n_heads, n_kv_heads, head_dim, window, n_splits,
+              seq_slot, tokens, out, ldo, part_o, part_ml, n_entries, n_heads, n_kv_heads, head_dim, window, n_splits,
               softcap > 0.f ? scale / softcap : scale * LOG2E, softcap * LOG2E, status};
     CUtensorMap mk, mv;
     if (!encode(&mk, k_pages, a) || !encode(&mv, v_pages, a)) return FX_ERR_SIZE;

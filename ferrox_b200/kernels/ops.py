@@ -125,7 +125,7 @@ _SIGNATURES = {
                             _I, _P, _P, _I, _I, _I, _P, _F, _P, _P],
     "fx_rope_kv_write_fp8": [_P, _I, _L, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "fx_read_kv_fp8": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _P],
-    "fx_decode_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F,
+    "fx_decode_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F,
                                 _I, _P, _P, _P, _P],
     "fx_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F, _P],
     "fx_argmax": [_P, _L, _I, _I, _P, _P],
@@ -2162,7 +2162,7 @@ def decode_fp8_runs(n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
     more than 128 elements) come to the least.  A function of the step's size and of ``reach``, the most positions a token may see, and
     not of the lengths, so that a captured step keeps its grid."""
     group = n_heads // n_kv_heads
-    per = 4 if group <= 4 else 8
+    per = 4 if group <= 4 or f32 else 8
     blocks, slots, tiles = max(1, n_tokens * n_kv_heads * -(-group // per)), sm_count() * (2 if head_dim <= 128 else 1), -(-reach // FP8_TILE)
     best, best_cost = 1, None
     for n in range(1, min(FP8_MAX_RUNS, tiles) + 1):
@@ -2185,20 +2185,19 @@ def decode_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_si
 
 
 def _decode_fp8(found, page_size, n_heads, window, scale, softcap, stream):
-    (device, now, x, kp, vp, kep, vep, tp, pp, sp, lp, qp, op, zp, ip, N, G, _, D, S, W, T, _, _, _, _, n, ldq, ldo) = found
+    (device, now, x, kp, vp, kep, vep, tp, pp, sp, lp, qp, op, zp, ip, N, G, _, D, S, W, T, B, _, _, _, n, ldq, ldo) = found
     if ip == 0 and n < 0:
         n = T
-    operands = (qp, ldq, x, kp, vp, kep, vep, tp, S, W, page_size, N, pp, sp, lp, ip, n, op, ldo, n_heads, G, D, int(window or 0), float(scale),
-                float(softcap or 0.0))
+    pages, heads = (qp, ldq, x, kp, vp, kep, vep, tp, S, W, page_size, N, pp, sp, lp), (ip, n, op, ldo, n_heads, G, D, int(window or 0), float(scale), float(softcap or 0.0))
     st = stream if stream is not None else _scoped_stream if _scoped_stream is not None else now
     if not decode_fp8_ok(kp, vp, D, page_size):
-        return call("fx_attention_fp8", *operands, st)
+        return call("fx_attention_fp8", *pages, *heads, st)
     reach = W * page_size
     if window is not None:
         reach = min(reach, (window + FP8_TILE - 2) // FP8_TILE * FP8_TILE + FP8_TILE)      # (the tiles that it straddles)
     runs = decode_fp8_runs(n, n_heads, G, D, x == F32, reach)
     if runs == 1:
-        return call("fx_decode_attention_fp8", *operands, 1, 0, 0, zp, st)
+        return call("fx_decode_attention_fp8", *pages, B, *heads, 1, 0, 0, zp, st)
     global _launches
     _launches += 1
     size = n * n_heads * runs * (D + 2)
@@ -2208,7 +2207,7 @@ def _decode_fp8(found, page_size, n_heads, window, scale, softcap, stream):
     else:
         work = torch.empty(size, dtype=torch.float32, device=device)
     base = work.data_ptr()
-    call("fx_decode_attention_fp8", *operands, runs, base, base + 4 * n * n_heads * runs * D, zp, st)
+    call("fx_decode_attention_fp8", *pages, B, *heads, runs, base, base + 4 * n * n_heads * runs * D, zp, st)
 
 
 FP8_FEW_TOKENS = 8                # entries that bring at most this many tokens are left to decode_attention_fp8
