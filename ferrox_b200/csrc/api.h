@@ -83,10 +83,11 @@ int fx_rope_kv_write_fp8(void* qkv, int dtype, long ld, const int* positions, co
                          const float* inv_freq, const float* cos_sin, int rotary_dim, int pairing, void* k_pages, void* v_pages,
                          void* k_exp, void* v_exp, const int* block_table, int n_slots, int table_width, int page_size, int n_pages,
                          int n_tokens, int n_heads, int n_kv_heads, int head_dim, int write_cache, int* status, void* stream);
-// spans null: k_out, v_out [n_rows][kv heads][head_dim] at the listed positions; else pages of n_spans stretches
+// spans null: k_out, v_out [n_rows][kv heads][head_dim] at the listed positions; else pages of out_page positions of n_spans
+// stretches; attend: a position that is not finite becomes a key of NaN and a value of 0
 int fx_read_kv_fp8(const void* k_pages, const void* v_pages, const void* k_exp, const void* v_exp, const int* block_table, int n_slots,
                    int table_width, int page_size, int n_pages, const int* positions, const int* token_seq, const int* seq_slot,
-                   const int* spans, int n_spans, int n_rows, void* k_out, void* v_out, int dtype, int n_kv_heads, int head_dim,
+                   const int* spans, int n_spans, int n_rows, int out_page, int attend, void* k_out, void* v_out, int dtype, int n_kv_heads, int head_dim,
                    void* stream);
 // tokens (optional): the n_tokens rows of q and out that are taken; fx_decode_attention_fp8: head sizes and pages in steps of 16,
 // n_splits > 1: part_o [tokens][heads][n_splits][head_dim], part_ml [tokens][heads][n_splits][2]; fx_attention_fp8: any up to 256
@@ -95,6 +96,11 @@ int fx_decode_attention_fp8(const void* q, long ldq, int dtype, const void* k_pa
                             const int* positions, const int* token_seq, const int* seq_slot, int n_entries, const int* tokens, int n_tokens,
                             void* out, long ldo, int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap,
                             int n_splits, float* part_o, float* part_ml, int* status, void* stream);
+// bfloat16 over pages of 128 positions, head sizes up to 128 in steps of 16, rows of (token, head): see attention_prefill_grouped.cu
+int fx_prefill_attention_grouped(const void* q, long ldq, int n_tokens, const void* k_pages, const void* v_pages, int n_pages,
+                                 const int* block_table, int table_width, const int* items, int n_items, void* out, long ldo, int n_heads,
+                                 int n_kv_heads, int head_dim, int window, float scale, float* part_o, float* part_ml, const int* merges,
+                                 int n_merges, int* status, void* stream);
 int fx_attention_fp8(const void* q, long ldq, int dtype, const void* k_pages, const void* v_pages, const void* k_exp,
                      const void* v_exp, const int* block_table, int n_slots, int table_width, int page_size, int n_pages,
                      const int* positions, const int* token_seq, const int* seq_slot, const int* tokens, int n_tokens, void* out,

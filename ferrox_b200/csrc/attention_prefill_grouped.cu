@@ -1,0 +1,403 @@
+// Attention for prompt portions whose query heads share key heads, on the 5th-generation tensor cores (bfloat16, heads of up to
+// 128 elements in steps of 16), over pages of 128 positions: what read_kv_fp8_spans makes of an 8-bit cache.
+//
+// A row is a (token, query head) pair; the rows of a tile are the query heads of one kv head for consecutive tokens of a
+// request, so that a block of keys and values that has been brought in serves all of them, and a portion of few tokens fills
+// its tiles with its heads (the kernel of attention_prefill_tc.cu has a head's tokens for rows: a portion of 300 tokens takes
+// tiles of 256 and 44 there, of 2,100 rows here).  One CTA takes two sub-tiles of up to 128 rows and walks the request's keys in
+// blocks of 128:
+//
+//   S_t = Q_t K_j^T    tcgen05.mma 128 x 128 x head_dim, Q by TMA ([token][head][64 elements] boxes), S_t in tensor memory
+//   P_t = 2^(S_t - m)  a thread a row: mask by absolute position, running maximum and sum in 32 bits, P in bfloat16 over S_t
+//   O_t += P_t V_j     tcgen05.mma, A from tensor memory, V as an N-major B operand
+//
+// What bounds it: the softmax threads' instructions, 4.5 a score.  (Converting the 8-bit pages in this kernel, by seven more
+// warps, cost those threads a third of their registers and the tile its pace: 28 heads of 128 on 4, six portions of 300 tokens
+// behind up to 3,800: 162 us; prompts of 2,048 of 16 heads each with its own keys 86 us against 67 with the pages read back.)
+//
+// A row of the cache that is not finite arrives as a key of NaN and a value of 0 (read_kv_fp8_spans): the scores against it are
+// NaN where a query sees it and masked away where none does, and 0 times the value is 0.  What lies behind a request's last
+// position in its last page is 0.
+//
+// The running maximum is raised only when it grows by more than 2^8; O is then scaled in tensor memory.  Warps: 0 brings keys
+// and values (TMA, two places each), 1 the queries and issues the products, 2 - 5 and 6 - 9 are the sub-tiles' rows.  Every wait
+// is bounded (status 3).  Tiles with many key blocks may be cut into runs, which a second kernel adds up in their order (items:
+// as the plan of the kernel above, with tokens for rows and kv heads for heads).
+#include "tc_common.cuh"
+#include "api.h"
+
+namespace {
+using namespace fxtc;
+
+constexpr int BQ = 128, BK = 128, NTHREADS = 320, TMEM_COLS = 512, ITEM_INTS = 8;
+constexpr float RAISE_MAX_BY = 8.f;   // in powers of two
+
+struct Args {
+    const int* block_table; int table_width, n_pages;       // [entries][blocks of 128 positions]
+    const int* items;
+    bf16* out; long ldo;
+    float *part_o, *part_ml;
+    int n_kv_heads, group, per_sub, head_dim, window;     // per_sub: tokens of a sub-tile
+    float scale_log2e;
+    int* status;
+};
+
+template <int D> struct Smem {
+    static constexpr int HALVES = D / 64, SUB = 128 * 128, TILE = HALVES * SUB;         // a [128 rows][128 bytes] piece; a tile
+    static constexpr int K_OFF = 2 * TILE, V_OFF = 4 * TILE, TOTAL = 6 * TILE + 1024;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int D>
+__global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __grid_constant__ CUtensorMap map_q,
+                                                                      const __grid_constant__ CUtensorMap map_k,
+                                                                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a)
+{
+    using L = Smem<D>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int abort_flag_s;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ __align__(8) uint64_t bars_s[16];
+    volatile int* abort_flag = &abort_flag_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    auto bar = [&](int i) { return smem_u32(&bars_s[i]); };
+    const uint32_t q_full = bar(0);
+    auto s_full = [&](int t) { return bar(1 + t); };
+    auto p_full = [&](int t) { return bar(3 + t); };
+    auto o_done = [&](int t) { return bar(5 + t); };
+    auto k_full = [&](int b) { return bar(7 + b); };
+    auto v_full = [&](int b) { return bar(9 + b); };
+    auto kv_empty = [&](int b) { return bar(11 + b); };
+    const uint32_t drained = bar(13);
+
+    const int* item = a.items + (long)blockIdx.y * ITEM_INTS;
+    const int tok0 = item[0], n_tok = item[1], entry = item[2], pos0 = item[3], kb_begin = item[4], kb_end = item[5], part = item[6];
+    const int kvh = blockIdx.x, per = a.per_sub, nt = n_tok > per ? 2 : 1;
+    auto tokens_of = [&](int t) { return min(per, n_tok - t * per); };
+    auto lo_of = [&](int t) { return max(fx_first_key(pos0 + t * per, a.window, 0) / BK, kb_begin); };
+    auto hi_of = [&](int t) { return min((pos0 + t * per + tokens_of(t) - 1) / BK, kb_end - 1); };
+    const int lo0 = lo_of(0), hi0 = hi_of(0), lo1 = nt > 1 ? lo_of(1) : 1, hi1 = nt > 1 ? hi_of(1) : 0;      // (none: lo > hi)
+    const bool act0 = lo0 <= hi0, act1 = lo1 <= hi1;
+    const int first_blk = act0 && act1 ? min(lo0, lo1) : act0 ? lo0 : lo1, last_blk = act0 && act1 ? max(hi0, hi1) : act0 ? hi0 : hi1;
+    const int n_walk = max(0, last_blk - first_blk + 1);
+    auto active = [&](int t, int i) { const int j = first_blk + i; return t < nt && i < n_walk && j >= (t ? lo1 : lo0) && j <= (t ? hi1 : hi0); };
+    auto last_of = [&](int t) { return (t ? act1 : act0) ? (t ? hi1 : hi0) - first_blk : -1; };
+
+    if (threadIdx.x == 0) {
+        abort_flag_s = 0;
+        for (int i = 0; i < 14; ++i) mbar_init(bar(i), i == 3 || i == 4 ? 4 : 1);      // (p_full: four warps)
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&tmem_base_s)), "r"((uint32_t)TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+    fx_pdl_wait();   // set up while the kernel before this one drains; its results from here on
+    auto tmem_s = [&](int t) { return tmem + 128u * t; };            // S_t, and P_t over its first 64 columns
+    auto tmem_o = [&](int t) { return tmem + 256u + 128u * t; };
+
+    int asked = 0;                                                   // blocks under way or there
+    if (warp == 1) {
+        // ---------------- the queries; products: PV_0(i), S_0(i + 1), PV_1(i), S_1(i + 1) ----------------
+        if (lane == 0) {
+            mbar_expect_tx(q_full, (uint32_t)(nt * L::HALVES * per * a.group * 128));
+            for (int t = 0; t < nt; ++t)
+                for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + t * L::TILE + h * L::SUB, &map_q, h * 64, 0, kvh, tok0 + t * per, q_full);
+            constexpr uint32_t idesc_s = instr_desc_ex(BQ, BK, 0), idesc_o = instr_desc_ex(BQ, D, 1);
+            int k_ready = -1, n_p[2] = {0, 0};
+            const int last0 = last_of(0), last1 = last_of(1);
+            bool ok = mbar_wait(q_full, 0, abort_flag);
+            auto issue_s = [&](int t, int i) {
+                const int b = i & 1;
+                if (k_ready < i) {
+                    if (!mbar_wait(k_full(b), (uint32_t)(i >> 1) & 1u, abort_flag)) return false;
+                    k_ready = i;
+                    tc_fence_after();
+                }
+#pragma unroll
+                for (int h = 0; h < L::HALVES; ++h) {
+                    const uint64_t dq = smem_desc(base + t * L::TILE + h * L::SUB), dk = smem_desc(base + L::K_OFF + b * L::TILE + h * L::SUB);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc_mma(tmem_s(t), dq + 2u * k, dk + 2u * k, idesc_s, (h | k) != 0);
+                }
+                tc_commit(s_full(t));
+                return true;
+            };
+            for (int t = 0; t < nt && ok; ++t)
+                if (active(t, 0)) ok = issue_s(t, 0);
+            for (int i = 0; i < n_walk && ok; ++i) {
+                const int b = i & 1;
+                bool v_ready = false;
+                for (int t = 0; t < nt && ok; ++t) {
+                    if (active(t, i)) {
+                        ok = mbar_wait(p_full(t), (uint32_t)n_p[t] & 1u, abort_flag);
+                        if (ok && !v_ready) { ok = mbar_wait(v_full(b), (uint32_t)(i >> 1) & 1u, abort_flag); v_ready = true; }
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int ks = 0; ks < BK / 16; ++ks)
+                            tc_mma_ts(tmem_o(t), tmem_s(t) + 8u * ks, smem_desc_lbo_sbo(base + L::V_OFF + b * L::TILE + ks * 2048, L::SUB, 1024), idesc_o,
+                                      (n_p[t] | ks) != 0);
+                        ++n_p[t];
+                        if (i == (t ? last1 : last0)) tc_commit(o_done(t));
+                    }
+                    if (t == nt - 1) tc_commit(kv_empty(b));   // every product that reads this block has been issued
+                    if (active(t, i + 1)) ok = issue_s(t, i + 1);
+                }
+            }
+            if (*abort_flag) {                                  // given up: no product may outlive tensor memory
+                tc_commit(drained);
+                for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(drained, 0); ++i) { }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 0) {
+        // ---------------- keys and values: a block is a page ----------------
+        if (lane == 0) {
+            const int* table = a.block_table + (long)entry * a.table_width;
+            for (int i = 0; i < n_walk; ++i, ++asked) {
+                const int b = i & 1, j = first_blk + i, found = j < a.table_width ? table[j] : -1, page = found < 0 ? a.n_pages : found;   // (none: zeros)
+                if (!mbar_wait(kv_empty(b), (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag)) break;
+                mbar_expect_tx(k_full(b), (uint32_t)L::TILE);
+                for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + L::K_OFF + b * L::TILE + h * L::SUB, &map_k, h * 64, 0, kvh, page, k_full(b));
+                mbar_expect_tx(v_full(b), (uint32_t)L::TILE);
+                for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + L::V_OFF + b * L::TILE + h * L::SUB, &map_v, h * 64, 0, kvh, page, v_full(b));
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------- softmax: a row a thread ----------------
+        const int t = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;      // (tensor memory: a warp may touch lanes 32 (warp % 4) ..)
+        if (t < nt) {
+            const int rows_t = tokens_of(t) * a.group, tok = r / a.group, pos_t = pos0 + t * per, p_r = pos_t + tok;
+            const int lo_r = fx_first_key(p_r, a.window, 0), lo_last = fx_first_key(pos_t + tokens_of(t) - 1, a.window, 0);
+            const uint32_t lane_off = (uint32_t)(quad * 32) << 16, ts = tmem_s(t) + lane_off, to = tmem_o(t) + lane_off;
+            float m = -INFINITY, l = 0.f;
+            bool ok = true;
+            int cnt = 0;
+            for (int i = 0; i < n_walk; ++i) {
+                if (!active(t, i)) continue;
+                ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), (uint32_t)cnt & 1u, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+                if (quad * 32 >= rows_t) {               // none of the warp's rows exists: what its rows of P hold reaches no others
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full(t));
+                    ++cnt;
+                    continue;
+                }
+                const int kb = (first_blk + i) * BK;
+                const bool interior = kb + BK - 1 <= pos_t && kb >= lo_last;   // every row sees all of the block: no masking (most blocks)
+                uint32_t ca[32], cb[32], pk[32];
+                auto mask = [&](uint32_t* c, int chunk, uint32_t with) {
+                    if (interior) return;
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        const int key = kb + chunk * 32 + k;
+                        if (key > p_r || key < lo_r) c[k] = with;
+                    }
+                };
+                constexpr uint32_t MINUS_INF = 0xff800000u, NO_NUMBER = 0x7fffffffu;
+                // first pass: the row's maximum (the next 32 columns are on their way while these are looked at)
+                float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+                auto take_max = [&](uint32_t* c, int chunk) {
+                    mask(c, chunk, NO_NUMBER);           // (what fmaxf passes over)
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        mx0 = fmaxf(mx0, __uint_as_float(c[k])); mx1 = fmaxf(mx1, __uint_as_float(c[k + 1]));
+                        mx2 = fmaxf(mx2, __uint_as_float(c[k + 2])); mx3 = fmaxf(mx3, __uint_as_float(c[k + 3]));
+                    }
+                };
+                tc_ld32(ts, ca);
+                tc_ld_wait_for(ca);
+                tc_ld32(ts + 32, cb); take_max(ca, 0); tc_ld_wait_for(cb);
+                tc_ld32(ts + 64, ca); take_max(cb, 1); tc_ld_wait_for(ca);
+                tc_ld32(ts + 96, cb); take_max(ca, 2); tc_ld_wait_for(cb);
+                tc_ld32(ts, ca);      take_max(cb, 3);   // the first columns again, for the second pass
+                const float mn = fmaxf(m, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)));
+                const bool raise = r < rows_t && mn > m && (m == -INFINITY || (mn - m) * a.scale_log2e > RAISE_MAX_BY);
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float alpha = m == -INFINITY ? 0.f : exp2_fast((m - mn) * a.scale_log2e);
+                    l *= alpha;
+                    m = mn;
+                    if (cnt > 0) {
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            tc_ld32(to + c * 32, cb);
+                            tc_ld_wait_for(cb);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) cb[k] = __float_as_uint(__uint_as_float(cb[k]) * alpha);
+                            tc_st32(to + c * 32, cb);
+                        }
+                    }
+                }
+                // second pass: weights in bfloat16 pairs over the first 64 columns of S, each behind its last reading
+                const float ref = m == -INFINITY ? 0.f : m * a.scale_log2e;
+                float sum0 = 0.f, sum1 = 0.f;
+                auto take_exp = [&](uint32_t* c, int chunk, uint32_t* out) {
+                    mask(c, chunk, MINUS_INF);
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        const float e0 = exp2_fast(fmaf(__uint_as_float(c[k]), a.scale_log2e, -ref)), e1 = exp2_fast(fmaf(__uint_as_float(c[k + 1]), a.scale_log2e, -ref));
+                        sum0 += e0; sum1 += e1;
+                        __nv_bfloat162 pr = __floats2bfloat162_rn(e0, e1);
+                        out[k >> 1] = *reinterpret_cast<uint32_t*>(&pr);
+                    }
+                };
+                tc_ld_wait_for(ca);
+                tc_ld32(ts + 32, cb); take_exp(ca, 0, pk);      tc_ld_wait_for(cb);
+                tc_ld32(ts + 64, ca); take_exp(cb, 1, pk + 16); tc_ld_wait_for(ca);
+                tc_ld32(ts + 96, cb);
+                tc_st32(ts, pk);
+                take_exp(ca, 2, pk);
+                tc_ld_wait_for(cb);
+                take_exp(cb, 3, pk + 16);
+                tc_st32(ts + 32, pk);
+                l += sum0 + sum1;
+                tc_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(t));
+                ++cnt;
+            }
+            const bool has = last_of(t) >= 0;
+            if (ok && has) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), 0, abort_flag));
+            if (ok) {
+                tc_fence_after();
+                const long slot = ((long)max(part, 0) * a.n_kv_heads + kvh) * (2 * BQ) + t * BQ + r;
+                if (part >= 0 && r < rows_t) { a.part_ml[slot * 2] = has ? m * a.scale_log2e : -INFINITY; a.part_ml[slot * 2 + 1] = has ? l : 0.f; }
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                bf16* dst = a.out + (long)(tok0 + t * per + tok) * a.ldo + ((long)kvh * a.group + r % a.group) * a.head_dim;
+                if (has || part < 0)
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t ob[32];
+                        __syncwarp();
+                        if (has) { tc_ld32(to + c * 32, ob); tc_ld_wait(); }
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            if (r >= rows_t || c * 32 + k >= a.head_dim) continue;
+                            if (part >= 0) {
+                                float* o = a.part_o + slot * D + c * 32 + k;
+                                *reinterpret_cast<uint4*>(o) = make_uint4(ob[k], ob[k + 1], ob[k + 2], ob[k + 3]);
+                                *reinterpret_cast<uint4*>(o + 4) = make_uint4(ob[k + 4], ob[k + 5], ob[k + 6], ob[k + 7]);
+                            } else {
+                                float x[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : __uint_as_float(ob[k + e]) * inv;
+                                Pack<bf16>::store(dst + c * 32 + k, x);
+                            }
+                        }
+                    }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)TMEM_COLS) : "memory");
+    }
+    if (threadIdx.x == 0 && abort_flag_s) {
+        // given up: the copies under way still land
+        auto settle = [](uint32_t at, uint32_t parity) { for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(at, parity); ++i) { } };
+        settle(q_full, 0);
+        for (int i = max(0, asked - 2); i < asked; ++i) { settle(k_full(i & 1), (uint32_t)(i >> 1) & 1u); settle(v_full(i & 1), (uint32_t)(i >> 1) & 1u); }
+        if (a.status) atomicExch(a.status, STATUS_TC_TIMEOUT);
+    }
+}
+
+// The runs of a tile that was cut: merges int32 [n][4] = (first token, tokens, first part, runs); a warp a row.
+template <int D> __global__ void __launch_bounds__(128) prefill_grouped_merge_kernel(const int* __restrict__ merges, const __grid_constant__ Args a)
+{
+    fx_pdl_wait();
+    const int* mg = merges + (long)blockIdx.x * 4;
+    const int tok0 = mg[0], n_tok = mg[1], part0 = mg[2], runs = mg[3], kvh = blockIdx.y;
+    const int lane = threadIdx.x & 31, row = blockIdx.z * 4 + (threadIdx.x >> 5), t = row / BQ, r = row % BQ;
+    if (r >= min(a.per_sub, n_tok - t * a.per_sub) * a.group) return;      // (a whole warp)
+    constexpr int PER = D / 32;
+    const long slot0 = ((long)part0 * a.n_kv_heads + kvh) * (2 * BQ) + row, step = (long)a.n_kv_heads * (2 * BQ);
+    float m = -INFINITY, l = 0.f;                                            // lane c: run c's (at most 32)
+    if (lane < runs) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (slot0 + lane * step) * 2);
+        m = ml.x; l = ml.y;
+    }
+    const float top = warp_max(m), w = l == 0.f ? 0.f : exp2f(m - top), sum = warp_sum(l * w);
+    float acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < runs; ++c) {
+        const float wc = __shfl_sync(0xffffffffu, w, c);
+        if (wc == 0.f) continue;                                             // (a run without keys for this row has written no sums)
+        const float* src = a.part_o + (slot0 + c * step) * D + lane * PER;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = fmaf(src[i], wc, acc[i]);
+    }
+    bf16* dst = a.out + (long)(tok0 + t * a.per_sub + r / a.group) * a.ldo + ((long)kvh * a.group + r % a.group) * a.head_dim + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (lane * PER + i < a.head_dim) dst[i] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc[i] / sum);
+}
+
+template <int D>
+int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int n_items, const int* merges, int n_merges, cudaStream_t s)
+{
+    auto kern = prefill_grouped_kernel<D>;
+    // of the current device: asked for each time
+    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL)) return (int)e;
+    fx_launch_pdl(kern, dim3(a.n_kv_heads, n_items), NTHREADS, Smem<D>::TOTAL, s, mq, mk, mv, a);
+    if (n_merges > 0) fx_launch_pdl(prefill_grouped_merge_kernel<D>, dim3(n_merges, a.n_kv_heads, 2 * BQ / 4), 128, 0, s, merges, a);
+    return fx_launch_status();
+}
+
+bool encode(CUtensorMap* map, const void* ptr, cuuint64_t d0, cuuint64_t d1, cuuint64_t d2, cuuint64_t d3, cuuint64_t s1, cuuint64_t s2, cuuint64_t s3,
+            cuuint32_t b1, cuuint32_t b3)
+{
+    EncodeTiledFn fn = encode_fn();
+    const cuuint64_t dims[4] = {d0, d1, d2, d3}, strides[3] = {s1 * 2, s2 * 2, s3 * 2};
+    const cuuint32_t box[4] = {64, b1, 1, b3}, ones[4] = {1, 1, 1, 1};
+    return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+// Keys and values: pages [n_pages][kv heads][128][head_dim], block_table [entries][table_width] names those of an entry's positions
+// 128 j .. 128 j + 127.  items: int32 [n_items][8] = (first flat token, tokens, entry, position of the first token, first key block, end
+// of the key blocks, part or -1, 0); a tile holds up to 2 * (128 / group) tokens, group = n_heads / n_kv_heads <= 128.  part_o [parts][kv
+// heads][256][64 or 128], part_ml [parts][kv heads][256][2].
+extern "C" int fx_prefill_attention_grouped(const void* q, long ldq, int n_tokens, const void* k_pages, const void* v_pages, int n_pages,
+                                            const int* block_table, int table_width, const int* items, int n_items, void* out, long ldo,
+                                            int n_heads, int n_kv_heads, int head_dim, int window, float scale, float* part_o, float* part_ml,
+                                            const int* merges, int n_merges, int* status, void* stream)
+{
+    if (n_items <= 0 || n_tokens <= 0) return FX_OK;
+    if (head_dim <= 0 || head_dim > 128 || head_dim % 16 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > BQ ||
+        n_pages <= 0 || table_width <= 0 || window < 0 || !(scale > 0.f) || n_items > 65535 || n_kv_heads > 65535 ||
+        (n_merges > 0 && (!part_o || !part_ml || !merges))) return FX_ERR_SIZE;
+    if (ldq % 8 || ldo % 8 || (uintptr_t)q % 16 || (uintptr_t)out % 16 || (uintptr_t)k_pages % 16 || (uintptr_t)v_pages % 16 || (uintptr_t)part_o % 16)
+        return FX_ERR_ALIGN;
+    const int group = n_heads / n_kv_heads, per = BQ / group;
+    const Args a = {block_table, table_width, n_pages, items, (bf16*)out, ldo, part_o, part_ml, n_kv_heads, group, per, head_dim, window,
+                    scale * 1.4426950408889634f, status};
+    CUtensorMap mq, mk, mv;
+    const cuuint64_t W = head_dim, G = n_kv_heads;
+    if (!encode(&mq, q, W, group, G, n_tokens, W, W * group, ldq, group, per) || !encode(&mk, k_pages, W, BK, G, n_pages, W, BK * W, G * BK * W, BK, 1) ||
+        !encode(&mv, v_pages, W, BK, G, n_pages, W, BK * W, G * BK * W, BK, 1)) return FX_ERR_SIZE;
+    cudaStream_t s = (cudaStream_t)stream;
+    return head_dim <= 64 ? launch<64>(mq, mk, mv, a, n_items, merges, n_merges, s) : launch<128>(mq, mk, mv, a, n_items, merges, n_merges, s);
+}

@@ -181,7 +181,7 @@ struct ReadArgs {
     const uint8_t *k_pages, *v_pages, *k_exp, *v_exp;
     const int* block_table; int n_slots, table_width, page_size, n_pages;
     const int *positions, *token_seq, *seq_slot;
-    const int* spans; int n_spans, n_rows;
+    const int* spans; int n_spans, n_rows, out_page, attend;
     void *k_out, *v_out;
     int n_kv_heads, head_dim;
 };
@@ -238,14 +238,16 @@ __global__ void __launch_bounds__(READ_THREADS) read_rows_kernel(ReadArgs a)
     }
 }
 
-// Stretches of requests (spans: entry, first position, end, first row; first position and row at a page's start, rows in
-// order) into pages [page of the rows][kv head][position][head_dim].  A block takes a page of a head, keys or values; what
-// lies behind a stretch's end in its last page is 0.
+// Stretches of requests (spans: entry, first position, end, first row; first rows at a page's start, in order) into pages
+// [page of the rows][kv head][position][head_dim] of out_page positions, which need not be the cache's.  A block takes a page of
+// a head, keys or values; what lies behind a stretch's end in its last page is 0.  For attention: a position of which the key or
+// the value is not finite becomes a key of NaN and a value of 0, so that it makes those queries' results NaN that see it, and no
+// other's (a weight of 0 times NaN is none).
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) read_spans_kernel(ReadArgs a)
+__global__ void __launch_bounds__(READ_THREADS) read_spans_kernel(ReadArgs a)
 {
     fx_pdl_wait();
-    const int D = a.head_dim, P = a.page_size, row0 = blockIdx.x * P, per_row = D / VEC;
+    const int D = a.head_dim, P = a.out_page, row0 = blockIdx.x * P, per_row = D / VEC, n = P * per_row;
     int lo = 0, hi = a.n_spans - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -255,19 +257,34 @@ __global__ void __launch_bounds__(256) read_spans_kernel(ReadArgs a)
     const int* span = a.spans + 4 * lo;
     const int pos0 = span[1] + row0 - span[3], live = min(P, span[2] - pos0);
     const int slot = a.seq_slot[span[0]], h = blockIdx.y >> 1;
-    const bool is_v = blockIdx.y & 1;
-    const int page = live > 0 && slot >= 0 && slot < a.n_slots
-        ? fx_page_of(a.block_table + (long)slot * a.table_width, a.table_width, a.n_pages, pos0, P) : -1;
-    const long at = ((long)max(page, 0) * a.n_kv_heads + h) * P;
-    const uint8_t* src = (is_v ? a.v_pages : a.k_pages) + at * D;
-    const uint8_t* exps = (is_v ? a.v_exp : a.k_exp) + at;
+    const bool is_v = blockIdx.y & 1, known = slot >= 0 && slot < a.n_slots;
+    const int* table = a.block_table + (long)(known ? slot : 0) * a.table_width;
+    const uint8_t *pages = is_v ? a.v_pages : a.k_pages, *own = is_v ? a.v_exp : a.k_exp, *other = is_v ? a.k_exp : a.v_exp;
     T* dst = reinterpret_cast<T*>(is_v ? a.v_out : a.k_out) + ((long)blockIdx.x * a.n_kv_heads + h) * P * D;
-    for (int i = threadIdx.x; i < P * per_row; i += blockDim.x) {
-        const int r = i / per_row;
-        const bool there = page >= 0 && r < live;
-        const float scale = there ? fx_fp8_scale(exps[r]) : 0.f;
-        if constexpr (VEC == 16) put16(dst + i * 16, there ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0), scale);
-        else dst[i] = from_f32<T>(there ? fx_fp8_float2(src[i]).x * scale : 0.f);
+    for (int i0 = threadIdx.x; i0 < n; i0 += READ_AHEAD * READ_THREADS) {
+        uint4 w[READ_AHEAD];
+        float scale[READ_AHEAD];
+#pragma unroll
+        for (int u = 0; u < READ_AHEAD; ++u) {
+            const int i = i0 + u * READ_THREADS, r = i / per_row;
+            w[u] = make_uint4(0, 0, 0, 0);
+            scale[u] = 0.f;
+            const int page = i < n && r < live && known ? fx_page_of(table, a.table_width, a.n_pages, pos0 + r, a.page_size) : -1;
+            if (page < 0) continue;
+            const long at = ((long)page * a.n_kv_heads + h) * a.page_size + (pos0 + r) % a.page_size;
+            const uint8_t* src = pages + at * D + (i - r * per_row) * VEC;
+            if constexpr (VEC == 16) w[u] = *reinterpret_cast<const uint4*>(src);
+            else w[u].x = *src;
+            const int e = own[at];
+            scale[u] = a.attend && (e == FX_FP8_NAN || other[at] == FX_FP8_NAN) ? (is_v ? 0.f : __uint_as_float(0x7fc00000u)) : fx_fp8_scale(e);
+        }
+#pragma unroll
+        for (int u = 0; u < READ_AHEAD; ++u) {
+            const int i = i0 + u * READ_THREADS;
+            if (i >= n) continue;
+            if constexpr (VEC == 16) put16(dst + (long)i * 16, w[u], scale[u]);
+            else dst[i] = from_f32<T>(fx_fp8_float2(w[u].x).x * scale[u]);
+        }
     }
 }
 
@@ -319,21 +336,21 @@ extern "C" int fx_rope_kv_write_fp8(void* qkv, int dtype, long ld, const int* po
 // spans null: the rows of the lists positions, token_seq; else n_spans stretches of n_rows rows together.
 extern "C" int fx_read_kv_fp8(const void* k_pages, const void* v_pages, const void* k_exp, const void* v_exp, const int* block_table,
                               int n_slots, int table_width, int page_size, int n_pages, const int* positions, const int* token_seq,
-                              const int* seq_slot, const int* spans, int n_spans, int n_rows, void* k_out, void* v_out, int dtype,
+                              const int* seq_slot, const int* spans, int n_spans, int n_rows, int out_page, int attend, void* k_out, void* v_out, int dtype,
                               int n_kv_heads, int head_dim, void* stream)
 {
     if (n_rows <= 0 || n_kv_heads <= 0) return FX_OK;
     if (head_dim <= 0 || page_size <= 0 || n_pages <= 0 || n_slots <= 0 || table_width <= 0 || n_kv_heads > 32767) return FX_ERR_SIZE;
     if (dtype != FX_F32 && dtype != FX_BF16) return FX_ERR_DTYPE;
     const ReadArgs a = {(const uint8_t*)k_pages, (const uint8_t*)v_pages, (const uint8_t*)k_exp, (const uint8_t*)v_exp, block_table, n_slots,
-                        table_width, page_size, n_pages, positions, token_seq, seq_slot, spans, n_spans, n_rows, k_out, v_out, n_kv_heads, head_dim};
+                        table_width, page_size, n_pages, positions, token_seq, seq_slot, spans, n_spans, n_rows, out_page, attend, k_out, v_out, n_kv_heads, head_dim};
     const bool vec = head_dim % 16 == 0 && (uintptr_t)k_pages % 16 == 0 && (uintptr_t)v_pages % 16 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0;
     cudaStream_t s = (cudaStream_t)stream;
     if (spans) {
-        if (n_spans <= 0 || n_rows % page_size || (long)page_size * head_dim > (1L << 30)) return FX_ERR_SIZE;
-        const dim3 grid(n_rows / page_size, 2 * n_kv_heads);
-        if (dtype == FX_F32) vec ? fx_launch_pdl(read_spans_kernel<float, 16>, grid, 256, 0, s, a) : fx_launch_pdl(read_spans_kernel<float, 1>, grid, 256, 0, s, a);
-        else vec ? fx_launch_pdl(read_spans_kernel<bf16, 16>, grid, 256, 0, s, a) : fx_launch_pdl(read_spans_kernel<bf16, 1>, grid, 256, 0, s, a);
+        if (n_spans <= 0 || out_page <= 0 || n_rows % out_page || (long)out_page * head_dim > (1L << 30)) return FX_ERR_SIZE;
+        const dim3 grid(n_rows / out_page, 2 * n_kv_heads);
+        if (dtype == FX_F32) vec ? fx_launch_pdl(read_spans_kernel<float, 16>, grid, READ_THREADS, 0, s, a) : fx_launch_pdl(read_spans_kernel<float, 1>, grid, READ_THREADS, 0, s, a);
+        else vec ? fx_launch_pdl(read_spans_kernel<bf16, 16>, grid, READ_THREADS, 0, s, a) : fx_launch_pdl(read_spans_kernel<bf16, 1>, grid, READ_THREADS, 0, s, a);
         return fx_launch_status();
     }
     const dim3 blocks(n_rows, (unsigned)fx_cdiv(2L * n_kv_heads * (head_dim / (vec ? 16 : 1)), READ_THREADS * READ_AHEAD));

@@ -124,9 +124,10 @@ _SIGNATURES = {
     "fx_decode_attention": [_P, _L, _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P, _L, _P, _P, _I, _I, _I, _I, _I, _F, _I,
                             _I, _P, _P, _I, _I, _I, _P, _F, _P, _P],
     "fx_rope_kv_write_fp8": [_P, _I, _L, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
-    "fx_read_kv_fp8": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _P],
+    "fx_read_kv_fp8": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _P],
     "fx_decode_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F,
                                 _I, _P, _P, _P, _P],
+    "fx_prefill_attention_grouped": [_P, _L, _I, _P, _P, _I, _P, _I, _P, _I, _P, _L, _I, _I, _I, _I, _F, _P, _P, _P, _I, _P, _P],
     "fx_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F, _P],
     "fx_argmax": [_P, _L, _I, _I, _P, _P],
     "fx_repetition_penalty": [_P, _L, _I, _I, _P, _P, _P, _P],
@@ -1701,7 +1702,7 @@ def prefill_tc_better(entries, window, n_heads: int, key_dim: int, value_dim: in
     return unit * max(longest, work * n_heads / sms) < 0.85 * mma
 
 
-def prefill_tc_plan(entries, window, n_heads: int, sms: int = 0, run_blocks: int = -1, chunk=None, keep_first: int = 0):
+def prefill_tc_plan(entries, window, n_heads: int, sms: int = 0, run_blocks: int = -1, chunk=None, keep_first: int = 0, tile: int = 0):
     """The work items of the tcgen05 prompt attention kernel for a step.  ``entries``: (tokens, first position) of
     each entry, in the order of the flattened batch.  A tile is up to 256 queries of one entry; it sees the key blocks
     (of 128 positions) from its first query's first visible key to its last query's own.  Tiles with many key blocks
@@ -1711,14 +1712,15 @@ def prefill_tc_plan(entries, window, n_heads: int, sms: int = 0, run_blocks: int
     :func:`_prefill_makespan`, and whole tiles stay unless a cut is 15 % faster by that estimate.  Returns (items int32 [n, 8], merges int32 [m, 4], parts) as
     ``fx_prefill_attention_tc`` takes them: heavy items first; a tile's runs have consecutive parts in the order of
     their keys.  ``keep_first`` (with a window): the positions below it stay visible; their blocks before a tile's own go to
-    its first run.  ``run_blocks`` >= 0: this many key blocks a run instead of the choice (0: no cut; tests)."""
+    its first run.  ``run_blocks`` >= 0: this many key blocks a run instead of the choice (0: no cut; tests).
+    ``tile``: tokens of a tile (default: 256)."""
     import numpy as np
 
-    sms = sms or sm_count()
+    sms, tile = sms or sm_count(), tile or WIDE_PREFILL_TILE
     tiles, flat = [], 0
     for b, (n, start) in enumerate(entries):
-        for i in range(0, n, WIDE_PREFILL_TILE):
-            rows, pos0 = min(WIDE_PREFILL_TILE, n - i), start + i
+        for i in range(0, n, tile):
+            rows, pos0 = min(tile, n - i), start + i
             first = first_key(pos0, window, chunk) // PREFILL_KEY_BLOCK
             end = (pos0 + rows - 1) // PREFILL_KEY_BLOCK + 1
             kept = min(first, -(-keep_first // PREFILL_KEY_BLOCK)) if window else 0
@@ -2099,7 +2101,7 @@ def rope_kv_write_fp8(qkv, positions, token_seq, seq_slot, inv_freq, rotary_dim,
          G, D, int(write_cache), zp, stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
 
 
-_READ_FP8, _READ_FP8_SPANS = "eNGPD eNGPD uNGP uNGP iSW iT iT iB xTGD xTGD", "eNGPD eNGPD uNGP uNGP iSW in4 iB xMGPD xMGPD"
+_READ_FP8, _READ_FP8_SPANS = "eNGPD eNGPD uNGP uNGP iSW iT iT iB xTGD xTGD", "eNGPD eNGPD uNGP uNGP iSW in4 iB xMGRD xMGRD"
 
 
 def read_kv_fp8(k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, k_out, v_out, stream=None):
@@ -2109,23 +2111,25 @@ def read_kv_fp8(k_pages, v_pages, k_exp, v_exp, block_table, page_size, position
         "read_kv_fp8", _READ_FP8, _CACHE_FP8 + _STEP + ("k_out", "v_out"), k_pages, v_pages, k_exp, v_exp, block_table, positions, token_seq,
         seq_slot, k_out, v_out)
     _check_fp8("read_kv_fp8", (N, G, P, D), page_size, None, None)
-    call("fx_read_kv_fp8", kp, vp, kep, vep, tp, S, W, page_size, N, pp, sp, lp, 0, 0, T, ko, vo, x, G, D,
+    call("fx_read_kv_fp8", kp, vp, kep, vep, tp, S, W, page_size, N, pp, sp, lp, 0, 0, T, 1, 0, ko, vo, x, G, D,
          stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
 
 
-def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, spans, n_rows, seq_slot, k_out, v_out, stream=None):
+def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, spans, n_rows, seq_slot, k_out, v_out, stream=None,
+                      attend=False):
     """Stretches of requests out of an 8-bit cache into pages that the other attention kernels take: ``k_out``, ``v_out`` [n_rows /
-    page, kv heads, page, head_dim].  ``spans``: int32 [n, 4] rows of (entry, first position, end, first row), first positions and
-    rows multiples of the page, the rows in order and without gaps up to ``n_rows``.  What lies behind a stretch's end in its last
-    page is 0, and so is a page that its request does not have."""
+    R, kv heads, R, head_dim] with pages of R positions, the cache's or others.  ``spans``: int32 [n, 4] rows of (entry, first position,
+    end, first row), first rows multiples of R, the rows in order and without gaps up to ``n_rows``.  What lies behind a stretch's end
+    in its last page is 0, and so is a position without a page.  ``attend``: a position of which the key or the value is not finite is
+    read as a key of NaN and a value of 0, which makes the results NaN of the queries that see it and of no others."""
     name = "read_kv_fp8_spans"
-    (_, now, x, kp, vp, kep, vep, tp, np_, lp, ko, vo, N, G, P, D, S, W, n, four, _, M) = _operands(
+    (_, now, x, kp, vp, kep, vep, tp, np_, lp, ko, vo, N, G, P, D, S, W, n, four, _, M, R) = _operands(
         name, _READ_FP8_SPANS, _CACHE_FP8 + ("spans", "seq_slot", "k_out", "v_out"), k_pages, v_pages, k_exp, v_exp, block_table, spans, seq_slot,
         k_out, v_out)
     _check_fp8(name, (N, G, P, D), page_size, None, None)
-    if n_rows != M * P or four != 4 or (M and not n):
-        raise KernelError(f"{name}: spans [n, 4] over {n_rows} rows, {M} pages of {P}: found [{n}, {four}]")
-    call("fx_read_kv_fp8", kp, vp, kep, vep, tp, S, W, page_size, N, 0, 0, lp, np_, n, n_rows, ko, vo, x, G, D,
+    if n_rows != M * R or four != 4 or (M and not n):
+        raise KernelError(f"{name}: spans [n, 4] over {n_rows} rows, {M} pages of {R}: found [{n}, {four}]")
+    call("fx_read_kv_fp8", kp, vp, kep, vep, tp, S, W, page_size, N, 0, 0, lp, np_, n, n_rows, R, int(attend), ko, vo, x, G, D,
          stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
 
 
@@ -2212,6 +2216,7 @@ def _decode_fp8(found, page_size, n_heads, window, scale, softcap, stream):
 
 FP8_FEW_TOKENS = 8                # entries that bring at most this many tokens are left to decode_attention_fp8
 FP8_READ_BACK_MAX = 1 << 30       # bytes of keys and values that are read back at a time
+FP8_READ_PAGE = 128               # positions of a page that is read back (whatever the cache's: what every tiled kernel takes)
 
 
 class PrefillFp8Plan:
@@ -2270,8 +2275,8 @@ class PrefillFp8Plan:
                                                        for g in self._groups(window, row_bytes)])
 
     def _rows_of(self, n, start, window):
-        p0 = first_key(start, window) // self.page_size * self.page_size
-        return p0, -(-(start + n - p0) // self.page_size) * self.page_size
+        p0 = first_key(start, window) // FP8_READ_PAGE * FP8_READ_PAGE
+        return p0, -(-(start + n - p0) // FP8_READ_PAGE) * FP8_READ_PAGE
 
     def _groups(self, window, row_bytes):
         groups, flat, rows, end = [], 0, 0, -1
@@ -2289,7 +2294,7 @@ class PrefillFp8Plan:
     def _part(self, window, group):
         import numpy as np
 
-        P, spans, row = self.page_size, [], 0
+        P, spans, row = FP8_READ_PAGE, [], 0
         for b, _, n, start in group:
             p0, rows = self._rows_of(n, start, window)
             spans.append((b, p0, start + n, row))
@@ -2321,8 +2326,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     :func:`decode_attention_fp8`, ``plan``: :func:`prefill_fp8_plan` of the step's entries.
 
     The keys and values that a portion sees are read back once into pages of q's type (exact: an element has four significant bits
-    and a power of two) and the attention kernels for such pages take them from there: a tile of queries then meets operands that
-    the tensor cores take as they are, where conversion in the attention kernel would be paid again for every tile and query head.
+    and a power of two) and the attention kernels for such pages take them from there: tensor cores then meet operands that they take
+    as they are, where conversion in the attention kernel would be paid again for every tile.  Every position that is seen has a page.
     Entries of up to FP8_FEW_TOKENS tokens, and shapes that no tiled kernel takes, go to :func:`decode_attention_fp8`."""
     name = "prefill_attention_fp8"
     found = _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, status, None,
@@ -2348,11 +2353,45 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
         decode_attention_fp8(q, *cache, *step, out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status,
                              tokens=plan.few(), stream=st)
     for tok0, n, entries, spans, rows, table, slots in plan.parts(window, 2 * n_kv_heads * head_dim * q.element_size()):
-        k, v = (torch.empty(rows // page_size, n_kv_heads, page_size, head_dim, dtype=q.dtype, device=q.device) for _ in range(2))
-        read_kv_fp8_spans(*cache, spans, rows, seq_slot, k, v, stream=st)
+        k, v = (torch.empty(rows // FP8_READ_PAGE, n_kv_heads, FP8_READ_PAGE, head_dim, dtype=q.dtype, device=q.device) for _ in range(2))
+        read_kv_fp8_spans(*cache, spans, rows, seq_slot, k, v, stream=st, attend=True)
         q_part, out_part = (q, out) if n == plan.n_tokens else (q[tok0:tok0 + n], out[tok0:tok0 + n])
-        _prefill_read_back(q_part, k, v, table, page_size, plan, (tok0, window), entries, slots, out_part, n_heads, n_kv_heads, head_dim,
+        _prefill_read_back(q_part, k, v, table, FP8_READ_PAGE, plan, (tok0, window), entries, slots, out_part, n_heads, n_kv_heads, head_dim,
                            window, scale, softcap, status, st)
+    return out
+
+
+def prefill_grouped_ok(q, out, n_heads: int, n_kv_heads: int, head_dim: int, scale: float) -> bool:
+    """Whether :func:`prefill_attention_grouped` takes these operands and has something to gain: query heads that share key heads."""
+    return (q.dtype is torch.bfloat16 and n_kv_heads < n_heads <= 128 * n_kv_heads and 0 < head_dim <= 128 and head_dim % 16 == 0 and scale > 0
+            and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
+
+
+def prefill_grouped_plan(entries, window, n_heads: int, n_kv_heads: int):
+    """:func:`prefill_tc_plan` for :func:`prefill_attention_grouped`: whole tokens of all the query heads of a kv head, in two halves of
+    up to 128 rows."""
+    return prefill_tc_plan(entries, window, n_kv_heads, tile=2 * (128 * n_kv_heads // n_heads))
+
+
+def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_heads, n_kv_heads, head_dim, window, scale, status=None,
+                              stream=None, merges=None, parts=0):
+    """Attention of prompt portions in bfloat16 whose query heads share key heads, over pages of 128 positions [pages, kv heads, 128,
+    head_dim] (see :func:`prefill_grouped_ok`).  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``,
+    ``parts``: device copies of what :func:`prefill_grouped_plan` returns, and its number of parts."""
+    if k_pages.shape != v_pages.shape or k_pages.shape[1:] != (n_kv_heads, 128, head_dim) or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise KernelError(f"prefill_attention_grouped: contiguous pages [pages, {n_kv_heads}, 128, {head_dim}], found {tuple(k_pages.shape)} and "
+                          f"{tuple(v_pages.shape)}")
+    po = pm = n_merges = 0
+    if parts:
+        global _launches
+        _launches += 1
+        width, n_merges = 64 if head_dim <= 64 else 128, merges.shape[0]
+        work = torch.empty(parts * n_kv_heads * 256 * (width + 2), dtype=torch.float32, device=q.device)
+        po = work.data_ptr()
+        pm = po + 4 * parts * n_kv_heads * 256 * width
+    call("fx_prefill_attention_grouped", _ptr(q), _rows(q), q.shape[0], _ptr(k_pages), _ptr(v_pages), k_pages.shape[0], _ptr(block_table),
+         block_table.shape[1], _ptr(items), items.shape[0], _ptr(out), _rows(out), n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), po,
+         pm, _ptr(merges) if n_merges else 0, n_merges, _ptr(status), stream if stream is not None else stream_ptr())
     return out
 
 
@@ -2374,6 +2413,10 @@ def _prefill_read_back(q, k, v, table, page_size, plan, key, entries, slots, out
             prefill_attention_f32(q, k, v, table, page_size, tiles, slots, out, *heads, **tail)
         return
     capped = softcap is not None
+    if not capped and prefill_grouped_ok(q, out, n_heads, n_kv_heads, head_dim, scale):
+        items, merges, parts = plan.kept(("grouped", n_heads, n_kv_heads) + key, lambda: prefill_grouped_plan(entries, window, n_heads, n_kv_heads))
+        prefill_attention_grouped(q, k, v, table, items, out, *heads, status=status, stream=stream, merges=merges, parts=parts)
+        return
     if (prefill_tc_general_ok(q, q.stride(0), head_dim, k, v, page_size, out, out.stride(0), head_dim, head_dim, head_dim, scale, softcap)
             and prefill_tc_better(entries, window, n_heads, head_dim, head_dim, capped=True) if capped
             else prefill_tc_ok(q, out, k, page_size, head_dim, scale=scale)):

@@ -165,8 +165,8 @@ def test_a_plan_of_another_step():
 @pytest.mark.parametrize("most", [1, 3000, 1 << 30])
 def test_parts_hold_what_the_tokens_see(window, most, monkeypatch):
     monkeypatch.setattr(ops, "FP8_READ_BACK_MAX", most)
-    P, entries = 16, [(40, 0), (3, 100), (17, 33), (9, 0), (0, 12), (200, 7), (8, 0)]
-    plan = ops.prefill_fp8_plan(entries, P, "cpu")
+    P, entries = ops.FP8_READ_PAGE, [(40, 0), (3, 100), (17, 33), (9, 0), (0, 12), (200, 7), (8, 0)]
+    plan = ops.prefill_fp8_plan(entries, 16, "cpu")
     few = plan.few().tolist()
     seen, first = set(few), [0]
     for n, _ in entries:

@@ -241,16 +241,16 @@ def test_positions_without_a_page(what):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("G,D,P", [(2, 64, 16), (1, 128, 64), (3, 20, 5), (1, 256, 32)])
-def test_stretches_of_requests(dtype, G, D, P):
+@pytest.mark.parametrize("G,D,P,R", [(2, 64, 16, 16), (1, 128, 64, 64), (3, 20, 5, 5), (1, 256, 32, 32), (2, 128, 16, 128), (1, 48, 5, 128), (1, 64, 128, 16)])
+def test_stretches_of_requests(dtype, G, D, P, R):
     lens = [5 * P - 1, 1, 3 * P, 2 * P + 1]
     c = Cache(lens, G, D, P, 11)
     c.table[int(c.slots[2]), 1] = -1                                        # a page in the middle is missing
     spans, row = [], 0
     for b, p0, end in [(0, 2 * P, lens[0]), (1, 0, 1), (2, 0, lens[2]), (3, P, 2 * P)]:
         spans.append((b, p0, end, row))
-        row += -(-(end - p0) // P) * P
-    k_out, v_out = (torch.full((row // P, G, P, D), 7.0, dtype=DTYPES[dtype], device=DEV) for _ in range(2))
+        row += -(-(end - p0) // R) * R
+    k_out, v_out = (torch.full((row // R, G, R, D), 7.0, dtype=DTYPES[dtype], device=DEV) for _ in range(2))
     ops.read_kv_fp8_spans(*c.operands, torch.tensor(spans, dtype=torch.int32, device=DEV), row, c.slots.to(DEV), k_out, v_out)
     for which, got in ((0, k_out), (1, v_out)):
         want = torch.zeros(row, G, D, dtype=torch.float64)
@@ -413,7 +413,8 @@ PROMPT_WEIGHT = {"bf16": 2.0 ** -8, "f32": 2.0 ** -20}
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("H,G,D,P", [(4, 2, 128, 64), (4, 4, 64, 64), (6, 3, 48, 32), (2, 1, 128, 16), (5, 1, 256, 64), (4, 2, 20, 16), (2, 2, 128, 5), (8, 8, 80, 128)])
+@pytest.mark.parametrize("H,G,D,P", [(4, 2, 128, 64), (4, 4, 64, 64), (6, 3, 48, 32), (2, 1, 128, 16), (5, 1, 256, 64), (4, 2, 20, 16), (2, 2, 128, 5), (8, 8, 80, 128),
+                                     (7, 1, 128, 64), (28, 4, 64, 16), (130, 2, 16, 64), (129, 1, 32, 16), (128, 1, 64, 5), (12, 4, 112, 64)])
 def test_prompts(dtype, H, G, D, P):
     entries = [(9, 0), (1, 40), (70, 0), (8, 3), (33, 100), (130, 17)]
     c = Cache([n + s for n, s in entries], G, D, P, 16)
@@ -445,10 +446,11 @@ def test_prompts_with_a_window(dtype, window, softcap, most, monkeypatch):
         check(out, c, entries, q, H, window, 0.2, softcap, PROMPT_WEIGHT[dtype])
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f32"])
-def test_a_prompt_next_to_rows_that_are_no_numbers(dtype):
-    """Garbage behind a request's last position, and a row that only some queries see."""
-    H, G, D, P = 2, 1, 64, 64
+@pytest.mark.parametrize("dtype,H,softcap", [("bf16", 2, None), ("bf16", 1, None), ("bf16", 2, 20.0), ("f32", 2, None)])
+def test_a_prompt_next_to_rows_that_are_no_numbers(dtype, H, softcap):
+    """Garbage behind a request's last position, and a row that only some queries see; heads that share their keys, and one that
+    does not."""
+    G, D, P = 1, 64, 64
     entries = [(100, 0), (90, 30)]
     c = Cache([170, 128], G, D, P, 20)
     for which in (0, 1):
@@ -458,10 +460,37 @@ def test_a_prompt_next_to_rows_that_are_no_numbers(dtype):
     T = 190
     q = rows(T, H, G, D, DTYPES[dtype], 21)
     out = torch.empty(T, H * D, dtype=q.dtype, device=DEV)
-    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, P, DEV), *step(entries, c.slots), out, H, G, D, None, 0.1)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, P, DEV), *step(entries, c.slots), out, H, G, D, None, 0.1, softcap=softcap)
     bad = torch.isnan(out).any(-1).cpu()
     assert bad[:60].sum() == 0 and bad[60:100].all() and not bad[100:].any()
     assert torch.isfinite(out[:60]).all() and torch.isfinite(out[100:]).all()
+
+
+@pytest.mark.parametrize("H,G,D", [(6, 2, 128), (7, 1, 64), (16, 4, 80)])
+@pytest.mark.parametrize("window", [None, 100, 700])
+@pytest.mark.parametrize("run_blocks", [0, 1, 3])
+def test_prompts_of_grouped_heads_cut_into_runs(H, G, D, window, run_blocks, monkeypatch):
+    own = ops.prefill_tc_plan
+    monkeypatch.setattr(ops, "prefill_tc_plan", lambda *a, **k: own(*a, run_blocks=run_blocks, **k))
+    entries = [(60, 900), (300, 0), (19, 333)]
+    c = Cache([n + s for n, s in entries], G, D, 64, 50)
+    T = sum(n for n, _ in entries)
+    q = rows(T, H, G, D, torch.bfloat16, 51)
+    out = torch.full((T, H * D), 7.0, dtype=q.dtype, device=DEV)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out, H, G, D, window, 0.15)
+    check(out, c, entries, q, H, window, 0.15, None, PROMPT_WEIGHT["bf16"])
+
+
+def test_results_beside_a_portion_stay():
+    """Rows of a wider result behind a head's, and a tile's places that no token has, are left as they were."""
+    H, G, D = 6, 2, 64
+    entries = [(50, 0), (23, 70)]
+    c = Cache([50, 93], G, D, 64, 52)
+    q = rows(73, H, G, D, torch.bfloat16, 53)
+    out = torch.full((75, H * D + 8), 7.0, dtype=q.dtype, device=DEV)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out[:73, :H * D], H, G, D, None, 0.1)
+    assert (out[73:] == 7).all() and (out[:, H * D:] == 7).all()
+    check(out[:73, :H * D], c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT["bf16"])
 
 
 # ---- streams, graphs, order -----------------------------------------------------------------------------------------
