@@ -246,45 +246,52 @@ __global__ void __launch_bounds__(READ_THREADS) read_rows_kernel(ReadArgs a)
 template <typename T, int VEC>
 __global__ void __launch_bounds__(READ_THREADS) read_spans_kernel(ReadArgs a)
 {
+    __shared__ int place_s[READ_THREADS * READ_AHEAD];                      // of a row among the cache's positions; -1: nowhere
     fx_pdl_wait();
-    const int D = a.head_dim, P = a.out_page, row0 = blockIdx.x * P, per_row = D / VEC, n = P * per_row;
-    int lo = 0, hi = a.n_spans - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.spans[4 * mid + 3] <= row0) lo = mid;
-        else hi = mid - 1;
+    const int D = a.head_dim, P = a.out_page, row0 = blockIdx.x * P, per_row = D / VEC;
+    int before = 0;                                                         // stretches that begin at this page or before it
+    for (int i = 0; i < a.n_spans; i += READ_THREADS) {
+        const int k = i + threadIdx.x;
+        before += __syncthreads_count(k < a.n_spans && a.spans[4 * k + 3] <= row0);
     }
-    const int* span = a.spans + 4 * lo;
-    const int pos0 = span[1] + row0 - span[3], live = min(P, span[2] - pos0);
-    const int slot = a.seq_slot[span[0]], h = blockIdx.y >> 1;
+    const int4 span = *reinterpret_cast<const int4*>(a.spans + 4 * max(before - 1, 0));
+    const int pos0 = span.y + row0 - span.w, live = min(P, span.z - pos0);
+    const int slot = a.seq_slot[span.x], h = blockIdx.y >> 1;
     const bool is_v = blockIdx.y & 1, known = slot >= 0 && slot < a.n_slots;
     const int* table = a.block_table + (long)(known ? slot : 0) * a.table_width;
+    // this block's elements: the pieces from `first` on, of the page's rows from row_a on
+    const long first = (long)blockIdx.z * (READ_AHEAD * READ_THREADS), n = (long)P * per_row;
+    const int row_a = (int)(first / per_row), row_b = (int)min((long)P, (first + READ_AHEAD * READ_THREADS - 1) / per_row + 1);
+    for (int r = row_a + threadIdx.x; r < row_b; r += READ_THREADS) {
+        const int page = r < live && known ? fx_page_of(table, a.table_width, a.n_pages, pos0 + r, a.page_size) : -1;
+        place_s[r - row_a] = page < 0 ? -1 : (page * a.n_kv_heads + h) * a.page_size + (pos0 + r) % a.page_size;
+    }
+    __syncthreads();
     const uint8_t *pages = is_v ? a.v_pages : a.k_pages, *own = is_v ? a.v_exp : a.k_exp, *other = is_v ? a.k_exp : a.v_exp;
     T* dst = reinterpret_cast<T*>(is_v ? a.v_out : a.k_out) + ((long)blockIdx.x * a.n_kv_heads + h) * P * D;
-    for (int i0 = threadIdx.x; i0 < n; i0 += READ_AHEAD * READ_THREADS) {
-        uint4 w[READ_AHEAD];
-        float scale[READ_AHEAD];
+    uint4 w[READ_AHEAD];
+    int e[READ_AHEAD], e2[READ_AHEAD];
 #pragma unroll
-        for (int u = 0; u < READ_AHEAD; ++u) {
-            const int i = i0 + u * READ_THREADS, r = i / per_row;
-            w[u] = make_uint4(0, 0, 0, 0);
-            scale[u] = 0.f;
-            const int page = i < n && r < live && known ? fx_page_of(table, a.table_width, a.n_pages, pos0 + r, a.page_size) : -1;
-            if (page < 0) continue;
-            const long at = ((long)page * a.n_kv_heads + h) * a.page_size + (pos0 + r) % a.page_size;
-            const uint8_t* src = pages + at * D + (i - r * per_row) * VEC;
-            if constexpr (VEC == 16) w[u] = *reinterpret_cast<const uint4*>(src);
-            else w[u].x = *src;
-            const int e = own[at];
-            scale[u] = a.attend && (e == FX_FP8_NAN || other[at] == FX_FP8_NAN) ? (is_v ? 0.f : __uint_as_float(0x7fc00000u)) : fx_fp8_scale(e);
-        }
+    for (int u = 0; u < READ_AHEAD; ++u) {
+        const long i = first + u * READ_THREADS + threadIdx.x;
+        const int r = (int)(i / per_row), at = i < n ? place_s[r - row_a] : -1;
+        w[u] = make_uint4(0, 0, 0, 0);
+        e[u] = e2[u] = 0;
+        if (at < 0) continue;
+        const uint8_t* src = pages + (long)at * D + (i - (long)r * per_row) * VEC;
+        if constexpr (VEC == 16) w[u] = *reinterpret_cast<const uint4*>(src);
+        else w[u].x = *src;
+        e[u] = own[at];
+        if (a.attend) e2[u] = other[at];
+    }
 #pragma unroll
-        for (int u = 0; u < READ_AHEAD; ++u) {
-            const int i = i0 + u * READ_THREADS;
-            if (i >= n) continue;
-            if constexpr (VEC == 16) put16(dst + (long)i * 16, w[u], scale[u]);
-            else dst[i] = from_f32<T>(fx_fp8_float2(w[u].x).x * scale[u]);
-        }
+    for (int u = 0; u < READ_AHEAD; ++u) {
+        const long i = first + u * READ_THREADS + threadIdx.x;
+        if (i >= n) continue;
+        float scale = fx_fp8_scale(e[u]);
+        if (a.attend && (e[u] == FX_FP8_NAN || e2[u] == FX_FP8_NAN)) scale = is_v ? 0.f : __uint_as_float(0x7fc00000u);
+        if constexpr (VEC == 16) put16(dst + i * 16, w[u], scale);
+        else dst[i] = from_f32<T>(fx_fp8_float2(w[u].x).x * scale);
     }
 }
 
@@ -340,15 +347,19 @@ extern "C" int fx_read_kv_fp8(const void* k_pages, const void* v_pages, const vo
                               int n_kv_heads, int head_dim, void* stream)
 {
     if (n_rows <= 0 || n_kv_heads <= 0) return FX_OK;
-    if (head_dim <= 0 || page_size <= 0 || n_pages <= 0 || n_slots <= 0 || table_width <= 0 || n_kv_heads > 32767) return FX_ERR_SIZE;
+    if (head_dim <= 0 || page_size <= 0 || n_pages <= 0 || n_slots <= 0 || table_width <= 0 || n_kv_heads > 32767 ||
+        (long)n_pages * n_kv_heads * page_size > 0x7fffffffL) return FX_ERR_SIZE;
     if (dtype != FX_F32 && dtype != FX_BF16) return FX_ERR_DTYPE;
     const ReadArgs a = {(const uint8_t*)k_pages, (const uint8_t*)v_pages, (const uint8_t*)k_exp, (const uint8_t*)v_exp, block_table, n_slots,
                         table_width, page_size, n_pages, positions, token_seq, seq_slot, spans, n_spans, n_rows, out_page, attend, k_out, v_out, n_kv_heads, head_dim};
     const bool vec = head_dim % 16 == 0 && (uintptr_t)k_pages % 16 == 0 && (uintptr_t)v_pages % 16 == 0 && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0;
+    if ((uintptr_t)spans % 16) return FX_ERR_ALIGN;
     cudaStream_t s = (cudaStream_t)stream;
     if (spans) {
         if (n_spans <= 0 || out_page <= 0 || n_rows % out_page || (long)out_page * head_dim > (1L << 30)) return FX_ERR_SIZE;
-        const dim3 grid(n_rows / out_page, 2 * n_kv_heads);
+        const long pieces = fx_cdiv((long)out_page * (head_dim / (vec ? 16 : 1)), READ_THREADS * READ_AHEAD);
+        if (pieces > 65535) return FX_ERR_SIZE;
+        const dim3 grid(n_rows / out_page, 2 * n_kv_heads, (unsigned)pieces);
         if (dtype == FX_F32) vec ? fx_launch_pdl(read_spans_kernel<float, 16>, grid, READ_THREADS, 0, s, a) : fx_launch_pdl(read_spans_kernel<float, 1>, grid, READ_THREADS, 0, s, a);
         else vec ? fx_launch_pdl(read_spans_kernel<bf16, 16>, grid, READ_THREADS, 0, s, a) : fx_launch_pdl(read_spans_kernel<bf16, 1>, grid, READ_THREADS, 0, s, a);
         return fx_launch_status();
