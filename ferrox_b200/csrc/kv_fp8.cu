@@ -250,9 +250,9 @@ __global__ void __launch_bounds__(READ_THREADS) read_spans_kernel(ReadArgs a)
     fx_pdl_wait();
     const int D = a.head_dim, P = a.out_page, row0 = blockIdx.x * P, per_row = D / VEC;
     int before = 0;                                                         // stretches that begin at this page or before it
-    for (int i = 0; i < a.n_spans; i += READ_THREADS) {
-        const int k = i + threadIdx.x;
-        before += __syncthreads_count(k < a.n_spans && a.spans[4 * k + 3] <= row0);
+    for (int i = 0; i < a.n_spans; i += 32) {
+        const int k = i + (threadIdx.x & 31);
+        before += __popc(__ballot_sync(0xffffffffu, k < a.n_spans && a.spans[4 * k + 3] <= row0));
     }
     const int4 span = *reinterpret_cast<const int4*>(a.spans + 4 * max(before - 1, 0));
     const int pos0 = span.y + row0 - span.w, live = min(P, span.z - pos0);
@@ -262,11 +262,18 @@ __global__ void __launch_bounds__(READ_THREADS) read_spans_kernel(ReadArgs a)
     // this block's elements: the pieces from `first` on, of the page's rows from row_a on
     const long first = (long)blockIdx.z * (READ_AHEAD * READ_THREADS), n = (long)P * per_row;
     const int row_a = (int)(first / per_row), row_b = (int)min((long)P, (first + READ_AHEAD * READ_THREADS - 1) / per_row + 1);
-    for (int r = row_a + threadIdx.x; r < row_b; r += READ_THREADS) {
-        const int page = r < live && known ? fx_page_of(table, a.table_width, a.n_pages, pos0 + r, a.page_size) : -1;
-        place_s[r - row_a] = page < 0 ? -1 : (page * a.n_kv_heads + h) * a.page_size + (pos0 + r) % a.page_size;
+    const bool whole = P == a.page_size && pos0 % P == 0;                   // (the block's rows are a page of the cache)
+    int place0 = -1;
+    if (whole) {
+        const int page = known ? fx_page_of(table, a.table_width, a.n_pages, pos0, P) : -1;
+        if (page >= 0) place0 = (page * a.n_kv_heads + h) * P;
+    } else {
+        for (int r = row_a + threadIdx.x; r < row_b; r += READ_THREADS) {
+            const int page = r < live && known ? fx_page_of(table, a.table_width, a.n_pages, pos0 + r, a.page_size) : -1;
+            place_s[r - row_a] = page < 0 ? -1 : (page * a.n_kv_heads + h) * a.page_size + (pos0 + r) % a.page_size;
+        }
+        __syncthreads();
     }
-    __syncthreads();
     const uint8_t *pages = is_v ? a.v_pages : a.k_pages, *own = is_v ? a.v_exp : a.k_exp, *other = is_v ? a.k_exp : a.v_exp;
     T* dst = reinterpret_cast<T*>(is_v ? a.v_out : a.k_out) + ((long)blockIdx.x * a.n_kv_heads + h) * P * D;
     uint4 w[READ_AHEAD];
@@ -274,7 +281,7 @@ __global__ void __launch_bounds__(READ_THREADS) read_spans_kernel(ReadArgs a)
 #pragma unroll
     for (int u = 0; u < READ_AHEAD; ++u) {
         const long i = first + u * READ_THREADS + threadIdx.x;
-        const int r = (int)(i / per_row), at = i < n ? place_s[r - row_a] : -1;
+        const int r = (int)(i / per_row), at = i >= n ? -1 : !whole ? place_s[r - row_a] : r < live && place0 >= 0 ? place0 + r : -1;
         w[u] = make_uint4(0, 0, 0, 0);
         e[u] = e2[u] = 0;
         if (at < 0) continue;
