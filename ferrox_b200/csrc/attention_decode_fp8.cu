@@ -369,6 +369,14 @@ __global__ void __launch_bounds__(NTHREADS, SLABS == 1 ? 2 : 1) decode_fp8_kerne
             page_next = next_page();
             const bool live = exps >= 0;
             const float k_scale = fx_fp8_scale(exps & 255), v_scale = live ? fx_fp8_scale(exps >> 8 & 255) : 0.f;
+            // What lies where nobody has written may be no number, and 0 times it is none: such values become zeros, while the scores
+            // are made.  (The tile is there: the scores' product waits for the same barrier.)
+            if (!live && mbar_wait(full(j % STAGES), (uint32_t)(j / STAGES) & 1u, abort_flag)) {
+                uint8_t* v = sm + j % STAGES * L::STAGE + SLABS * SLAB + r * 128;
+#pragma unroll
+                for (int i = 0; i < SLABS * 8; ++i) *reinterpret_cast<uint4*>(v + i / 8 * SLAB + ((i ^ r) & 7) * 16) = make_uint4(0, 0, 0, 0);   // (rows side by side: other banks)
+            }
+            __syncwarp();
             bool ok = mbar_wait(s_full(b), (uint32_t)(j / S_PLACES) & 1u, abort_flag);
             tc_fence_after();
             float s[HB], p[HB], w[HB];

@@ -238,9 +238,9 @@ __global__ void __launch_bounds__(READ_THREADS) read_rows_kernel(ReadArgs a)
     }
 }
 
-// Stretches of requests (spans: entry, first position, end, first row; first rows at a page's start, in order) into pages
+// Stretches of requests (spans: entry, first position, end, first row; each in pages of its own, in order) into pages
 // [page of the rows][kv head][position][head_dim] of out_page positions, which need not be the cache's.  A block takes a page of
-// a head, keys or values; what lies behind a stretch's end in its last page is 0.  For attention: a position of which the key or
+// a head, keys or values; what lies before a stretch in its first page and behind its end in its last is 0.  For attention: a position of which the key or
 // the value is not finite becomes a key of NaN and a value of 0, so that it makes those queries' results NaN that see it, and no
 // other's (a weight of 0 times NaN is none).
 template <typename T, int VEC>
@@ -252,10 +252,10 @@ __global__ void __launch_bounds__(READ_THREADS) read_spans_kernel(ReadArgs a)
     int before = 0;                                                         // stretches that begin at this page or before it
     for (int i = 0; i < a.n_spans; i += 32) {
         const int k = i + (threadIdx.x & 31);
-        before += __popc(__ballot_sync(0xffffffffu, k < a.n_spans && a.spans[4 * k + 3] <= row0));
+        before += __popc(__ballot_sync(0xffffffffu, k < a.n_spans && a.spans[4 * k + 3] - row0 < P));
     }
     const int4 span = *reinterpret_cast<const int4*>(a.spans + 4 * max(before - 1, 0));
-    const int pos0 = span.y + row0 - span.w, live = min(P, span.z - pos0);
+    const int pos0 = span.y + row0 - span.w, skip = span.w - row0, live = min(P, span.z - pos0);
     const int slot = a.seq_slot[span.x], h = blockIdx.y >> 1;
     const bool is_v = blockIdx.y & 1, known = slot >= 0 && slot < a.n_slots;
     const int* table = a.block_table + (long)(known ? slot : 0) * a.table_width;
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(READ_THREADS) read_spans_kernel(ReadArgs a)
         if (page >= 0) place0 = (page * a.n_kv_heads + h) * P;
     } else {
         for (int r = row_a + threadIdx.x; r < row_b; r += READ_THREADS) {
-            const int page = r < live && known ? fx_page_of(table, a.table_width, a.n_pages, pos0 + r, a.page_size) : -1;
+            const int page = r >= skip && r < live && known ? fx_page_of(table, a.table_width, a.n_pages, pos0 + r, a.page_size) : -1;
             place_s[r - row_a] = page < 0 ? -1 : (page * a.n_kv_heads + h) * a.page_size + (pos0 + r) % a.page_size;
         }
         __syncthreads();
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(READ_THREADS) read_spans_kernel(ReadArgs a)
 #pragma unroll
     for (int u = 0; u < READ_AHEAD; ++u) {
         const long i = first + u * READ_THREADS + threadIdx.x;
-        const int r = (int)(i / per_row), at = i >= n ? -1 : !whole ? place_s[r - row_a] : r < live && place0 >= 0 ? place0 + r : -1;
+        const int r = (int)(i / per_row), at = i >= n ? -1 : !whole ? place_s[r - row_a] : r >= skip && r < live && place0 >= 0 ? place0 + r : -1;
         w[u] = make_uint4(0, 0, 0, 0);
         e[u] = e2[u] = 0;
         if (at < 0) continue;

@@ -2060,8 +2060,6 @@ def gemm_tc2(x, w, out, *, bias=None, accumulate=False, gated=False, unary=None,
 
 # ---- the 8-bit cache: e4m3 elements and one exponent a position and head (csrc/fp8.cuh) --------------------------------------
 FP8_MAX_DIM = 256                 # elements of a head
-FP8_LARGEST, FP8_MIN_EXP, FP8_NAN = 448.0, -119, 255
-
 
 _CACHE_FP8 = ("k_pages", "v_pages", "k_exp", "v_exp", "block_table")
 _STEP = ("positions", "token_seq", "seq_slot")
@@ -2073,6 +2071,11 @@ def _check_fp8(name, found, page_size, n_kv_heads, head_dim):
     if P != page_size or N == 0 or not 0 < D <= FP8_MAX_DIM or (n_kv_heads is not None and (G != n_kv_heads or D != head_dim)):
         raise KernelError(f"{name}: pages of {page_size} positions, {n_kv_heads or 'any'} heads of {head_dim or 'up to'} {'' if head_dim else FP8_MAX_DIM}"
                           f" elements (at most {FP8_MAX_DIM}), at least one: found [{N}, {G}, {P}, {D}]")
+
+
+def _check_entries(name, n, entries):
+    if n and not entries:
+        raise KernelError(f"{name}: a step of no entries with something to do")
 
 
 _WRITE_FP8 = "eNGPD eNGPD uNGP uNGP iSW iT iT iB xTQ~ ?fF ?fThc ?iZ"
@@ -2089,10 +2092,11 @@ def rope_kv_write_fp8(qkv, positions, token_seq, seq_slot, inv_freq, rotary_dim,
     reads as NaN.  A position without a page, or outside its table, is written nowhere and raises ``status`` 2.  Positions of a
     request are distinct."""
     name = "rope_kv_write_fp8"
-    (_, now, x, kp, vp, kep, vep, tp, pp, sp, lp, qp, fp, cp, zp, N, G, P, D, S, W, T, _, Q, F, h, c, _, ld) = _operands(
+    (_, now, x, kp, vp, kep, vep, tp, pp, sp, lp, qp, fp, cp, zp, N, G, P, D, S, W, T, B, Q, F, h, c, _, ld) = _operands(
         name, _WRITE_FP8, _CACHE_FP8 + _STEP + ("qkv", "inv_freq", "cos_sin", "status"), k_pages, v_pages, k_exp, v_exp, block_table,
         positions, token_seq, seq_slot, qkv, inv_freq, cos_sin, status)
     _check_fp8(name, (N, G, P, D), page_size, n_kv_heads, head_dim)
+    _check_entries(name, T, B)
     half = rotary_dim // 2
     if n_heads < 0 or Q < (n_heads + 2 * G) * D or W == 0 or (inv_freq is not None and F < half) or (cos_sin is not None and (h != half or c != 2)):
         raise KernelError(f"{name}: rows of {n_heads} + 2 * {G} heads of {D}, {half} frequencies, (cos, sin) pairs [{T}, {half}, 2]: found rows of "
@@ -2107,10 +2111,11 @@ _READ_FP8, _READ_FP8_SPANS = "eNGPD eNGPD uNGP uNGP iSW iT iT iB xTGD xTGD", "eN
 def read_kv_fp8(k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, k_out, v_out, stream=None):
     """What an 8-bit cache holds at the given positions: ``k_out``, ``v_out`` [tokens, kv heads, head_dim] (bfloat16, in which every
     value is exact, or float32).  A position without a page reads as 0."""
-    (_, now, x, kp, vp, kep, vep, tp, pp, sp, lp, ko, vo, N, G, P, D, S, W, T, _) = _operands(
+    (_, now, x, kp, vp, kep, vep, tp, pp, sp, lp, ko, vo, N, G, P, D, S, W, T, B) = _operands(
         "read_kv_fp8", _READ_FP8, _CACHE_FP8 + _STEP + ("k_out", "v_out"), k_pages, v_pages, k_exp, v_exp, block_table, positions, token_seq,
         seq_slot, k_out, v_out)
     _check_fp8("read_kv_fp8", (N, G, P, D), page_size, None, None)
+    _check_entries("read_kv_fp8", T, B)
     call("fx_read_kv_fp8", kp, vp, kep, vep, tp, S, W, page_size, N, pp, sp, lp, 0, 0, T, 1, 0, ko, vo, x, G, D,
          stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
 
@@ -2119,14 +2124,15 @@ def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, sp
                       attend=False):
     """Stretches of requests out of an 8-bit cache into pages that the other attention kernels take: ``k_out``, ``v_out`` [n_rows /
     R, kv heads, R, head_dim] with pages of R positions, the cache's or others.  ``spans``: int32 [n, 4] rows of (entry, first position,
-    end, first row), first rows multiples of R, the rows in order and without gaps up to ``n_rows``.  What lies behind a stretch's end
-    in its last page is 0, and so is a position without a page.  ``attend``: a position of which the key or the value is not finite is
+    end, first row), in order; each has pages of its own, without gaps up to ``n_rows``.  What lies before a stretch in its first page
+    and behind its end in its last is 0, and so is a position without a page.  ``attend``: a position of which the key or the value is not finite is
     read as a key of NaN and a value of 0, which makes the results NaN of the queries that see it and of no others."""
     name = "read_kv_fp8_spans"
-    (_, now, x, kp, vp, kep, vep, tp, np_, lp, ko, vo, N, G, P, D, S, W, n, four, _, M, R) = _operands(
+    (_, now, x, kp, vp, kep, vep, tp, np_, lp, ko, vo, N, G, P, D, S, W, n, four, B, M, R) = _operands(
         name, _READ_FP8_SPANS, _CACHE_FP8 + ("spans", "seq_slot", "k_out", "v_out"), k_pages, v_pages, k_exp, v_exp, block_table, spans, seq_slot,
         k_out, v_out)
     _check_fp8(name, (N, G, P, D), page_size, None, None)
+    _check_entries(name, M, B)
     if n_rows != M * R or four != 4 or (M and not n):
         raise KernelError(f"{name}: spans [n, 4] over {n_rows} rows, {M} pages of {R}: found [{n}, {four}]")
     call("fx_read_kv_fp8", kp, vp, kep, vep, tp, S, W, page_size, N, 0, 0, lp, np_, n, n_rows, R, int(attend), ko, vo, x, G, D,
@@ -2141,11 +2147,12 @@ def _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table,
     found = _operands(name, _ATTEND_FP8, _CACHE_FP8 + _STEP + ("q", "out", "status", "tokens"), k_pages, v_pages, k_exp, v_exp, block_table, positions,
                       token_seq, seq_slot, q, out, status, tokens)
     _check_fp8(name, found[15:19], page_size, n_kv_heads, head_dim)
+    _check_entries(name, found[21], found[22])
     need = n_heads * head_dim
     if n_heads < 1 or n_heads % n_kv_heads or found[20] == 0 or found[23] < need or found[24] < need:
         raise KernelError(f"{name}: {n_heads} heads on {n_kv_heads} of {head_dim}, {found[20]} pages a request: found rows of {found[23]} and {found[24]}")
-    if (window is not None and window < 1) or (softcap is not None and not softcap > 0) or not abs(scale) < float("inf"):
-        raise KernelError(f"{name}: window={window}, softcap={softcap}, scale={scale}: positive (or None), positive (or None), finite")
+    if (window is not None and not 1 <= window < 1 << 31) or (softcap is not None and not softcap > 0) or not abs(scale) < float("inf"):
+        raise KernelError(f"{name}: window={window}, softcap={softcap}, scale={scale}: positive 32-bit (or None), positive (or None), finite")
     return found
 
 
@@ -2226,6 +2233,8 @@ class PrefillFp8Plan:
 
     def __init__(self, entries, page_size, device):
         self.entries, self.page_size, self.device = [(int(n), int(start)) for n, start in entries], int(page_size), torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         if self.page_size < 1 or any(n < 0 or start < 0 for n, start in self.entries):
             raise KernelError(f"prefill_fp8_plan: entries {self.entries} of pages of {page_size}")
         self.n_tokens = sum(n for n, _ in self.entries)
@@ -2250,6 +2259,9 @@ class PrefillFp8Plan:
         if x is None:
             x = make()
             if isinstance(x, tuple):
+                if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                    raise KernelError("prefill_attention_fp8: a plan's lists are made by its first use, which cannot be captured: a replay would "
+                                      "copy them from memory that is given back (use the plan once before the capture)")
                 x = tuple(upload(v, self.device) if hasattr(v, "__array__") else v for v in x)
                 self._tensors += [v for v in x if isinstance(v, torch.Tensor) and v.numel() and v.is_cuda]
             self._kept[key] = x
@@ -2295,13 +2307,14 @@ class PrefillFp8Plan:
         import numpy as np
 
         P, spans, row = FP8_READ_PAGE, [], 0
-        for b, _, n, start in group:
+        for b, _, n, start in group:                     # (from the first position that is seen: what is before it may never have been written)
             p0, rows = self._rows_of(n, start, window)
-            spans.append((b, p0, start + n, row))
+            seen = first_key(start, window)
+            spans.append((b, seen, start + n, row + seen - p0))
             row += rows
         table = np.full((len(group), max(-(-s[2] // P) for s in spans)), -1, dtype=np.int32)
-        for i, (_, p0, end, r) in enumerate(spans):
-            table[i, p0 // P:-(-end // P)] = r // P + np.arange(-(-end // P) - p0 // P)
+        for i, (_, seen, end, r) in enumerate(spans):
+            table[i, seen // P:-(-end // P)] = r // P + np.arange(-(-end // P) - seen // P)
         return (group[0][1], sum(n for _, _, n, _ in group), [(n, start) for _, _, n, start in group], np.asarray(spans, dtype=np.int32), row,
                 table, np.arange(len(group), dtype=np.int32))
 
@@ -2333,6 +2346,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     found = _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, status, None,
                                    out, n_heads, n_kv_heads, head_dim, window, scale, softcap)
     T, B = found[21:23]
+    if plan.device.index != found[0]:
+        raise KernelError(f"{name}: a plan made for {plan.device}, operands on cuda:{found[0]}")
     if plan.n_tokens != T or plan.page_size != page_size or len(plan.entries) > B:
         raise KernelError(f"{name}: a plan of {len(plan.entries)} entries, {plan.n_tokens} tokens and pages of {plan.page_size} for "
                           f"{B} entries, {T} tokens and pages of {page_size}")

@@ -174,9 +174,10 @@ def test_parts_hold_what_the_tokens_see(window, most, monkeypatch):
     for tok0, n, own, spans, rows, table, slots in plan.parts(window, 10):
         assert sum(m for m, _ in own) == n and slots.tolist() == list(range(len(own))) and (len(own) == 1 or rows * 10 <= most)
         at, row = tok0, 0
-        for (m, start), (b, p0, end, r), pages in zip(own, spans.tolist(), table.tolist()):
-            assert (m, start) == entries[b] and at == first[b] and end == start + m and r == row and p0 % P == 0
-            assert p0 <= ops.first_key(start, window) < p0 + P
+        for (m, start), (b, seen_from, end, r), pages in zip(own, spans.tolist(), table.tolist()):
+            p0 = seen_from // P * P
+            assert (m, start) == entries[b] and at == first[b] and end == start + m and r == row + seen_from - p0
+            assert seen_from == ops.first_key(start, window)
             for p in range(len(pages)):
                 inside = p0 <= p * P < end
                 assert pages[p] == (row // P + p - p0 // P if inside else -1)

@@ -493,6 +493,59 @@ def test_results_beside_a_portion_stay():
     check(out[:73, :H * D], c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT["bf16"])
 
 
+def only_seen(c, entries, window):
+    """Everything in the cache but what the entries' tokens see becomes bytes that are no numbers, with exponents of any kind."""
+    g = torch.Generator().manual_seed(60)
+    keep = torch.zeros(c.dev[0][0].shape[0], c.P, dtype=torch.bool)
+    for b, (n, start) in enumerate(entries):
+        for p in range(max(0, start - window + 1) if window else 0, start + n):
+            keep[int(c.table[int(c.slots[b]), p // c.P]), p % c.P] = True
+    keep = keep[:, None].expand(-1, c.G, -1)
+    for i, (pages, e) in enumerate(c.dev):
+        bad = torch.where(torch.rand(pages.shape, generator=g) < 0.5, 127, 255).to(torch.uint8)
+        pages = torch.where(keep[..., None], pages.view(torch.uint8).cpu(), bad).to(DEV).view(torch.float8_e4m3fn)
+        c.dev[i] = (pages, torch.where(keep, e.cpu(), torch.randint(8, 256, e.shape, generator=g).to(torch.uint8)).to(DEV))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("H,G,D,P", [(4, 2, 128, 64), (6, 2, 64, 16), (4, 1, 256, 128), (2, 2, 20, 5), (1, 1, 64, 48)])
+@pytest.mark.parametrize("window", [None, 37])
+def test_what_nobody_has_written_counts_for_nothing(dtype, H, G, D, P, window):
+    lens = [1, 5, 127, 130, 400]
+    c = Cache(lens, G, D, P, 61)
+    entries = [(1, n - 1) for n in lens]
+    only_seen(c, entries, window)
+    q = rows(len(lens), H, G, D, DTYPES[dtype], 62)
+    out = torch.empty(len(lens), H * D, dtype=q.dtype, device=DEV)
+    ops.decode_attention_fp8(q, *c.operands, *step(entries, c.slots), out, H, G, D, window, 0.1)
+    check(out, c, entries, q, H, window, 0.1, None, WEIGHT[dtype])
+    entries = [(1, 0), (5, 0), (60, 67), (2, 128), (40, 360)]
+    c = Cache(lens, G, D, P, 63)
+    only_seen(c, entries, window)
+    T = sum(n for n, _ in entries)
+    q = rows(T, H, G, D, DTYPES[dtype], 64)
+    out = torch.empty(T, H * D, dtype=q.dtype, device=DEV)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, P, DEV), *step(entries, c.slots), out, H, G, D, window, 0.1)
+    check(out, c, entries, q, H, window, 0.1, None, PROMPT_WEIGHT[dtype])
+
+
+@pytest.mark.parametrize("R,P", [(128, 64), (64, 64), (16, 5)])
+def test_stretches_that_begin_inside_a_page(R, P):
+    G, D = 2, 64
+    c = Cache([300, 200], G, D, P, 65)
+    spans, row = [], 0
+    for b, p0, end in [(0, 130, 300), (1, 64, 200), (0, 7, 9)]:
+        spans.append((b, p0, end, row + p0 % R))
+        row += (-(-end // R) - p0 // R) * R
+    k, v = (torch.full((row // R, G, R, D), 7.0, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    ops.read_kv_fp8_spans(*c.operands, torch.tensor(spans, dtype=torch.int32, device=DEV), row, c.slots.to(DEV), k, v)
+    for which, got in ((0, k), (1, v)):
+        want = torch.zeros(row, G, D, dtype=torch.float64)
+        for b, p0, end, r in spans:
+            want[r:r + end - p0] = c.of(b, end, which)[0][p0:]
+        assert torch.equal(got.double().cpu().transpose(1, 2).reshape(row, G, D), want)
+
+
 # ---- streams, graphs, order -----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_on_a_stream_of_its_own_and_in_a_graph(dtype):
@@ -623,3 +676,52 @@ def test_operands_are_found_the_same_without_the_extension(dtype, monkeypatch):
     got = torch.empty_like(want)
     ops.decode_attention_fp8(q, *c.operands, *st, got, H, G, D, 40, 0.1)
     assert torch.equal(got, want)
+
+
+# ---- refusals that take operands on the device ----------------------------------------------------------------------
+def test_steps_without_entries():
+    """A token has to belong to one."""
+    H, G, D, P = 2, 1, 64, 16
+    c = Cache([4], G, D, P, 66)
+    q, out = rows(2, H, G, D, torch.bfloat16, 67), torch.zeros(2, H * D, dtype=torch.bfloat16, device=DEV)
+    pos, seq, _ = step([(2, 2)], c.slots)
+    st, k = (pos, seq, pos[:0]), torch.zeros(2, G, D, dtype=torch.bfloat16, device=DEV)
+    pages, spans = torch.zeros(1, G, P, D, device=DEV), torch.tensor([[0, 0, 4, 0]], dtype=torch.int32, device=DEV)
+    for call in (lambda: ops.rope_kv_write_fp8(q, *st, None, 0, *c.operands, H, G, D), lambda: ops.read_kv_fp8(*c.operands, *st, k, k),
+                 lambda: ops.read_kv_fp8_spans(*c.operands, spans, P, pos[:0], pages, pages),
+                 lambda: ops.decode_attention_fp8(q, *c.operands, *st, out, H, G, D, None, 1.0),
+                 lambda: ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan([(2, 2)], P, DEV), *st, out, H, G, D, None, 1.0)):
+        with pytest.raises(ops.KernelError, match="no entries"):
+            call()
+
+
+def test_a_prompt_in_a_graph():
+    """A plan's lists are made before a capture; a graph made of a plan that has them follows what the buffers hold."""
+    H, G, D, P = 4, 2, 64, 64
+    entries = [(300, 50), (5, 20), (40, 0)]
+    c = Cache([350, 25, 40], G, D, P, 68)
+    q = rows(345, H, G, D, torch.bfloat16, 69)
+    st, operands, plan = step(entries, c.slots), c.operands, ops.prefill_fp8_plan(entries, P, DEV)
+    want, out = (torch.zeros(345, H * D, dtype=q.dtype, device=DEV) for _ in range(2))
+    with pytest.raises(ops.KernelError, match="cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.prefill_attention_fp8(q, *operands, plan, *st, out, H, G, D, None, 0.1)
+    ops.prefill_attention_fp8(q, *operands, plan, *st, want, H, G, D, None, 0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.prefill_attention_fp8(q, *operands, plan, *st, out, H, G, D, None, 0.1)
+    for seed in (70, 71):
+        q.copy_(rows(345, H, G, D, torch.bfloat16, seed))
+        graph.replay()
+        ops.prefill_attention_fp8(q, *operands, plan, *st, want, H, G, D, None, 0.1)
+        assert torch.equal(out, want)
+    check(want, c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT["bf16"])
+
+
+def test_a_plan_of_another_device():
+    H, G, D, P = 2, 1, 64, 16
+    c = Cache([20], G, D, P, 72)
+    q, out = rows(20, H, G, D, torch.bfloat16, 73), torch.zeros(20, H * D, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ops.KernelError, match="a plan made for cpu"):
+        ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan([(20, 0)], P, "cpu"), *step([(20, 0)], c.slots), out, H, G, D, None, 1.0)
