@@ -1,37 +1,48 @@
 // Attention of few tokens a request over 8-bit cache pages (the form: fp8.cuh) on the 5th-generation tensor cores, which take
 // the pages' bytes as they are: nothing converts a cached element.
 //
-//   grid = (token, kv head x block of HB query heads, run of keys); a tile is 128 positions.
+//   grid = (token, kv head x block of HB = 4 or 8 query heads, run of keys); a tile is 128 positions.
 //
 //   S^T = K Q^T     tcgen05.mma kind::f8f6f4, 128 keys x (heads x parts) x head_dim.  K as TMA lays it down ([key][128 bytes],
-//                   128-byte swizzle).  A query is e4m3 in PARTS parts: with q' = q 2^-x (its largest element between 128 and
+//                   128-byte swizzle).  A query is e4m3 in PARTS_Q parts: with q' = q 2^-x (its largest element between 128 and
 //                   256), part 1 is q' rounded to e4m3, part n + 1 what is left times 16 rounded again, each part a column of
 //                   its own; two parts hold a bfloat16 element exactly (4 + 4 bits), six a 32-bit one.
 //   softmax         a thread owns a key: it adds up its heads' parts in 32 bits, multiplies by the key's 2^K, caps and masks,
 //                   and makes p = 2^(s - ref) for the denominator and w = p 2^V / 2^refw for the second product.
 //   O^T += V^T W^T  tcgen05.mma, 128 elements x (heads x parts) x 128 keys.  V as TMA lays it down is its transpose with the
-//                   elements side by side (M-major A); W in three parts of e4m3 (six in 32 bits), written [key][64 bytes] with
-//                   the 64-byte swizzle (N-major B).
+//                   elements side by side (M-major A); W in three parts of e4m3 (six in 32 bits), written [key][32 bytes] with
+//                   the 32-byte swizzle (N-major B).
 //
 // Why parts: e4m3 keeps 4 bits, and products of e4m3 are added up in 32 bits (measured: beside a sum of 2^16 in the same
 // instruction a product of 2^-9 is kept, in the next one of 2^-7), so that the sum over the parts is the product of the wider
 // number.  Weights are first rounded to 16-bit floating numbers (2^-12 of the weight) for 16-bit rows; the third part ends at
 // 2^-13 of a weight and at 2^-18 of 1 where the largest weight lies between 2^5 and 2^8, six parts at 2^-24 and 2^-30.
-// What it costs is columns, of which the instruction has more than 16 heads need.
+// What it costs is columns, of which the instruction has more than 8 heads need.
 //
-// The references ref and refw are whole powers of two, for each head, the same in all threads: ref for the sum of weights, refw
-// for the weights times 2^V (a cached value's scale belongs to its key, and with it the weight may be of any size).  They are
-// raised when a score passes ref by 6 or a weighted scale refw by 8; then O in tensor memory is multiplied by the power of two
-// between the old and the new one.  After the first tile that is rare.  One barrier a tile asks all 128 threads.
+// The references ref and refw are whole powers of two, for each head, the same in all threads of a group: ref for the sum of
+// weights, refw for the weights times 2^V (a cached value's scale belongs to its key, and with it the weight may be of any size).
+// They are raised when a score passes ref by 6 or a weighted scale refw by 8; then O in tensor memory is multiplied by the power
+// of two between the old and the new one.  After the first tile that is rare.
 //
 // Warp 0 asks for tiles (TMA, a ring of 3 stages; a stage of heads up to 128 elements is 32 KB, two blocks an SM), warp 1 issues
-// the products in the order S(j + 1), O(j), warps 2 - 5 are the softmax threads.  Every wait is bounded (status 3).
+// the products S(j) as their keys land, warps 2 - 5 and 6 - 9 are two groups of softmax threads: a group takes every other tile,
+// with references, W and O of its own, and its first thread issues its O(j).  While one group waits for its product the other
+// works.  The two are added up at the end.  Every wait is bounded (status 3).
+//
+// What bounds it, B200.  A step long enough streams 7.35 TB/s (two tiles of 32 KB in 1.32 us an SM: the memory), and a launch
+// costs 8 to 11 us beside that, the last blocks of a round among them: 64 requests of up to 4,096 positions, 28 heads on 4 of 128,
+// 39.6 us of which the bytes are 27.4; one request of 131,072 in 33.0 of 20.6 (its 74 runs a kv head: 2.2 us to add them up); one of 37 in 5.4, a
+// chain of waits (lookups 0.9 us, boxes asked 1.6, all met 2.0, keys landed 2.3, S 2.6, W 3.1, O 3.5, written 4.2).
+// Measured beside it: one group of softmax threads 57 us for the 64 requests; two groups that share a place for W 40.5; rings of
+// their own for keys and values 41.3; blocks in order of their lengths 39.8 (and requests with a window 29.1 -> 30.5).
 //
 // Positions outside the run or without a page: their boxes are asked for behind the last page, where TMA fills in zeros without
-// reading; their weights are 0.  Bytes of pages are finite (the writer makes no other), so that 0 times them is 0.  A position
-// whose row is not finite has E = 255: its scale is NaN, and so is the result of the queries that see it.
+// reading, or hold what is in the page beside the run's own; their weights are 0, and their values are made 0, so that bytes that
+// nobody has written reach nothing.  A position whose row is not finite has E = 255: its scale is NaN, and so is the result of the
+// queries that see it.
 //
-// Runs of a token's keys leave (mean of the values, ref, sum of weights) and a second kernel adds them up in their order.
+// Runs of a token's keys leave (sum of weighted values over the sum of weights, ref, sum of weights) and a second kernel adds them
+// up in their order.
 #include "fp8.cuh"
 #include "tc_common.cuh"
 #include "api.h"

@@ -52,6 +52,37 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                   "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+// Two 32-bit numbers in a register pair.
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float2 parts_of(uint64_t a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
 template <int D>
 __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                       const __grid_constant__ CUtensorMap map_k,
@@ -73,7 +104,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
     auto k_full = [&](int b) { return bar(7 + b); };
     auto v_full = [&](int b) { return bar(9 + b); };
     auto kv_empty = [&](int b) { return bar(11 + b); };
-    const uint32_t drained = bar(13);
+    auto p_half = [&](int t) { return bar(13 + t); };
+    const uint32_t drained = bar(15);
 
     const int* item = a.items + (long)blockIdx.y * ITEM_INTS;
     const int tok0 = item[0], n_tok = item[1], entry = item[2], pos0 = item[3], kb_begin = item[4], kb_end = item[5], part = item[6];
@@ -90,7 +122,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
 
     if (threadIdx.x == 0) {
         abort_flag_s = 0;
-        for (int i = 0; i < 14; ++i) mbar_init(bar(i), i == 3 || i == 4 ? 4 : 1);      // (p_full: four warps)
+        for (int i = 0; i < 16; ++i) mbar_init(bar(i), i == 3 || i == 4 || i == 13 || i == 14 ? 4 : 1);      // (p_full, p_half: four warps)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -115,16 +147,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
             for (int t = 0; t < nt; ++t)
                 for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + t * L::TILE + h * L::SUB, &map_q, h * 64, 0, kvh, tok0 + t * per, q_full);
             constexpr uint32_t idesc_s = instr_desc_ex(BQ, BK, 0), idesc_o = instr_desc_ex(BQ, D, 1);
-            int k_ready = -1, n_p[2] = {0, 0};
+            int n_p[2] = {0, 0};
             const int last0 = last_of(0), last1 = last_of(1);
             bool ok = mbar_wait(q_full, 0, abort_flag);
             auto issue_s = [&](int t, int i) {
                 const int b = i & 1;
-                if (k_ready < i) {
-                    if (!mbar_wait(k_full(b), (uint32_t)(i >> 1) & 1u, abort_flag)) return false;
-                    k_ready = i;
-                    tc_fence_after();
-                }
 #pragma unroll
                 for (int h = 0; h < L::HALVES; ++h) {
                     const uint64_t dq = smem_desc(base + t * L::TILE + h * L::SUB), dk = smem_desc(base + L::K_OFF + b * L::TILE + h * L::SUB);
@@ -132,28 +159,38 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                     for (int k = 0; k < 4; ++k) tc_mma(tmem_s(t), dq + 2u * k, dk + 2u * k, idesc_s, (h | k) != 0);
                 }
                 tc_commit(s_full(t));
-                return true;
             };
+            auto k_there = [&](int i) { return i >= n_walk || mbar_wait(k_full(i & 1), (uint32_t)(i >> 1) & 1u, abort_flag); };
+            ok = ok && k_there(0);
+            tc_fence_after();
             for (int t = 0; t < nt && ok; ++t)
-                if (active(t, 0)) ok = issue_s(t, 0);
+                if (active(t, 0)) issue_s(t, 0);
             for (int i = 0; i < n_walk && ok; ++i) {
                 const int b = i & 1;
-                bool v_ready = false;
+                ok = mbar_wait(v_full(b), (uint32_t)(i >> 1) & 1u, abort_flag) && k_there(i + 1);
                 for (int t = 0; t < nt && ok; ++t) {
                     if (active(t, i)) {
-                        ok = mbar_wait(p_full(t), (uint32_t)n_p[t] & 1u, abort_flag);
-                        if (ok && !v_ready) { ok = mbar_wait(v_full(b), (uint32_t)(i >> 1) & 1u, abort_flag); v_ready = true; }
-                        if (!ok) break;
-                        tc_fence_after();
+                        const uint32_t phase = (uint32_t)n_p[t] & 1u;
+                        auto issue_o = [&](int ks0) {
+                            tc_fence_after();
 #pragma unroll
-                        for (int ks = 0; ks < BK / 16; ++ks)
-                            tc_mma_ts(tmem_o(t), tmem_s(t) + 8u * ks, smem_desc_lbo_sbo(base + L::V_OFF + b * L::TILE + ks * 2048, L::SUB, 1024), idesc_o,
-                                      (n_p[t] | ks) != 0);
+                            for (int k = 0; k < BK / 32; ++k) {
+                                const int ks = ks0 + k;
+                                tc_mma_ts(tmem_o(t), tmem_s(t) + 8u * ks, smem_desc_lbo_sbo(base + L::V_OFF + b * L::TILE + ks * 2048, L::SUB, 1024), idesc_o,
+                                          (n_p[t] | ks) != 0);
+                            }
+                        };
+                        ok = mbar_wait(p_half(t), phase, abort_flag);
+                        if (!ok) break;
+                        issue_o(0);
+                        ok = mbar_wait(p_full(t), phase, abort_flag);
+                        if (!ok) break;
+                        issue_o(BK / 32);
                         ++n_p[t];
                         if (i == (t ? last1 : last0)) tc_commit(o_done(t));
                     }
                     if (t == nt - 1) tc_commit(kv_empty(b));   // every product that reads this block has been issued
-                    if (active(t, i + 1)) ok = issue_s(t, i + 1);
+                    if (active(t, i + 1)) issue_s(t, i + 1);
                 }
             }
             if (*abort_flag) {                                  // given up: no product may outlive tensor memory
@@ -194,82 +231,87 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                 if (quad * 32 >= rows_t) {               // none of the warp's rows exists: what its rows of P hold reaches no others
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(p_full(t));
+                    if (lane == 0) { mbar_arrive(p_half(t)); mbar_arrive(p_full(t)); }
                     ++cnt;
                     continue;
                 }
                 const int kb = (first_blk + i) * BK;
                 const bool interior = kb + BK - 1 <= pos_t && kb >= lo_last;   // every row sees all of the block: no masking (most blocks)
-                uint32_t ca[32], cb[32], pk[32];
-                auto mask = [&](uint32_t* c, int chunk, uint32_t with) {
-                    if (interior) return;
+                uint32_t c[4][32];                       // the row's scores
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto look = [&](int chunk) {
+                    if (!interior)
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const int key = kb + chunk * 32 + k;
-                        if (key > p_r || key < lo_r) c[k] = with;
-                    }
-                };
-                constexpr uint32_t MINUS_INF = 0xff800000u, NO_NUMBER = 0x7fffffffu;
-                // first pass: the row's maximum (the next 32 columns are on their way while these are looked at)
-                float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
-                auto take_max = [&](uint32_t* c, int chunk) {
-                    mask(c, chunk, NO_NUMBER);           // (what fmaxf passes over)
+                        for (int k = 0; k < 32; ++k) {
+                            const int key = kb + chunk * 32 + k;
+                            if (key > p_r || key < lo_r) c[chunk][k] = 0xff800000u;      // -infinity
+                        }
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4) {
-                        mx0 = fmaxf(mx0, __uint_as_float(c[k])); mx1 = fmaxf(mx1, __uint_as_float(c[k + 1]));
-                        mx2 = fmaxf(mx2, __uint_as_float(c[k + 2])); mx3 = fmaxf(mx3, __uint_as_float(c[k + 3]));
-                    }
+                    for (int k = 0; k < 32; k += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(c[chunk][k + e])), __uint_as_float(c[chunk][k + 4 + e]));
                 };
-                tc_ld32(ts, ca);
-                tc_ld_wait_for(ca);
-                tc_ld32(ts + 32, cb); take_max(ca, 0); tc_ld_wait_for(cb);
-                tc_ld32(ts + 64, ca); take_max(cb, 1); tc_ld_wait_for(ca);
-                tc_ld32(ts + 96, cb); take_max(ca, 2); tc_ld_wait_for(cb);
-                tc_ld32(ts, ca);      take_max(cb, 3);   // the first columns again, for the second pass
-                const float mn = fmaxf(m, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)));
+                tc_ld32(ts, c[0]);
+                tc_ld32(ts + 32, c[1]);
+                tc_ld_wait_for(c[0]);
+                tc_ld_wait_for(c[1]);
+                tc_ld32(ts + 64, c[2]);
+                tc_ld32(ts + 96, c[3]);
+                look(0);
+                look(1);
+                tc_ld_wait_for(c[2]);
+                tc_ld_wait_for(c[3]);
+                look(2);
+                look(3);
+                const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
                 const bool raise = r < rows_t && mn > m && (m == -INFINITY || (mn - m) * a.scale_log2e > RAISE_MAX_BY);
                 if (__any_sync(0xffffffffu, raise)) {
                     const float alpha = m == -INFINITY ? 0.f : exp2_fast((m - mn) * a.scale_log2e);
                     l *= alpha;
                     m = mn;
                     if (cnt > 0) {
+#pragma unroll 1
+                        for (int col = 0; col < D; col += 16) {
+                            uint32_t o[16];
+                            tc_ld16(to + col, o);
+                            tc_ld_wait();
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            tc_ld32(to + c * 32, cb);
-                            tc_ld_wait_for(cb);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) cb[k] = __float_as_uint(__uint_as_float(cb[k]) * alpha);
-                            tc_st32(to + c * 32, cb);
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                            tc_st16(to + col, o);
                         }
                     }
                 }
-                // second pass: weights in bfloat16 pairs over the first 64 columns of S, each behind its last reading
+                // weights in bfloat16 pairs over the first 64 columns of S, all of which has been read
                 const float ref = m == -INFINITY ? 0.f : m * a.scale_log2e;
-                float sum0 = 0.f, sum1 = 0.f;
-                auto take_exp = [&](uint32_t* c, int chunk, uint32_t* out) {
-                    mask(c, chunk, MINUS_INF);
+                const uint64_t scale2 = pair_of(__float_as_uint(a.scale_log2e), __float_as_uint(a.scale_log2e)), ref2 = pair_of(__float_as_uint(-ref), __float_as_uint(-ref));
+                uint64_t sum2[2] = {0, 0};
+                auto weigh = [&](int chunk) {
+                    uint32_t out[16];
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
-                        const float e0 = exp2_fast(fmaf(__uint_as_float(c[k]), a.scale_log2e, -ref)), e1 = exp2_fast(fmaf(__uint_as_float(c[k + 1]), a.scale_log2e, -ref));
-                        sum0 += e0; sum1 += e1;
-                        __nv_bfloat162 pr = __floats2bfloat162_rn(e0, e1);
+                        float2 e = parts_of(pair_fma(pair_of(c[chunk][k], c[chunk][k + 1]), scale2, ref2));
+                        e.x = exp2_fast(e.x); e.y = exp2_fast(e.y);
+                        sum2[k / 2 % 2] = pair_add(sum2[k / 2 % 2], pair_of(__float_as_uint(e.x), __float_as_uint(e.y)));
+                        __nv_bfloat162 pr = __floats2bfloat162_rn(e.x, e.y);
                         out[k >> 1] = *reinterpret_cast<uint32_t*>(&pr);
                     }
+                    tc_st16(ts + chunk * 16, out);
                 };
-                tc_ld_wait_for(ca);
-                tc_ld32(ts + 32, cb); take_exp(ca, 0, pk);      tc_ld_wait_for(cb);
-                tc_ld32(ts + 64, ca); take_exp(cb, 1, pk + 16); tc_ld_wait_for(ca);
-                tc_ld32(ts + 96, cb);
-                tc_st32(ts, pk);
-                take_exp(ca, 2, pk);
-                tc_ld_wait_for(cb);
-                take_exp(cb, 3, pk + 16);
-                tc_st32(ts + 32, pk);
-                l += sum0 + sum1;
+                weigh(0);
+                weigh(1);
+                tc_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_half(t));
+                weigh(2);
+                weigh(3);
                 tc_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(t));
+                const float2 sum = parts_of(pair_add(sum2[0], sum2[1]));
+                l += sum.x + sum.y;
                 ++cnt;
             }
             const bool has = last_of(t) >= 0;
