@@ -29,7 +29,8 @@
 namespace {
 using namespace fxtc;
 
-constexpr int BQ = 128, BK = 128, NTHREADS = 320, TMEM_COLS = 512, ITEM_INTS = 8;
+constexpr int BQ = 128, BK = 128, NTHREADS = 384, TMEM_COLS = 512, ITEM_INTS = 8, N_BARS = 22;
+constexpr int REGS_FEW = 88, REGS_MANY = 208;   // a thread of the first four warps, of the softmax: together what the block is launched with
 constexpr float RAISE_MAX_BY = 8.f;   // in powers of two
 
 struct Args {
@@ -78,10 +79,16 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ uint64_t both(float x) { return pair_of(__float_as_uint(x), __float_as_uint(x)); }
 __device__ __forceinline__ float2 parts_of(uint64_t a) {
     float2 r;
     asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
     return r;
+}
+// mbar_wait whose first answer is mostly yes.
+__device__ __forceinline__ bool met(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
+    return mbar_wait(bar, parity, abort_flag);
 }
 template <int D>
 __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __grid_constant__ CUtensorMap map_q,
@@ -92,20 +99,22 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag_s;
     __shared__ uint32_t tmem_base_s;
-    __shared__ __align__(8) uint64_t bars_s[16];
+    __shared__ __align__(8) uint64_t bars_s[N_BARS];
     volatile int* abort_flag = &abort_flag_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     auto bar = [&](int i) { return smem_u32(&bars_s[i]); };
-    const uint32_t q_full = bar(0);
-    auto s_full = [&](int t) { return bar(1 + t); };
-    auto p_full = [&](int t) { return bar(3 + t); };
-    auto o_done = [&](int t) { return bar(5 + t); };
-    auto k_full = [&](int b) { return bar(7 + b); };
-    auto v_full = [&](int b) { return bar(9 + b); };
-    auto kv_empty = [&](int b) { return bar(11 + b); };
-    auto p_half = [&](int t) { return bar(13 + t); };
-    const uint32_t drained = bar(15);
+    auto q_full = [&](int t) { return bar(t); };
+    auto s_full = [&](int t) { return bar(2 + t); };
+    auto p_half = [&](int t) { return bar(4 + t); };
+    auto p_full = [&](int t) { return bar(6 + t); };
+    auto k_empty = [&](int b) { return bar(8 + b); };
+    auto v_empty = [&](int b) { return bar(10 + b); };
+    auto o_done = [&](int t) { return bar(12 + t); };
+    auto k_full = [&](int b) { return bar(14 + b); };
+    auto v_full = [&](int b) { return bar(16 + b); };
+    auto drained = [&](int t) { return bar(18 + t); };
+    auto turn = [&](int t) { return bar(20 + t); };
 
     const int* item = a.items + (long)blockIdx.y * ITEM_INTS;
     const int tok0 = item[0], n_tok = item[1], entry = item[2], pos0 = item[3], kb_begin = item[4], kb_end = item[5], part = item[6];
@@ -122,7 +131,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
 
     if (threadIdx.x == 0) {
         abort_flag_s = 0;
-        for (int i = 0; i < 16; ++i) mbar_init(bar(i), i == 3 || i == 4 || i == 13 || i == 14 ? 4 : 1);      // (p_full, p_half: four warps)
+        for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), (i >= 4 && i < 8) || i >= 20 ? 4 : i >= 8 && i < 12 ? nt : 1);      // (p_half, p_full, turn: four warps; k_empty, v_empty: the sub-tiles)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -139,83 +148,89 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
     auto tmem_s = [&](int t) { return tmem + 128u * t; };            // S_t, and P_t over its first 64 columns
     auto tmem_o = [&](int t) { return tmem + 256u + 128u * t; };
 
-    int asked = 0;                                                   // blocks under way or there
-    if (warp == 1) {
-        // ---------------- the queries; products: PV_0(i), S_0(i + 1), PV_1(i), S_1(i + 1) ----------------
-        if (lane == 0) {
-            mbar_expect_tx(q_full, (uint32_t)(nt * L::HALVES * per * a.group * 128));
-            for (int t = 0; t < nt; ++t)
-                for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + t * L::TILE + h * L::SUB, &map_q, h * 64, 0, kvh, tok0 + t * per, q_full);
-            constexpr uint32_t idesc_s = instr_desc_ex(BQ, BK, 0), idesc_o = instr_desc_ex(BQ, D, 1);
-            int n_p[2] = {0, 0};
-            const int last0 = last_of(0), last1 = last_of(1);
-            bool ok = mbar_wait(q_full, 0, abort_flag);
-            auto issue_s = [&](int t, int i) {
-                const int b = i & 1;
+    int k_asked = 0, v_asked = 0;                                    // blocks under way or there
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
+        if (warp == 1 || warp == 2) {
+            // ---------------- a sub-tile's queries; its products: S(0), then PV(i), S(i + 1) ----------------
+            const int t = warp - 1;
+            if (lane == 0 && t < nt) {
+                mbar_expect_tx(q_full(t), (uint32_t)(L::HALVES * per * a.group * 128));
+                for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + t * L::TILE + h * L::SUB, &map_q, h * 64, 0, kvh, tok0 + t * per, q_full(t));
+                constexpr uint32_t idesc_s = instr_desc_ex(BQ, BK, 0), idesc_o = instr_desc_ex(BQ, D, 1);
+                const uint32_t ts = tmem_s(t), to = tmem_o(t);
+                const int last = last_of(t);
+                uint32_t n_p = 0;
+                bool ok = met(q_full(t), 0, abort_flag);
+                auto issue_s = [&](int b) {
+                    tc_fence_after();
 #pragma unroll
-                for (int h = 0; h < L::HALVES; ++h) {
-                    const uint64_t dq = smem_desc(base + t * L::TILE + h * L::SUB), dk = smem_desc(base + L::K_OFF + b * L::TILE + h * L::SUB);
+                    for (int h = 0; h < L::HALVES; ++h) {
+                        const uint64_t dq = smem_desc(base + t * L::TILE + h * L::SUB), dk = smem_desc(base + L::K_OFF + b * L::TILE + h * L::SUB);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc_mma(tmem_s(t), dq + 2u * k, dk + 2u * k, idesc_s, (h | k) != 0);
+                        for (int k = 0; k < 4; ++k) tc_mma(ts, dq + 2u * k, dk + 2u * k, idesc_s, (h | k) != 0);
+                    }
+                    tc_commit(s_full(t));
+                };
+                auto k_there = [&](int i) { return i >= n_walk || met(k_full(i & 1), (uint32_t)(i >> 1) & 1u, abort_flag); };
+                ok = ok && k_there(0);
+                if (ok && n_walk > 0) {
+                    if (active(t, 0)) issue_s(0);
+                    tc_commit(k_empty(0));
                 }
-                tc_commit(s_full(t));
-            };
-            auto k_there = [&](int i) { return i >= n_walk || mbar_wait(k_full(i & 1), (uint32_t)(i >> 1) & 1u, abort_flag); };
-            ok = ok && k_there(0);
-            tc_fence_after();
-            for (int t = 0; t < nt && ok; ++t)
-                if (active(t, 0)) issue_s(t, 0);
-            for (int i = 0; i < n_walk && ok; ++i) {
-                const int b = i & 1;
-                ok = mbar_wait(v_full(b), (uint32_t)(i >> 1) & 1u, abort_flag) && k_there(i + 1);
-                for (int t = 0; t < nt && ok; ++t) {
-                    if (active(t, i)) {
-                        const uint32_t phase = (uint32_t)n_p[t] & 1u;
+                for (int i = 0; i < n_walk && ok; ++i) {
+                    const int b = i & 1;
+                    ok = met(v_full(b), (uint32_t)(i >> 1) & 1u, abort_flag) && k_there(i + 1);      // (while the weights are made)
+                    if (ok && active(t, i)) {
                         auto issue_o = [&](int ks0) {
                             tc_fence_after();
 #pragma unroll
-                            for (int k = 0; k < BK / 32; ++k) {
-                                const int ks = ks0 + k;
-                                tc_mma_ts(tmem_o(t), tmem_s(t) + 8u * ks, smem_desc_lbo_sbo(base + L::V_OFF + b * L::TILE + ks * 2048, L::SUB, 1024), idesc_o,
-                                          (n_p[t] | ks) != 0);
-                            }
+                            for (int k = 0; k < BK / 32; ++k)
+                                tc_mma_ts(to, ts + 8u * (ks0 + k), smem_desc_lbo_sbo(base + L::V_OFF + b * L::TILE + (ks0 + k) * 2048, L::SUB, 1024), idesc_o,
+                                          (n_p | (ks0 + k)) != 0);
                         };
-                        ok = mbar_wait(p_half(t), phase, abort_flag);
+                        ok = met(p_half(t), n_p & 1u, abort_flag);
                         if (!ok) break;
                         issue_o(0);
-                        ok = mbar_wait(p_full(t), phase, abort_flag);
+                        ok = met(p_full(t), n_p & 1u, abort_flag);
                         if (!ok) break;
                         issue_o(BK / 32);
-                        ++n_p[t];
-                        if (i == (t ? last1 : last0)) tc_commit(o_done(t));
+                        ++n_p;
+                        if (i == last) tc_commit(o_done(t));
                     }
-                    if (t == nt - 1) tc_commit(kv_empty(b));   // every product that reads this block has been issued
-                    if (active(t, i + 1)) issue_s(t, i + 1);
+                    if (!ok) break;
+                    if (active(t, i + 1)) issue_s(b ^ 1);
+                    tc_commit(v_empty(b));                          // every product that reads these has been issued
+                    if (i + 1 < n_walk) tc_commit(k_empty(b ^ 1));
+                }
+                if (*abort_flag) {                                  // given up: no product may outlive tensor memory
+                    tc_commit(drained(t));
+                    for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(drained(t), 0); ++i) { }
                 }
             }
-            if (*abort_flag) {                                  // given up: no product may outlive tensor memory
-                tc_commit(drained);
-                for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(drained, 0); ++i) { }
+            __syncwarp();
+        } else if (warp == 0) {
+            // ---------------- keys and values: a block is a page ----------------
+            if (lane == 0) {
+                const int* table = a.block_table + (long)entry * a.table_width;
+                for (int i = 0; i < n_walk; ++i) {
+                    const int b = i & 1, j = first_blk + i, found = j < a.table_width ? table[j] : -1, page = found < 0 ? a.n_pages : found;   // (none: zeros)
+                    if (!met(k_empty(b), (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag)) break;
+                    mbar_expect_tx(k_full(b), (uint32_t)L::TILE);
+                    for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + L::K_OFF + b * L::TILE + h * L::SUB, &map_k, h * 64, 0, kvh, page, k_full(b));
+                    ++k_asked;
+                    if (!met(v_empty(b), (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag)) break;
+                    mbar_expect_tx(v_full(b), (uint32_t)L::TILE);
+                    for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + L::V_OFF + b * L::TILE + h * L::SUB, &map_v, h * 64, 0, kvh, page, v_full(b));
+                    ++v_asked;
+                }
             }
+            __syncwarp();
         }
-        __syncwarp();
-    } else if (warp == 0) {
-        // ---------------- keys and values: a block is a page ----------------
-        if (lane == 0) {
-            const int* table = a.block_table + (long)entry * a.table_width;
-            for (int i = 0; i < n_walk; ++i, ++asked) {
-                const int b = i & 1, j = first_blk + i, found = j < a.table_width ? table[j] : -1, page = found < 0 ? a.n_pages : found;   // (none: zeros)
-                if (!mbar_wait(kv_empty(b), (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag)) break;
-                mbar_expect_tx(k_full(b), (uint32_t)L::TILE);
-                for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + L::K_OFF + b * L::TILE + h * L::SUB, &map_k, h * 64, 0, kvh, page, k_full(b));
-                mbar_expect_tx(v_full(b), (uint32_t)L::TILE);
-                for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + L::V_OFF + b * L::TILE + h * L::SUB, &map_v, h * 64, 0, kvh, page, v_full(b));
-            }
-        }
-        __syncwarp();
     } else {
         // ---------------- softmax: a row a thread ----------------
-        const int t = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;      // (tensor memory: a warp may touch lanes 32 (warp % 4) ..)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
+        const int t = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;      // (tensor memory: a warp may touch lanes 32 (warp % 4) ..)
         if (t < nt) {
             const int rows_t = tokens_of(t) * a.group, tok = r / a.group, pos_t = pos0 + t * per, p_r = pos_t + tok;
             const int lo_r = fx_first_key(p_r, a.window, 0), lo_last = fx_first_key(pos_t + tokens_of(t) - 1, a.window, 0);
@@ -224,49 +239,48 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
             bool ok = true;
             int cnt = 0;
             for (int i = 0; i < n_walk; ++i) {
-                if (!active(t, i)) continue;
-                ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), (uint32_t)cnt & 1u, abort_flag));
+                auto my_turn = [&]() { return nt == 1 || (t == 0 && i == 0) || __all_sync(0xffffffffu, met(turn(t), (uint32_t)(i - 1 + t) & 1u, abort_flag)); };
+                auto your_turn = [&]() { if (nt > 1 && lane == 0) mbar_arrive(turn(t ^ 1)); };
+                if (__builtin_expect(!active(t, i), 0)) {
+                    ok = my_turn();
+                    if (!ok) break;
+                    your_turn();
+                    continue;
+                }
+                ok = __all_sync(0xffffffffu, met(s_full(t), (uint32_t)cnt & 1u, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
-                if (quad * 32 >= rows_t) {               // none of the warp's rows exists: what its rows of P hold reaches no others
+                if (__builtin_expect(quad * 32 >= rows_t, 0)) {               // none of the warp's rows exists: what its rows of P hold reaches no others
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) { mbar_arrive(p_half(t)); mbar_arrive(p_full(t)); }
                     ++cnt;
+                    ok = my_turn();
+                    if (!ok) break;
+                    your_turn();
                     continue;
                 }
                 const int kb = (first_blk + i) * BK;
                 const bool interior = kb + BK - 1 <= pos_t && kb >= lo_last;   // every row sees all of the block: no masking (most blocks)
                 uint32_t c[4][32];                       // the row's scores
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, c[i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tc_ld_wait_for(c[i]);
+                if (__builtin_expect(!interior, 0)) {    // (out of the way of what most blocks run through)
+#pragma unroll
+                    for (int k = 0; k < BK; ++k)
+                        if (kb + k > p_r || kb + k < lo_r) c[k / 32][k % 32] = 0xff800000u;      // -infinity
+                }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                auto look = [&](int chunk) {
-                    if (!interior)
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const int key = kb + chunk * 32 + k;
-                            if (key > p_r || key < lo_r) c[chunk][k] = 0xff800000u;      // -infinity
-                        }
+                for (int k = 0; k < BK; k += 8)
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(c[chunk][k + e])), __uint_as_float(c[chunk][k + 4 + e]));
-                };
-                tc_ld32(ts, c[0]);
-                tc_ld32(ts + 32, c[1]);
-                tc_ld_wait_for(c[0]);
-                tc_ld_wait_for(c[1]);
-                tc_ld32(ts + 64, c[2]);
-                tc_ld32(ts + 96, c[3]);
-                look(0);
-                look(1);
-                tc_ld_wait_for(c[2]);
-                tc_ld_wait_for(c[3]);
-                look(2);
-                look(3);
+                    for (int e = 0; e < 4; ++e)
+                        mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(c[k / 32][k % 32 + e])), __uint_as_float(c[k / 32][k % 32 + 4 + e]));
                 const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
                 const bool raise = r < rows_t && mn > m && (m == -INFINITY || (mn - m) * a.scale_log2e > RAISE_MAX_BY);
-                if (__any_sync(0xffffffffu, raise)) {
+                if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
                     const float alpha = m == -INFINITY ? 0.f : exp2_fast((m - mn) * a.scale_log2e);
                     l *= alpha;
                     m = mn;
@@ -284,7 +298,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                 }
                 // weights in bfloat16 pairs over the first 64 columns of S, all of which has been read
                 const float ref = m == -INFINITY ? 0.f : m * a.scale_log2e;
-                const uint64_t scale2 = pair_of(__float_as_uint(a.scale_log2e), __float_as_uint(a.scale_log2e)), ref2 = pair_of(__float_as_uint(-ref), __float_as_uint(-ref));
+                const uint64_t scale2 = both(a.scale_log2e), ref2 = both(-ref);
                 uint64_t sum2[2] = {0, 0};
                 auto weigh = [&](int chunk) {
                     uint32_t out[16];
@@ -298,6 +312,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                     }
                     tc_st16(ts + chunk * 16, out);
                 };
+                ok = my_turn();
+                if (!ok) break;
                 weigh(0);
                 weigh(1);
                 tc_st_wait();
@@ -305,6 +321,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_half(t));
                 weigh(2);
+                your_turn();
                 weigh(3);
                 tc_st_wait();
                 tc_fence_before();
@@ -315,7 +332,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                 ++cnt;
             }
             const bool has = last_of(t) >= 0;
-            if (ok && has) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), 0, abort_flag));
+            if (ok && has) ok = __all_sync(0xffffffffu, met(o_done(t), 0, abort_flag));
             if (ok) {
                 tc_fence_after();
                 const long slot = ((long)max(part, 0) * a.n_kv_heads + kvh) * (2 * BQ) + t * BQ + r;
@@ -356,8 +373,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
     if (threadIdx.x == 0 && abort_flag_s) {
         // given up: the copies under way still land
         auto settle = [](uint32_t at, uint32_t parity) { for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(at, parity); ++i) { } };
-        settle(q_full, 0);
-        for (int i = max(0, asked - 2); i < asked; ++i) { settle(k_full(i & 1), (uint32_t)(i >> 1) & 1u); settle(v_full(i & 1), (uint32_t)(i >> 1) & 1u); }
+        for (int t = 0; t < nt; ++t) settle(q_full(t), 0);
+        for (int i = max(0, k_asked - 2); i < k_asked; ++i) settle(k_full(i & 1), (uint32_t)(i >> 1) & 1u);
+        for (int i = max(0, v_asked - 2); i < v_asked; ++i) settle(v_full(i & 1), (uint32_t)(i >> 1) & 1u);
         if (a.status) atomicExch(a.status, STATUS_TC_TIMEOUT);
     }
 }
@@ -399,6 +417,9 @@ template <int D>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int n_items, const int* merges, int n_merges, cudaStream_t s)
 {
     auto kern = prefill_grouped_kernel<D>;
+    // what the softmax threads ask for has to be there: the block's registers at its launch
+    static const bool fits = [&] { cudaFuncAttributes at; return cudaFuncGetAttributes(&at, kern) == cudaSuccess && at.numRegs * 3 >= REGS_FEW + 2 * REGS_MANY; }();
+    if (!fits) return FX_ERR_SIZE;
     // of the current device: asked for each time
     if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL)) return (int)e;
     fx_launch_pdl(kern, dim3(a.n_kv_heads, n_items), NTHREADS, Smem<D>::TOTAL, s, mq, mk, mv, a);

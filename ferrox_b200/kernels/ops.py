@@ -2377,8 +2377,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
 
 
 def prefill_grouped_ok(q, out, n_heads: int, n_kv_heads: int, head_dim: int, scale: float) -> bool:
-    """Whether :func:`prefill_attention_grouped` takes these operands and has something to gain: query heads that share key heads."""
-    return (q.dtype is torch.bfloat16 and n_kv_heads < n_heads <= 128 * n_kv_heads and 0 < head_dim <= 128 and head_dim % 16 == 0 and scale > 0
+    """Whether :func:`prefill_attention_grouped` takes these operands."""
+    return (q.dtype is torch.bfloat16 and n_heads <= 128 * n_kv_heads and 0 < head_dim <= 128 and head_dim % 16 == 0 and scale > 0
             and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
 
 
@@ -2390,7 +2390,7 @@ def prefill_grouped_plan(entries, window, n_heads: int, n_kv_heads: int):
 
 def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_heads, n_kv_heads, head_dim, window, scale, status=None,
                               stream=None, merges=None, parts=0):
-    """Attention of prompt portions in bfloat16 whose query heads share key heads, over pages of 128 positions [pages, kv heads, 128,
+    """Attention of prompt portions in bfloat16, of query heads that may share key heads, over pages of 128 positions [pages, kv heads, 128,
     head_dim] (see :func:`prefill_grouped_ok`).  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``,
     ``parts``: device copies of what :func:`prefill_grouped_plan` returns, and its number of parts."""
     if k_pages.shape != v_pages.shape or k_pages.shape[1:] != (n_kv_heads, 128, head_dim) or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
