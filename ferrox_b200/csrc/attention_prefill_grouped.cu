@@ -1,35 +1,45 @@
-// Attention for prompt portions whose query heads share key heads, on the 5th-generation tensor cores (bfloat16, heads of up to
-// 128 elements in steps of 16), over pages of 128 positions: what read_kv_fp8_spans makes of an 8-bit cache.
+// Attention for prompt portions on the 5th-generation tensor cores (bfloat16, heads of up to 128 elements in steps of 16), over
+// pages of 128 positions: what read_kv_fp8_spans makes of an 8-bit cache.
 //
 // A row is a (token, query head) pair; the rows of a tile are the query heads of one kv head for consecutive tokens of a
 // request, so that a block of keys and values that has been brought in serves all of them, and a portion of few tokens fills
 // its tiles with its heads (the kernel of attention_prefill_tc.cu has a head's tokens for rows: a portion of 300 tokens takes
-// tiles of 256 and 44 there, of 2,100 rows here).  One CTA takes two sub-tiles of up to 128 rows and walks the request's keys in
-// blocks of 128:
+// tiles of 256 and 44 there, of 2,100 rows here where 7 heads share their keys).  One CTA takes two sub-tiles of up to 128 rows
+// and walks the request's keys in blocks of 128:
 //
 //   S_t = Q_t K_j^T    tcgen05.mma 128 x 128 x head_dim, Q by TMA ([token][head][64 elements] boxes), S_t in tensor memory
 //   P_t = 2^(S_t - m)  a thread a row: mask by absolute position, running maximum and sum in 32 bits, P in bfloat16 over S_t
-//   O_t += P_t V_j     tcgen05.mma, A from tensor memory, V as an N-major B operand
+//   O_t += P_t V_j     tcgen05.mma, A from tensor memory, V as an N-major B operand; its first half as soon as half of P_t is
+//                      written
 //
-// What bounds it: the softmax threads' instructions, 4.5 a score.  (Converting the 8-bit pages in this kernel, by seven more
-// warps, cost those threads a third of their registers and the tile its pace: 28 heads of 128 on 4, six portions of 300 tokens
-// behind up to 3,800: 162 us; prompts of 2,048 of 16 heads each with its own keys 86 us against 67 with the pages read back.)
+// Warps: 0 brings keys and values (TMA, two places each), 1 the queries and issues the products in the order PV_0(i), S_0(i + 1),
+// PV_1(i), S_1(i + 1), which keeps the sub-tiles half a block apart: one's products run under the other's softmax.  4 - 7 and 8 -
+// 11 are the sub-tiles' rows; they hold a row's 128 scores in registers, which the first four warps have left to them.
+//
+// What bounds it, in clocks of a pair of blocks, of which the four products are 2,056: a sub-tile's chain of waits.  Scores read and
+// their maximum found 500, asked whether it is to be raised 190, weights 1,540 (their 2^x alone 1,024), the rest of PV and the next
+// S 1,330.  B200: 3,600 clocks a pair with few blocks running, 2.39 us with all (982 TFLOP/s over long contexts; 28 heads of 128 on 4).  Six
+// portions of 300 tokens behind up to 3,800, the pages' reading back included: 86 us; a prompt of 2,048 of 16 heads with their own
+// keys 49.5 (by the kernel of attention_prefill_tc.cu 65).  Tried: scores read twice instead of held, P in one piece 2.91 us a pair; a
+// thread of its own for each sub-tile's products, softmaxes in turns 2.56, without turns 2.89 (both then do the same at the same
+// time); a quarter of the 2^x by polynomial 2.64; rolled loops around the products 2.71.  Converting the 8-bit pages in this
+// kernel, by seven more warps, cost the softmax threads a third of their registers and the tile its pace (162 us and 86 us where
+// reading back first then took 124 and 67).
 //
 // A row of the cache that is not finite arrives as a key of NaN and a value of 0 (read_kv_fp8_spans): the scores against it are
 // NaN where a query sees it and masked away where none does, and 0 times the value is 0.  What lies behind a request's last
 // position in its last page is 0.
 //
-// The running maximum is raised only when it grows by more than 2^8; O is then scaled in tensor memory.  Warps: 0 brings keys
-// and values (TMA, two places each), 1 the queries and issues the products, 2 - 5 and 6 - 9 are the sub-tiles' rows.  Every wait
-// is bounded (status 3).  Tiles with many key blocks may be cut into runs, which a second kernel adds up in their order (items:
-// as the plan of the kernel above, with tokens for rows and kv heads for heads).
+// The running maximum is raised only when it grows by more than 2^8; O is then scaled in tensor memory.  Every wait is bounded
+// (status 3).  Tiles with many key blocks may be cut into runs, which a second kernel adds up in their order (items: as the plan of
+// the kernel above, with tokens for rows and kv heads for heads).
 #include "tc_common.cuh"
 #include "api.h"
 
 namespace {
 using namespace fxtc;
 
-constexpr int BQ = 128, BK = 128, NTHREADS = 384, TMEM_COLS = 512, ITEM_INTS = 8, N_BARS = 22;
+constexpr int BQ = 128, BK = 128, NTHREADS = 384, TMEM_COLS = 512, ITEM_INTS = 8, N_BARS = 19;
 constexpr int REGS_FEW = 88, REGS_MANY = 208;   // a thread of the first four warps, of the softmax: together what the block is launched with
 constexpr float RAISE_MAX_BY = 8.f;   // in powers of two
 
@@ -113,8 +123,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
     auto o_done = [&](int t) { return bar(12 + t); };
     auto k_full = [&](int b) { return bar(14 + b); };
     auto v_full = [&](int b) { return bar(16 + b); };
-    auto drained = [&](int t) { return bar(18 + t); };
-    auto turn = [&](int t) { return bar(20 + t); };
+    const uint32_t drained = bar(18);
 
     const int* item = a.items + (long)blockIdx.y * ITEM_INTS;
     const int tok0 = item[0], n_tok = item[1], entry = item[2], pos0 = item[3], kb_begin = item[4], kb_end = item[5], part = item[6];
@@ -131,7 +140,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
 
     if (threadIdx.x == 0) {
         abort_flag_s = 0;
-        for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), (i >= 4 && i < 8) || i >= 20 ? 4 : i >= 8 && i < 12 ? nt : 1);      // (p_half, p_full, turn: four warps; k_empty, v_empty: the sub-tiles)
+        for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= 4 && i < 8 ? 4 : 1);      // (p_half, p_full: four warps)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -151,61 +160,67 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
     int k_asked = 0, v_asked = 0;                                    // blocks under way or there
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
-        if (warp == 1 || warp == 2) {
-            // ---------------- a sub-tile's queries; its products: S(0), then PV(i), S(i + 1) ----------------
-            const int t = warp - 1;
-            if (lane == 0 && t < nt) {
-                mbar_expect_tx(q_full(t), (uint32_t)(L::HALVES * per * a.group * 128));
-                for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + t * L::TILE + h * L::SUB, &map_q, h * 64, 0, kvh, tok0 + t * per, q_full(t));
+        if (warp == 1) {
+            // ---------------- queries; products: S_0(0), S_1(0), then PV_0(i), S_0(i + 1), PV_1(i), S_1(i + 1) ----------------
+            if (lane == 0) {
+                for (int t = 0; t < nt; ++t) {
+                    mbar_expect_tx(q_full(t), (uint32_t)(L::HALVES * per * a.group * 128));
+                    for (int h = 0; h < L::HALVES; ++h) tma_load_4d(base + t * L::TILE + h * L::SUB, &map_q, h * 64, 0, kvh, tok0 + t * per, q_full(t));
+                }
                 constexpr uint32_t idesc_s = instr_desc_ex(BQ, BK, 0), idesc_o = instr_desc_ex(BQ, D, 1);
-                const uint32_t ts = tmem_s(t), to = tmem_o(t);
-                const int last = last_of(t);
-                uint32_t n_p = 0;
-                bool ok = met(q_full(t), 0, abort_flag);
-                auto issue_s = [&](int b) {
+                uint32_t n_p[2] = {0, 0};
+                auto issue_s = [&](int t, int b) {
                     tc_fence_after();
 #pragma unroll
                     for (int h = 0; h < L::HALVES; ++h) {
                         const uint64_t dq = smem_desc(base + t * L::TILE + h * L::SUB), dk = smem_desc(base + L::K_OFF + b * L::TILE + h * L::SUB);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) tc_mma(ts, dq + 2u * k, dk + 2u * k, idesc_s, (h | k) != 0);
+                        for (int k = 0; k < 4; ++k) tc_mma(tmem_s(t), dq + 2u * k, dk + 2u * k, idesc_s, (h | k) != 0);
                     }
                     tc_commit(s_full(t));
                 };
                 auto k_there = [&](int i) { return i >= n_walk || met(k_full(i & 1), (uint32_t)(i >> 1) & 1u, abort_flag); };
-                ok = ok && k_there(0);
-                if (ok && n_walk > 0) {
-                    if (active(t, 0)) issue_s(0);
-                    tc_commit(k_empty(0));
+                bool ok = k_there(0);
+                for (int t = 0; t < nt && ok; ++t) {
+                    ok = met(q_full(t), 0, abort_flag);
+                    if (ok && active(t, 0)) issue_s(t, 0);
                 }
+                if (ok && n_walk > 0) tc_commit(k_empty(0));
+                ok = ok && (n_walk == 0 || met(v_full(0), 0, abort_flag)) && k_there(1);
                 for (int i = 0; i < n_walk && ok; ++i) {
                     const int b = i & 1;
-                    ok = met(v_full(b), (uint32_t)(i >> 1) & 1u, abort_flag) && k_there(i + 1);      // (while the weights are made)
-                    if (ok && active(t, i)) {
-                        auto issue_o = [&](int ks0) {
-                            tc_fence_after();
 #pragma unroll
-                            for (int k = 0; k < BK / 32; ++k)
-                                tc_mma_ts(to, ts + 8u * (ks0 + k), smem_desc_lbo_sbo(base + L::V_OFF + b * L::TILE + (ks0 + k) * 2048, L::SUB, 1024), idesc_o,
-                                          (n_p | (ks0 + k)) != 0);
-                        };
-                        ok = met(p_half(t), n_p & 1u, abort_flag);
-                        if (!ok) break;
-                        issue_o(0);
-                        ok = met(p_full(t), n_p & 1u, abort_flag);
-                        if (!ok) break;
-                        issue_o(BK / 32);
-                        ++n_p;
-                        if (i == last) tc_commit(o_done(t));
+                    for (int t = 0; t < 2; ++t) {
+                        if (t >= nt || !ok) continue;
+                        if (active(t, i)) {
+                            auto issue_o = [&](int ks0) {
+                                tc_fence_after();
+#pragma unroll
+                                for (int k = 0; k < BK / 32; ++k)
+                                    tc_mma_ts(tmem_o(t), tmem_s(t) + 8u * (ks0 + k), smem_desc_lbo_sbo(base + L::V_OFF + b * L::TILE + (ks0 + k) * 2048, L::SUB, 1024),
+                                              idesc_o, (n_p[t] | (ks0 + k)) != 0);
+                            };
+                            ok = met(p_half(t), n_p[t] & 1u, abort_flag);
+                            if (!ok) continue;
+                            issue_o(0);
+                            ok = met(p_full(t), n_p[t] & 1u, abort_flag);
+                            if (!ok) continue;
+                            issue_o(BK / 32);
+                            ++n_p[t];
+                        }
+                        if (active(t, i + 1)) issue_s(t, b ^ 1);
+                        else if (i == last_of(t)) tc_commit(o_done(t));
                     }
                     if (!ok) break;
-                    if (active(t, i + 1)) issue_s(b ^ 1);
                     tc_commit(v_empty(b));                          // every product that reads these has been issued
-                    if (i + 1 < n_walk) tc_commit(k_empty(b ^ 1));
+                    if (i + 1 < n_walk) {
+                        tc_commit(k_empty(b ^ 1));
+                        ok = met(v_full(b ^ 1), (uint32_t)((i + 1) >> 1) & 1u, abort_flag) && k_there(i + 2);      // (while the weights are made)
+                    }
                 }
                 if (*abort_flag) {                                  // given up: no product may outlive tensor memory
-                    tc_commit(drained(t));
-                    for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(drained(t), 0); ++i) { }
+                    tc_commit(drained);
+                    for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(drained, 0); ++i) { }
                 }
             }
             __syncwarp();
@@ -239,14 +254,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
             bool ok = true;
             int cnt = 0;
             for (int i = 0; i < n_walk; ++i) {
-                auto my_turn = [&]() { return nt == 1 || (t == 0 && i == 0) || __all_sync(0xffffffffu, met(turn(t), (uint32_t)(i - 1 + t) & 1u, abort_flag)); };
-                auto your_turn = [&]() { if (nt > 1 && lane == 0) mbar_arrive(turn(t ^ 1)); };
-                if (__builtin_expect(!active(t, i), 0)) {
-                    ok = my_turn();
-                    if (!ok) break;
-                    your_turn();
-                    continue;
-                }
+                if (!active(t, i)) continue;
                 ok = __all_sync(0xffffffffu, met(s_full(t), (uint32_t)cnt & 1u, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
@@ -255,9 +263,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                     __syncwarp();
                     if (lane == 0) { mbar_arrive(p_half(t)); mbar_arrive(p_full(t)); }
                     ++cnt;
-                    ok = my_turn();
-                    if (!ok) break;
-                    your_turn();
                     continue;
                 }
                 const int kb = (first_blk + i) * BK;
@@ -312,8 +317,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                     }
                     tc_st16(ts + chunk * 16, out);
                 };
-                ok = my_turn();
-                if (!ok) break;
                 weigh(0);
                 weigh(1);
                 tc_st_wait();
@@ -321,7 +324,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_half(t));
                 weigh(2);
-                your_turn();
                 weigh(3);
                 tc_st_wait();
                 tc_fence_before();
