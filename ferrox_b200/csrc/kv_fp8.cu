@@ -52,7 +52,7 @@ __device__ __forceinline__ float turned(const WriteArgs& a, int t, int pos, floa
 // Rows of LANES lanes with 16 bytes each (or 32 lanes with 32 bytes), a rotation of the whole head in halves or none.  A block
 // takes a token's rows, or a share of them (blockIdx.y); a lane loads R rows' parts before it works on the first.  What bounds
 // it is how many bytes are under way: the place of a token's position is four loads that hang on one another, beside which its
-// rows arrive.  B200, 2,705 tokens with 16 heads of 128 for keys and for values, written and read back: one row a warp 34.4 us,
+// rows arrive.  B200, 2,709 tokens with 16 heads of 128 for keys and for values, written and read back: one row a warp 34.4 us,
 // four rows a lane 20.5 (each of the two launches moves 33 MB, 5.1 us of the memory); 32 tokens of 4 heads 4.5, which are the launches.
 template <typename T, int DIM, int R>
 __global__ void __launch_bounds__(WRITE_WARPS * 32) write_rows_kernel(WriteArgs a)
@@ -342,6 +342,7 @@ extern "C" int fx_rope_kv_write_fp8(void* qkv, int dtype, long ld, const int* po
                          (uint8_t*)k_exp, (uint8_t*)v_exp, block_table, n_slots, table_width, page_size, n_pages, n_tokens, n_heads, n_kv_heads,
                          head_dim, inv_freq ? 0 : n_heads, write_cache, status};
     if ((long)n_tokens * (n_heads + 2 * n_kv_heads) > 0x7fffffffL || n_heads + 2 * n_kv_heads > 65535) return FX_ERR_SIZE;
+    if (inv_freq && (uintptr_t)cos_sin % 8) return FX_ERR_ALIGN;
     const int es = dtype == FX_F32 ? 4 : 2;
     const bool whole = (!inv_freq || (rotary_dim == head_dim && pairing == 0)) && (head_dim == 64 || head_dim == 128 || head_dim == 256) &&
                        ld * es % 16 == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)k_pages % 8 == 0 && (uintptr_t)v_pages % 8 == 0;

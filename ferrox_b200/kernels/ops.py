@@ -2341,7 +2341,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     The keys and values that a portion sees are read back once into pages of q's type (exact: an element has four significant bits
     and a power of two) and the attention kernels for such pages take them from there: tensor cores then meet operands that they take
     as they are, where conversion in the attention kernel would be paid again for every tile.  Every position that is seen has a page.
-    Entries of up to FP8_FEW_TOKENS tokens, and shapes that no tiled kernel takes, go to :func:`decode_attention_fp8`."""
+    Entries of up to FP8_FEW_TOKENS tokens, and shapes that no tiled kernel takes, go to :func:`decode_attention_fp8`.  A call
+    may be captured once the plan has been used; the plan lives as long as the graph."""
     name = "prefill_attention_fp8"
     found = _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, status, None,
                                    out, n_heads, n_kv_heads, head_dim, window, scale, softcap)
@@ -2360,7 +2361,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     step = (positions, token_seq, seq_slot)
     f32 = q.dtype == torch.float32
     # (asked with q in the pages' place: pages that are read back have its type and lie on the allocator's grid)
-    if not (prefill_f32_ok(q, out, q, head_dim) if f32 else prefill_ok(q, out, q, head_dim)):
+    # (and the tiled kernels find a row's maximum before they scale it)
+    if scale <= 0 or not (prefill_f32_ok(q, out, q, head_dim) if f32 else prefill_ok(q, out, q, head_dim)):
         _decode_fp8(found, page_size, n_heads, window, scale, softcap, st)
         return out
     plan.on_stream(st)
@@ -2388,25 +2390,32 @@ def prefill_grouped_plan(entries, window, n_heads: int, n_kv_heads: int):
     return prefill_tc_plan(entries, window, n_kv_heads, tile=2 * (128 * n_kv_heads // n_heads))
 
 
+_GROUPED = "xTQ~ xNGPD xNGPD iBW in8 xTO~ ?im4 ?iZ"
+
+
 def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_heads, n_kv_heads, head_dim, window, scale, status=None,
                               stream=None, merges=None, parts=0):
     """Attention of prompt portions in bfloat16, of query heads that may share key heads, over pages of 128 positions [pages, kv heads, 128,
     head_dim] (see :func:`prefill_grouped_ok`).  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``,
     ``parts``: device copies of what :func:`prefill_grouped_plan` returns, and its number of parts."""
-    if k_pages.shape != v_pages.shape or k_pages.shape[1:] != (n_kv_heads, 128, head_dim) or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
-        raise KernelError(f"prefill_attention_grouped: contiguous pages [pages, {n_kv_heads}, 128, {head_dim}], found {tuple(k_pages.shape)} and "
-                          f"{tuple(v_pages.shape)}")
-    po = pm = n_merges = 0
+    name = "prefill_attention_grouped"
+    (_, now, x, qp, kp, vp, tp, ip, op, mp, zp, T, Q, N, G, P, D, B, W, n, eight, O, n_merges, four, _, ldq, ldo) = _operands(
+        name, _GROUPED, ("q", "k_pages", "v_pages", "block_table", "items", "out", "merges", "status"), q, k_pages, v_pages, block_table, items, out,
+        merges, status)
+    if (x != BF16 or (G, P, D) != (n_kv_heads, 128, head_dim) or n_heads < 1 or n_heads % G or min(Q, O) < n_heads * D or eight != 8 or four not in (-1, 4)
+            or (parts and n_merges < 1)):
+        raise KernelError(f"{name}: bfloat16, {n_heads} heads on pages [pages, {n_kv_heads}, 128, {head_dim}], items [n, 8], merges [n, 4] of {parts} parts: "
+                          f"found {q.dtype}, pages [{N}, {G}, {P}, {D}], rows of {Q} and {O}, items [{n}, {eight}], merges [{n_merges}, {four}]")
+    po = pm = 0
     if parts:
         global _launches
         _launches += 1
-        width, n_merges = 64 if head_dim <= 64 else 128, merges.shape[0]
+        width = 64 if head_dim <= 64 else 128
         work = torch.empty(parts * n_kv_heads * 256 * (width + 2), dtype=torch.float32, device=q.device)
         po = work.data_ptr()
         pm = po + 4 * parts * n_kv_heads * 256 * width
-    call("fx_prefill_attention_grouped", _ptr(q), _rows(q), q.shape[0], _ptr(k_pages), _ptr(v_pages), k_pages.shape[0], _ptr(block_table),
-         block_table.shape[1], _ptr(items), items.shape[0], _ptr(out), _rows(out), n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), po,
-         pm, _ptr(merges) if n_merges else 0, n_merges, _ptr(status), stream if stream is not None else stream_ptr())
+    call("fx_prefill_attention_grouped", qp, ldq, T, kp, vp, N, tp, W, ip, n, op, ldo, n_heads, G, D, int(window or 0), float(scale), po, pm,
+         mp if parts else 0, n_merges if parts else 0, zp, stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
     return out
 
 

@@ -53,7 +53,7 @@ def held(pages, exps, table_row, upto):
 
 def attention(q, k, v, there, positions, heads, window, scale, softcap):
     """q [tokens, heads, dim], k and v [positions, kv heads, dim]; (results, sum of weights times |v|, the largest
-    scale * sum |q_i k_i|), each [tokens, heads, dim] or a number."""
+    |scale| * sum |q_i k_i|), each [tokens, heads, dim] or a number."""
     out, mag, most = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64), 0.0
     group = heads // k.shape[1]
     q = q.double()
@@ -66,7 +66,7 @@ def attention(q, k, v, there, positions, heads, window, scale, softcap):
         for h in range(heads):
             kk, vv = k[at, h // group], v[at, h // group]
             s = kk @ q[t, h] * scale
-            most = max(most, float(torch.nan_to_num((kk.abs() @ q[t, h].abs()).amax() * scale)))
+            most = max(most, float(torch.nan_to_num((kk.abs() @ q[t, h].abs()).amax() * abs(scale))))
             if softcap:
                 s = softcap * torch.tanh(s / softcap)
             w = torch.softmax(s, 0)

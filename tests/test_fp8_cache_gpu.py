@@ -546,6 +546,53 @@ def test_stretches_that_begin_inside_a_page(R, P):
         assert torch.equal(got.double().cpu().transpose(1, 2).reshape(row, G, D), want)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+@pytest.mark.parametrize("softcap", [None, 4.0])
+def test_scales_that_are_not_positive(dtype, scale, softcap):
+    H, G, D, P = 4, 2, 64, 64
+    entries = [(1, 149), (40, 60), (12, 0)]
+    c = Cache([150, 100, 12], G, D, P, 74)
+    q = rows(53, H, G, D, DTYPES[dtype], 75)
+    st, out = step(entries, c.slots), torch.empty(53, H * D, dtype=DTYPES[dtype], device=DEV)
+    ops.decode_attention_fp8(q, *c.operands, *st, out, H, G, D, None, scale, softcap=softcap)
+    check(out, c, entries, q, H, None, scale, softcap, WEIGHT[dtype])
+    out.fill_(7.0)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, P, DEV), *st, out, H, G, D, None, scale, softcap=softcap)
+    check(out, c, entries, q, H, None, scale, softcap, PROMPT_WEIGHT[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("H,G,D,P", [(4, 2, 128, 256), (3, 1, 64, 384), (2, 2, 20, 1), (2, 1, 256, 512), (8, 1, 16, 1024)])
+def test_pages_longer_than_a_tile(dtype, H, G, D, P):
+    lens = [1, 100, 700, 1500]
+    c = Cache(lens, G, D, P, 76)
+    entries = [(1, n - 1) for n in lens]
+    q = rows(4, H, G, D, DTYPES[dtype], 77)
+    st, out = step(entries, c.slots), torch.empty(4, H * D, dtype=DTYPES[dtype], device=DEV)
+    ops.rope_kv_write_fp8(q, *st, None, 0, *c.operands, H, G, D)
+    ops.decode_attention_fp8(q, *c.operands, *st, out, H, G, D, None, 0.1)
+    check(out, c, entries, q, H, None, 0.1, None, WEIGHT[dtype])
+    entries = [(1, 0), (50, 50), (300, 400), (20, 1480)]
+    q = rows(371, H, G, D, DTYPES[dtype], 78)
+    out = torch.empty(371, H * D, dtype=DTYPES[dtype], device=DEV)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, P, DEV), *step(entries, c.slots), out, H, G, D, None, 0.1)
+    check(out, c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT[dtype])
+
+
+@pytest.mark.parametrize("H,G,D", [(4, 4, 128), (3, 3, 48), (12, 12, 64)])
+@pytest.mark.parametrize("window", [None, 90])
+def test_prompts_of_heads_with_their_own_keys(H, G, D, window):
+    """Portions around the sizes of a sub-tile and a tile."""
+    entries = [(127, 0), (128, 5), (129, 0), (256, 131), (257, 0), (9, 300)]
+    c = Cache([n + s for n, s in entries], G, D, 64, 79)
+    T = sum(n for n, _ in entries)
+    q = rows(T, H, G, D, torch.bfloat16, 80)
+    out = torch.full((T, H * D), 7.0, dtype=q.dtype, device=DEV)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out, H, G, D, window, 0.15)
+    check(out, c, entries, q, H, window, 0.15, None, PROMPT_WEIGHT["bf16"])
+
+
 # ---- streams, graphs, order -----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_on_a_stream_of_its_own_and_in_a_graph(dtype):
@@ -717,6 +764,30 @@ def test_a_prompt_in_a_graph():
         ops.prefill_attention_fp8(q, *operands, plan, *st, want, H, G, D, None, 0.1)
         assert torch.equal(out, want)
     check(want, c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT["bf16"])
+
+
+def test_refusals_of_the_kernel_over_pages_of_128():
+    H, G, D = 4, 2, 64
+    q, out = torch.zeros(20, H * D, dtype=torch.bfloat16, device=DEV), torch.zeros(20, H * D, dtype=torch.bfloat16, device=DEV)
+    k, table = torch.zeros(1, G, 128, D, dtype=torch.bfloat16, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    items, merges, parts = ops.prefill_grouped_plan([(20, 0)], None, H, G)
+    items = torch.from_numpy(items).to(DEV)
+    good = dict(q=q, k_pages=k, v_pages=k, block_table=table, items=items, out=out, n_heads=H, n_kv_heads=G, head_dim=D, window=None, scale=1.0)
+    ops.prefill_attention_grouped(**good)
+    for bad in (dict(q=q.float()), dict(q=q.float(), out=out.float(), k_pages=k.float(), v_pages=k.float()), dict(v_pages=k[:0]), dict(k_pages=k[:, :1]),
+                dict(k_pages=k[:, :, :64], v_pages=k[:, :, :64]), dict(block_table=table.long()), dict(items=items.long()), dict(items=items[:, :7]),
+                dict(out=out[:, :64]), dict(n_heads=8), dict(n_heads=3), dict(n_kv_heads=4), dict(scale=0.0), dict(scale=-1.0), dict(parts=3),
+                dict(parts=1, merges=torch.zeros(1, 3, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ops.KernelError):
+            ops.prefill_attention_grouped(**{**good, **bad})
+
+
+def test_pairs_of_cosine_and_sine_off_their_grid():
+    H, G, D, P = 2, 1, 64, 16
+    c = Cache([4], G, D, P, 81)
+    q, cs = rows(2, H, G, D, torch.bfloat16, 82), torch.zeros(2 * 32 * 2 + 1, device=DEV)
+    with pytest.raises(ops.KernelError):
+        ops.rope_kv_write_fp8(q, *step([(2, 2)], c.slots), torch.ones(32, device=DEV), 64, *c.operands, H, G, D, cos_sin=cs[1:].reshape(2, 32, 2))
 
 
 def test_a_plan_of_another_device():
