@@ -2222,8 +2222,39 @@ def _decode_fp8(found, page_size, n_heads, window, scale, softcap, stream):
 
 
 FP8_FEW_TOKENS = 8                # entries that bring at most this many tokens are left to decode_attention_fp8
+FP8_JOIN_KEYS = 4096              # unless they stand between others and see no more keys than this: a second launch of everything costs more
 FP8_READ_BACK_MAX = 1 << 30       # bytes of keys and values that are read back at a time
 FP8_READ_PAGE = 128               # positions of a page that is read back (whatever the cache's: what every tiled kernel takes)
+
+
+def fp8_token_by_token(kind, entries, window, n_heads, n_kv_heads, head_dim, sms=0) -> bool:
+    """Whether :func:`prefill_attention_fp8` is done sooner if every token of the step goes through the decode kernel by itself: portions
+    of few tokens, whose keys would be read back and walked through by a nearly empty tile.  Microseconds, as measured on a B200.
+
+    ``kind``: the tiled kernel that would take the step.  A tile of ``rows`` (token, query head) pairs costs ``block`` a 128 keys that it sees, all
+    SMs sharing the tiles; one that is not cut into runs takes ``chain`` a key by itself; ``base`` are the launches.  20 requests of up
+    to 600 positions and 8 of up to 4,000, 24 tokens each, decode against tiled: 28 heads of 128 on 4 (grouped) 50 against 28 and 89
+    against 43, 96 tokens of one request of 600 19 against 23; the same with capped scores (tc) 52 against 82 and 94 against 176; 16 heads of
+    256 on 4 (mma) 85 against 109 and 95 against 429; 16 heads of 128 on 4 in 32 bits 48 against 119 and 81 against 322;
+    prompts of 300, 193 and 97 tokens of 4 heads of 64 on 2 in 32 bits 28 against 24."""
+    rows, base, block, chain = {"grouped": (256 * n_kv_heads // n_heads, 14.0, 2.4, 0.0), "tc": (256, 30.0, 4.5, 0.0), "mma": (PREFILL_TILE, 12.0, 3.0, 0.107 * head_dim / 256),
+                                "f32": (128, 14.0, 4.0, 0.057 * head_dim / 128)}[kind]
+    sms, group = sms or sm_count(), n_heads // n_kv_heads
+    heads = n_kv_heads if kind == "grouped" else n_heads
+    per_tile, per_run = (0.45, 1.4) if head_dim <= 128 else (0.75, 2.5)      # of the decode kernel, a run of heads that share their keys
+    runs = n_kv_heads * -(-group // (4 if group <= 4 or kind == "f32" else 8))
+    decode = tiled = back = longest = 0
+    for n, start in entries:
+        seen, most = start + n - first_key(start, window), min(start + n, int(window or 0) or start + n)
+        decode += n * runs * (per_run + per_tile * -(-most // FP8_TILE))
+        if n > FP8_FEW_TOKENS:
+            tiled += -(-n // max(rows, 1)) * heads * block * -(-seen // FP8_TILE)
+            back += seen
+            longest = max(longest, seen)
+        else:
+            tiled += n * runs * (per_run + per_tile * -(-most // FP8_TILE))
+    read = back * n_kv_heads * head_dim * (10 if kind == "f32" else 6) / 5.3e6
+    return longest == 0 or 8.0 + decode / sms < base + read + chain * longest + tiled / sms
 
 
 class PrefillFp8Plan:
@@ -2238,7 +2269,6 @@ class PrefillFp8Plan:
         if self.page_size < 1 or any(n < 0 or start < 0 for n, start in self.entries):
             raise KernelError(f"prefill_fp8_plan: entries {self.entries} of pages of {page_size}")
         self.n_tokens = sum(n for n, _ in self.entries)
-        self.has_few = any(0 < n <= FP8_FEW_TOKENS for n, _ in self.entries)
         self._kept, self._tensors, self._stream = {}, [], None
 
     def on_stream(self, stream: int):
@@ -2267,21 +2297,26 @@ class PrefillFp8Plan:
             self._kept[key] = x
         return x
 
-    def few(self):
-        """Flat indices of the tokens of entries that bring few."""
+    def token_by_token(self, kind, window, n_heads, n_kv_heads, head_dim):
+        return self.kept(("token by token", kind, window, n_heads, n_kv_heads, head_dim),
+                         lambda: fp8_token_by_token(kind, self.entries, window, n_heads, n_kv_heads, head_dim))
+
+    def few(self, window, row_bytes):
+        """Flat indices of the tokens that are in none of the parts."""
         import numpy as np
 
         def make():
-            at, flat = [], 0
-            for n, _ in self.entries:
-                if n <= FP8_FEW_TOKENS:
+            at, flat, taken = [], 0, {e[0] for g in self._groups(window, row_bytes) for e in g}
+            for b, (n, _) in enumerate(self.entries):
+                if b not in taken:
                     at += range(flat, flat + n)
                 flat += n
             return (np.asarray(at, dtype=np.int32),)
-        return self.kept("few", make)[0]
+        return self.kept(("few", window, row_bytes), make)[0]
 
     def parts(self, window, row_bytes):
-        """Neighbouring entries whose visible keys and values are read back together: (first token, tokens, entries, spans, rows,
+        """Neighbouring entries of more than FP8_FEW_TOKENS tokens (and of fewer between them, where they see few keys) whose visible keys
+        and values are read back together: (first token, tokens, entries, spans, rows,
         block table over the rows' pages, its slots), at most FP8_READ_BACK_MAX bytes each where that holds an entry at all."""
         return self.kept((window, row_bytes), lambda: [self.kept(("part", window, row_bytes, g[0][0]), lambda: self._part(window, g))
                                                        for g in self._groups(window, row_bytes)])
@@ -2291,16 +2326,23 @@ class PrefillFp8Plan:
         return p0, -(-(start + n - p0) // FP8_READ_PAGE) * FP8_READ_PAGE
 
     def _groups(self, window, row_bytes):
-        groups, flat, rows, end = [], 0, 0, -1
+        groups, flat, rows, between = [], 0, 0, None         # between: the entries of few tokens behind the last one that was taken
         for b, (n, start) in enumerate(self.entries):
-            if n > FP8_FEW_TOKENS:
-                need = self._rows_of(n, start, window)[1]
-                if end != flat or (rows + need) * row_bytes > FP8_READ_BACK_MAX:
-                    groups.append([])
-                    rows = 0
-                groups[-1].append((b, flat, n, start))
-                rows, end = rows + need, flat + n
+            entry = (b, flat, n, start)
             flat += n
+            if n <= FP8_FEW_TOKENS:
+                if between is not None and n:
+                    between.append(entry)
+                continue
+            own = self._rows_of(n, start, window)[1]
+            joined = [(e, self._rows_of(e[2], e[3], window)[1]) for e in between or ()]
+            need = own + sum(r for _, r in joined)
+            if between is None or sum(e[2] + e[3] - first_key(e[3], window) for e, _ in joined) > FP8_JOIN_KEYS or (rows + need) * row_bytes > FP8_READ_BACK_MAX:
+                groups.append([])
+                rows, need, joined = 0, own, []
+            groups[-1] += [e for e, _ in joined] + [entry]
+            rows += need
+            between = []
         return groups
 
     def _part(self, window, group):
@@ -2341,7 +2383,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     The keys and values that a portion sees are read back once into pages of q's type (exact: an element has four significant bits
     and a power of two) and the attention kernels for such pages take them from there: tensor cores then meet operands that they take
     as they are, where conversion in the attention kernel would be paid again for every tile.  Every position that is seen has a page.
-    Entries of up to FP8_FEW_TOKENS tokens, and shapes that no tiled kernel takes, go to :func:`decode_attention_fp8`.  A call
+    Entries of up to FP8_FEW_TOKENS tokens, steps that are done sooner token by token (:func:`fp8_token_by_token`), scales that are not
+    positive and shapes that no tiled kernel takes go to :func:`decode_attention_fp8`.  A call
     may be captured once the plan has been used; the plan lives as long as the graph."""
     name = "prefill_attention_fp8"
     found = _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, status, None,
@@ -2360,16 +2403,21 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     cache = (k_pages, v_pages, k_exp, v_exp, block_table, page_size)
     step = (positions, token_seq, seq_slot)
     f32 = q.dtype == torch.float32
+    kind = ("f32" if f32 else "grouped" if softcap is None and prefill_grouped_ok(q, out, n_heads, n_kv_heads, head_dim, scale) else
+            "tc" if head_dim <= 128 else "mma")
     # (asked with q in the pages' place: pages that are read back have its type and lie on the allocator's grid)
     # (and the tiled kernels find a row's maximum before they scale it)
-    if scale <= 0 or not (prefill_f32_ok(q, out, q, head_dim) if f32 else prefill_ok(q, out, q, head_dim)):
+    if (scale <= 0 or not (prefill_f32_ok(q, out, q, head_dim) if f32 else prefill_ok(q, out, q, head_dim))
+            or plan.token_by_token(kind, window, n_heads, n_kv_heads, head_dim)):
         _decode_fp8(found, page_size, n_heads, window, scale, softcap, st)
         return out
     plan.on_stream(st)
-    if plan.has_few:
+    row_bytes = 2 * n_kv_heads * head_dim * q.element_size()
+    few = plan.few(window, row_bytes)
+    if few.shape[0]:
         decode_attention_fp8(q, *cache, *step, out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status,
-                             tokens=plan.few(), stream=st)
-    for tok0, n, entries, spans, rows, table, slots in plan.parts(window, 2 * n_kv_heads * head_dim * q.element_size()):
+                             tokens=few, stream=st)
+    for tok0, n, entries, spans, rows, table, slots in plan.parts(window, row_bytes):
         k, v = (torch.empty(rows // FP8_READ_PAGE, n_kv_heads, FP8_READ_PAGE, head_dim, dtype=q.dtype, device=q.device) for _ in range(2))
         read_kv_fp8_spans(*cache, spans, rows, seq_slot, k, v, stream=st, attend=True)
         q_part, out_part = (q, out) if n == plan.n_tokens else (q[tok0:tok0 + n], out[tok0:tok0 + n])

@@ -167,7 +167,8 @@ def test_parts_hold_what_the_tokens_see(window, most, monkeypatch):
     monkeypatch.setattr(ops, "FP8_READ_BACK_MAX", most)
     P, entries = ops.FP8_READ_PAGE, [(40, 0), (3, 100), (17, 33), (9, 0), (0, 12), (200, 7), (8, 0)]
     plan = ops.prefill_fp8_plan(entries, 16, "cpu")
-    few = plan.few().tolist()
+    few = plan.few(window, 10).tolist()
+    placed = len(few)
     seen, first = set(few), [0]
     for n, _ in entries:
         first.append(first[-1] + n)
@@ -183,6 +184,29 @@ def test_parts_hold_what_the_tokens_see(window, most, monkeypatch):
                 assert pages[p] == (row // P + p - p0 // P if inside else -1)
             seen |= set(range(at, at + m))
             at += m
+            placed += m
             row += -(-(end - p0) // P) * P
         assert row == rows
-    assert seen == set(range(first[-1])) and len(few) == 3 + 8
+    assert seen == set(range(first[-1])) and placed == first[-1] and len(few) == 8 + (3 if most < 1 << 30 else 0)      # (the 3 go with their neighbours)
+
+
+@pytest.mark.parametrize("keys,parts", [(0, 2), (102, 2), (103, 1)])
+def test_few_tokens_between_others(keys, parts, monkeypatch):
+    monkeypatch.setattr(ops, "FP8_JOIN_KEYS", keys)
+    plan = ops.prefill_fp8_plan([(2, 5), (40, 0), (3, 100), (0, 4), (17, 33), (5, 0)], 16, "cpu")
+    found = plan.parts(None, 10)
+    assert len(found) == parts and found[0][0] == 2
+    few = list(range(2)) + list(range(62, 67))
+    assert plan.few(None, 10).tolist() == (few if parts == 1 else few[:2] + [42, 43, 44] + few[2:])
+    assert plan.few(8, 10).tolist() != [] and len(plan.parts(8, 10)) == (2 if keys < 11 else 1)      # (the 3 see 10 keys there)
+
+
+@pytest.mark.parametrize("kind,heads,kv_heads,dim", [("grouped", 28, 4, 128), ("tc", 16, 16, 128), ("mma", 16, 4, 256), ("f32", 16, 4, 128)])
+def test_what_goes_token_by_token(kind, heads, kv_heads, dim):
+    def choice(entries, window=None):
+        return ops.fp8_token_by_token(kind, entries, window, heads, kv_heads, dim, sms=148)
+    assert choice([(1, 5000)] * 30) and choice([(8, 0), (3, 100)]) and choice([])
+    assert choice([(12, 100)]) and choice([(1, 4000)] * 40 + [(12, 20)])
+    assert not choice([(2048, 0)]) and not choice([(300, 3700)] * 6)
+    sizes = [choice([(n, 1000)] * 4) for n in (9, 16, 32, 64, 128, 256, 1024)]
+    assert sizes == sorted(sizes, reverse=True)                             # (once tiled, tiled with more tokens)

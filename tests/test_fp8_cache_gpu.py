@@ -12,6 +12,15 @@ DEV = "cuda:0"
 DTYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
 
 
+CHOICE = ops.fp8_token_by_token
+
+
+@pytest.fixture(autouse=True)
+def tiled(monkeypatch):
+    """Steps this small would go through the decode kernel; the tests are of the others (test_prompts_as_chosen: as they come)."""
+    monkeypatch.setattr(ops, "fp8_token_by_token", lambda kind, entries, *a: all(n <= ops.FP8_FEW_TOKENS for n, _ in entries))
+
+
 class Cache:
     """A cache of ``lens`` positions for each request in scattered pages of a pool, and what it holds by the definition."""
 
@@ -479,6 +488,21 @@ def test_prompts_of_grouped_heads_cut_into_runs(H, G, D, window, run_blocks, mon
     out = torch.full((T, H * D), 7.0, dtype=q.dtype, device=DEV)
     ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out, H, G, D, window, 0.15)
     check(out, c, entries, q, H, window, 0.15, None, PROMPT_WEIGHT["bf16"])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("H,G,D", [(4, 2, 128), (2, 2, 256)])
+@pytest.mark.parametrize("entries", [[(12, 100), (9, 3)], [(1, 200), (1, 7), (30, 0), (3, 50), (400, 100), (1, 90)]])
+def test_prompts_as_chosen(dtype, H, G, D, entries, monkeypatch):
+    """Tokens one by one where that is sooner, portions with single tokens between them where it is not."""
+    monkeypatch.setattr(ops, "fp8_token_by_token", CHOICE)
+    c = Cache([n + s for n, s in entries], G, D, 64, 83)
+    T = sum(n for n, _ in entries)
+    q = rows(T, H, G, D, DTYPES[dtype], 84)
+    for window in (None, 33):
+        out = torch.full((T, H * D), 7.0, dtype=q.dtype, device=DEV)
+        ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out, H, G, D, window, 0.15)
+        check(out, c, entries, q, H, window, 0.15, None, PROMPT_WEIGHT[dtype])
 
 
 def test_results_beside_a_portion_stay():
