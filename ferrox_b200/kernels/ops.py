@@ -2238,7 +2238,7 @@ def fp8_token_by_token(kind, entries, window, n_heads, n_kv_heads, head_dim, sms
     256 on 4 (mma) 85 against 109 and 95 against 429; 16 heads of 128 on 4 in 32 bits 48 against 119 and 81 against 322;
     prompts of 300, 193 and 97 tokens of 4 heads of 64 on 2 in 32 bits 28 against 24."""
     rows, base, block, chain = {"grouped": (256 * n_kv_heads // n_heads, 14.0, 2.4, 0.0), "tc": (256, 30.0, 4.5, 0.0), "mma": (PREFILL_TILE, 12.0, 3.0, 0.107 * head_dim / 256),
-                                "f32": (128, 14.0, 4.0, 0.057 * head_dim / 128)}[kind]
+                                "f32": (128, 10.0, 4.0, 0.035 + 0.00017 * head_dim)}[kind]
     sms, group = sms or sm_count(), n_heads // n_kv_heads
     heads = n_kv_heads if kind == "grouped" else n_heads
     per_tile, per_run = (0.45, 1.4) if head_dim <= 128 else (0.75, 2.5)      # of the decode kernel, a run of heads that share their keys
@@ -2408,7 +2408,7 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     # (asked with q in the pages' place: pages that are read back have its type and lie on the allocator's grid)
     # (and the tiled kernels find a row's maximum before they scale it)
     if (scale <= 0 or not (prefill_f32_ok(q, out, q, head_dim) if f32 else prefill_ok(q, out, q, head_dim))
-            or plan.token_by_token(kind, window, n_heads, n_kv_heads, head_dim)):
+            or (decode_fp8_ok(found[3], found[4], head_dim, page_size) and plan.token_by_token(kind, window, n_heads, n_kv_heads, head_dim))):
         _decode_fp8(found, page_size, n_heads, window, scale, softcap, st)
         return out
     plan.on_stream(st)
@@ -2474,7 +2474,7 @@ def _prefill_read_back(q, k, v, table, page_size, plan, key, entries, slots, out
     heads = (n_heads, n_kv_heads, head_dim, window, scale)
     if q.dtype == torch.float32:
         tiles = None
-        if prefill_f32_tc_ok(q, out, k, page_size, head_dim):
+        if head_dim % 8 == 0:
             items, spans, rest, n_items, rows = plan.kept(("f32", head_dim) + key, lambda: _f32_lists(entries, window, head_dim))
             if prefill_f32_tc_fits(n_items, q.shape[0], rows, n_heads, n_kv_heads, head_dim):
                 prefill_attention_f32_tc(q, k, v, table, page_size, items, spans, rows, slots, out, *heads, status=status, **tail)
