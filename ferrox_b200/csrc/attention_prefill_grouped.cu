@@ -125,19 +125,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
     auto v_full = [&](int b) { return bar(16 + b); };
     const uint32_t drained = bar(18);
 
-    const int* item = a.items + (long)blockIdx.y * ITEM_INTS;
-    const int tok0 = item[0], n_tok = item[1], entry = item[2], pos0 = item[3], kb_begin = item[4], kb_end = item[5], part = item[6];
-    const int kvh = blockIdx.x, per = a.per_sub, nt = n_tok > per ? 2 : 1;
-    auto tokens_of = [&](int t) { return min(per, n_tok - t * per); };
-    auto lo_of = [&](int t) { return max(fx_first_key(pos0 + t * per, a.window, 0) / BK, kb_begin); };
-    auto hi_of = [&](int t) { return min((pos0 + t * per + tokens_of(t) - 1) / BK, kb_end - 1); };
-    const int lo0 = lo_of(0), hi0 = hi_of(0), lo1 = nt > 1 ? lo_of(1) : 1, hi1 = nt > 1 ? hi_of(1) : 0;      // (none: lo > hi)
-    const bool act0 = lo0 <= hi0, act1 = lo1 <= hi1;
-    const int first_blk = act0 && act1 ? min(lo0, lo1) : act0 ? lo0 : lo1, last_blk = act0 && act1 ? max(hi0, hi1) : act0 ? hi0 : hi1;
-    const int n_walk = max(0, last_blk - first_blk + 1);
-    auto active = [&](int t, int i) { const int j = first_blk + i; return t < nt && i < n_walk && j >= (t ? lo1 : lo0) && j <= (t ? hi1 : hi0); };
-    auto last_of = [&](int t) { return (t ? act1 : act0) ? (t ? hi1 : hi0) - first_blk : -1; };
-
     if (threadIdx.x == 0) {
         abort_flag_s = 0;
         for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= 4 && i < 8 ? 4 : 1);      // (p_half, p_full: four warps)
@@ -153,7 +140,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;
-    fx_pdl_wait();   // set up while the kernel before this one drains; its results from here on
+    fx_pdl_wait();   // set up while the kernel before this one drains; its results (and the lists, which may be new) from here on
+
+    const int* item = a.items + (long)blockIdx.y * ITEM_INTS;
+    const int tok0 = item[0], n_tok = item[1], entry = item[2], pos0 = item[3], kb_begin = item[4], kb_end = item[5], part = item[6];
+    const int kvh = blockIdx.x, per = a.per_sub, nt = n_tok > per ? 2 : 1;
+    auto tokens_of = [&](int t) { return min(per, n_tok - t * per); };
+    auto lo_of = [&](int t) { return max(fx_first_key(pos0 + t * per, a.window, 0) / BK, kb_begin); };
+    auto hi_of = [&](int t) { return min((pos0 + t * per + tokens_of(t) - 1) / BK, kb_end - 1); };
+    const int lo0 = lo_of(0), hi0 = hi_of(0), lo1 = nt > 1 ? lo_of(1) : 1, hi1 = nt > 1 ? hi_of(1) : 0;      // (none: lo > hi)
+    const bool act0 = lo0 <= hi0, act1 = lo1 <= hi1;
+    const int first_blk = act0 && act1 ? min(lo0, lo1) : act0 ? lo0 : lo1, last_blk = act0 && act1 ? max(hi0, hi1) : act0 ? hi0 : hi1;
+    const int n_walk = max(0, last_blk - first_blk + 1);
+    auto active = [&](int t, int i) { const int j = first_blk + i; return t < nt && i < n_walk && j >= (t ? lo1 : lo0) && j <= (t ? hi1 : hi0); };
+    auto last_of = [&](int t) { return (t ? act1 : act0) ? (t ? hi1 : hi0) - first_blk : -1; };
     auto tmem_s = [&](int t) { return tmem + 128u * t; };            // S_t, and P_t over its first 64 columns
     auto tmem_o = [&](int t) { return tmem + 256u + 128u * t; };
 
