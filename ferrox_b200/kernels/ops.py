@@ -2297,9 +2297,17 @@ class PrefillFp8Plan:
             self._kept[key] = x
         return x
 
-    def token_by_token(self, kind, window, n_heads, n_kv_heads, head_dim):
-        return self.kept(("token by token", kind, window, n_heads, n_kv_heads, head_dim),
-                         lambda: fp8_token_by_token(kind, self.entries, window, n_heads, n_kv_heads, head_dim))
+    def route(self, kind, window, n_heads, n_kv_heads, head_dim, size):
+        """None where every token goes by itself (``kind`` None: never for its speed); else the tokens that do (or None) and the parts."""
+        key = (kind, window, n_heads, n_kv_heads, head_dim, size)
+        found = self._kept.get(key, self)
+        if found is self:
+            found, row_bytes = None, 2 * n_kv_heads * head_dim * size
+            if not (fp8_token_by_token(kind, self.entries, window, n_heads, n_kv_heads, head_dim) if kind else all(n <= FP8_FEW_TOKENS for n, _ in self.entries)):
+                few = self.few(window, row_bytes)
+                found = (few if few.shape[0] else None, self.parts(window, row_bytes))
+            self._kept[key] = found
+        return found
 
     def few(self, window, row_bytes):
         """Flat indices of the tokens that are in none of the parts."""
@@ -2402,34 +2410,30 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
                                          out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status)
     cache = (k_pages, v_pages, k_exp, v_exp, block_table, page_size)
     step = (positions, token_seq, seq_slot)
-    f32 = q.dtype == torch.float32
-    kind = ("f32" if f32 else "grouped" if softcap is None and prefill_grouped_ok(q, out, n_heads, n_kv_heads, head_dim, scale) else
-            "tc" if head_dim <= 128 else "mma")
-    # (asked with q in the pages' place: pages that are read back have its type and lie on the allocator's grid)
-    # (and the tiled kernels find a row's maximum before they scale it)
-    if (scale <= 0 or not (prefill_f32_ok(q, out, q, head_dim) if f32 else prefill_ok(q, out, q, head_dim))
-            or (decode_fp8_ok(found[3], found[4], head_dim, page_size) and plan.token_by_token(kind, window, n_heads, n_kv_heads, head_dim))):
+    # Which kernel (:func:`prefill_f32_ok`, :func:`prefill_ok` and what the grouped one asks, from what is known already; pages that are
+    # read back have q's type and lie on the allocator's grid).  The tiled kernels find a row's maximum before they scale it.
+    x, kp, vp, qp, op, ldq, ldo = found[2], found[3], found[4], found[11], found[12], found[27], found[28]
+    f32, wide = x == F32, 4 if x == F32 else 8
+    tiled = scale > 0 and ldq % wide == 0 and qp % 16 == 0 and (head_dim <= 128 and head_dim % 4 == 0 and ldo % 4 == 0 and op % 16 == 0 if f32 else
+                                                                head_dim % 16 == 0 and ldo % 2 == 0)
+    kind = ("f32" if f32 else "mma" if head_dim > 128 else "tc" if softcap is not None or n_heads > 128 * n_kv_heads or ldo % 8 or op % 16 else "grouped")
+    route = tiled and plan.route(kind if decode_fp8_ok(kp, vp, head_dim, page_size) else None, window, n_heads, n_kv_heads, head_dim, 4 if f32 else 2)
+    if not route:
         _decode_fp8(found, page_size, n_heads, window, scale, softcap, st)
         return out
     plan.on_stream(st)
-    row_bytes = 2 * n_kv_heads * head_dim * q.element_size()
-    few = plan.few(window, row_bytes)
-    if few.shape[0]:
+    few, parts = route
+    if few is not None:
         decode_attention_fp8(q, *cache, *step, out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status,
                              tokens=few, stream=st)
-    for tok0, n, entries, spans, rows, table, slots in plan.parts(window, row_bytes):
-        k, v = (torch.empty(rows // FP8_READ_PAGE, n_kv_heads, FP8_READ_PAGE, head_dim, dtype=q.dtype, device=q.device) for _ in range(2))
+    for tok0, n, entries, spans, rows, table, slots in parts:
+        shape = (rows // FP8_READ_PAGE, n_kv_heads, FP8_READ_PAGE, head_dim)
+        k, v = torch.empty(shape, dtype=q.dtype, device=q.device), torch.empty(shape, dtype=q.dtype, device=q.device)
         read_kv_fp8_spans(*cache, spans, rows, seq_slot, k, v, stream=st, attend=True)
-        q_part, out_part = (q, out) if n == plan.n_tokens else (q[tok0:tok0 + n], out[tok0:tok0 + n])
-        _prefill_read_back(q_part, k, v, table, FP8_READ_PAGE, plan, (tok0, window), entries, slots, out_part, n_heads, n_kv_heads, head_dim,
+        q_part, out_part = (q, out) if n == T else (q[tok0:tok0 + n], out[tok0:tok0 + n])
+        _prefill_read_back(kind, q_part, k, v, table, FP8_READ_PAGE, plan, (tok0, window), entries, slots, out_part, n_heads, n_kv_heads, head_dim,
                            window, scale, softcap, status, st)
     return out
-
-
-def prefill_grouped_ok(q, out, n_heads: int, n_kv_heads: int, head_dim: int, scale: float) -> bool:
-    """Whether :func:`prefill_attention_grouped` takes these operands."""
-    return (q.dtype is torch.bfloat16 and n_heads <= 128 * n_kv_heads and 0 < head_dim <= 128 and head_dim % 16 == 0 and scale > 0
-            and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
 
 
 def prefill_grouped_plan(entries, window, n_heads: int, n_kv_heads: int):
@@ -2444,8 +2448,9 @@ _GROUPED = "xTQ~ xNGPD xNGPD iBW in8 xTO~ ?im4 ?iZ"
 def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_heads, n_kv_heads, head_dim, window, scale, status=None,
                               stream=None, merges=None, parts=0):
     """Attention of prompt portions in bfloat16, of query heads that may share key heads, over pages of 128 positions [pages, kv heads, 128,
-    head_dim] (see :func:`prefill_grouped_ok`).  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``,
-    ``parts``: device copies of what :func:`prefill_grouped_plan` returns, and its number of parts."""
+    head_dim]: heads of up to 128 elements in steps of 16, at most 128 query heads a kv head, rows on the 16-byte grid, a positive
+    scale.  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``, ``parts``: device copies of what
+    :func:`prefill_grouped_plan` returns, and its number of parts."""
     name = "prefill_attention_grouped"
     (_, now, x, qp, kp, vp, tp, ip, op, mp, zp, T, Q, N, G, P, D, B, W, n, eight, O, n_merges, four, _, ldq, ldo) = _operands(
         name, _GROUPED, ("q", "k_pages", "v_pages", "block_table", "items", "out", "merges", "status"), q, k_pages, v_pages, block_table, items, out,
@@ -2467,12 +2472,12 @@ def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_he
     return out
 
 
-def _prefill_read_back(q, k, v, table, page_size, plan, key, entries, slots, out, n_heads, n_kv_heads, head_dim, window, scale, softcap,
+def _prefill_read_back(kind, q, k, v, table, page_size, plan, key, entries, slots, out, n_heads, n_kv_heads, head_dim, window, scale, softcap,
                        status, stream):
     """Prompt attention of neighbouring entries over pages of q's type, by the kernel that the attention mixer takes for such pages."""
     tail = dict(stream=stream, softcap=softcap)
     heads = (n_heads, n_kv_heads, head_dim, window, scale)
-    if q.dtype == torch.float32:
+    if kind == "f32":
         tiles = None
         if head_dim % 8 == 0:
             items, spans, rest, n_items, rows = plan.kept(("f32", head_dim) + key, lambda: _f32_lists(entries, window, head_dim))
@@ -2485,7 +2490,7 @@ def _prefill_read_back(q, k, v, table, page_size, plan, key, entries, slots, out
             prefill_attention_f32(q, k, v, table, page_size, tiles, slots, out, *heads, **tail)
         return
     capped = softcap is not None
-    if not capped and prefill_grouped_ok(q, out, n_heads, n_kv_heads, head_dim, scale):
+    if kind == "grouped":
         items, merges, parts = plan.kept(("grouped", n_heads, n_kv_heads) + key, lambda: prefill_grouped_plan(entries, window, n_heads, n_kv_heads))
         prefill_attention_grouped(q, k, v, table, items, out, *heads, status=status, stream=stream, merges=merges, parts=parts)
         return
