@@ -99,8 +99,8 @@ int fx_decode_attention_fp8(const void* q, long ldq, int dtype, const void* k_pa
 // bfloat16 over pages of 128 positions, head sizes up to 128 in steps of 16, rows of (token, head): see attention_prefill_grouped.cu
 int fx_prefill_attention_grouped(const void* q, long ldq, int n_tokens, const void* k_pages, const void* v_pages, int n_pages,
                                  const int* block_table, int table_width, const int* items, int n_items, void* out, long ldo, int n_heads,
-                                 int n_kv_heads, int head_dim, int window, float scale, float* part_o, float* part_ml, const int* merges,
-                                 int n_merges, int* status, void* stream);
+                                 int n_kv_heads, int head_dim, int window, float scale, float softcap, float* part_o, float* part_ml,
+                                 const int* merges, int n_merges, int* status, void* stream);
 int fx_attention_fp8(const void* q, long ldq, int dtype, const void* k_pages, const void* v_pages, const void* k_exp,
                      const void* v_exp, const int* block_table, int n_slots, int table_width, int page_size, int n_pages,
                      const int* positions, const int* token_seq, const int* seq_slot, const int* tokens, int n_tokens, void* out,

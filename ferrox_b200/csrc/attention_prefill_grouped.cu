@@ -8,7 +8,7 @@
 // and walks the request's keys in blocks of 128:
 //
 //   S_t = Q_t K_j^T    tcgen05.mma 128 x 128 x head_dim, Q by TMA ([token][head][64 elements] boxes), S_t in tensor memory
-//   P_t = 2^(S_t - m)  a thread a row: mask by absolute position, running maximum and sum in 32 bits, P in bfloat16 over S_t
+//   P_t = 2^(S_t - m)  a thread a row: cap, mask by absolute position, running maximum and sum in 32 bits, P in bfloat16 over S_t
 //   O_t += P_t V_j     tcgen05.mma, A from tensor memory, V as an N-major B operand; its first half as soon as half of P_t is
 //                      written
 //
@@ -20,7 +20,8 @@
 // their maximum found 500, asked whether it is to be raised 190, weights 1,540 (their 2^x alone 1,024), the rest of PV and the next
 // S 1,330.  B200: 3,600 clocks a pair with few blocks running, 2.39 us with all (982 TFLOP/s over long contexts; 28 heads of 128 on 4).  Six
 // portions of 300 tokens behind up to 3,800, the pages' reading back included: 86 us; a prompt of 2,048 of 16 heads with their own
-// keys 49.5 (by the kernel of attention_prefill_tc.cu 65).  Tried: scores read twice instead of held, P in one piece 2.91 us a pair; a
+// keys 49.5 (by the kernel of attention_prefill_tc.cu 65); with capped scores, whose tanh is two more operations of the special-function
+// unit a score, 152 and 80 (there 280 and 139).  Tried: scores read twice instead of held, P in one piece 2.91 us a pair; a
 // thread of its own for each sub-tile's products, softmaxes in turns 2.56, without turns 2.89 (both then do the same at the same
 // time); a quarter of the 2^x by polynomial 2.64; rolled loops around the products 2.71.  Converting the 8-bit pages in this
 // kernel, by seven more warps, cost the softmax threads a third of their registers and the tile its pace (162 us and 86 us where
@@ -49,7 +50,7 @@ struct Args {
     bf16* out; long ldo;
     float *part_o, *part_ml;
     int n_kv_heads, group, per_sub, head_dim, window;     // per_sub: tokens of a sub-tile
-    float scale_log2e;
+    float scale_log2e, cap_in, cap;                       // capped: score = cap tanh(q.k scale / softcap), cap and scores in powers of two
     int* status;
 };
 
@@ -72,6 +73,11 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
                    "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 // Two 32-bit numbers in a register pair.
 __device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
@@ -100,7 +106,7 @@ __device__ __forceinline__ bool met(uint32_t bar, uint32_t parity, volatile int*
     if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
     return mbar_wait(bar, parity, abort_flag);
 }
-template <int D>
+template <int D, bool CAPPED>
 __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                       const __grid_constant__ CUtensorMap map_k,
                                                                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a)
@@ -272,6 +278,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                 for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, c[i]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) tc_ld_wait_for(c[i]);
+                if constexpr (CAPPED) {                  // tanh(x) = 1 - 2 / (e^2x + 1)
+#pragma unroll
+                    for (int k = 0; k < BK; ++k) {
+                        const float e = exp2_fast(__uint_as_float(c[k / 32][k % 32]) * a.cap_in);
+                        c[k / 32][k % 32] = __float_as_uint(fmaf(-2.f * a.cap, reciprocal_fast(e + 1.f), a.cap));
+                    }
+                }
                 if (__builtin_expect(!interior, 0)) {    // (out of the way of what most blocks run through)
 #pragma unroll
                     for (int k = 0; k < BK; ++k)
@@ -415,10 +428,10 @@ template <int D> __global__ void __launch_bounds__(128) prefill_grouped_merge_ke
         if (lane * PER + i < a.head_dim) dst[i] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc[i] / sum);
 }
 
-template <int D>
+template <int D, bool CAPPED>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int n_items, const int* merges, int n_merges, cudaStream_t s)
 {
-    auto kern = prefill_grouped_kernel<D>;
+    auto kern = prefill_grouped_kernel<D, CAPPED>;
     // what the softmax threads ask for has to be there: the block's registers at its launch
     static const bool fits = [&] { cudaFuncAttributes at; return cudaFuncGetAttributes(&at, kern) == cudaSuccess && at.numRegs * 3 >= REGS_FEW + 2 * REGS_MANY; }();
     if (!fits) return FX_ERR_SIZE;
@@ -447,22 +460,25 @@ bool encode(CUtensorMap* map, const void* ptr, cuuint64_t d0, cuuint64_t d1, cuu
 // heads][256][64 or 128], part_ml [parts][kv heads][256][2].
 extern "C" int fx_prefill_attention_grouped(const void* q, long ldq, int n_tokens, const void* k_pages, const void* v_pages, int n_pages,
                                             const int* block_table, int table_width, const int* items, int n_items, void* out, long ldo,
-                                            int n_heads, int n_kv_heads, int head_dim, int window, float scale, float* part_o, float* part_ml,
+                                            int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap, float* part_o, float* part_ml,
                                             const int* merges, int n_merges, int* status, void* stream)
 {
     if (n_items <= 0 || n_tokens <= 0) return FX_OK;
     if (head_dim <= 0 || head_dim > 128 || head_dim % 16 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > BQ ||
-        n_pages <= 0 || table_width <= 0 || window < 0 || !(scale > 0.f) || n_items > 65535 || n_kv_heads > 65535 ||
+        n_pages <= 0 || table_width <= 0 || window < 0 || !(scale > 0.f) || !(softcap >= 0.f) || n_items > 65535 || n_kv_heads > 65535 ||
         (n_merges > 0 && (!part_o || !part_ml || !merges))) return FX_ERR_SIZE;
     if (ldq % 8 || ldo % 8 || (uintptr_t)q % 16 || (uintptr_t)out % 16 || (uintptr_t)k_pages % 16 || (uintptr_t)v_pages % 16 || (uintptr_t)part_o % 16)
         return FX_ERR_ALIGN;
     const int group = n_heads / n_kv_heads, per = BQ / group;
+    constexpr float LOG2E = 1.4426950408889634f;
+    const bool capped = softcap > 0.f;
     const Args a = {block_table, table_width, n_pages, items, (bf16*)out, ldo, part_o, part_ml, n_kv_heads, group, per, head_dim, window,
-                    scale * 1.4426950408889634f, status};
+                    capped ? 1.f : scale * LOG2E, capped ? 2.f * LOG2E * scale / softcap : 0.f, softcap * LOG2E, status};
     CUtensorMap mq, mk, mv;
     const cuuint64_t W = head_dim, G = n_kv_heads;
     if (!encode(&mq, q, W, group, G, n_tokens, W, W * group, ldq, group, per) || !encode(&mk, k_pages, W, BK, G, n_pages, W, BK * W, G * BK * W, BK, 1) ||
         !encode(&mv, v_pages, W, BK, G, n_pages, W, BK * W, G * BK * W, BK, 1)) return FX_ERR_SIZE;
     cudaStream_t s = (cudaStream_t)stream;
-    return head_dim <= 64 ? launch<64>(mq, mk, mv, a, n_items, merges, n_merges, s) : launch<128>(mq, mk, mv, a, n_items, merges, n_merges, s);
+    if (capped) return head_dim <= 64 ? launch<64, true>(mq, mk, mv, a, n_items, merges, n_merges, s) : launch<128, true>(mq, mk, mv, a, n_items, merges, n_merges, s);
+    return head_dim <= 64 ? launch<64, false>(mq, mk, mv, a, n_items, merges, n_merges, s) : launch<128, false>(mq, mk, mv, a, n_items, merges, n_merges, s);
 }

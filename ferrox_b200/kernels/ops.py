@@ -127,7 +127,7 @@ _SIGNATURES = {
     "fx_read_kv_fp8": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _P],
     "fx_decode_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F,
                                 _I, _P, _P, _P, _P],
-    "fx_prefill_attention_grouped": [_P, _L, _I, _P, _P, _I, _P, _I, _P, _I, _P, _L, _I, _I, _I, _I, _F, _P, _P, _P, _I, _P, _P],
+    "fx_prefill_attention_grouped": [_P, _L, _I, _P, _P, _I, _P, _I, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F, _P, _P, _P, _I, _P, _P],
     "fx_attention_fp8": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _F, _F, _P],
     "fx_argmax": [_P, _L, _I, _I, _P, _P],
     "fx_repetition_penalty": [_P, _L, _I, _I, _P, _P, _P, _P],
@@ -2234,13 +2234,15 @@ def fp8_token_by_token(kind, entries, window, n_heads, n_kv_heads, head_dim, sms
     ``kind``: the tiled kernel that would take the step.  A tile of ``rows`` (token, query head) pairs costs ``block`` a 128 keys that it sees, all
     SMs sharing the tiles; one that is not cut into runs takes ``chain`` a key by itself; ``base`` are the launches.  20 requests of up
     to 600 positions and 8 of up to 4,000, 24 tokens each, decode against tiled: 28 heads of 128 on 4 (grouped) 50 against 28 and 89
-    against 43, 96 tokens of one request of 600 19 against 23; the same with capped scores (tc) 52 against 82 and 94 against 176; 16 heads of
+    against 43, 96 tokens of one request of 600 19 against 23; the same with capped scores 51 against 37, 93 against 54, 20 against 32; 16 heads of
     256 on 4 (mma) 85 against 109 and 95 against 429; 16 heads of 128 on 4 in 32 bits 48 against 119 and 81 against 322;
     prompts of 300, 193 and 97 tokens of 4 heads of 64 on 2 in 32 bits 28 against 24."""
-    rows, base, block, chain = {"grouped": (256 * n_kv_heads // n_heads, 14.0, 2.4, 0.0), "tc": (256, 30.0, 4.5, 0.0), "mma": (PREFILL_TILE, 12.0, 3.0, 0.107 * head_dim / 256),
+    together = 256 * n_kv_heads // n_heads                                   # tokens of a tile that holds the heads of a kv head
+    rows, base, block, chain = {"grouped": (together, 14.0, 2.4, 0.0), "capped": (together, 24.0, 4.0, 0.0), "tc": (256, 30.0, 4.5, 0.0),
+                                "mma": (PREFILL_TILE, 12.0, 3.0, 0.107 * head_dim / 256),
                                 "f32": (128, 10.0, 4.0, 0.035 + 0.00017 * head_dim)}[kind]
     sms, group = sms or sm_count(), n_heads // n_kv_heads
-    heads = n_kv_heads if kind == "grouped" else n_heads
+    heads = n_kv_heads if kind in ("grouped", "capped") else n_heads
     per_tile, per_run = (0.45, 1.4) if head_dim <= 128 else (0.75, 2.5)      # of the decode kernel, a run of heads that share their keys
     runs = n_kv_heads * -(-group // (4 if group <= 4 or kind == "f32" else 8))
     decode = tiled = back = longest = 0
@@ -2416,7 +2418,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     f32, wide = x == F32, 4 if x == F32 else 8
     tiled = scale > 0 and ldq % wide == 0 and qp % 16 == 0 and (head_dim <= 128 and head_dim % 4 == 0 and ldo % 4 == 0 and op % 16 == 0 if f32 else
                                                                 head_dim % 16 == 0 and ldo % 2 == 0)
-    kind = ("f32" if f32 else "mma" if head_dim > 128 else "tc" if softcap is not None or n_heads > 128 * n_kv_heads or ldo % 8 or op % 16 else "grouped")
+    kind = ("f32" if f32 else "mma" if head_dim > 128 else "tc" if n_heads > 128 * n_kv_heads or ldo % 8 or op % 16 else
+            "grouped" if softcap is None else "capped")
     route = tiled and plan.route(kind if decode_fp8_ok(kp, vp, head_dim, page_size) else None, window, n_heads, n_kv_heads, head_dim, 4 if f32 else 2)
     if not route:
         _decode_fp8(found, page_size, n_heads, window, scale, softcap, st)
@@ -2446,10 +2449,10 @@ _GROUPED = "xTQ~ xNGPD xNGPD iBW in8 xTO~ ?im4 ?iZ"
 
 
 def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_heads, n_kv_heads, head_dim, window, scale, status=None,
-                              stream=None, merges=None, parts=0):
+                              stream=None, merges=None, parts=0, softcap=None):
     """Attention of prompt portions in bfloat16, of query heads that may share key heads, over pages of 128 positions [pages, kv heads, 128,
     head_dim]: heads of up to 128 elements in steps of 16, at most 128 query heads a kv head, rows on the 16-byte grid, a positive
-    scale.  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``, ``parts``: device copies of what
+    scale, scores capped or not.  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``, ``parts``: device copies of what
     :func:`prefill_grouped_plan` returns, and its number of parts."""
     name = "prefill_attention_grouped"
     (_, now, x, qp, kp, vp, tp, ip, op, mp, zp, T, Q, N, G, P, D, B, W, n, eight, O, n_merges, four, _, ldq, ldo) = _operands(
@@ -2467,7 +2470,7 @@ def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_he
         work = torch.empty(parts * n_kv_heads * 256 * (width + 2), dtype=torch.float32, device=q.device)
         po = work.data_ptr()
         pm = po + 4 * parts * n_kv_heads * 256 * width
-    call("fx_prefill_attention_grouped", qp, ldq, T, kp, vp, N, tp, W, ip, n, op, ldo, n_heads, G, D, int(window or 0), float(scale), po, pm,
+    call("fx_prefill_attention_grouped", qp, ldq, T, kp, vp, N, tp, W, ip, n, op, ldo, n_heads, G, D, int(window or 0), float(scale), float(softcap or 0.0), po, pm,
          mp if parts else 0, n_merges if parts else 0, zp, stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
     return out
 
@@ -2490,9 +2493,9 @@ def _prefill_read_back(kind, q, k, v, table, page_size, plan, key, entries, slot
             prefill_attention_f32(q, k, v, table, page_size, tiles, slots, out, *heads, **tail)
         return
     capped = softcap is not None
-    if kind == "grouped":
+    if kind in ("grouped", "capped"):
         items, merges, parts = plan.kept(("grouped", n_heads, n_kv_heads) + key, lambda: prefill_grouped_plan(entries, window, n_heads, n_kv_heads))
-        prefill_attention_grouped(q, k, v, table, items, out, *heads, status=status, stream=stream, merges=merges, parts=parts)
+        prefill_attention_grouped(q, k, v, table, items, out, *heads, status=status, merges=merges, parts=parts, **tail)
         return
     if (prefill_tc_general_ok(q, q.stride(0), head_dim, k, v, page_size, out, out.stride(0), head_dim, head_dim, head_dim, scale, softcap)
             and prefill_tc_better(entries, window, n_heads, head_dim, head_dim, capped=True) if capped

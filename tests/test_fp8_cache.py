@@ -201,7 +201,7 @@ def test_few_tokens_between_others(keys, parts, monkeypatch):
     assert plan.few(8, 10).tolist() != [] and len(plan.parts(8, 10)) == (2 if keys < 11 else 1)      # (the 3 see 10 keys there)
 
 
-@pytest.mark.parametrize("kind,heads,kv_heads,dim", [("grouped", 28, 4, 128), ("tc", 16, 16, 128), ("mma", 16, 4, 256), ("f32", 16, 4, 128)])
+@pytest.mark.parametrize("kind,heads,kv_heads,dim", [("grouped", 28, 4, 128), ("capped", 28, 4, 128), ("tc", 16, 16, 128), ("mma", 16, 4, 256), ("f32", 16, 4, 128)])
 def test_what_goes_token_by_token(kind, heads, kv_heads, dim):
     def choice(entries, window=None):
         return ops.fp8_token_by_token(kind, entries, window, heads, kv_heads, dim, sms=148)

@@ -478,7 +478,8 @@ def test_a_prompt_next_to_rows_that_are_no_numbers(dtype, H, softcap):
 @pytest.mark.parametrize("H,G,D", [(6, 2, 128), (7, 1, 64), (16, 4, 80)])
 @pytest.mark.parametrize("window", [None, 100, 700])
 @pytest.mark.parametrize("run_blocks", [0, 1, 3])
-def test_prompts_of_grouped_heads_cut_into_runs(H, G, D, window, run_blocks, monkeypatch):
+@pytest.mark.parametrize("softcap", [None, 6.0])
+def test_prompts_of_grouped_heads_cut_into_runs(H, G, D, window, run_blocks, softcap, monkeypatch):
     own = ops.prefill_tc_plan
     monkeypatch.setattr(ops, "prefill_tc_plan", lambda *a, **k: own(*a, run_blocks=run_blocks, **k))
     entries = [(60, 900), (300, 0), (19, 333)]
@@ -486,8 +487,8 @@ def test_prompts_of_grouped_heads_cut_into_runs(H, G, D, window, run_blocks, mon
     T = sum(n for n, _ in entries)
     q = rows(T, H, G, D, torch.bfloat16, 51)
     out = torch.full((T, H * D), 7.0, dtype=q.dtype, device=DEV)
-    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out, H, G, D, window, 0.15)
-    check(out, c, entries, q, H, window, 0.15, None, PROMPT_WEIGHT["bf16"])
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out, H, G, D, window, 0.15, softcap=softcap)
+    check(out, c, entries, q, H, window, 0.15, softcap, PROMPT_WEIGHT["bf16"])
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -605,16 +606,16 @@ def test_pages_longer_than_a_tile(dtype, H, G, D, P):
 
 
 @pytest.mark.parametrize("H,G,D", [(4, 4, 128), (3, 3, 48), (12, 12, 64)])
-@pytest.mark.parametrize("window", [None, 90])
-def test_prompts_of_heads_with_their_own_keys(H, G, D, window):
+@pytest.mark.parametrize("window,softcap", [(None, None), (90, None), (90, 40.0)])
+def test_prompts_of_heads_with_their_own_keys(H, G, D, window, softcap):
     """Portions around the sizes of a sub-tile and a tile."""
     entries = [(127, 0), (128, 5), (129, 0), (256, 131), (257, 0), (9, 300)]
     c = Cache([n + s for n, s in entries], G, D, 64, 79)
     T = sum(n for n, _ in entries)
     q = rows(T, H, G, D, torch.bfloat16, 80)
     out = torch.full((T, H * D), 7.0, dtype=q.dtype, device=DEV)
-    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out, H, G, D, window, 0.15)
-    check(out, c, entries, q, H, window, 0.15, None, PROMPT_WEIGHT["bf16"])
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out, H, G, D, window, 0.15, softcap=softcap)
+    check(out, c, entries, q, H, window, 0.15, softcap, PROMPT_WEIGHT["bf16"])
 
 
 # ---- streams, graphs, order -----------------------------------------------------------------------------------------
