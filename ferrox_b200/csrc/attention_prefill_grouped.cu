@@ -1,5 +1,6 @@
-// Attention for prompt portions on the 5th-generation tensor cores (bfloat16, heads of up to 128 elements in steps of 16), over
-// pages of 128 positions: what read_kv_fp8_spans makes of an 8-bit cache.
+// Attention for prompt portions on the 5th-generation tensor cores (bfloat16, heads of up to 256 elements in steps of 16), over
+// pages of 128 positions: what read_kv_fp8_spans makes of an 8-bit cache.  Heads of up to 128 elements here, longer ones below
+// (prefill_wide_kernel).
 //
 // A row is a (token, query head) pair; the rows of a tile are the query heads of one kv head for consecutive tokens of a
 // request, so that a block of keys and values that has been brought in serves all of them, and a portion of few tokens fills
@@ -105,6 +106,84 @@ __device__ __forceinline__ float2 parts_of(uint64_t a) {
 __device__ __forceinline__ bool met(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
     return mbar_wait(bar, parity, abort_flag);
+}
+// A row's scores into registers, capped and masked, and the largest of them.
+template <bool CAPPED>
+__device__ __forceinline__ float scores_of(uint32_t (&c)[4][32], uint32_t ts, const Args& a, bool interior, int kb, int lo_r, int p_r) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, c[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tc_ld_wait_for(c[i]);
+    if constexpr (CAPPED) {                              // tanh(x) = 1 - 2 / (e^2x + 1)
+#pragma unroll
+        for (int k = 0; k < BK; ++k) {
+            const float e = exp2_fast(__uint_as_float(c[k / 32][k % 32]) * a.cap_in);
+            c[k / 32][k % 32] = __float_as_uint(fmaf(-2.f * a.cap, reciprocal_fast(e + 1.f), a.cap));
+        }
+    }
+    if (__builtin_expect(!interior, 0)) {                // (out of the way of what most blocks run through)
+#pragma unroll
+        for (int k = 0; k < BK; ++k)
+            if (kb + k > p_r || kb + k < lo_r) c[k / 32][k % 32] = 0xff800000u;      // -infinity
+    }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int k = 0; k < BK; k += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(c[k / 32][k % 32 + e])), __uint_as_float(c[k / 32][k % 32 + 4 + e]));
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+// 32 scores' weights in bfloat16 pairs into 16 columns of tensor memory, their sums (before they are rounded) onto sum2.
+__device__ __forceinline__ void weights_of(const uint32_t* c, uint32_t at, uint64_t scale2, uint64_t ref2, uint64_t* sum2) {
+    uint32_t out[16];
+#pragma unroll
+    for (int k = 0; k < 32; k += 2) {
+        float2 e = parts_of(pair_fma(pair_of(c[k], c[k + 1]), scale2, ref2));
+        e.x = exp2_fast(e.x); e.y = exp2_fast(e.y);
+        sum2[k / 2 % 2] = pair_add(sum2[k / 2 % 2], pair_of(__float_as_uint(e.x), __float_as_uint(e.y)));
+        __nv_bfloat162 pr = __floats2bfloat162_rn(e.x, e.y);
+        out[k >> 1] = *reinterpret_cast<uint32_t*>(&pr);
+    }
+    tc_st16(at, out);
+}
+template <int D> __device__ __forceinline__ void shrink(uint32_t to, float alpha) {
+#pragma unroll 1
+    for (int col = 0; col < D; col += 16) {
+        uint32_t o[16];
+        tc_ld16(to + col, o);
+        tc_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+        tc_st16(to + col, o);
+    }
+}
+// A row's result, or its part of a tile that was cut (slot: among the parts' rows).  has: it has seen keys.
+template <int D>
+__device__ __forceinline__ void put_row(uint32_t to, const Args& a, bool row_ok, bool has, float m, float l, int part, long slot, bf16* dst) {
+    if (part >= 0 && row_ok) { a.part_ml[slot * 2] = has ? m * a.scale_log2e : -INFINITY; a.part_ml[slot * 2 + 1] = has ? l : 0.f; }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (!has && part >= 0) return;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+        uint32_t ob[32];
+        __syncwarp();
+        if (has) { tc_ld32(to + c * 32, ob); tc_ld_wait(); }
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+            if (!row_ok || c * 32 + k >= a.head_dim) continue;
+            if (part >= 0) {
+                float* o = a.part_o + slot * D + c * 32 + k;
+                *reinterpret_cast<uint4*>(o) = make_uint4(ob[k], ob[k + 1], ob[k + 2], ob[k + 3]);
+                *reinterpret_cast<uint4*>(o + 4) = make_uint4(ob[k + 4], ob[k + 5], ob[k + 6], ob[k + 7]);
+            } else {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : __uint_as_float(ob[k + e]) * inv;
+                Pack<bf16>::store(dst + c * 32 + k, x);
+            }
+        }
+    }
 }
 template <int D, bool CAPPED>
 __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __grid_constant__ CUtensorMap map_q,
@@ -273,63 +352,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                 }
                 const int kb = (first_blk + i) * BK;
                 const bool interior = kb + BK - 1 <= pos_t && kb >= lo_last;   // every row sees all of the block: no masking (most blocks)
-                uint32_t c[4][32];                       // the row's scores
-#pragma unroll
-                for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, c[i]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) tc_ld_wait_for(c[i]);
-                if constexpr (CAPPED) {                  // tanh(x) = 1 - 2 / (e^2x + 1)
-#pragma unroll
-                    for (int k = 0; k < BK; ++k) {
-                        const float e = exp2_fast(__uint_as_float(c[k / 32][k % 32]) * a.cap_in);
-                        c[k / 32][k % 32] = __float_as_uint(fmaf(-2.f * a.cap, reciprocal_fast(e + 1.f), a.cap));
-                    }
-                }
-                if (__builtin_expect(!interior, 0)) {    // (out of the way of what most blocks run through)
-#pragma unroll
-                    for (int k = 0; k < BK; ++k)
-                        if (kb + k > p_r || kb + k < lo_r) c[k / 32][k % 32] = 0xff800000u;      // -infinity
-                }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int k = 0; k < BK; k += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(c[k / 32][k % 32 + e])), __uint_as_float(c[k / 32][k % 32 + 4 + e]));
-                const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                uint32_t c[4][32];
+                const float mn = fmaxf(m, scores_of<CAPPED>(c, ts, a, interior, kb, lo_r, p_r));
                 const bool raise = r < rows_t && mn > m && (m == -INFINITY || (mn - m) * a.scale_log2e > RAISE_MAX_BY);
                 if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
                     const float alpha = m == -INFINITY ? 0.f : exp2_fast((m - mn) * a.scale_log2e);
                     l *= alpha;
                     m = mn;
-                    if (cnt > 0) {
-#pragma unroll 1
-                        for (int col = 0; col < D; col += 16) {
-                            uint32_t o[16];
-                            tc_ld16(to + col, o);
-                            tc_ld_wait();
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                            tc_st16(to + col, o);
-                        }
-                    }
+                    if (cnt > 0) shrink<D>(to, alpha);
                 }
                 // weights in bfloat16 pairs over the first 64 columns of S, all of which has been read
                 const float ref = m == -INFINITY ? 0.f : m * a.scale_log2e;
                 const uint64_t scale2 = both(a.scale_log2e), ref2 = both(-ref);
                 uint64_t sum2[2] = {0, 0};
-                auto weigh = [&](int chunk) {
-                    uint32_t out[16];
-#pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        float2 e = parts_of(pair_fma(pair_of(c[chunk][k], c[chunk][k + 1]), scale2, ref2));
-                        e.x = exp2_fast(e.x); e.y = exp2_fast(e.y);
-                        sum2[k / 2 % 2] = pair_add(sum2[k / 2 % 2], pair_of(__float_as_uint(e.x), __float_as_uint(e.y)));
-                        __nv_bfloat162 pr = __floats2bfloat162_rn(e.x, e.y);
-                        out[k >> 1] = *reinterpret_cast<uint32_t*>(&pr);
-                    }
-                    tc_st16(ts + chunk * 16, out);
-                };
+                auto weigh = [&](int chunk) { weights_of(c[chunk], ts + chunk * 16, scale2, ref2, sum2); };
                 weigh(0);
                 weigh(1);
                 tc_st_wait();
@@ -351,30 +387,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
             if (ok) {
                 tc_fence_after();
                 const long slot = ((long)max(part, 0) * a.n_kv_heads + kvh) * (2 * BQ) + t * BQ + r;
-                if (part >= 0 && r < rows_t) { a.part_ml[slot * 2] = has ? m * a.scale_log2e : -INFINITY; a.part_ml[slot * 2 + 1] = has ? l : 0.f; }
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                bf16* dst = a.out + (long)(tok0 + t * per + tok) * a.ldo + ((long)kvh * a.group + r % a.group) * a.head_dim;
-                if (has || part < 0)
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t ob[32];
-                        __syncwarp();
-                        if (has) { tc_ld32(to + c * 32, ob); tc_ld_wait(); }
-#pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            if (r >= rows_t || c * 32 + k >= a.head_dim) continue;
-                            if (part >= 0) {
-                                float* o = a.part_o + slot * D + c * 32 + k;
-                                *reinterpret_cast<uint4*>(o) = make_uint4(ob[k], ob[k + 1], ob[k + 2], ob[k + 3]);
-                                *reinterpret_cast<uint4*>(o + 4) = make_uint4(ob[k + 4], ob[k + 5], ob[k + 6], ob[k + 7]);
-                            } else {
-                                float x[8];
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : __uint_as_float(ob[k + e]) * inv;
-                                Pack<bf16>::store(dst + c * 32 + k, x);
-                            }
-                        }
-                    }
+                put_row<D>(to, a, r < rows_t, has, m, l, part, slot,
+                           a.out + (long)(tok0 + t * per + tok) * a.ldo + ((long)kvh * a.group + r % a.group) * a.head_dim);
             }
         }
     }
@@ -395,16 +409,204 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
     }
 }
 
+// Heads of 129 to 256 elements: one tile of up to 128 rows a CTA, whose O takes 256 columns.  S has two places, so that S(i + 1) is
+// made while P(i) is, and PV(i) runs under the softmax of block i + 1; keys and values have one place each, keys given back when S has
+// read them.  B200, reading back included: 2,048 tokens of 8 heads of 256 with their own keys 40 us (by attention_prefill.cu 250), 25
+// portions of up to 499 tokens behind up to 1,000, 8 heads on 1, 99 (621).
+constexpr int WIDE_THREADS = 256, WIDE_D = 256, WIDE_BARS = 13;
+struct WideSmem { static constexpr int SUB = 128 * 128, TILE = 4 * SUB, K_OFF = TILE, V_OFF = 2 * TILE, TOTAL = 3 * TILE + 1024; };
+
+template <bool CAPPED>
+__global__ void __launch_bounds__(WIDE_THREADS, 1) prefill_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a)
+{
+    using L = WideSmem;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int abort_flag_s;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ __align__(8) uint64_t bars_s[WIDE_BARS];
+    volatile int* abort_flag = &abort_flag_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    auto bar = [&](int i) { return smem_u32(&bars_s[i]); };
+    auto s_full = [&](int b) { return bar(b); };
+    auto p_half = [&](int b) { return bar(2 + b); };                     // (of either place: a warp may be a block ahead of another)
+    auto p_full = [&](int b) { return bar(4 + b); };
+    const uint32_t q_full = bar(6), k_full = bar(7), v_full = bar(8), k_empty = bar(9), v_empty = bar(10), o_done = bar(11), drained = bar(12);
+    if (threadIdx.x == 0) {
+        abort_flag_s = 0;
+        for (int i = 0; i < WIDE_BARS; ++i) mbar_init(bar(i), i >= 2 && i < 6 ? 4 : 1);      // (p_half, p_full: four warps)
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&tmem_base_s)), "r"((uint32_t)TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s, tmem_o = tmem + 256u;
+    fx_pdl_wait();
+
+    const int* item = a.items + (long)blockIdx.y * ITEM_INTS;
+    const int tok0 = item[0], n_tok = item[1], entry = item[2], pos0 = item[3], kb_begin = item[4], kb_end = item[5], part = item[6];
+    const int kvh = blockIdx.x, first_blk = max(fx_first_key(pos0, a.window, 0) / BK, kb_begin), last_blk = min((pos0 + n_tok - 1) / BK, kb_end - 1);
+    const int n = max(0, last_blk - first_blk + 1);
+    const int* table = a.block_table + (long)entry * a.table_width;
+    auto page_of = [&](int i) {                                          // (none: behind the last, zeros)
+        const int j = first_blk + i, found = j < a.table_width ? table[j] : -1;
+        return found < 0 ? a.n_pages : found;
+    };
+
+    int asked = 0;                                                       // of this thread's copies: keys', values'
+    if (warp == 0 || warp == 2) {
+        // ---------------- keys, values ----------------
+        if (lane == 0) {
+            const bool keys = warp == 0;
+            const uint32_t full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty, at = base + (keys ? L::K_OFF : L::V_OFF);
+            for (int i = 0; i < n; ++i, ++asked) {
+                const int page = page_of(i);
+                if (!met(empty, ((uint32_t)i & 1u) ^ 1u, abort_flag)) break;
+                mbar_expect_tx(full, (uint32_t)L::TILE);
+                for (int h = 0; h < 4; ++h) tma_load_4d(at + h * L::SUB, keys ? &map_k : &map_v, h * 64, 0, kvh, page, full);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------- the queries; products: S(0), then S(i + 1), PV(i) ----------------
+        if (lane == 0) {
+            mbar_expect_tx(q_full, (uint32_t)(4 * a.per_sub * a.group * 128));
+            for (int h = 0; h < 4; ++h) tma_load_4d(base + h * L::SUB, &map_q, h * 64, 0, kvh, tok0, q_full);
+            constexpr uint32_t idesc_s = instr_desc_ex(BQ, BK, 0), idesc_o = instr_desc_ex(BQ, WIDE_D, 1);
+            bool ok = met(q_full, 0, abort_flag);
+            auto issue_s = [&](int i) {
+                if (!met(k_full, (uint32_t)i & 1u, abort_flag)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const uint64_t dq = smem_desc(base + h * L::SUB), dk = smem_desc(base + L::K_OFF + h * L::SUB);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc_mma(tmem + 128u * (i & 1), dq + 2u * k, dk + 2u * k, idesc_s, (h | k) != 0);
+                }
+                tc_commit(s_full(i & 1));
+                tc_commit(k_empty);
+                return true;
+            };
+            ok = ok && (n == 0 || issue_s(0));
+            for (int i = 0; i < n && ok; ++i) {
+                if (i + 1 < n) ok = issue_s(i + 1);
+                ok = ok && met(v_full, (uint32_t)i & 1u, abort_flag) && met(p_half(i & 1), (uint32_t)(i >> 1) & 1u, abort_flag);
+                auto issue_o = [&](int ks0) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < BK / 32; ++k)
+                        tc_mma_ts(tmem_o, tmem + 128u * (i & 1) + 8u * (ks0 + k), smem_desc_lbo_sbo(base + L::V_OFF + (ks0 + k) * 2048, L::SUB, 1024), idesc_o,
+                                  (i | (ks0 + k)) != 0);
+                };
+                if (!ok) break;
+                issue_o(0);
+                ok = met(p_full(i & 1), (uint32_t)(i >> 1) & 1u, abort_flag);
+                if (!ok) break;
+                issue_o(BK / 32);
+                tc_commit(o_done);
+                tc_commit(v_empty);
+            }
+            if (*abort_flag) {                                           // given up: no product may outlive tensor memory
+                tc_commit(drained);
+                for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(drained, 0); ++i) { }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ---------------- softmax: a row a thread ----------------
+        const int quad = warp & 3, r = quad * 32 + lane, rows = n_tok * a.group, tok = r / a.group, p_r = pos0 + tok;
+        const int lo_r = fx_first_key(p_r, a.window, 0), lo_last = fx_first_key(pos0 + n_tok - 1, a.window, 0);
+        const uint32_t lane_off = (uint32_t)(quad * 32) << 16, to = tmem_o + lane_off;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            ok = __all_sync(0xffffffffu, met(s_full(i & 1), (uint32_t)(i >> 1) & 1u, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            if (__builtin_expect(quad * 32 >= rows, 0)) {                // none of the warp's rows exists
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(p_half(i & 1)); mbar_arrive(p_full(i & 1)); }
+                continue;
+            }
+            const int kb = (first_blk + i) * BK;
+            const bool interior = kb + BK - 1 <= pos0 && kb >= lo_last;
+            const uint32_t ts = tmem + 128u * (i & 1) + lane_off;
+            uint32_t c[4][32];
+            const float mn = fmaxf(m, scores_of<CAPPED>(c, ts, a, interior, kb, lo_r, p_r));
+            const bool raise = r < rows && mn > m && (m == -INFINITY || (mn - m) * a.scale_log2e > RAISE_MAX_BY);
+            if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
+                const float alpha = m == -INFINITY ? 0.f : exp2_fast((m - mn) * a.scale_log2e);
+                l *= alpha;
+                m = mn;
+                if (i > 0) {                                             // (S(i) was made behind PV(i - 2) and ahead of PV(i - 1))
+                    ok = __all_sync(0xffffffffu, met(o_done, (uint32_t)(i - 1) & 1u, abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+                    shrink<WIDE_D>(to, alpha);
+                }
+            }
+            const float ref = m == -INFINITY ? 0.f : m * a.scale_log2e;
+            const uint64_t scale2 = both(a.scale_log2e), ref2 = both(-ref);
+            uint64_t sum2[2] = {0, 0};
+            weights_of(c[0], ts, scale2, ref2, sum2);
+            weights_of(c[1], ts + 16, scale2, ref2, sum2);
+            tc_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_half(i & 1));
+            weights_of(c[2], ts + 32, scale2, ref2, sum2);
+            weights_of(c[3], ts + 48, scale2, ref2, sum2);
+            tc_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(i & 1));
+            const float2 sum = parts_of(pair_add(sum2[0], sum2[1]));
+            l += sum.x + sum.y;
+        }
+        // (what S(n - 1) says is that PV(n - 3) has ended: a phase at a time from there)
+        if (ok && n > 1) ok = __all_sync(0xffffffffu, met(o_done, (uint32_t)(n - 2) & 1u, abort_flag));
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, met(o_done, (uint32_t)(n - 1) & 1u, abort_flag));
+        if (ok) {
+            tc_fence_after();
+            put_row<WIDE_D>(to, a, r < rows, n > 0, m, l, part, ((long)max(part, 0) * a.n_kv_heads + kvh) * BQ + r,
+                            a.out + (long)(tok0 + tok) * a.ldo + ((long)kvh * a.group + r % a.group) * a.head_dim);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)TMEM_COLS) : "memory");
+    }
+    if (abort_flag_s && lane == 0 && warp < 3) {
+        // given up: this thread's copies under way still land
+        auto settle = [](uint32_t at, uint32_t parity) { for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try_wait(at, parity); ++i) { } };
+        if (warp == 1) settle(q_full, 0);
+        else if (asked > 0) settle(warp == 0 ? k_full : v_full, (uint32_t)(asked - 1) & 1u);
+        if (a.status) atomicExch(a.status, STATUS_TC_TIMEOUT);
+    }
+}
+
 // The runs of a tile that was cut: merges int32 [n][4] = (first token, tokens, first part, runs); a warp a row.
 template <int D> __global__ void __launch_bounds__(128) prefill_grouped_merge_kernel(const int* __restrict__ merges, const __grid_constant__ Args a)
 {
     fx_pdl_wait();
     const int* mg = merges + (long)blockIdx.x * 4;
     const int tok0 = mg[0], n_tok = mg[1], part0 = mg[2], runs = mg[3], kvh = blockIdx.y;
+    constexpr int ROWS = D > 128 ? BQ : 2 * BQ;
     const int lane = threadIdx.x & 31, row = blockIdx.z * 4 + (threadIdx.x >> 5), t = row / BQ, r = row % BQ;
     if (r >= min(a.per_sub, n_tok - t * a.per_sub) * a.group) return;      // (a whole warp)
     constexpr int PER = D / 32;
-    const long slot0 = ((long)part0 * a.n_kv_heads + kvh) * (2 * BQ) + row, step = (long)a.n_kv_heads * (2 * BQ);
+    const long slot0 = ((long)part0 * a.n_kv_heads + kvh) * ROWS + row, step = (long)a.n_kv_heads * ROWS;
     float m = -INFINITY, l = 0.f;                                            // lane c: run c's (at most 32)
     if (lane < runs) {
         const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (slot0 + lane * step) * 2);
@@ -442,6 +644,17 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
     return fx_launch_status();
 }
 
+template <bool CAPPED>
+int launch_wide(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int n_items, const int* merges, int n_merges, cudaStream_t s)
+{
+    auto kern = prefill_wide_kernel<CAPPED>;
+    // of the current device: asked for each time
+    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WideSmem::TOTAL)) return (int)e;
+    fx_launch_pdl(kern, dim3(a.n_kv_heads, n_items), WIDE_THREADS, WideSmem::TOTAL, s, mq, mk, mv, a);
+    if (n_merges > 0) fx_launch_pdl(prefill_grouped_merge_kernel<WIDE_D>, dim3(n_merges, a.n_kv_heads, BQ / 4), 128, 0, s, merges, a);
+    return fx_launch_status();
+}
+
 bool encode(CUtensorMap* map, const void* ptr, cuuint64_t d0, cuuint64_t d1, cuuint64_t d2, cuuint64_t d3, cuuint64_t s1, cuuint64_t s2, cuuint64_t s3,
             cuuint32_t b1, cuuint32_t b3)
 {
@@ -456,15 +669,15 @@ bool encode(CUtensorMap* map, const void* ptr, cuuint64_t d0, cuuint64_t d1, cuu
 
 // Keys and values: pages [n_pages][kv heads][128][head_dim], block_table [entries][table_width] names those of an entry's positions
 // 128 j .. 128 j + 127.  items: int32 [n_items][8] = (first flat token, tokens, entry, position of the first token, first key block, end
-// of the key blocks, part or -1, 0); a tile holds up to 2 * (128 / group) tokens, group = n_heads / n_kv_heads <= 128.  part_o [parts][kv
-// heads][256][64 or 128], part_ml [parts][kv heads][256][2].
+// of the key blocks, part or -1, 0); a tile holds up to 2 * (128 / group) tokens (128 / group of heads above 128 elements), group = n_heads
+// / n_kv_heads <= 128.  part_o [parts][kv heads][256][64 or 128] ([128][256]), part_ml [parts][kv heads][256 (128)][2].
 extern "C" int fx_prefill_attention_grouped(const void* q, long ldq, int n_tokens, const void* k_pages, const void* v_pages, int n_pages,
                                             const int* block_table, int table_width, const int* items, int n_items, void* out, long ldo,
                                             int n_heads, int n_kv_heads, int head_dim, int window, float scale, float softcap, float* part_o, float* part_ml,
                                             const int* merges, int n_merges, int* status, void* stream)
 {
     if (n_items <= 0 || n_tokens <= 0) return FX_OK;
-    if (head_dim <= 0 || head_dim > 128 || head_dim % 16 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > BQ ||
+    if (head_dim <= 0 || head_dim > WIDE_D || head_dim % 16 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > BQ ||
         n_pages <= 0 || table_width <= 0 || window < 0 || !(scale > 0.f) || !(softcap >= 0.f) || n_items > 65535 || n_kv_heads > 65535 ||
         (n_merges > 0 && (!part_o || !part_ml || !merges))) return FX_ERR_SIZE;
     if (ldq % 8 || ldo % 8 || (uintptr_t)q % 16 || (uintptr_t)out % 16 || (uintptr_t)k_pages % 16 || (uintptr_t)v_pages % 16 || (uintptr_t)part_o % 16)
@@ -479,6 +692,7 @@ extern "C" int fx_prefill_attention_grouped(const void* q, long ldq, int n_token
     if (!encode(&mq, q, W, group, G, n_tokens, W, W * group, ldq, group, per) || !encode(&mk, k_pages, W, BK, G, n_pages, W, BK * W, G * BK * W, BK, 1) ||
         !encode(&mv, v_pages, W, BK, G, n_pages, W, BK * W, G * BK * W, BK, 1)) return FX_ERR_SIZE;
     cudaStream_t s = (cudaStream_t)stream;
+    if (head_dim > 128) return capped ? launch_wide<true>(mq, mk, mv, a, n_items, merges, n_merges, s) : launch_wide<false>(mq, mk, mv, a, n_items, merges, n_merges, s);
     if (capped) return head_dim <= 64 ? launch<64, true>(mq, mk, mv, a, n_items, merges, n_merges, s) : launch<128, true>(mq, mk, mv, a, n_items, merges, n_merges, s);
     return head_dim <= 64 ? launch<64, false>(mq, mk, mv, a, n_items, merges, n_merges, s) : launch<128, false>(mq, mk, mv, a, n_items, merges, n_merges, s);
 }

@@ -2235,9 +2235,9 @@ def fp8_token_by_token(kind, entries, window, n_heads, n_kv_heads, head_dim, sms
     SMs sharing the tiles; one that is not cut into runs takes ``chain`` a key by itself; ``base`` are the launches.  20 requests of up
     to 600 positions and 8 of up to 4,000, 24 tokens each, decode against tiled: 28 heads of 128 on 4 (grouped) 50 against 28 and 89
     against 43, 96 tokens of one request of 600 19 against 23; the same with capped scores 51 against 37, 93 against 54, 20 against 32; 16 heads of
-    256 on 4 (mma) 85 against 109 and 95 against 429; 16 heads of 128 on 4 in 32 bits 48 against 119 and 81 against 322;
+    256 on 4 83 against 29 and 94 against 64 (by the mma.sync kernel 109 and 429); 16 heads of 128 on 4 in 32 bits 48 against 119 and 81 against 322;
     prompts of 300, 193 and 97 tokens of 4 heads of 64 on 2 in 32 bits 28 against 24."""
-    together = 256 * n_kv_heads // n_heads                                   # tokens of a tile that holds the heads of a kv head
+    together = (256 if head_dim <= 128 else 128) * n_kv_heads // n_heads     # tokens of a tile that holds the heads of a kv head
     rows, base, block, chain = {"grouped": (together, 14.0, 2.4, 0.0), "capped": (together, 24.0, 4.0, 0.0), "tc": (256, 30.0, 4.5, 0.0),
                                 "mma": (PREFILL_TILE, 12.0, 3.0, 0.107 * head_dim / 256),
                                 "f32": (128, 10.0, 4.0, 0.035 + 0.00017 * head_dim)}[kind]
@@ -2418,8 +2418,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     f32, wide = x == F32, 4 if x == F32 else 8
     tiled = scale > 0 and ldq % wide == 0 and qp % 16 == 0 and (head_dim <= 128 and head_dim % 4 == 0 and ldo % 4 == 0 and op % 16 == 0 if f32 else
                                                                 head_dim % 16 == 0 and ldo % 2 == 0)
-    kind = ("f32" if f32 else "mma" if head_dim > 128 else "tc" if n_heads > 128 * n_kv_heads or ldo % 8 or op % 16 else
-            "grouped" if softcap is None else "capped")
+    kind = ("f32" if f32 else ("tc" if head_dim <= 128 else "mma") if n_heads > 128 * n_kv_heads or ldo % 8 or op % 16 else
+            "capped" if softcap is not None else "grouped")
     route = tiled and plan.route(kind if decode_fp8_ok(kp, vp, head_dim, page_size) else None, window, n_heads, n_kv_heads, head_dim, 4 if f32 else 2)
     if not route:
         _decode_fp8(found, page_size, n_heads, window, scale, softcap, st)
@@ -2439,10 +2439,10 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     return out
 
 
-def prefill_grouped_plan(entries, window, n_heads: int, n_kv_heads: int):
+def prefill_grouped_plan(entries, window, n_heads: int, n_kv_heads: int, head_dim: int):
     """:func:`prefill_tc_plan` for :func:`prefill_attention_grouped`: whole tokens of all the query heads of a kv head, in two halves of
-    up to 128 rows."""
-    return prefill_tc_plan(entries, window, n_kv_heads, tile=2 * (128 * n_kv_heads // n_heads))
+    up to 128 rows, or one for heads of more than 128 elements."""
+    return prefill_tc_plan(entries, window, n_kv_heads, tile=(2 if head_dim <= 128 else 1) * (128 * n_kv_heads // n_heads))
 
 
 _GROUPED = "xTQ~ xNGPD xNGPD iBW in8 xTO~ ?im4 ?iZ"
@@ -2451,7 +2451,7 @@ _GROUPED = "xTQ~ xNGPD xNGPD iBW in8 xTO~ ?im4 ?iZ"
 def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_heads, n_kv_heads, head_dim, window, scale, status=None,
                               stream=None, merges=None, parts=0, softcap=None):
     """Attention of prompt portions in bfloat16, of query heads that may share key heads, over pages of 128 positions [pages, kv heads, 128,
-    head_dim]: heads of up to 128 elements in steps of 16, at most 128 query heads a kv head, rows on the 16-byte grid, a positive
+    head_dim]: heads of up to 256 elements in steps of 16, at most 128 query heads a kv head, rows on the 16-byte grid, a positive
     scale, scores capped or not.  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``, ``parts``: device copies of what
     :func:`prefill_grouped_plan` returns, and its number of parts."""
     name = "prefill_attention_grouped"
@@ -2466,10 +2466,10 @@ def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_he
     if parts:
         global _launches
         _launches += 1
-        width = 64 if head_dim <= 64 else 128
-        work = torch.empty(parts * n_kv_heads * 256 * (width + 2), dtype=torch.float32, device=q.device)
+        width, rows = 64 if D <= 64 else 128 if D <= 128 else 256, parts * G * (256 if D <= 128 else 128)
+        work = torch.empty(rows * (width + 2), dtype=torch.float32, device=q.device)
         po = work.data_ptr()
-        pm = po + 4 * parts * n_kv_heads * 256 * width
+        pm = po + 4 * rows * width
     call("fx_prefill_attention_grouped", qp, ldq, T, kp, vp, N, tp, W, ip, n, op, ldo, n_heads, G, D, int(window or 0), float(scale), float(softcap or 0.0), po, pm,
          mp if parts else 0, n_merges if parts else 0, zp, stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
     return out
@@ -2494,7 +2494,8 @@ def _prefill_read_back(kind, q, k, v, table, page_size, plan, key, entries, slot
         return
     capped = softcap is not None
     if kind in ("grouped", "capped"):
-        items, merges, parts = plan.kept(("grouped", n_heads, n_kv_heads) + key, lambda: prefill_grouped_plan(entries, window, n_heads, n_kv_heads))
+        items, merges, parts = plan.kept(("grouped", n_heads, n_kv_heads, head_dim > 128) + key,
+                                           lambda: prefill_grouped_plan(entries, window, n_heads, n_kv_heads, head_dim))
         prefill_attention_grouped(q, k, v, table, items, out, *heads, status=status, merges=merges, parts=parts, **tail)
         return
     if (prefill_tc_general_ok(q, q.stride(0), head_dim, k, v, page_size, out, out.stride(0), head_dim, head_dim, head_dim, scale, softcap)

@@ -475,7 +475,7 @@ def test_a_prompt_next_to_rows_that_are_no_numbers(dtype, H, softcap):
     assert torch.isfinite(out[:60]).all() and torch.isfinite(out[100:]).all()
 
 
-@pytest.mark.parametrize("H,G,D", [(6, 2, 128), (7, 1, 64), (16, 4, 80)])
+@pytest.mark.parametrize("H,G,D", [(6, 2, 128), (7, 1, 64), (16, 4, 80), (6, 2, 256), (5, 1, 144)])
 @pytest.mark.parametrize("window", [None, 100, 700])
 @pytest.mark.parametrize("run_blocks", [0, 1, 3])
 @pytest.mark.parametrize("softcap", [None, 6.0])
@@ -605,7 +605,7 @@ def test_pages_longer_than_a_tile(dtype, H, G, D, P):
     check(out, c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT[dtype])
 
 
-@pytest.mark.parametrize("H,G,D", [(4, 4, 128), (3, 3, 48), (12, 12, 64)])
+@pytest.mark.parametrize("H,G,D", [(4, 4, 128), (3, 3, 48), (12, 12, 64), (2, 2, 256), (3, 3, 192)])
 @pytest.mark.parametrize("window,softcap", [(None, None), (90, None), (90, 40.0)])
 def test_prompts_of_heads_with_their_own_keys(H, G, D, window, softcap):
     """Portions around the sizes of a sub-tile and a tile."""
@@ -795,7 +795,7 @@ def test_refusals_of_the_kernel_over_pages_of_128():
     H, G, D = 4, 2, 64
     q, out = torch.zeros(20, H * D, dtype=torch.bfloat16, device=DEV), torch.zeros(20, H * D, dtype=torch.bfloat16, device=DEV)
     k, table = torch.zeros(1, G, 128, D, dtype=torch.bfloat16, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
-    items, merges, parts = ops.prefill_grouped_plan([(20, 0)], None, H, G)
+    items, merges, parts = ops.prefill_grouped_plan([(20, 0)], None, H, G, D)
     items = torch.from_numpy(items).to(DEV)
     good = dict(q=q, k_pages=k, v_pages=k, block_table=table, items=items, out=out, n_heads=H, n_kv_heads=G, head_dim=D, window=None, scale=1.0)
     ops.prefill_attention_grouped(**good)
