@@ -456,10 +456,11 @@ def test_prompts_with_a_window(dtype, window, softcap, most, monkeypatch):
 
 
 @pytest.mark.parametrize("dtype,H,softcap", [("bf16", 2, None), ("bf16", 1, None), ("bf16", 2, 20.0), ("f32", 2, None)])
-def test_a_prompt_next_to_rows_that_are_no_numbers(dtype, H, softcap):
+@pytest.mark.parametrize("D", [64, 256])
+def test_a_prompt_next_to_rows_that_are_no_numbers(dtype, H, softcap, D):
     """Garbage behind a request's last position, and a row that only some queries see; heads that share their keys, and one that
     does not."""
-    G, D, P = 1, 64, 64
+    G, P = 1, 64
     entries = [(100, 0), (90, 30)]
     c = Cache([170, 128], G, D, P, 20)
     for which in (0, 1):
