@@ -2434,7 +2434,9 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
         k, v = torch.empty(shape, dtype=q.dtype, device=q.device), torch.empty(shape, dtype=q.dtype, device=q.device)
         read_kv_fp8_spans(*cache, spans, rows, seq_slot, k, v, stream=st, attend=True)
         q_part, out_part = (q, out) if n == T else (q[tok0:tok0 + n], out[tok0:tok0 + n])
-        _prefill_read_back(kind, q_part, k, v, table, FP8_READ_PAGE, plan, (tok0, window), entries, slots, out_part, n_heads, n_kv_heads, head_dim,
+        # (which entries a portion has goes by the bytes that the layer reads back of a position)
+        of_part = (tok0, window, 2 * n_kv_heads * head_dim * (4 if f32 else 2))
+        _prefill_read_back(kind, q_part, k, v, table, FP8_READ_PAGE, plan, of_part, entries, slots, out_part, n_heads, n_kv_heads, head_dim,
                            window, scale, softcap, status, st)
     return out
 

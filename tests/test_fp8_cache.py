@@ -210,3 +210,64 @@ def test_what_goes_token_by_token(kind, heads, kv_heads, dim):
     assert not choice([(2048, 0)]) and not choice([(300, 3700)] * 6)
     sizes = [choice([(n, 1000)] * 4) for n in (9, 16, 32, 64, 128, 256, 1024)]
     assert sizes == sorted(sizes, reverse=True)                             # (once tiled, tiled with more tokens)
+
+
+# ---- one plan, layers of several shapes -----------------------------------------------------------------------------
+def _prompt_layer(plan, monkeypatch, heads, kv_heads, dim, dtype=torch.bfloat16, window=None, dim_out=0):
+    """What a layer of a prompt step hands to the kernels over read-back pages: [(first token, tokens, block table, tile lists)], the
+    launches put aside."""
+    T, found = plan.n_tokens, []
+
+    def look(name, q, *rest):
+        x = ops.BF16 if q.dtype == torch.bfloat16 else ops.F32
+        return (None, 0, x, *[256] * 12, 9, kv_heads, plan.page_size, dim, 1, 9, T, len(plan.entries), heads * dim, heads * dim, 1, -1, q.stride(0), heads * dim + dim_out)
+
+    def kernel(rows, stays):
+        def record(q, k, v, table, *lists_and_rest, **kw):
+            at = (q.data_ptr() - q_all.data_ptr()) // (q_all.stride(0) * q_all.element_size())
+            found.append((at, q.shape[0], table, rows([x for x in lists_and_rest if isinstance(x, torch.Tensor) and x.dim() == 2 and x.dtype == torch.int32])))
+            return stays
+        return record
+
+    q_all = torch.zeros(T, heads * dim, dtype=dtype)
+    monkeypatch.setattr(ops, "_look_at_attention_fp8", look)
+    monkeypatch.setattr(ops, "sm_count", lambda: 148)
+    monkeypatch.setattr(ops, "fp8_token_by_token", lambda *a: False)
+    monkeypatch.setattr(ops, "read_kv_fp8_spans", lambda *a, **k: None)
+    monkeypatch.setattr(ops, "decode_attention_fp8", lambda *a, **k: None)
+    monkeypatch.setattr(ops, "prefill_attention_grouped", kernel(lambda t: t[0][:, :3], None))
+    monkeypatch.setattr(ops, "prefill_attention_tc", kernel(lambda t: t[0][:, :3], None))
+    monkeypatch.setattr(ops, "prefill_attention", kernel(lambda t: t[0][:, :3], None))
+    monkeypatch.setattr(ops, "prefill_attention_f32_tc", kernel(lambda t: t[0][:, :3], None))
+    monkeypatch.setattr(ops, "prefill_attention_f32", kernel(lambda t: t[0][:, :3], None))
+    ops.prefill_attention_fp8(q_all, *[None] * 5, plan.page_size, plan, None, None, None, torch.zeros(T, heads * dim, dtype=dtype), heads, kv_heads, dim,
+                              window, 1.0)
+    return found
+
+
+SHAPES = [("grouped", dict(heads=16, kv_heads=16, dim=64)), ("grouped", dict(heads=16, kv_heads=16, dim=128)), ("grouped", dict(heads=16, kv_heads=4, dim=64)),
+          ("tc", dict(heads=130, kv_heads=1, dim=64)), ("tc", dict(heads=130, kv_heads=1, dim=128)),
+          ("mma", dict(heads=130, kv_heads=1, dim=144)), ("mma", dict(heads=130, kv_heads=1, dim=256)),
+          ("f32", dict(heads=16, kv_heads=16, dim=64, dtype=torch.float32)), ("f32", dict(heads=16, kv_heads=4, dim=64, dtype=torch.float32)),
+          ("f32", dict(heads=16, kv_heads=4, dim=68, dtype=torch.float32)), ("f32", dict(heads=16, kv_heads=2, dim=68, dtype=torch.float32))]
+
+
+@pytest.mark.parametrize("a", range(len(SHAPES)))
+@pytest.mark.parametrize("b", range(len(SHAPES)))
+def test_a_plan_serves_layers_that_are_cut_differently(a, b, monkeypatch):
+    """A step is cut into portions by the bytes that a layer reads back, so that layers of other heads, head sizes or types have other
+    portions.  Every list names entries of its own portion only and holds all of its tokens, whatever layer has used the plan before."""
+    monkeypatch.setattr(ops, "FP8_READ_BACK_MAX", 4 * 512 * 2 * 16 * 64 * 2)              # (four entries of the first shape)
+    plan = ops.prefill_fp8_plan([(40, 460)] * 6, 64, "cpu")
+    for kind, shape in (SHAPES[a], SHAPES[b]):
+        row_bytes = 2 * shape["kv_heads"] * shape["dim"] * (4 if shape.get("dtype") else 2)
+        found = _prompt_layer(plan, monkeypatch, **shape)
+        assert sum(n for _, n, _, _ in found) == 240
+        assert all(n <= 40 or n // 40 * 512 * row_bytes <= ops.FP8_READ_BACK_MAX for _, n, _, _ in found)
+        at = 0
+        for first, n, table, tiles in found:
+            assert first == at and table.shape[0] == n // 40
+            covered = sorted((t, t + m, e) for t, m, e in set(map(tuple, tiles.tolist())))
+            assert covered[0][0] == 0 and covered[-1][1] == n and all(x[1] == y[0] for x, y in zip(covered, covered[1:]))
+            assert all(0 <= e < table.shape[0] and t // 40 == e == (end - 1) // 40 for t, end, e in covered)
+            at += n

@@ -619,6 +619,27 @@ def test_prompts_of_heads_with_their_own_keys(H, G, D, window, softcap):
     check(out, c, entries, q, H, window, 0.15, softcap, PROMPT_WEIGHT["bf16"])
 
 
+@pytest.mark.parametrize("first,second", [((8, 8, 64, "bf16"), (8, 8, 128, "bf16")), ((8, 8, 128, "bf16"), (8, 8, 64, "bf16")), ((8, 2, 64, "f32"), (8, 8, 64, "f32")),
+                                          ((8, 8, 64, "f32"), (8, 2, 64, "f32")), ((4, 1, 256, "bf16"), (4, 4, 256, "bf16")), ((4, 4, 64, "f32"), (4, 4, 64, "bf16"))])
+def test_a_plan_of_layers_that_are_cut_differently(first, second, monkeypatch):
+    """Layers whose steps are cut into other portions, by what they read back of a position, use one plan in turn: every result is that of
+    a plan of the layer's own, bit for bit."""
+    monkeypatch.setattr(ops, "FP8_READ_BACK_MAX", 1 << 20)
+    entries = [(40, 460), (12, 100), (3, 90), (100, 20), (30, 300), (20, 0)]
+    plan, cuts = ops.prefill_fp8_plan(entries, 64, DEV), []
+    for H, G, D, dtype in (first, second, first):
+        c = Cache([n + s for n, s in entries], G, D, 64, 90)
+        T = sum(n for n, _ in entries)
+        q, st, own = rows(T, H, G, D, DTYPES[dtype], 91), step(entries, c.slots), ops.prefill_fp8_plan(entries, 64, DEV)
+        want, out = (torch.full((T, H * D), 7.0, dtype=q.dtype, device=DEV) for _ in range(2))
+        ops.prefill_attention_fp8(q, *c.operands, own, *st, want, H, G, D, None, 0.1)
+        ops.prefill_attention_fp8(q, *c.operands, plan, *st, out, H, G, D, None, 0.1)
+        assert torch.equal(out, want)
+        cuts.append([n for _, n, *_ in own.parts(None, 2 * G * D * q.element_size())])
+    assert cuts[0] != cuts[1] and cuts[0] == cuts[2]
+    check(out, c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT[first[3]])
+
+
 # ---- streams, graphs, order -----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_on_a_stream_of_its_own_and_in_a_graph(dtype):
