@@ -21,8 +21,8 @@
 // their maximum found 500, asked whether it is to be raised 190, weights 1,540 (their 2^x alone 1,024), the rest of PV and the next
 // S 1,330.  B200: 3,600 clocks a pair with few blocks running, 2.39 us with all (982 TFLOP/s over long contexts; 28 heads of 128 on 4).  Six
 // portions of 300 tokens behind up to 3,800, the pages' reading back included: 86 us; a prompt of 2,048 of 16 heads with their own
-// keys 49.5 (by the kernel of attention_prefill_tc.cu 65); with capped scores, whose tanh is two more operations of the special-function
-// unit a score, 152 and 80 (there 280 and 139).  Tried: scores read twice instead of held, P in one piece 2.91 us a pair; a
+// keys 49.5 (by the kernel of attention_prefill_tc.cu 65); with capped scores 129 and 70, and 152 and 83 where
+// scores come near the cap (there 280 and 139).  Tried: scores read twice instead of held, P in one piece 2.91 us a pair; a
 // thread of its own for each sub-tile's products, softmaxes in turns 2.56, without turns 2.89 (both then do the same at the same
 // time); a quarter of the 2^x by polynomial 2.64; rolled loops around the products 2.71.  Converting the 8-bit pages in this
 // kernel, by seven more warps, cost the softmax threads a third of their registers and the tile its pace (162 us and 86 us where
@@ -44,6 +44,7 @@ using namespace fxtc;
 constexpr int BQ = 128, BK = 128, NTHREADS = 384, TMEM_COLS = 512, ITEM_INTS = 8, N_BARS = 19;
 constexpr int REGS_FEW = 88, REGS_MANY = 208;   // a thread of the first four warps, of the softmax: together what the block is launched with
 constexpr float RAISE_MAX_BY = 8.f;   // in powers of two
+constexpr float CAP_SMALL = 0.8f, CAP_LARGE = 0.66f;      // (tanh(CAP_SMALL) = 0.664)
 
 struct Args {
     const int* block_table; int table_width, n_pages;       // [entries][blocks of 128 positions]
@@ -51,7 +52,7 @@ struct Args {
     bf16* out; long ldo;
     float *part_o, *part_ml;
     int n_kv_heads, group, per_sub, head_dim, window;     // per_sub: tokens of a sub-tile
-    float scale_log2e, cap_in, cap;                       // capped: score = cap tanh(q.k scale / softcap), cap and scores in powers of two
+    float scale_log2e, cap_in;                            // scores in powers of two: q.k scale_log2e, capped scale_log2e tanh(q.k cap_in)
     int* status;
 };
 
@@ -96,6 +97,11 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ uint64_t both(float x) { return pair_of(__float_as_uint(x), __float_as_uint(x)); }
 __device__ __forceinline__ float2 parts_of(uint64_t a) {
     float2 r;
@@ -107,32 +113,84 @@ __device__ __forceinline__ bool met(uint32_t bar, uint32_t parity, volatile int*
     if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
     return mbar_wait(bar, parity, abort_flag);
 }
-// A row's scores into registers, capped and masked, and the largest of them.
-template <bool CAPPED>
-__device__ __forceinline__ float scores_of(uint32_t (&c)[4][32], uint32_t ts, const Args& a, bool interior, int kb, int lo_r, int p_r) {
+// Capped scores: a warp's of a block become tanh(k s).  Where none that counts is beyond |k s| = 0.8 (mostly so: caps are several times what
+// scores come to), the odd polynomial x + x z p(z), z = x^2, p fitted by a linear program for the smallest largest relative error (4.3e-8; in
+// 32 bits 1.4e-7 of each score).  Else 1 - 2 / (e^2x + 1), which is off by some 3e-7 of the cap however small the score: at most 5e-7 of the
+// largest score that the warp's rows have met.  Two scores an instruction, for what a cap costs is instructions.  A block behind one with a
+// score that large is not looked at first (`look`).  B200, the portions of 300 tokens and the prompt of 2,048 named above, scores of up to
+// some 20: 129 and 70 us under caps of 30 and more, 152 and 83 under one of 15, 151 and 80 under one of 4; with the second form alone 150 and
+// 80; always looking 159 and 85 under the cap of 4; the polynomial up to 1/2 only, of a term less, 120 and 65 under a cap of 50, 164 and 87
+// under one of 15; one rational function for every size 173 and 87.
+// Hidden scores are no numbers while they are looked at, which fmaxf passes over, and rows that do not exist have no say: which form is taken
+// hangs on the request's own scores.
+__device__ __forceinline__ uint64_t tanh_small(uint64_t x) {
+    const uint64_t z = pair_mul(x, x);
+    const uint64_t p = pair_fma(pair_fma(pair_fma(pair_fma(both(-4.390075137e-03f), z, both(1.916173016e-02f)), z, both(-5.316196404e-02f)), z,
+                                         both(1.332244125e-01f)), z, both(-3.333283229e-01f));
+    return pair_fma(pair_mul(x, z), p, x);
+}
+__device__ __forceinline__ uint64_t tanh_any(uint64_t x2log2e) {
+    const float2 x = parts_of(x2log2e);
+    const float2 d = parts_of(pair_add(pair_of(__float_as_uint(exp2_fast(x.x)), __float_as_uint(exp2_fast(x.y))), both(1.f)));
+    return pair_fma(pair_of(__float_as_uint(reciprocal_fast(d.x)), __float_as_uint(reciprocal_fast(d.y))), both(-2.f), both(1.f));
+}
+template <typename F> __device__ __forceinline__ void each_pair(uint32_t (&c)[32], float k, F&& f) {
+    const uint64_t k2 = both(k);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, c[i]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) tc_ld_wait_for(c[i]);
-    if constexpr (CAPPED) {                              // tanh(x) = 1 - 2 / (e^2x + 1)
-#pragma unroll
-        for (int k = 0; k < BK; ++k) {
-            const float e = exp2_fast(__uint_as_float(c[k / 32][k % 32]) * a.cap_in);
-            c[k / 32][k % 32] = __float_as_uint(fmaf(-2.f * a.cap, reciprocal_fast(e + 1.f), a.cap));
-        }
+    for (int i = 0; i < 32; i += 2) {
+        const float2 y = parts_of(f(pair_mul(pair_of(c[i], c[i + 1]), k2)));
+        c[i] = __float_as_uint(y.x); c[i + 1] = __float_as_uint(y.y);
     }
-    if (__builtin_expect(!interior, 0)) {                // (out of the way of what most blocks run through)
+}
+// A row's scores into registers, capped (then what they are multiplied with, scale_log2e, is the cap) and masked, and the largest of them.
+template <bool CAPPED>
+__device__ __forceinline__ float scores_of(uint32_t (&c)[4][32], uint32_t ts, const Args& a, bool interior, int kb, int lo_r, int p_r, bool row_ok, bool& look) {
+    auto hide = [&](uint32_t as) {
+        if (__builtin_expect(interior, 1)) return;       // (out of the way of what most blocks run through)
 #pragma unroll
         for (int k = 0; k < BK; ++k)
-            if (kb + k > p_r || kb + k < lo_r) c[k / 32][k % 32] = 0xff800000u;      // -infinity
+            if (kb + k > p_r || kb + k < lo_r) c[k / 32][k % 32] = as;
+    };
+    bool small = !CAPPED;
+    if (!CAPPED || look) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, c[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tc_ld_wait_for(c[i]);
+        if constexpr (CAPPED) {
+            hide(0x7fffffffu);                           // no number
+            float size[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < BK; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    size[e] = fmaxf(fmaxf(size[e], fabsf(__uint_as_float(c[i / 32][i % 32 + e]))), fabsf(__uint_as_float(c[i / 32][i % 32 + 4 + e])));
+            small = __all_sync(0xffffffffu, !row_ok || fmaxf(fmaxf(size[0], size[1]), fmaxf(size[2], size[3])) * a.cap_in <= CAP_SMALL);
+            if (small) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) each_pair(c[i], a.cap_in, tanh_small);
+            }
+        }
     }
+    if (!small) {                                        // (read again where they have been looked at: no copy of what is still on its way)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, c[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            tc_ld_wait_for(c[i]);
+            each_pair(c[i], a.cap_in * 2.8853900817779268f, tanh_any);      // 2 log2(e)
+        }
+    }
+    hide(0xff800000u);                                   // -infinity
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int k = 0; k < BK; k += 8)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(c[k / 32][k % 32 + e])), __uint_as_float(c[k / 32][k % 32 + 4 + e]));
-    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    if constexpr (CAPPED) look = !__any_sync(0xffffffffu, row_ok && top > CAP_LARGE);
+    return top;
 }
 // 32 scores' weights in bfloat16 pairs into 16 columns of tensor memory, their sums (before they are rounded) onto sum2.
 __device__ __forceinline__ void weights_of(const uint32_t* c, uint32_t at, uint64_t scale2, uint64_t ref2, uint64_t* sum2) {
@@ -336,7 +394,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
             const int lo_r = fx_first_key(p_r, a.window, 0), lo_last = fx_first_key(pos_t + tokens_of(t) - 1, a.window, 0);
             const uint32_t lane_off = (uint32_t)(quad * 32) << 16, ts = tmem_s(t) + lane_off, to = tmem_o(t) + lane_off;
             float m = -INFINITY, l = 0.f;
-            bool ok = true;
+            bool ok = true, look = true;
             int cnt = 0;
             for (int i = 0; i < n_walk; ++i) {
                 if (!active(t, i)) continue;
@@ -353,7 +411,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_grouped_kernel(const __gr
                 const int kb = (first_blk + i) * BK;
                 const bool interior = kb + BK - 1 <= pos_t && kb >= lo_last;   // every row sees all of the block: no masking (most blocks)
                 uint32_t c[4][32];
-                const float mn = fmaxf(m, scores_of<CAPPED>(c, ts, a, interior, kb, lo_r, p_r));
+                const float mn = fmaxf(m, scores_of<CAPPED>(c, ts, a, interior, kb, lo_r, p_r, r < rows_t, look));
                 const bool raise = r < rows_t && mn > m && (m == -INFINITY || (mn - m) * a.scale_log2e > RAISE_MAX_BY);
                 if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
                     const float alpha = m == -INFINITY ? 0.f : exp2_fast((m - mn) * a.scale_log2e);
@@ -525,7 +583,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) prefill_wide_kernel(const __g
         const int lo_r = fx_first_key(p_r, a.window, 0), lo_last = fx_first_key(pos0 + n_tok - 1, a.window, 0);
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16, to = tmem_o + lane_off;
         float m = -INFINITY, l = 0.f;
-        bool ok = true;
+        bool ok = true, look = true;
         for (int i = 0; i < n; ++i) {
             ok = __all_sync(0xffffffffu, met(s_full(i & 1), (uint32_t)(i >> 1) & 1u, abort_flag));
             if (!ok) break;
@@ -540,7 +598,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) prefill_wide_kernel(const __g
             const bool interior = kb + BK - 1 <= pos0 && kb >= lo_last;
             const uint32_t ts = tmem + 128u * (i & 1) + lane_off;
             uint32_t c[4][32];
-            const float mn = fmaxf(m, scores_of<CAPPED>(c, ts, a, interior, kb, lo_r, p_r));
+            const float mn = fmaxf(m, scores_of<CAPPED>(c, ts, a, interior, kb, lo_r, p_r, r < rows, look));
             const bool raise = r < rows && mn > m && (m == -INFINITY || (mn - m) * a.scale_log2e > RAISE_MAX_BY);
             if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
                 const float alpha = m == -INFINITY ? 0.f : exp2_fast((m - mn) * a.scale_log2e);
@@ -686,7 +744,7 @@ extern "C" int fx_prefill_attention_grouped(const void* q, long ldq, int n_token
     constexpr float LOG2E = 1.4426950408889634f;
     const bool capped = softcap > 0.f;
     const Args a = {block_table, table_width, n_pages, items, (bf16*)out, ldo, part_o, part_ml, n_kv_heads, group, per, head_dim, window,
-                    capped ? 1.f : scale * LOG2E, capped ? 2.f * LOG2E * scale / softcap : 0.f, softcap * LOG2E, status};
+                    (capped ? softcap : scale) * LOG2E, capped ? scale / softcap : 0.f, status};
     CUtensorMap mq, mk, mv;
     const cuuint64_t W = head_dim, G = n_kv_heads;
     if (!encode(&mq, q, W, group, G, n_tokens, W, W * group, ldq, group, per) || !encode(&mk, k_pages, W, BK, G, n_pages, W, BK * W, G * BK * W, BK, 1) ||

@@ -640,6 +640,43 @@ def test_a_plan_of_layers_that_are_cut_differently(first, second, monkeypatch):
     check(out, c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT[first[3]])
 
 
+@pytest.mark.parametrize("softcap", [1e5, 1e6, 1e7, 1e30])
+@pytest.mark.parametrize("dtype,H,G,D", [("bf16", 4, 2, 128), ("bf16", 3, 3, 64), ("bf16", 6, 2, 256), ("f32", 4, 2, 128)])
+def test_caps_far_beyond_the_scores(dtype, H, G, D, softcap):
+    """A capped score is exact in proportion to itself, not to its cap.  Against the definition without a cap: scores are below 32 in size,
+    and c tanh(s / c) is off s by at most |s|^3 / (3 c^2), 1.1e-6 here and below what a score's own arithmetic may be off by."""
+    entries = [(9, 0), (33, 2), (200, 70), (1, 90), (300, 0)]
+    c = Cache([n + s for n, s in entries], G, D, 64, 92)
+    T = sum(n for n, _ in entries)
+    q, st = rows(T, H, G, D, DTYPES[dtype], 93), step(entries, c.slots)
+    out = torch.full((T, H * D), 7.0, dtype=q.dtype, device=DEV)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *st, out, H, G, D, None, D ** -0.5, softcap=softcap)
+    check(out, c, entries, q, H, None, D ** -0.5, None, PROMPT_WEIGHT[dtype])
+    ops.decode_attention_fp8(q, *c.operands, *st, out, H, G, D, None, D ** -0.5, softcap=softcap)
+    check(out, c, entries, q, H, None, D ** -0.5, None, WEIGHT[dtype])
+
+
+@pytest.mark.parametrize("softcap", [0.3, 2.0])
+@pytest.mark.parametrize("D", [64, 256])
+def test_scores_on_either_side_of_half_the_cap(softcap, D):
+    """Scores from far below the cap to far beyond it in one row, and a request's bits whatever the request beside it has: which of the
+    two forms a score takes is its own affair."""
+    H, G = 4, 2
+    entries = [(70, 60), (150, 0)]
+    c = Cache([130, 150], G, D, 64, 94)
+    q = rows(220, H, G, D, torch.bfloat16, 95)
+    q[:70] *= torch.exp2(torch.linspace(-12, 4, 70)).to(DEV)[:, None].bfloat16()
+    st, plan, outs = step(entries, c.slots), ops.prefill_fp8_plan(entries, 64, DEV), []
+    for size in (1.0, 0.0, 1000.0):
+        x = q.clone()
+        x[70:] *= size
+        out = torch.full((220, H * D), 7.0, dtype=q.dtype, device=DEV)
+        ops.prefill_attention_fp8(x, *c.operands, plan, *st, out, H, G, D, None, D ** -0.5, softcap=softcap)
+        outs.append(out)
+    check(outs[0], c, entries, q, H, None, D ** -0.5, softcap, PROMPT_WEIGHT["bf16"])
+    assert torch.equal(outs[0][:70], outs[1][:70]) and torch.equal(outs[0][:70], outs[2][:70])
+
+
 # ---- streams, graphs, order -----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_on_a_stream_of_its_own_and_in_a_graph(dtype):
