@@ -2195,6 +2195,15 @@ def decode_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_si
     return out
 
 
+def _scratch(n, device, stream, now):
+    """``n`` floats for kernels on ``stream``, which they belong to (``now``: the current stream): given back, they are handed out again
+    behind those kernels only."""
+    if stream != now:
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream)):
+            return torch.empty(n, dtype=torch.float32, device=device)
+    return torch.empty(n, dtype=torch.float32, device=device)
+
+
 def _decode_fp8(found, page_size, n_heads, window, scale, softcap, stream):
     (device, now, x, kp, vp, kep, vep, tp, pp, sp, lp, qp, op, zp, ip, N, G, _, D, S, W, T, B, _, _, _, n, ldq, ldo) = found
     if ip == 0 and n < 0:
@@ -2211,12 +2220,7 @@ def _decode_fp8(found, page_size, n_heads, window, scale, softcap, stream):
         return call("fx_decode_attention_fp8", *pages, B, *heads, 1, 0, 0, zp, st)
     global _launches
     _launches += 1
-    size = n * n_heads * runs * (D + 2)
-    if st != now:                              # (scratch belongs to the stream that the kernels run on)
-        with torch.cuda.stream(torch.cuda.ExternalStream(st)):
-            work = torch.empty(size, dtype=torch.float32, device=device)
-    else:
-        work = torch.empty(size, dtype=torch.float32, device=device)
+    work = _scratch(n * n_heads * runs * (D + 2), device, st, now)
     base = work.data_ptr()
     call("fx_decode_attention_fp8", *pages, B, *heads, runs, base, base + 4 * n * n_heads * runs * D, zp, st)
 
@@ -2457,23 +2461,24 @@ def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_he
     scale, scores capped or not.  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``, ``parts``: device copies of what
     :func:`prefill_grouped_plan` returns, and its number of parts."""
     name = "prefill_attention_grouped"
-    (_, now, x, qp, kp, vp, tp, ip, op, mp, zp, T, Q, N, G, P, D, B, W, n, eight, O, n_merges, four, _, ldq, ldo) = _operands(
+    (device, now, x, qp, kp, vp, tp, ip, op, mp, zp, T, Q, N, G, P, D, B, W, n, eight, O, n_merges, four, _, ldq, ldo) = _operands(
         name, _GROUPED, ("q", "k_pages", "v_pages", "block_table", "items", "out", "merges", "status"), q, k_pages, v_pages, block_table, items, out,
         merges, status)
     if (x != BF16 or (G, P, D) != (n_kv_heads, 128, head_dim) or n_heads < 1 or n_heads % G or min(Q, O) < n_heads * D or eight != 8 or four not in (-1, 4)
             or (parts and n_merges < 1)):
         raise KernelError(f"{name}: bfloat16, {n_heads} heads on pages [pages, {n_kv_heads}, 128, {head_dim}], items [n, 8], merges [n, 4] of {parts} parts: "
                           f"found {q.dtype}, pages [{N}, {G}, {P}, {D}], rows of {Q} and {O}, items [{n}, {eight}], merges [{n_merges}, {four}]")
+    st = stream if stream is not None else _scoped_stream if _scoped_stream is not None else now
     po = pm = 0
     if parts:
         global _launches
         _launches += 1
         width, rows = 64 if D <= 64 else 128 if D <= 128 else 256, parts * G * (256 if D <= 128 else 128)
-        work = torch.empty(rows * (width + 2), dtype=torch.float32, device=q.device)
+        work = _scratch(rows * (width + 2), device, st, now)
         po = work.data_ptr()
         pm = po + 4 * rows * width
     call("fx_prefill_attention_grouped", qp, ldq, T, kp, vp, N, tp, W, ip, n, op, ldo, n_heads, G, D, int(window or 0), float(scale), float(softcap or 0.0), po, pm,
-         mp if parts else 0, n_merges if parts else 0, zp, stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
+         mp if parts else 0, n_merges if parts else 0, zp, st)
     return out
 
 

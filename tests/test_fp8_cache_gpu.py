@@ -738,6 +738,28 @@ def test_a_prompt_on_a_stream_of_its_own():
     assert torch.equal(other, want)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_runs_on_a_stream_of_their_own(D):
+    """The kernel over pages of 128 on a named stream that begins late: what its runs leave is not handed to the current stream meanwhile."""
+    H, G, entries = 4, 2, [(50, 1200)]
+    items, merges, parts = ops.prefill_tc_plan(entries, None, G, tile=(2 if D <= 128 else 1) * 64, run_blocks=2)
+    assert parts > 1
+    g = torch.Generator().manual_seed(97)
+    q, k, v = (torch.randn(*shape, generator=g).bfloat16().to(DEV) for shape in ((50, H * D), (10, G, 128, D), (10, G, 128, D)))
+    table, items, merges = torch.arange(10, dtype=torch.int32, device=DEV)[None], torch.from_numpy(items).to(DEV), torch.from_numpy(merges).to(DEV)
+    args = (q, k, v, table, items)
+    want, out = torch.zeros(50, H * D, dtype=q.dtype, device=DEV), torch.zeros(50, H * D, dtype=q.dtype, device=DEV)
+    ops.prefill_attention_grouped(*args, want, H, G, D, None, 0.1, merges=merges, parts=parts)
+    torch.cuda.synchronize()
+    side, floats = torch.cuda.Stream(), parts * G * (256 if D <= 128 else 128) * (max(D, 64) + 2)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)                                       # (some 10 ms)
+    ops.prefill_attention_grouped(*args, out, H, G, D, None, 0.1, merges=merges, parts=parts, stream=side.cuda_stream)
+    others = [torch.full((floats,), 3.0, device=DEV) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and all(bool((x == 3).all()) for x in others)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_a_request_has_the_same_bits_alone_and_twice(dtype):
     """The order of a token's sums depends on the step's size and the table's width only."""
