@@ -2139,11 +2139,20 @@ def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, sp
          stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
 
 
+SCORE_SCALE_MAX = 2.0 ** 127     # of a scale, a cap and a scale over its cap: times log2(e), still a number of 32 bits
 _ATTEND_FP8 = "eNGPD eNGPD uNGP uNGP iSW iT iT iB xTQ~ xTO~ ?iZ ?in"
+
+
+def _check_scores(name, window, scale, softcap):
+    if ((window is not None and not 1 <= window < 1 << 31) or not abs(scale) <= SCORE_SCALE_MAX
+            or (softcap is not None and not (2.0 ** -149 <= softcap <= SCORE_SCALE_MAX and abs(scale) <= SCORE_SCALE_MAX * softcap))):
+        raise KernelError(f"{name}: window={window}, softcap={softcap}, scale={scale}: positive 32-bit (or None), positive (or None), finite, and the cap, the "
+                          "scale and the scale over the cap at most 2^127: they are numbers of 32 bits")
 
 
 def _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, status, tokens, out,
                            n_heads, n_kv_heads, head_dim, window, scale, softcap):
+    _check_scores(name, window, scale, softcap)
     found = _operands(name, _ATTEND_FP8, _CACHE_FP8 + _STEP + ("q", "out", "status", "tokens"), k_pages, v_pages, k_exp, v_exp, block_table, positions,
                       token_seq, seq_slot, q, out, status, tokens)
     _check_fp8(name, found[15:19], page_size, n_kv_heads, head_dim)
@@ -2151,8 +2160,6 @@ def _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table,
     need = n_heads * head_dim
     if n_heads < 1 or n_heads % n_kv_heads or found[20] == 0 or found[23] < need or found[24] < need:
         raise KernelError(f"{name}: {n_heads} heads on {n_kv_heads} of {head_dim}, {found[20]} pages a request: found rows of {found[23]} and {found[24]}")
-    if (window is not None and not 1 <= window < 1 << 31) or (softcap is not None and not softcap > 0) or not abs(scale) < float("inf"):
-        raise KernelError(f"{name}: window={window}, softcap={softcap}, scale={scale}: positive 32-bit (or None), positive (or None), finite")
     return found
 
 
@@ -2417,11 +2424,12 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
     cache = (k_pages, v_pages, k_exp, v_exp, block_table, page_size)
     step = (positions, token_seq, seq_slot)
     # Which kernel (:func:`prefill_f32_ok`, :func:`prefill_ok` and what the grouped one asks, from what is known already; pages that are
-    # read back have q's type and lie on the allocator's grid).  The tiled kernels find a row's maximum before they scale it.
+    # read back have q's type and lie on the allocator's grid).  The tiled kernels find a row's maximum before they scale it, by a number
+    # of 32 bits that is none of its smallest.
     x, kp, vp, qp, op, ldq, ldo = found[2], found[3], found[4], found[11], found[12], found[27], found[28]
     f32, wide = x == F32, 4 if x == F32 else 8
-    tiled = scale > 0 and ldq % wide == 0 and qp % 16 == 0 and (head_dim <= 128 and head_dim % 4 == 0 and ldo % 4 == 0 and op % 16 == 0 if f32 else
-                                                                head_dim % 16 == 0 and ldo % 2 == 0)
+    tiled = scale >= 2.0 ** -126 and ldq % wide == 0 and qp % 16 == 0 and (head_dim <= 128 and head_dim % 4 == 0 and ldo % 4 == 0 and op % 16 == 0 if f32 else
+                                                                             head_dim % 16 == 0 and ldo % 2 == 0)
     kind = ("f32" if f32 else ("tc" if head_dim <= 128 else "mma") if n_heads > 128 * n_kv_heads or ldo % 8 or op % 16 else
             "capped" if softcap is not None else "grouped")
     route = tiled and plan.route(kind if decode_fp8_ok(kp, vp, head_dim, page_size) else None, window, n_heads, n_kv_heads, head_dim, 4 if f32 else 2)
@@ -2461,6 +2469,7 @@ def prefill_attention_grouped(q, k_pages, v_pages, block_table, items, out, n_he
     scale, scores capped or not.  ``block_table``: int32 [entries, blocks], a row an entry; ``items``, ``merges``, ``parts``: device copies of what
     :func:`prefill_grouped_plan` returns, and its number of parts."""
     name = "prefill_attention_grouped"
+    _check_scores(name, window or None, scale, softcap or None)
     (device, now, x, qp, kp, vp, tp, ip, op, mp, zp, T, Q, N, G, P, D, B, W, n, eight, O, n_merges, four, _, ldq, ldo) = _operands(
         name, _GROUPED, ("q", "k_pages", "v_pages", "block_table", "items", "out", "merges", "status"), q, k_pages, v_pages, block_table, items, out,
         merges, status)

@@ -132,6 +132,26 @@ def test_bad_attention(which, bad):
         _calls(_cache(), _step())[which](**bad)
 
 
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("bad", [dict(softcap=math.inf), dict(softcap=math.nan), dict(softcap=1e39), dict(softcap=3e38), dict(softcap=1e-46), dict(scale=1e39),
+                                 dict(scale=-3e38), dict(softcap=1e-30, scale=1e10), dict(softcap=1e-44), dict(softcap=10 ** 400), dict(window=1 << 31)])
+def test_scores_beyond_32_bits(which, bad):
+    """A cap of which 32 bits hold 0 would be none at all, an infinite one or an infinite scale no number: refused, whatever the operands."""
+    with pytest.raises(ops.KernelError, match="softcap="):
+        _calls(_cache(), _step())[which](**bad)
+    if which == 3:
+        with pytest.raises(ops.KernelError, match="prefill_attention_grouped: window=.* softcap="):
+            ops.prefill_attention_grouped(*[torch.zeros(1)] * 6, 4, 2, 32, **{**dict(window=None, scale=1.0), **bad})
+
+
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("good", [dict(softcap=1e30), dict(softcap=1e-30), dict(scale=1e37, softcap=1.0), dict(scale=-1e-50), dict(scale=0.0, softcap=2.0 ** -149),
+                                  dict(window=(1 << 31) - 1)])
+def test_scores_within_32_bits(which, good):
+    with pytest.raises(ops.KernelError, match="an operand on cpu"):
+        _calls(_cache(), _step())[which](**good)
+
+
 @pytest.mark.parametrize("bad", [dict(n_heads=8), dict(head_dim=16), dict(inv_freq=torch.zeros(3), rotary_dim=32),
                                  dict(inv_freq=torch.zeros(16, dtype=torch.float64), rotary_dim=32),
                                  dict(inv_freq=torch.zeros(16), rotary_dim=32, cos_sin=torch.zeros(2, 16, 2))])

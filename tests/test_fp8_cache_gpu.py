@@ -589,6 +589,20 @@ def test_scales_that_are_not_positive(dtype, scale, softcap):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [1e-50, 1e-40, 2.0 ** -126])
+@pytest.mark.parametrize("softcap", [None, 4.0])
+def test_scales_that_32_bits_hardly_hold(dtype, scale, softcap):
+    """All keys that are seen count the same then."""
+    H, G, D, P = 4, 2, 64, 64
+    entries = [(40, 60), (120, 0)]
+    c = Cache([100, 120], G, D, P, 98)
+    q = rows(160, H, G, D, DTYPES[dtype], 99)
+    st, out = step(entries, c.slots), torch.full((160, H * D), 7.0, dtype=DTYPES[dtype], device=DEV)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, P, DEV), *st, out, H, G, D, None, scale, softcap=softcap)
+    check(out, c, entries, q, H, None, scale, softcap, PROMPT_WEIGHT[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("H,G,D,P", [(4, 2, 128, 256), (3, 1, 64, 384), (2, 2, 20, 1), (2, 1, 256, 512), (8, 1, 16, 1024)])
 def test_pages_longer_than_a_tile(dtype, H, G, D, P):
     lens = [1, 100, 700, 1500]
