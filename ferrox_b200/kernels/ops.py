@@ -2068,7 +2068,7 @@ _STEP = ("positions", "token_seq", "seq_slot")
 def _check_fp8(name, found, page_size, n_kv_heads, head_dim):
     """The sizes of an 8-bit cache, which come first in ``found``: pages, kv heads, page, head size."""
     N, G, P, D = found
-    if P != page_size or N == 0 or not 0 < D <= FP8_MAX_DIM or (n_kv_heads is not None and (G != n_kv_heads or D != head_dim)):
+    if P != page_size or N == 0 or not 0 < D <= FP8_MAX_DIM or (n_kv_heads is not None and (G == 0 or G != n_kv_heads or D != head_dim)):
         raise KernelError(f"{name}: pages of {page_size} positions, {n_kv_heads or 'any'} heads of {head_dim or 'up to'} {'' if head_dim else FP8_MAX_DIM}"
                           f" elements (at most {FP8_MAX_DIM}), at least one: found [{N}, {G}, {P}, {D}]")
 

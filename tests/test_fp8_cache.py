@@ -180,6 +180,14 @@ def test_a_plan_of_another_step():
             ops.prefill_fp8_plan(entries, page, "cpu")
 
 
+def test_no_kv_heads():
+    """Nothing to write for, and nothing for a query to read: refused where the heads are named (the queries would stay unrotated)."""
+    with pytest.raises(ops.KernelError, match="pages of 16 positions"):
+        ops._check_fp8("x", (3, 0, 16, 32), 16, 0, 32)
+    ops._check_fp8("x", (3, 0, 16, 32), 16, None, None)                     # (reading none of them back is nothing to do)
+    ops._check_fp8("x", (3, 2, 16, 32), 16, 2, 32)
+
+
 # ---- how a prompt step is planned -----------------------------------------------------------------------------------
 @pytest.mark.parametrize("window", [None, 5, 40])
 @pytest.mark.parametrize("most", [1, 3000, 1 << 30])
