@@ -194,6 +194,20 @@ def test_rotation_without_a_write_leaves_the_cache():
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("D,rot", [(64, 64), (20, 8)])
+def test_no_byte_is_written_without_a_write(dtype, D, rot):
+    c = Cache([20], 2, D, 16, 6)
+    pos, seq, slots = step([(4, 10)], c.slots)
+    qkv = rows(4, 2, 2, D, DTYPES[dtype], 7)
+    inv, was = (10000.0 ** (-torch.arange(rot // 2).float() / (rot // 2))).to(DEV), qkv.clone()
+    before = [(p.view(torch.uint8).clone(), e.clone()) for p, e in c.dev]
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.rope_kv_write_fp8(qkv, pos, seq, slots, inv, rot, *c.operands, 2, 2, D, write_cache=False, status=status)
+    assert not torch.equal(qkv[:, :4 * D], was[:, :4 * D]) and torch.equal(qkv[:, 4 * D:], was[:, 4 * D:]) and int(status) == 0
+    assert all(torch.equal(p.view(torch.uint8), p0) and torch.equal(e, e0) for (p, e), (p0, e0) in zip(c.dev, before))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_rows_at_the_ends_of_the_range(dtype):
     G, D, P = 1, 64, 16
     c = Cache([P], G, D, P, 8)
@@ -474,6 +488,23 @@ def test_a_prompt_next_to_rows_that_are_no_numbers(dtype, H, softcap, D):
     bad = torch.isnan(out).any(-1).cpu()
     assert bad[:60].sum() == 0 and bad[60:100].all() and not bad[100:].any()
     assert torch.isfinite(out[:60]).all() and torch.isfinite(out[100:]).all()
+
+
+@pytest.mark.parametrize("dtype,H,G,D,extra", [("bf16", 4, 2, 64, 2), ("bf16", 2, 2, 128, 2), ("bf16", 4, 1, 256, 2), ("bf16", 129, 1, 32, 0), ("bf16", 130, 1, 144, 0),
+                                               ("f32", 4, 2, 20, 0), ("f32", 3, 1, 68, 0), ("f32", 4, 2, 64, 1), ("f32", 2, 2, 128, 0)])
+@pytest.mark.parametrize("window,softcap", [(None, None), (25, None), (None, 20.0)])
+def test_rows_that_are_no_numbers_by_every_route(dtype, H, G, D, extra, window, softcap):
+    """Results off the 16-byte grid, more query heads a kv head than a tile has rows, odd head sizes: who sees such a row, and nobody else."""
+    entries = [(100, 0), (70, 30), (9, 4)]
+    c = Cache([100, 128, 13], G, D, 64, 100)
+    for b, at, which in ((0, 60, 1), (0, 99, 0), (1, 20, 0), (1, 29, 1), (1, 120, 0)):      # (behind 120, 20 and 29: in the window of some)
+        c.dev[which][1][int(c.table[int(c.slots[b]), at // 64]), :, at % 64] = 255
+    T = 179
+    q = rows(T, H, G, D, DTYPES[dtype], 101)
+    out = torch.full((T, H * D + extra), 7.0, dtype=q.dtype, device=DEV)
+    ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan(entries, 64, DEV), *step(entries, c.slots), out[:, :H * D], H, G, D, window, 0.1, softcap=softcap)
+    check(out[:, :H * D], c, entries, q, H, window, 0.1, softcap, PROMPT_WEIGHT[dtype])
+    assert (out[:, H * D:] == 7).all()
 
 
 @pytest.mark.parametrize("H,G,D", [(6, 2, 128), (7, 1, 64), (16, 4, 80), (6, 2, 256), (5, 1, 144)])
@@ -789,6 +820,24 @@ def test_a_request_has_the_same_bits_alone_and_twice(dtype):
         ops.decode_attention_fp8(q, *c.operands, *step(entries, c.slots), out, H, G, D, None, 0.09)
         outs.append(out)
     assert all(torch.equal(o, outs[0]) for o in outs) and all(torch.equal(outs[0][b], outs[0][0]) for b in range(8))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("window", [None, 200])
+def test_single_tokens_have_their_bits_whoever_is_beside_them(dtype, window):
+    """In a step of as many tokens over a table as wide, a request's results do not hang on the other requests' lengths or places."""
+    H, G, D, P, outs = 16, 4, 128, 64, []
+    for others in ([1500] * 7, [1, 40, 128, 129, 700, 1400, 1500], [1] * 7):
+        for place in (0, 5):
+            c = Cache([1500] * 8, G, D, P, 102)
+            lens = others[:place] + [1333] + others[place:]
+            slots = torch.cat([c.slots[1:1 + place], c.slots[:1], c.slots[1 + place:]])
+            q = rows(8, H, G, D, DTYPES[dtype], 103 + place)
+            q[place] = rows(1, H, G, D, DTYPES[dtype], 104)[0]
+            out = torch.empty(8, H * D, dtype=q.dtype, device=DEV)
+            ops.decode_attention_fp8(q, *c.operands, *step([(1, n - 1) for n in lens], slots), out, H, G, D, window, 0.09)
+            outs.append(out[place])
+    assert all(torch.equal(o, outs[0]) for o in outs)
 
 
 # ---- the operators as an engine uses them ---------------------------------------------------------------------------
