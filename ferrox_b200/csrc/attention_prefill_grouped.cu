@@ -693,8 +693,13 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
 {
     auto kern = prefill_grouped_kernel<D, CAPPED>;
     // what the softmax threads ask for has to be there: the block's registers at its launch
-    static const bool fits = [&] { cudaFuncAttributes at; return cudaFuncGetAttributes(&at, kern) == cudaSuccess && at.numRegs * 3 >= REGS_FEW + 2 * REGS_MANY; }();
-    if (!fits) return FX_ERR_SIZE;
+    static int regs = 0;                                 // (found once; a call that could not be answered is asked again)
+    if (!regs) {
+        cudaFuncAttributes at;
+        if (const cudaError_t e = cudaFuncGetAttributes(&at, kern)) return (int)e;
+        regs = at.numRegs;
+    }
+    if (regs * 3 < REGS_FEW + 2 * REGS_MANY) return FX_ERR_REGISTERS;
     // of the current device: asked for each time
     if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL)) return (int)e;
     fx_launch_pdl(kern, dim3(a.n_kv_heads, n_items), NTHREADS, Smem<D>::TOTAL, s, mq, mk, mv, a);

@@ -16,6 +16,7 @@
 #define FX_ERR_SIZE -2      // a size outside what the kernel handles
 #define FX_ERR_ALIGN -3     // pointer or stride not aligned as required
 #define FX_ERR_TIMEOUT -4   // a bounded wait inside a kernel ran out
+#define FX_ERR_REGISTERS -6 // built with fewer registers a thread than the kernel hands out among its warps
 
 typedef __nv_bfloat16 bf16;
 

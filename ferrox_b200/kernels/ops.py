@@ -26,6 +26,7 @@ _ERRORS = {
     -3: "pointer or stride not aligned as the kernel requires",
     -4: "a bounded wait inside a kernel ran out",
     -5: "the request needs more scratch than the library's fixed array holds",
+    -6: "the compiler gave the kernel fewer registers a thread than it hands out among its warps",
 }
 
 

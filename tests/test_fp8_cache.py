@@ -180,6 +180,17 @@ def test_a_plan_of_another_step():
             ops.prefill_fp8_plan(entries, page, "cpu")
 
 
+def test_every_error_of_the_library_has_its_words():
+    import os
+    import re
+    from ferrox_b200.kernels import lib
+    codes = set()
+    for name in ("common.cuh", "no_alloc.h"):
+        with open(os.path.join(lib.CSRC, name)) as f:
+            codes |= {int(c) for c in re.findall(r"#define FX_ERR_\w+ (-\d+)", f.read())}
+    assert codes == set(ops._ERRORS) and len(set(ops._ERRORS.values())) == len(codes) >= 6
+
+
 def test_no_kv_heads():
     """Nothing to write for, and nothing for a query to read: refused where the heads are named (the queries would stay unrotated)."""
     with pytest.raises(ops.KernelError, match="pages of 16 positions"):
