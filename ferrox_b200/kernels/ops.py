@@ -2203,11 +2203,16 @@ def decode_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_si
     return out
 
 
+def _stream_of(pointer, device):
+    """The stream at an address as an object.  (The default stream's is 0, of which ExternalStream makes a new stream.)"""
+    return torch.cuda.ExternalStream(pointer, device=device) if pointer else torch.cuda.default_stream(device)
+
+
 def _scratch(n, device, stream, now):
     """``n`` floats for kernels on ``stream``, which they belong to (``now``: the current stream): given back, they are handed out again
     behind those kernels only."""
     if stream != now:
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream)):
+        with torch.cuda.stream(_stream_of(stream, device)):
             return torch.empty(n, dtype=torch.float32, device=device)
     return torch.empty(n, dtype=torch.float32, device=device)
 
@@ -2292,7 +2297,7 @@ class PrefillFp8Plan:
         if self._stream != stream:
             if self._stream is not None and not torch.cuda.is_current_stream_capturing():
                 now = torch.cuda.current_stream(self.device)
-                now.wait_stream(torch.cuda.ExternalStream(self._stream, device=self.device))
+                now.wait_stream(_stream_of(self._stream, self.device))
                 for t in self._tensors:
                     t.record_stream(now)
             self._stream = stream
@@ -2419,7 +2424,7 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
                           f"{B} entries, {T} tokens and pages of {page_size}")
     st = stream if stream is not None else _scoped_stream if _scoped_stream is not None else found[1]
     if st != found[1]:                   # (scratch and lists belong to the stream that the kernels run on)
-        with torch.cuda.stream(torch.cuda.ExternalStream(st)), stream_scope(st):
+        with torch.cuda.stream(_stream_of(st, found[0])), stream_scope(st):
             return prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, plan, positions, token_seq, seq_slot,
                                          out, n_heads, n_kv_heads, head_dim, window, scale, softcap=softcap, status=status)
     cache = (k_pages, v_pages, k_exp, v_exp, block_table, page_size)

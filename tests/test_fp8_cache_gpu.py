@@ -805,6 +805,51 @@ def test_runs_on_a_stream_of_their_own(D):
     assert torch.equal(out, want) and all(bool((x == 3).all()) for x in others)
 
 
+def test_the_default_stream_named_from_another():
+    """Calls that name the default stream while another is current; a plan that goes from one to the other and back."""
+    H, G, D, P = 4, 2, 64, 64
+    entries = [(300, 50), (3, 1400)]
+    c = Cache([350, 1403], G, D, P, 105)
+    q = rows(303, H, G, D, torch.bfloat16, 106)
+    st, plan, operands = step(entries, c.slots), ops.prefill_fp8_plan(entries, P, DEV), c.operands
+    outs = [torch.zeros(303, H * D, dtype=q.dtype, device=DEV) for _ in range(6)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.prefill_attention_fp8(q, *operands, plan, *st, outs[0], H, G, D, None, 0.1, stream=0)
+        ops.prefill_attention_fp8(q, *operands, plan, *st, outs[1], H, G, D, None, 0.1)
+        ops.decode_attention_fp8(q, *operands, *st, outs[2], H, G, D, None, 0.1, stream=0)
+        ops.decode_attention_fp8(q, *operands, *st, outs[3], H, G, D, None, 0.1)
+    ops.prefill_attention_fp8(q, *operands, plan, *st, outs[4], H, G, D, None, 0.1)
+    ops.prefill_attention_fp8(q, *operands, plan, *st, outs[5], H, G, D, None, 0.1, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    check(outs[0], c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT["bf16"])
+    check(outs[2], c, entries, q, H, None, 0.1, None, WEIGHT["bf16"])
+    assert all(torch.equal(outs[0], outs[i]) for i in (1, 4, 5)) and torch.equal(outs[2], outs[3])
+
+
+@pytest.mark.parametrize("first_named", [False, True])
+def test_a_plan_made_on_a_default_stream_that_is_late(first_named):
+    """Another stream's use of a plan waits for the lists, which the default stream has still to copy."""
+    H, G, D, P = 4, 2, 64, 64
+    entries = [(300, 50), (40, 1400), (200, 0)]
+    c = Cache([350, 1440, 200], G, D, P, 107)
+    q = rows(540, H, G, D, torch.bfloat16, 108)
+    st, plan, operands = step(entries, c.slots), ops.prefill_fp8_plan(entries, P, DEV), c.operands
+    late, out = (torch.zeros(540, H * D, dtype=q.dtype, device=DEV) for _ in range(2))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert ops._stream_of(0, 0) == torch.cuda.default_stream(0) and ops._stream_of(side.cuda_stream, 0).cuda_stream == side.cuda_stream
+    torch.cuda._sleep(40_000_000)                                           # (some 20 ms)
+    with torch.cuda.stream(side if first_named else torch.cuda.default_stream()):
+        ops.prefill_attention_fp8(q, *operands, plan, *st, late, H, G, D, None, 0.1, stream=0)
+    with torch.cuda.stream(side):
+        ops.prefill_attention_fp8(q, *operands, plan, *st, out, H, G, D, None, 0.1)
+    torch.cuda.synchronize()
+    check(out, c, entries, q, H, None, 0.1, None, PROMPT_WEIGHT["bf16"])
+    assert torch.equal(late, out)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_a_request_has_the_same_bits_alone_and_twice(dtype):
     """The order of a token's sums depends on the step's size and the table's width only."""
