@@ -29,7 +29,8 @@
 // with references, W and O of its own, and its first thread issues its O(j).  While one group waits for its product the other
 // works.  The two are added up at the end.  Every wait is bounded (status 3).
 //
-// What bounds it, B200.  A step long enough streams 7.35 TB/s (two tiles of 32 KB in 1.32 us an SM: the memory), and a launch
+// What bounds it, B200.  74 requests of 16,384 positions stream 6.88 TB/s, their second half 7.35 (1.25 GB a step and three steps' caches in
+// turn: none of it from the L2; torch's sum reads 4 GiB at 6.8, a copy moves 6.55, reads and writes together), and a launch
 // costs 8 to 11 us beside that, the last blocks of a round among them: 64 requests of up to 4,096 positions, 28 heads on 4 of 128,
 // 39.6 us of which the bytes are 27.4; one request of 131,072 in 33.0 of 20.6 (its 74 runs a kv head: 2.2 us to add them up); one of 37 in 5.4, a
 // chain of waits (lookups 0.9 us, boxes asked 1.6, all met 2.0, keys landed 2.3, S 2.6, W 3.1, O 3.5, written 4.2).

@@ -19,7 +19,7 @@
 //
 // What bounds it, in clocks of a pair of blocks, of which the four products are 2,056: a sub-tile's chain of waits.  Scores read and
 // their maximum found 500, asked whether it is to be raised 190, weights 1,540 (their 2^x alone 1,024), the rest of PV and the next
-// S 1,330.  B200: 3,600 clocks a pair with few blocks running, 2.39 us with all (982 TFLOP/s over long contexts; 28 heads of 128 on 4).  Six
+// S 1,330.  B200: 3,600 clocks a pair with few blocks running, 2.39 us with all (966 TFLOP/s for 4,096 tokens behind 28,672; 28 heads of 128 on 4).  Six
 // portions of 300 tokens behind up to 3,800, the pages' reading back included: 86 us; a prompt of 2,048 of 16 heads with their own
 // keys 49.5 (by the kernel of attention_prefill_tc.cu 65); with capped scores 129 and 70, and 152 and 83 where
 // scores come near the cap (there 280 and 139).  Tried: scores read twice instead of held, P in one piece 2.91 us a pair; a
@@ -31,6 +31,14 @@
 // A row of the cache that is not finite arrives as a key of NaN and a value of 0 (read_kv_fp8_spans): the scores against it are
 // NaN where a query sees it and masked away where none does, and 0 times the value is 0.  What lies behind a request's last
 // position in its last page is 0.
+//
+// Weights are rounded to bfloat16 (at most 2^-8 of the weight) for the second product, whose other operand is bfloat16; the denominator
+// adds them up unrounded.  Adding up what the product has, as the general forms of attention_prefill_tc.cu do, is an instruction a score more:
+// the portions 89 us instead of 86, capped 140 instead of 129, for results off by 2.05e-3 of their size instead of 2.16e-3, and where all
+// values lie around 1 by 0.0083 at most instead of 0.0134.
+//
+// Registers: 168 a thread at the launch, of which the first four warps give their share away.  The forms for heads of 128 spill 60 bytes a
+// thread, those for 64 20, the wide ones none.
 //
 // The running maximum is raised only when it grows by more than 2^8; O is then scaled in tensor memory.  Every wait is bounded
 // (status 3).  Tiles with many key blocks may be cut into runs, which a second kernel adds up in their order (items: as the plan of

@@ -2165,7 +2165,8 @@ def _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table,
 
 
 def decode_fp8_ok(k_address: int, v_address: int, head_dim: int, page_size: int) -> bool:
-    """Whether the tensor-core kernel takes such pages (head sizes and pages in steps of 16); others go to a warp a (token, head)."""
+    """Whether the tensor-core kernel takes such pages (head sizes and pages in steps of 16); others go to
+    eight warps a (token, head) on the CUDA cores."""
     return head_dim % 16 == 0 and page_size % 16 == 0 and k_address % 16 == 0 and v_address % 16 == 0
 
 
@@ -2253,7 +2254,9 @@ def fp8_token_by_token(kind, entries, window, n_heads, n_kv_heads, head_dim, sms
     to 600 positions and 8 of up to 4,000, 24 tokens each, decode against tiled: 28 heads of 128 on 4 (grouped) 50 against 28 and 89
     against 43, 96 tokens of one request of 600 19 against 23; the same with capped scores 51 against 37, 93 against 54, 20 against 32; 16 heads of
     256 on 4 83 against 29 and 94 against 64 (by the mma.sync kernel 109 and 429); 16 heads of 128 on 4 in 32 bits 48 against 119 and 81 against 322;
-    prompts of 300, 193 and 97 tokens of 4 heads of 64 on 2 in 32 bits 28 against 24."""
+    prompts of 300, 193 and 97 tokens of 4 heads of 64 on 2 in 32 bits 28 against 24.  Heads of 129 to 256 elements are rated by the
+    constants of the shorter ones' kernels, which have not been fitted to theirs.  The choice is the whole step's: a portion's rounding
+    hangs on who else is in the step."""
     together = (256 if head_dim <= 128 else 128) * n_kv_heads // n_heads     # tokens of a tile that holds the heads of a kv head
     rows, base, block, chain = {"grouped": (together, 14.0, 2.4, 0.0), "capped": (together, 24.0, 4.0, 0.0), "tc": (256, 30.0, 4.5, 0.0),
                                 "mma": (PREFILL_TILE, 12.0, 3.0, 0.107 * head_dim / 256),
@@ -2409,7 +2412,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
 
     The keys and values that a portion sees are read back once into pages of q's type (exact: an element has four significant bits
     and a power of two) and the attention kernels for such pages take them from there: tensor cores then meet operands that they take
-    as they are, where conversion in the attention kernel would be paid again for every tile.  Every position that is seen has a page.
+    as they are, where conversion in the attention kernel would be paid again for every tile.  Every position that is seen has a page
+    (one without counts for nothing or as a key and a value of zeros, whichever way its portion goes).
     Entries of up to FP8_FEW_TOKENS tokens, steps that are done sooner token by token (:func:`fp8_token_by_token`), scales that are not
     positive and shapes that no tiled kernel takes go to :func:`decode_attention_fp8`.  A call
     may be captured once the plan has been used; the plan lives as long as the graph."""
@@ -2461,7 +2465,8 @@ def prefill_attention_fp8(q, k_pages, v_pages, k_exp, v_exp, block_table, page_s
 
 def prefill_grouped_plan(entries, window, n_heads: int, n_kv_heads: int, head_dim: int):
     """:func:`prefill_tc_plan` for :func:`prefill_attention_grouped`: whole tokens of all the query heads of a kv head, in two halves of
-    up to 128 rows, or one for heads of more than 128 elements."""
+    up to 128 rows, or one for heads of more than 128 elements.  (Where a tile is cut goes by what an item costs the kernel of
+    :func:`prefill_tc_plan`; what it costs this one beside its blocks has not been measured.)"""
     return prefill_tc_plan(entries, window, n_kv_heads, tile=(2 if head_dim <= 128 else 1) * (128 * n_kv_heads // n_heads))
 
 

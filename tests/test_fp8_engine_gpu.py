@@ -138,6 +138,12 @@ def test_windowed_capped_attention_beside_another_mixer(tmp_path, monkeypatch, n
     assert off.median() < 1e-4 and off.max() < 5e-2
 
 
+@pytest.mark.parametrize("name", ["A", "B", "C", "E"])
+def test_portions_beside_another_mixer(tmp_path, monkeypatch, name):
+    """Portions of so few tokens that the mixers of a sum run side by side, prompts by the tiled kernels and by the decode kernel."""
+    test_windowed_capped_attention_beside_another_mixer(tmp_path, monkeypatch, name, [20, 33, 9, 8, 12])
+
+
 def test_models_with_other_caches_are_refused(tmp_path):
     import bobepel_configs
     from ferrox_b200 import Engine
