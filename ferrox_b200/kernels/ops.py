@@ -2140,15 +2140,16 @@ def read_kv_fp8_spans(k_pages, v_pages, k_exp, v_exp, block_table, page_size, sp
          stream if stream is not None else _scoped_stream if _scoped_stream is not None else now)
 
 
-SCORE_SCALE_MAX = 2.0 ** 127     # of a scale, a cap and a scale over its cap: times log2(e), still a number of 32 bits
+# of a scale or a cap, and of a scale over its cap: times log2(e), and 2 log2(e), still numbers of 32 bits
+SCORE_SCALE_MAX, SCORE_RATIO_MAX = 2.0 ** 127, 2.0 ** 125
 _ATTEND_FP8 = "eNGPD eNGPD uNGP uNGP iSW iT iT iB xTQ~ xTO~ ?iZ ?in"
 
 
 def _check_scores(name, window, scale, softcap):
     if ((window is not None and not 1 <= window < 1 << 31) or not abs(scale) <= SCORE_SCALE_MAX
-            or (softcap is not None and not (2.0 ** -149 <= softcap <= SCORE_SCALE_MAX and abs(scale) <= SCORE_SCALE_MAX * softcap))):
-        raise KernelError(f"{name}: window={window}, softcap={softcap}, scale={scale}: positive 32-bit (or None), positive (or None), finite, and the cap, the "
-                          "scale and the scale over the cap at most 2^127: they are numbers of 32 bits")
+            or (softcap is not None and not (2.0 ** -149 <= softcap <= SCORE_SCALE_MAX and abs(scale) <= SCORE_RATIO_MAX * softcap))):
+        raise KernelError(f"{name}: window={window}, softcap={softcap}, scale={scale}: positive 32-bit (or None), positive (or None), finite, as numbers "
+                          "of 32 bits: a cap and a scale of at most 2^127, 2^125 times the cap")
 
 
 def _look_at_attention_fp8(name, q, k_pages, v_pages, k_exp, v_exp, block_table, page_size, positions, token_seq, seq_slot, status, tokens, out,

@@ -145,6 +145,14 @@ def test_scores_beyond_32_bits(which, bad):
 
 
 @pytest.mark.parametrize("which", [2, 3])
+def test_scales_so_far_over_their_cap_that_nothing_times_them_is_no_number(which):
+    """2^127 times 2 log2(e), which the prompt kernel multiplies a score with, is infinite, and a score may be 0."""
+    for over, refused in ((2.0 ** 126, True), (2.0 ** 125, False)):
+        with pytest.raises(ops.KernelError, match="2\\^125 times the cap" if refused else "an operand on cpu"):
+            _calls(_cache(), _step())[which](softcap=0.5, scale=over / 2)
+
+
+@pytest.mark.parametrize("which", [2, 3])
 @pytest.mark.parametrize("good", [dict(softcap=1e30), dict(softcap=1e-30), dict(scale=1e37, softcap=1.0), dict(scale=-1e-50), dict(scale=0.0, softcap=2.0 ** -149),
                                   dict(window=(1 << 31) - 1)])
 def test_scores_within_32_bits(which, good):
