@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import plain_fp8_cache as plain
+import test_fp8_cache as host
 from ferrox_b200.kernels import ops
 
 pytestmark = pytest.mark.gpu
@@ -313,6 +314,24 @@ def test_decode(dtype, H, G, D, P):
     ops.decode_attention_fp8(q, *c.operands, *step(entries, c.slots), out, H, G, D, None, D ** -0.5, status=status)
     assert int(status) == 0
     check(out, c, entries, q, H, None, D ** -0.5, None, WEIGHT[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("H,G,D,P", [(4, 2, 144, 16), (3, 1, 192, 32), (18, 2, 240, 64), (9, 1, 32, 48), (2, 2, 112, 80), (12, 1, 128, 16)])
+@pytest.mark.parametrize("window", [None, 70])
+def test_decode_of_other_head_sizes(dtype, H, G, D, P, window):
+    """Heads that end inside a slab of 128 elements or a step of 32, pages that hold no whole tile; a row named twice."""
+    lens = [1, 63, 128, 500, 1300]
+    c = Cache(lens, G, D, P, H + D + 1)
+    entries = [(1, n - 1) for n in lens]
+    q, st = rows(5, H, G, D, DTYPES[dtype], 5, extra=3), step(entries, c.slots)
+    out = torch.full((5, H * D + 1), 7.0, dtype=q.dtype, device=DEV)
+    ops.decode_attention_fp8(q, *c.operands, *st, out[:, :H * D], H, G, D, window, D ** -0.5, softcap=30.0)
+    check(out[:, :H * D], c, entries, q, H, window, D ** -0.5, 30.0, WEIGHT[dtype])
+    some = torch.full_like(out, 7.0)
+    ops.decode_attention_fp8(q, *c.operands, *st, some[:, :H * D], H, G, D, window, D ** -0.5, softcap=30.0,
+                             tokens=torch.tensor([4, 0, 4, 3, 0], dtype=torch.int32, device=DEV))
+    assert torch.equal(some[[0, 3, 4]], out[[0, 3, 4]]) and (some[[1, 2]] == 7).all() and (out[:, H * D:] == 7).all()
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -954,6 +973,66 @@ def test_steps_without_entries():
                  lambda: ops.prefill_attention_fp8(q, *c.operands, ops.prefill_fp8_plan([(2, 2)], P, DEV), *st, out, H, G, D, None, 1.0)):
         with pytest.raises(ops.KernelError, match="no entries"):
             call()
+
+
+LABELS = {"k_pages": "k_pages", "v_pages": "v_pages", "k_exp": "k_exp", "v_exp": "v_exp", "block_table": "block_table|pages a request|a size", "page_size": "pages of 8"}
+
+
+def on_device(x):
+    if isinstance(x, torch.Tensor):
+        return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=DEV).copy_(x)
+    return x
+
+
+def calls_on_device(cache, step, **over):
+    """The calls of the host's tests with every operand on the device."""
+    T, H, G, D = 3, 4, 2, 32
+    qkv, out, kv = (torch.zeros(*shape, dtype=torch.bfloat16, device=DEV) for shape in ((T, (H + 2 * G) * D), (T, H * D), (T, G, D)))
+    plan = ops.prefill_fp8_plan([(T, 0)], cache["page_size"], DEV)
+    own = (dict(qkv=qkv), dict(k_out=kv, v_out=kv.clone()), dict(q=qkv, out=out), dict(q=qkv, out=out, plan=plan))
+    calls = host._calls(*({k: on_device(v) for k, v in x.items()} for x in (cache, step)))
+    return [lambda call=call, x=x: call(**{**x, **{k: on_device(v) for k, v in over.items()}}) for call, x in zip(calls, own)]
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("bad", range(len(host.BAD_CACHES)))
+def test_bad_caches_on_the_device(which, bad):
+    """What is refused on the host is refused by the operand's name where all of them lie on the device."""
+    with pytest.raises(ops.KernelError, match=LABELS[next(iter(host.BAD_CACHES[bad]))]):
+        calls_on_device(host._cache(**host.BAD_CACHES[bad]), host._step())[which]()
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("bad", range(len(host.BAD_STEPS)))
+def test_bad_steps_on_the_device(which, bad):
+    name = next(iter(host.BAD_STEPS[bad]))
+    with pytest.raises(ops.KernelError, match="token_seq|positions" if name == "token_seq" else name):
+        calls_on_device(host._cache(), {**host._step(), **host.BAD_STEPS[bad]})[which]()
+
+
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("bad", [dict(n_heads=3), dict(n_heads=0), dict(head_dim=64), dict(n_kv_heads=4), dict(out=torch.zeros(3, 128)),
+                                 dict(out=torch.zeros(3, 100, dtype=torch.bfloat16)), dict(out=torch.zeros(2, 128, dtype=torch.bfloat16)),
+                                 dict(q=torch.zeros(3, 96, dtype=torch.bfloat16))])
+def test_bad_attention_on_the_device(which, bad):
+    with pytest.raises(ops.KernelError, match="out is a|rows of" if "out" in bad else "heads"):
+        calls_on_device(host._cache(), host._step(), **bad)[which]()
+
+
+@pytest.mark.parametrize("bad", [dict(n_heads=8), dict(head_dim=16), dict(inv_freq=torch.zeros(3), rotary_dim=32),
+                                 dict(inv_freq=torch.zeros(16, dtype=torch.float64), rotary_dim=32),
+                                 dict(inv_freq=torch.zeros(16), rotary_dim=32, cos_sin=torch.zeros(2, 16, 2))])
+def test_bad_writes_on_the_device(bad):
+    with pytest.raises(ops.KernelError, match="cos_sin" if "cos_sin" in bad else "inv_freq" if bad.get("inv_freq") is not None and bad["inv_freq"].dtype == torch.float64
+                       else "heads"):
+        calls_on_device(host._cache(), host._step(), **bad)[0]()
+
+
+def test_good_calls_on_the_device():
+    """The calls that the refusals above are variants of."""
+    for call in calls_on_device(host._cache(), host._step()):
+        call()
+    torch.cuda.synchronize()
 
 
 def test_a_prompt_in_a_graph():
