@@ -2298,13 +2298,14 @@ class PrefillFp8Plan:
         """The next uses are on the (current) stream ``stream``: behind the uses before on another one, which copied the lists, and
         the lists are not freed under its kernels.  (A capture begins behind everything that was under way, and its graph needs
         the plan for as long as it lives.)"""
-        if self._stream != stream:
-            if self._stream is not None and not torch.cuda.is_current_stream_capturing():
-                now = torch.cuda.current_stream(self.device)
-                now.wait_stream(_stream_of(self._stream, self.device))
-                for t in self._tensors:
-                    t.record_stream(now)
-            self._stream = stream
+        if self._stream == stream or (self._stream is not None and torch.cuda.is_current_stream_capturing()):
+            return
+        if self._stream is not None:
+            now = torch.cuda.current_stream(self.device)
+            now.wait_stream(_stream_of(self._stream, self.device))
+            for t in self._tensors:
+                t.record_stream(now)
+        self._stream = stream
 
     def kept(self, key, make):
         """What ``make`` returns, made once: a tuple's numpy arrays as tensors on the device."""

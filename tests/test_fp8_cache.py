@@ -318,3 +318,30 @@ def test_a_plan_serves_layers_that_are_cut_differently(a, b, monkeypatch):
             assert covered[0][0] == 0 and covered[-1][1] == n and all(x[1] == y[0] for x, y in zip(covered, covered[1:]))
             assert all(0 <= e < table.shape[0] and t // 40 == e == (end - 1) // 40 for t, end, e in covered)
             at += n
+
+
+# ---- a plan on several streams --------------------------------------------------------------------------------------
+def test_a_capture_does_not_stand_for_the_stream_before_it(monkeypatch):
+    """The stream that copied a plan's lists is waited for by the next one that is no capture's, a capture between them or not."""
+    waited, capturing = [], False
+
+    class Stream:
+        def wait_stream(self, other):
+            waited.append(other)
+
+    monkeypatch.setattr(ops, "_stream_of", lambda pointer, device: pointer)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    plan = ops.prefill_fp8_plan([(20, 0)], 16, "cpu")
+    plan.on_stream(1)
+    plan.on_stream(1)
+    assert waited == []
+    capturing = True
+    plan.on_stream(2)
+    assert waited == []
+    capturing = False
+    plan.on_stream(3)
+    assert waited == [1]
+    plan.on_stream(1)
+    plan.on_stream(3)
+    assert waited == [1, 3, 1]
