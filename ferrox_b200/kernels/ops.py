@@ -2253,10 +2253,11 @@ def fp8_token_by_token(kind, entries, window, n_heads, n_kv_heads, head_dim, sms
     ``kind``: the tiled kernel that would take the step.  A tile of ``rows`` (token, query head) pairs costs ``block`` a 128 keys that it sees, all
     SMs sharing the tiles; one that is not cut into runs takes ``chain`` a key by itself; ``base`` are the launches.  20 requests of up
     to 600 positions and 8 of up to 4,000, 24 tokens each, decode against tiled: 28 heads of 128 on 4 (grouped) 50 against 28 and 89
-    against 43, 96 tokens of one request of 600 19 against 23; the same with capped scores 51 against 37, 93 against 54, 20 against 32; 16 heads of
+    against 43, 96 tokens of one request of 600 19 against 23; the same with capped scores 51 against 35, 92 against 51, 20 against 29; 16 heads of
     256 on 4 83 against 29 and 94 against 64 (by the mma.sync kernel 109 and 429); 16 heads of 128 on 4 in 32 bits 48 against 119 and 81 against 322;
     prompts of 300, 193 and 97 tokens of 4 heads of 64 on 2 in 32 bits 28 against 24.  Heads of 129 to 256 elements are rated by the
-    constants of the shorter ones' kernels, which have not been fitted to theirs.  The choice is the whole step's: a portion's rounding
+    constants of the shorter ones' kernels: of 12 steps of 16 heads of 256 on 4, capped or not, the sooner way is chosen in 11 (96 tokens of one
+    request of 600, capped: 28 token by token, 23 tiled).  The choice is the whole step's: a portion's rounding
     hangs on who else is in the step."""
     together = (256 if head_dim <= 128 else 128) * n_kv_heads // n_heads     # tokens of a tile that holds the heads of a kv head
     rows, base, block, chain = {"grouped": (together, 14.0, 2.4, 0.0), "capped": (together, 24.0, 4.0, 0.0), "tc": (256, 30.0, 4.5, 0.0),
